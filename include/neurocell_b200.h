@@ -22,6 +22,9 @@
  *   nc_softmax_ce_loss -> optax.softmax_cross_entropy_with_integer_labels(...).mean()
  *                       as used by the reference's classification drivers
  *   nc_sgd_update    -> optax.sgd update + apply_updates inside trainer.py:101-106
+ *   nc_linear_ce_*, nc_orthogonalize, nc_muon_update -> no counterpart in the reference: a
+ *                       readout of the output ports over a large vocabulary, and an update
+ *                       by orthogonalised momentum beside nc_sgd_update
  */
 #ifndef NEUROCELL_B200_H_
 #define NEUROCELL_B200_H_
@@ -33,7 +36,7 @@
 extern "C" {
 #endif
 
-#define NC_ABI_VERSION 7
+#define NC_ABI_VERSION 8
 
 typedef enum nc_status {
   NC_OK = 0,
@@ -250,6 +253,49 @@ nc_status nc_mse_loss(const float* out, const float* targets, int32_t batch, int
 /* Mean softmax cross-entropy over `batch` rows of `n` logits with int32 labels. */
 nc_status nc_softmax_ce_loss(const float* logits, const int32_t* labels, int32_t batch,
                              int32_t n, float* loss, float* g_logits, void* stream);
+
+/* Element types of the operators that take more than float32. */
+typedef enum nc_dtype { NC_F32 = 0, NC_BF16 = 1 } nc_dtype;
+
+typedef enum nc_reduction { NC_REDUCE_MEAN = 0, NC_REDUCE_SUM = 1, NC_REDUCE_NONE = 2 } nc_reduction;
+
+/*
+ * Softmax cross-entropy of a linear readout over a (large) vocabulary, without the
+ * (rows, classes) logits in memory: z = features weight^T + bias, and for every row
+ * loss = log sum exp z - z[label].
+ *   features (rows, dim), weight (classes, dim), bias (classes) or null: row-major, `dtype`
+ *   labels (rows) int32.  A row whose label is ignore_index (which must lie outside
+ *   [0, classes)) takes no part: its loss and feature gradient are 0 and its features are
+ *   not used, whatever they hold.  Any other label outside [0, classes) makes the loss and
+ *   the gradients NaN; nothing is read out of range.
+ * A bias of -inf takes its class out; a row with every class taken out has a NaN loss, as
+ * has one with a logit of NaN or +inf.  Sums and statistics are held in float32.
+ */
+typedef struct nc_linear_ce {
+  int32_t rows, dim, classes;   /* rows may be 0: the loss and the weight's gradients are 0 */
+  int32_t dtype;                /* nc_dtype of features, weight, bias and their gradients   */
+  int32_t ignore_index;
+  int32_t reduction;            /* nc_reduction; the mean is over the rows that take part
+                                   (0 when none does)                                       */
+} nc_linear_ce;
+
+/* Workspace bytes of one nc_linear_ce_forward (grad 0) or nc_linear_ce_backward (grad 1);
+   the two share nothing through it.  0 for a bad descriptor. */
+size_t nc_linear_ce_workspace_bytes(const nc_linear_ce* desc, int32_t grad);
+
+/* loss: float32 device memory, 1 value (mean, sum) or `rows` values (none).  lse (rows)
+   float32 receives the log-sum-exp that nc_linear_ce_backward takes. */
+nc_status nc_linear_ce_forward(const nc_linear_ce* desc, const void* features, const void* weight,
+                               const void* bias, const int32_t* labels, float* loss, float* lse,
+                               void* d_ws, size_t ws_bytes, void* stream);
+
+/* Gradients (overwritten; each may be null) for the loss gradient g_loss: a device float32
+   (mean, sum), `rows` of them (none), or null for ones.  Deterministic: no floating-point
+   atomics, sums in a fixed order. */
+nc_status nc_linear_ce_backward(const nc_linear_ce* desc, const void* features, const void* weight,
+                                const void* bias, const int32_t* labels, const float* lse,
+                                const float* g_loss, void* g_features, void* g_weight, void* g_bias,
+                                void* d_ws, size_t ws_bytes, void* stream);
 
 /*
  * Batch staging without the copy engine (no counterpart in the reference): copies `nseg`

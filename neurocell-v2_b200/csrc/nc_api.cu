@@ -135,7 +135,7 @@ static nc_status check_codd(const nc_codd* c) {
 // or page-locked host memory that is mapped into the device's address space (cudaHostAlloc,
 // cudaHostRegister with mapping; under unified addressing the same pointer).  Anything else
 // (pageable host memory, unknown pointers) is refused on the host, before any launch.
-static nc_status device_address(const void* p, const char* name, const void** dev) {
+nc_status device_address(const void* p, const char* name, const void** dev) {
   if (!p) return set_error(NC_ERR_INVALID, "%s is null", name);
   cudaPointerAttributes at;
   cudaError_t e = cudaPointerGetAttributes(&at, p);
@@ -155,7 +155,7 @@ static nc_status device_address(const void* p, const char* name, const void** de
                    "pass device memory or page-locked host memory", name);
 }
 
-static nc_status check_ptr(const void* p, const char* name) {
+nc_status check_ptr(const void* p, const char* name) {
   if (!p) return set_error(NC_ERR_INVALID, "%s is null", name);
   if (reinterpret_cast<uintptr_t>(p) % 4 != 0) return set_error(NC_ERR_INVALID, "%s is not 4-byte aligned", name);
   return NC_OK;
@@ -193,7 +193,7 @@ static nc_status set_smem_attr(const void* fn, size_t bytes) {
   return NC_OK;
 }
 
-static nc_status launch_check(const char* what) {
+nc_status launch_check(const char* what) {
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_error(e, what);
   note_launch();

@@ -15,6 +15,12 @@ nc_status cuda_error(cudaError_t e, const char* what);
 void clear_error();
 // Counts one successful kernel launch (reported by nc_launch_count).
 void note_launch();
+// After a kernel launch: its error, or NC_OK with the launch counted.
+nc_status launch_check(const char* what);
+// Refuses null and misaligned (4 bytes) pointers.
+nc_status check_ptr(const void* p, const char* name);
+// The device address of `p`; memory that the device cannot access is refused.
+nc_status device_address(const void* p, const char* name, const void** dev);
 
 // Launch configuration with programmatic dependent launch: the grid may be scheduled
 // before the kernel it follows on the stream has finished, once every CTA of that kernel

@@ -12,7 +12,7 @@ import threading
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libneurocell_b200.so")
-ABI_VERSION = 7
+ABI_VERSION = 8
 
 NC_OK, NC_ERR_INVALID, NC_ERR_WORKSPACE, NC_ERR_UNSUPPORTED, NC_ERR_CUDA = 0, 1, 2, 3, 4
 NC_PAD = {"VALID": 0, "SAME": 1, "CIRCULAR": 2}
@@ -20,6 +20,8 @@ NC_ACT = {"identity": 0, "tanh": 1, "sigmoid": 2, "relu": 3, "leaky_relu": 4, "g
 NC_CODD = {"continuous": 0, "annealed": 1, "ste_binary": 2, "ste_ternary": 3}
 NC_CONV = {"auto": 0, "direct": 1, "fft": 2}
 NC_FLAG_TRAIN = 1
+NC_DTYPE = {"float32": 0, "bfloat16": 1}
+NC_REDUCE = {"mean": 0, "sum": 1, "none": 2}
 
 # Every symbol the header declares (checked by the CPU test-suite).
 EXPORTED = (
@@ -31,6 +33,7 @@ EXPORTED = (
     "nc_dp_allreduce_sgd", "nc_dp_status", "nc_launch_count", "nc_conv_path",
     "nc_vnn_forward_universe", "nc_vnn_backward_universe", "nc_universe_embed_forward",
     "nc_universe_embed_backward", "nc_workspace_status", "nc_dp_reset", "nc_stage_from_host",
+    "nc_linear_ce_workspace_bytes", "nc_linear_ce_forward", "nc_linear_ce_backward",
 )
 NC_DP_MAX_RANKS = 8
 NC_IPC_HANDLE_BYTES = 64
@@ -62,10 +65,17 @@ class NcStageSeg(ctypes.Structure):
 NC_MAX_STAGE_SEGS = 4
 
 
+class NcLinearCe(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_int32), ("dim", ctypes.c_int32), ("classes", ctypes.c_int32),
+                ("dtype", ctypes.c_int32), ("ignore_index", ctypes.c_int32),
+                ("reduction", ctypes.c_int32)]
+
+
 _vp, _sz, _i32, _u32, _i64, _f32 = (ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int32,
                                     ctypes.c_uint32, ctypes.c_int64, ctypes.c_float)
 _TP = ctypes.POINTER(NcTopo)
 _CP = ctypes.POINTER(NcCodd)
+_LP = ctypes.POINTER(NcLinearCe)
 
 _SIGS = {
     "nc_plan_bytes": (_sz, [_TP]),
@@ -105,6 +115,9 @@ _SIGS = {
     "nc_workspace_status": (_i32, [_vp, ctypes.POINTER(_i32), _vp]),
     "nc_dp_reset": (_i32, [_vp, _vp, _sz, _vp]),
     "nc_stage_from_host": (_i32, [ctypes.c_void_p, _i32, _vp]),
+    "nc_linear_ce_workspace_bytes": (_sz, [_LP, _i32]),
+    "nc_linear_ce_forward": (_i32, [_LP, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "nc_linear_ce_backward": (_i32, [_LP, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
 }
 
 _lib = None

@@ -502,3 +502,147 @@ def sgd_(params: torch.Tensor, grads: torch.Tensor, lr: float) -> None:
     lib = _lib.load()
     _lib.check(lib.nc_sgd_update(_ptr(params), _ptr(grads), params.numel(), float(lr),
                                  _stream(params.device)), "nc_sgd_update")
+
+
+# ---------------------------------------------------------------------------------------
+# softmax cross-entropy of a linear readout over a large vocabulary
+# ---------------------------------------------------------------------------------------
+def _dtype_name(t: torch.Tensor) -> str:
+    return str(t.dtype).replace("torch.", "")
+
+
+class _on:
+    """Makes ``device`` current for the calls inside (launches go to the current device)."""
+
+    def __init__(self, device: torch.device):
+        self.index = device.index
+
+    def __enter__(self):
+        self.back = torch.cuda.current_device()
+        if self.back != self.index:
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc):
+        if self.back != self.index:
+            torch.cuda.set_device(self.back)
+        return False
+
+
+def _linear_ce_args(features, weight, labels, bias, ignore_index, reduction):
+    """Checks the arguments; returns the descriptor and contiguous tensors."""
+    for t, n in ((features, "features"), (weight, "weight"), (labels, "labels")):
+        _require_cuda(t, n)
+    if bias is not None:
+        _require_cuda(bias, "bias")
+    if reduction not in _lib.NC_REDUCE:
+        raise ValueError(f"Unsupported reduction '{reduction}'; choose from {tuple(_lib.NC_REDUCE)}.")
+    if features.ndim != 2 or weight.ndim != 2 or features.shape[1] != weight.shape[1]:
+        raise ValueError(f"features (rows, dim) and weight (classes, dim) expected, got "
+                         f"{tuple(features.shape)} and {tuple(weight.shape)}")
+    if labels.ndim != 1 or labels.shape[0] != features.shape[0]:
+        raise ValueError(f"labels (rows,) expected, got {tuple(labels.shape)} for {features.shape[0]} rows")
+    if labels.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"labels must be int32 or int64, got {labels.dtype}")
+    if _dtype_name(features) not in _lib.NC_DTYPE:
+        raise ValueError(f"features must be float32 or bfloat16, got {features.dtype}")
+    if bias is not None and (bias.ndim != 1 or bias.shape[0] != weight.shape[0]):
+        raise ValueError(f"bias (classes,) expected, got {tuple(bias.shape)}")
+    for t, n in ((weight, "weight"), (bias, "bias")):
+        if t is not None and t.dtype != features.dtype:
+            raise ValueError(f"{n} is {t.dtype}, features are {features.dtype}")
+    for t, n in ((weight, "weight"), (bias, "bias"), (labels, "labels")):
+        if t is not None and t.device != features.device:
+            raise ValueError(f"{n} is on {t.device}, features are on {features.device}")
+    d = _lib.NcLinearCe(features.shape[0], features.shape[1], weight.shape[0],
+                        _lib.NC_DTYPE[_dtype_name(features)], int(ignore_index),
+                        _lib.NC_REDUCE[reduction])
+    # int64 labels beyond int32 stay out of range instead of wrapping into it
+    if labels.dtype == torch.int64:
+        labels = labels.clamp(-2 ** 31, 2 ** 31 - 1).to(torch.int32)
+    return (d, features.contiguous(), weight.contiguous(), labels.contiguous(),
+            None if bias is None else bias.contiguous())
+
+
+def _linear_ce_ws(lib, d, grad: int, device) -> torch.Tensor:
+    n = lib.nc_linear_ce_workspace_bytes(ctypes.byref(d), grad)
+    if n == 0:
+        raise ValueError(f"linear_softmax_ce: {lib.nc_last_error().decode(errors='replace')}")
+    return torch.empty(n, dtype=torch.uint8, device=device)
+
+
+def _linear_ce_forward(lib, d, f, w, labels, b):
+    dev = f.device
+    ws = _linear_ce_ws(lib, d, 0, dev)
+    none = d.reduction == _lib.NC_REDUCE["none"]
+    loss = torch.empty((d.rows,) if none else (), dtype=torch.float32, device=dev)
+    lse = torch.empty(d.rows, dtype=torch.float32, device=dev)
+    if none and d.rows == 0:
+        return loss, lse
+    _lib.check(lib.nc_linear_ce_forward(ctypes.byref(d), _ptr(f), _ptr(w), _ptr(b), _ptr(labels),
+                                        _ptr(loss), _ptr(lse), _ptr(ws), ws.numel(), _stream(dev)),
+               "nc_linear_ce_forward")
+    return loss, lse
+
+
+def _linear_ce_backward(lib, d, f, w, labels, b, lse, g_loss, need_f, need_w, need_b):
+    dev = f.device
+    ws = _linear_ce_ws(lib, d, 1, dev)
+    g_f = torch.empty_like(f) if need_f else None
+    g_w = torch.empty_like(w) if need_w else None
+    g_b = torch.empty_like(b) if need_b else None
+    _lib.check(lib.nc_linear_ce_backward(ctypes.byref(d), _ptr(f), _ptr(w), _ptr(b), _ptr(labels),
+                                         _ptr(lse), _ptr(g_loss), _ptr(g_f), _ptr(g_w), _ptr(g_b),
+                                         _ptr(ws), ws.numel(), _stream(dev)),
+               "nc_linear_ce_backward")
+    return g_f, g_w, g_b
+
+
+class _LinearCE(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, features, weight, bias, labels, ignore_index, reduction):
+        lib = _lib.load()
+        d, f, w, lab, b = _linear_ce_args(features, weight, labels, bias, ignore_index, reduction)
+        with _on(f.device):
+            loss, lse = _linear_ce_forward(lib, d, f, w, lab, b)
+        ctx.save_for_backward(f, w, lab, lse, *(() if b is None else (b,)))
+        ctx.desc = d
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_loss):
+        lib = _lib.load()
+        f, w, lab, lse = ctx.saved_tensors[:4]
+        b = ctx.saved_tensors[4] if len(ctx.saved_tensors) > 4 else None
+        need_f, need_w, need_b = ctx.needs_input_grad[:3]
+        with _on(f.device):
+            g = _linear_ce_backward(lib, ctx.desc, f, w, lab, b, lse, g_loss.contiguous().float(),
+                                    need_f, need_w, need_b)
+        return (*g, None, None, None)
+
+
+def linear_softmax_ce_loss(features: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor,
+                           bias: torch.Tensor | None = None, ignore_index: int = -100,
+                           reduction: str = "mean") -> torch.Tensor:
+    """Softmax cross-entropy of the readout ``features @ weight.T + bias`` with integer
+    labels; the (rows, classes) logits are never held in memory.
+
+    ``features`` (rows, dim), ``weight`` (classes, dim) and ``bias`` (classes,) share one
+    type, float32 or bfloat16; the loss is float32.  ``reduction``: "mean" over the rows
+    whose label is not ``ignore_index`` (0 when there are none), "sum", or "none" (one loss
+    per row).  Any other label outside the classes gives NaN.  Differentiable once in
+    features, weight and bias (the gradient computes the logits a second time)."""
+    return _LinearCE.apply(features, weight, bias, labels, ignore_index, reduction)
+
+
+def linear_softmax_ce_value_and_grad(features: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor,
+                                     bias: torch.Tensor | None = None, ignore_index: int = -100,
+                                     reduction: str = "mean"):
+    """``(loss, g_features, g_weight, g_bias)`` of :func:`linear_softmax_ce_loss` without
+    autograd (``g_bias`` is None without a bias; with ``reduction="none"`` the gradients are
+    those of the losses' sum)."""
+    lib = _lib.load()
+    d, f, w, lab, b = _linear_ce_args(features, weight, labels, bias, ignore_index, reduction)
+    with _on(f.device):
+        loss, lse = _linear_ce_forward(lib, d, f, w, lab, b)
+        return (loss, *_linear_ce_backward(lib, d, f, w, lab, b, lse, None, True, True, b is not None))
