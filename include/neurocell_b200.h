@@ -319,6 +319,37 @@ nc_status nc_stage_from_host(const nc_stage_seg* segs, int32_t nseg, void* strea
 /* In-place SGD: params[i] -= lr * grads[i]  (lr read from host scalar). */
 nc_status nc_sgd_update(float* params, const float* grads, int64_t n, float lr, void* stream);
 
+/*
+ * Newton-Schulz orthogonalisation of `batch` matrices (rows, cols), row-major and packed:
+ * X0 = x / (|x|_F + eps), then `steps` times A = X X^T, X <- a X + (b A + c A^2) X (A = X^T X
+ * and X <- a X + X (b A + c A^2) when rows > cols).  Each singular value goes through the
+ * polynomial a s + b s^3 + c s^5; the singular vectors stay.  A zero matrix stays zero; a
+ * matrix that holds NaN or an infinity gives NaN in that matrix.
+ */
+typedef struct nc_newton_schulz {
+  int32_t batch, rows, cols;   /* batch may be 0                      */
+  int32_t dtype;               /* nc_dtype of x and out               */
+  int32_t steps;               /* 0..64                               */
+  float a, b, c;
+  float eps;                   /* >= 0                                */
+} nc_newton_schulz;
+
+size_t nc_newton_schulz_workspace_bytes(const nc_newton_schulz* desc);
+
+/* out = the orthogonalised x; out may be x itself. */
+nc_status nc_orthogonalize(const nc_newton_schulz* desc, const void* x, void* out, void* d_ws,
+                           size_t ws_bytes, void* stream);
+
+/*
+ * In-place update of `batch` float32 parameter matrices by orthogonalised momentum:
+ *   momentum <- beta momentum + grads;  u = grads + beta momentum (nesterov) or momentum
+ *   params <- (1 - lr weight_decay) params - lr sqrt(max(1, rows / cols)) orthogonalised(u)
+ * params, grads and momentum are different buffers.
+ */
+nc_status nc_muon_update(const nc_newton_schulz* desc, float* params, const float* grads,
+                         float* momentum, float lr, float beta, int32_t nesterov,
+                         float weight_decay, void* d_ws, size_t ws_bytes, void* stream);
+
 /* ---- data-parallel gradient exchange over NVLink ---------------------------------------- */
 /*
  * No counterpart in the reference (it has no multi-GPU code; the north star asks for the

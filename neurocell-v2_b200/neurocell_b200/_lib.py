@@ -34,6 +34,7 @@ EXPORTED = (
     "nc_vnn_forward_universe", "nc_vnn_backward_universe", "nc_universe_embed_forward",
     "nc_universe_embed_backward", "nc_workspace_status", "nc_dp_reset", "nc_stage_from_host",
     "nc_linear_ce_workspace_bytes", "nc_linear_ce_forward", "nc_linear_ce_backward",
+    "nc_newton_schulz_workspace_bytes", "nc_orthogonalize", "nc_muon_update",
 )
 NC_DP_MAX_RANKS = 8
 NC_IPC_HANDLE_BYTES = 64
@@ -71,11 +72,18 @@ class NcLinearCe(ctypes.Structure):
                 ("reduction", ctypes.c_int32)]
 
 
+class NcNewtonSchulz(ctypes.Structure):
+    _fields_ = [("batch", ctypes.c_int32), ("rows", ctypes.c_int32), ("cols", ctypes.c_int32),
+                ("dtype", ctypes.c_int32), ("steps", ctypes.c_int32), ("a", ctypes.c_float),
+                ("b", ctypes.c_float), ("c", ctypes.c_float), ("eps", ctypes.c_float)]
+
+
 _vp, _sz, _i32, _u32, _i64, _f32 = (ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int32,
                                     ctypes.c_uint32, ctypes.c_int64, ctypes.c_float)
 _TP = ctypes.POINTER(NcTopo)
 _CP = ctypes.POINTER(NcCodd)
 _LP = ctypes.POINTER(NcLinearCe)
+_NP = ctypes.POINTER(NcNewtonSchulz)
 
 _SIGS = {
     "nc_plan_bytes": (_sz, [_TP]),
@@ -118,6 +126,9 @@ _SIGS = {
     "nc_linear_ce_workspace_bytes": (_sz, [_LP, _i32]),
     "nc_linear_ce_forward": (_i32, [_LP, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "nc_linear_ce_backward": (_i32, [_LP, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "nc_newton_schulz_workspace_bytes": (_sz, [_NP]),
+    "nc_orthogonalize": (_i32, [_NP, _vp, _vp, _vp, _sz, _vp]),
+    "nc_muon_update": (_i32, [_NP, _vp, _vp, _vp, _f32, _f32, _i32, _f32, _vp, _sz, _vp]),
 }
 
 _lib = None

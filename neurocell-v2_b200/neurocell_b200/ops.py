@@ -646,3 +646,69 @@ def linear_softmax_ce_value_and_grad(features: torch.Tensor, weight: torch.Tenso
     with _on(f.device):
         loss, lse = _linear_ce_forward(lib, d, f, w, lab, b)
         return (loss, *_linear_ce_backward(lib, d, f, w, lab, b, lse, None, True, True, b is not None))
+
+
+# ---------------------------------------------------------------------------------------
+# orthogonalisation by Newton-Schulz products, and the update by orthogonalised momentum
+# ---------------------------------------------------------------------------------------
+NEWTON_SCHULZ_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+
+
+def _newton_schulz_desc(shape, dtype: str, steps, coefficients, eps) -> _lib.NcNewtonSchulz:
+    if len(shape) < 2 or shape[-1] < 1 or shape[-2] < 1:
+        raise ValueError(f"matrices (..., rows, cols) expected, got shape {tuple(shape)}")
+    if dtype not in _lib.NC_DTYPE:
+        raise ValueError(f"float32 or bfloat16 expected, got {dtype}")
+    a, b, c = coefficients
+    batch = int(np.prod(shape[:-2], dtype=np.int64))
+    return _lib.NcNewtonSchulz(batch, shape[-2], shape[-1], _lib.NC_DTYPE[dtype], int(steps), float(a),
+                               float(b), float(c), float(eps))
+
+
+def _newton_schulz_ws(lib, d, device) -> torch.Tensor:
+    n = lib.nc_newton_schulz_workspace_bytes(ctypes.byref(d))
+    if n == 0:
+        raise ValueError(f"newton_schulz: {lib.nc_last_error().decode(errors='replace')}")
+    return torch.empty(n, dtype=torch.uint8, device=device)
+
+
+def orthogonalize(x: torch.Tensor, steps: int = 5, coefficients=NEWTON_SCHULZ_COEFFICIENTS,
+                  eps: float = 1e-7) -> torch.Tensor:
+    """Newton-Schulz orthogonalisation of the matrices of ``x`` (..., rows, cols), float32 or
+    bfloat16: ``x / (|x| + eps)``, then ``steps`` times ``X <- a X + (b A + c A^2) X`` with
+    the Gram matrix ``A`` of the short side.  Returns a new tensor of ``x``'s type; products
+    and sums are as exact as float32 ones for either type.  Not differentiable."""
+    _require_cuda(x, "x")
+    lib = _lib.load()
+    d = _newton_schulz_desc(x.shape, _dtype_name(x), steps, coefficients, eps)
+    x = x.detach().contiguous()
+    out = torch.empty_like(x)
+    with _on(x.device):
+        ws = _newton_schulz_ws(lib, d, x.device)
+        _lib.check(lib.nc_orthogonalize(ctypes.byref(d), _ptr(x), _ptr(out), _ptr(ws), ws.numel(),
+                                        _stream(x.device)), "nc_orthogonalize")
+    return out
+
+
+def muon_(params: torch.Tensor, grads: torch.Tensor, momentum: torch.Tensor, lr: float,
+          beta: float = 0.95, nesterov: bool = True, weight_decay: float = 0.0, steps: int = 5,
+          coefficients=NEWTON_SCHULZ_COEFFICIENTS, eps: float = 1e-7) -> None:
+    """In-place update of the float32 matrices ``params`` (..., rows, cols) by orthogonalised
+    momentum, on the current stream: ``momentum = beta momentum + grads``, then
+    ``params = (1 - lr weight_decay) params - lr sqrt(max(1, rows / cols)) O`` with O the
+    orthogonalised ``grads + beta momentum`` (``nesterov``) or ``momentum``."""
+    for t, n in ((params, "params"), (grads, "grads"), (momentum, "momentum")):
+        _require_cuda(t, n)
+        if t.dtype != torch.float32:
+            raise ValueError(f"muon_ needs float32 tensors, {n} is {t.dtype}")
+        if t.shape != params.shape or t.device != params.device:
+            raise ValueError(f"muon_ needs tensors of one shape and device, {n} is {tuple(t.shape)} on {t.device}")
+        if not t.is_contiguous():
+            raise ValueError("muon_ needs contiguous tensors")
+    lib = _lib.load()
+    d = _newton_schulz_desc(params.shape, "float32", steps, coefficients, eps)
+    with _on(params.device):
+        ws = _newton_schulz_ws(lib, d, params.device)
+        _lib.check(lib.nc_muon_update(ctypes.byref(d), _ptr(params), _ptr(grads), _ptr(momentum), float(lr),
+                                      float(beta), int(nesterov), float(weight_decay), _ptr(ws), ws.numel(),
+                                      _stream(params.device)), "nc_muon_update")
