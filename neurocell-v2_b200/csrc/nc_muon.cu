@@ -12,6 +12,7 @@
 #include "nc_common.cuh"
 #include "nc_errors.h"
 #include "nc_readout.h"
+#include "nc_tc.cuh"
 
 namespace nc {
 
@@ -40,9 +41,11 @@ __device__ __forceinline__ double block_sum_f64(double v, double* red) {
 template <typename T>
 __global__ void __launch_bounds__(kNormThreads) ns_norm_kernel(const T* __restrict__ x, float* __restrict__ momentum,
                                                                MuonArgs mu, int64_t n, float* __restrict__ u,
-                                                               double* __restrict__ part) {
+                                                               double* __restrict__ part,
+                                                               int32_t* __restrict__ status) {
   __shared__ double red[kNormThreads / 32];
   pdl_enter();
+  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *status = 0;
   const size_t base = (size_t)blockIdx.y * n;
   const int64_t i0 = (int64_t)blockIdx.x * kNormThreads * kNormPer + threadIdx.x;
   double s = 0.0;
@@ -148,9 +151,169 @@ __global__ void ns_store_kernel(const float* __restrict__ x, int64_t n, T* __res
     store_as(out + i, x[i]);
 }
 
+// ---- products on the tensor cores --------------------------------------------------------
+// X, A = X X^T and b A + c A^2 are kept as two float16 planes each (nc_tc.cuh), scaled by
+// 2^12: |entries| stay below 16 while the singular values do, and an entry of 2^-26 still has
+// its 11 bits in the high plane.
+constexpr float kPlaneScale = 4096.f, kPlaneInv = 1.f / 4096.f;
+
+struct Planes {   // (batch, plane, rows, pitch)
+  __half* p;
+  int pitch;
+  int64_t plane;
+};
+
+// X0 of one matrix as planes.
+template <typename T>
+__global__ void __launch_bounds__(kNormThreads) ns_split_kernel(const T* __restrict__ x, int64_t n, int cols, int parts,
+                                                                const double* __restrict__ part, double eps,
+                                                                Planes out) {
+  __shared__ double red[kNormThreads / 32];
+  pdl_enter();
+  double s = 0.0;
+  for (int i = threadIdx.x; i < parts; i += kNormThreads) s += part[(size_t)blockIdx.y * parts + i];
+  s = block_sum_f64(s, red);
+  const double inv = 1.0 / (sqrt(s) + eps);
+  const size_t base = (size_t)blockIdx.y * n;
+  __half* hi = out.p + (size_t)blockIdx.y * 2 * out.plane;
+  const int64_t i0 = (int64_t)blockIdx.x * kNormThreads * kNormPer + threadIdx.x;
+#pragma unroll 4
+  for (int k = 0; k < kNormPer; ++k) {
+    const int64_t i = i0 + (int64_t)k * kNormThreads;
+    if (i >= n) break;
+    const int r = (int)i / cols, c = (int)i - r * cols;
+    uint16_t h, l;
+    tc::split_f16((float)((double)to_f32(x[base + i]) * inv) * kPlaneScale, &h, &l);
+    const size_t o = (size_t)r * out.pitch + c;
+    hi[o] = __ushort_as_half(h);
+    hi[out.plane + o] = __ushort_as_half(l);
+  }
+}
+
+enum NsMode { kGram, kPoly, kUpdate, kFinal };
+
+// 16 values of both planes, added up (still scaled).
+__device__ __forceinline__ void load_planes(const Planes& s, size_t o, float (&v)[16]) {
+  uint32_t h[8], l[8];
+  tc::load_v8(s.p + o, h);
+  tc::load_v8(s.p + s.plane + o, l);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float2 a = __half22float2(*reinterpret_cast<__half2*>(&h[i]));
+    const float2 b = __half22float2(*reinterpret_cast<__half2*>(&l[i]));
+    v[2 * i] = a.x + b.x, v[2 * i + 1] = a.y + b.y;
+  }
+}
+
+// Epilogue of the three products of a step, on scaled values:
+//   gram: A = acc;  poly: b A + c acc;  update: a X + acc;  final: the same, to the caller
+template <int MODE, typename T>
+struct NsEpilogue {
+  Planes src, dst;   // same shape: A for poly, X for update
+  int m, n;
+  float mul, add;    // value = mul acc + add src
+  T* out;            // final: the result (rows, cols), or
+  float* params;     // params <- decay params - step result
+  float decay, step;
+  bool wide;         // rows of out or params start on 32 bytes
+
+  template <int HALF>
+  __device__ __forceinline__ void run(const tc::Tile& x, int row, int col, float (&acc)[HALF]) const {
+    if (row >= m) return;
+    const size_t base = (size_t)x.batch * 2 * src.plane + (size_t)row * src.pitch;
+    const bool mirror = (MODE == kGram || MODE == kPoly) && x.n0 > x.m0;
+#pragma unroll
+    for (int j = 0; j < HALF; j += 16) {
+      if (col + j >= n) break;
+      float v[16];
+      if constexpr (MODE == kGram) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[e] = acc[j + e] * mul;
+      } else {
+        load_planes(src, base + col + j, v);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[e] = fmaf(acc[j + e], mul, v[e] * add);
+      }
+      if constexpr (MODE == kFinal) {
+        const size_t o = ((size_t)x.batch * m + row) * n + col + j;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[e] *= kPlaneInv;
+        if (params) {
+          if (wide && col + j + 16 <= n) {
+#pragma unroll
+            for (int e = 0; e < 16; e += 8) {
+              uint32_t q[8];
+              tc::load_v8(params + o + e, q);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) q[i] = __float_as_uint(__uint_as_float(q[i]) * decay - step * v[e + i]);
+              tc::store_v8(params + o + e, q);
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if (col + j + e < n) params[o + e] = params[o + e] * decay - step * v[e];
+          }
+        } else if (wide && col + j + 16 <= n) {
+          uint32_t q[8];
+          if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int e = 0; e < 16; e += 8) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) q[i] = __float_as_uint(v[e + i]);
+              tc::store_v8(out + o + e, q);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+              q[i] = *reinterpret_cast<const uint32_t*>(&b);
+            }
+            tc::store_v8(out + o, q);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (col + j + e < n) store_as(out + o + e, v[e]);
+        }
+      } else {
+        uint32_t h[8], l[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          uint16_t h0, l0, h1, l1;
+          tc::split_f16(v[2 * i], &h0, &l0);
+          tc::split_f16(v[2 * i + 1], &h1, &l1);
+          h[i] = h0 | (uint32_t)h1 << 16, l[i] = l0 | (uint32_t)l1 << 16;
+        }
+        __half* d = dst.p + base + col + j;
+        tc::store_v8(d, h);
+        tc::store_v8(d + dst.plane, l);
+        if (mirror) {   // lanes hold consecutive rows: the transposed store is contiguous over them
+          __half* t = dst.p + (size_t)x.batch * 2 * dst.plane + row;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            if (col + j + i >= n) break;
+            const size_t o = (size_t)(col + j + i) * dst.pitch;
+            t[o] = __ushort_as_half((uint16_t)(h[i / 2] >> (16 * (i & 1))));
+            t[o + dst.plane] = __ushort_as_half((uint16_t)(l[i / 2] >> (16 * (i & 1))));
+          }
+        }
+      }
+    }
+  }
+};
+
 size_t pad256(size_t n) { return (n + 255) / 256 * 256; }
 
 int norm_blocks(int64_t n) { return (int)((n + kNormThreads * kNormPer - 1) / (kNormThreads * kNormPer)); }
+
+// k-tiles (of 32) that one accumulator takes before it is added to the registers.
+constexpr int kNsChunk = 2;
+constexpr int kNsTile = 128;
+
+// The tensor cores from a short side of 65 on; below, one 64 x 64 float32 tile holds A.
+bool on_tensor_cores(const nc_newton_schulz* d) { return d->rows > 64 && d->cols > 64 && d->steps > 0; }
+
+int plane_pitch(int cols) { return (cols + 63) / 64 * 64; }
 
 struct NsLayout {
   size_t status, part, u, x, y, gram, poly, total;
@@ -159,6 +322,9 @@ struct NsLayout {
 NsLayout ns_layout(const nc_newton_schulz* d) {
   NsLayout L{};
   const size_t n = (size_t)d->rows * d->cols, s = d->rows < d->cols ? d->rows : d->cols;
+  // float32 (rows, cols), or two planes of float16 with padded rows
+  const bool tensor = on_tensor_cores(d);
+  const size_t x = tensor ? (size_t)d->rows * plane_pitch(d->cols) : n, g = tensor ? s * plane_pitch((int)s) : s * s;
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t o = at;
@@ -168,10 +334,10 @@ NsLayout ns_layout(const nc_newton_schulz* d) {
   L.status = take(4);
   L.part = take((size_t)d->batch * norm_blocks(n) * 8);
   L.u = take(d->batch * n * 4);
-  L.x = take(d->batch * n * 4);
-  L.y = take(d->batch * n * 4);
-  L.gram = take(d->batch * s * s * 4);
-  L.poly = take(d->batch * s * s * 4);
+  L.x = take(d->batch * x * 4);
+  L.y = take(d->batch * x * 4);
+  L.gram = take(d->batch * g * 4);
+  L.poly = take(d->batch * g * 4);
   L.total = at;
   return L;
 }
@@ -201,6 +367,69 @@ nc_status product(const Product& p, int batch, cudaStream_t st) {
   return launch_check("ns_product_kernel launch");
 }
 
+template <int MODE, typename T>
+nc_status tensor_product(const nc_newton_schulz* d, const Planes& A, bool a_mn, const Planes& B, bool b_mn, int m, int n,
+                         int k, const NsEpilogue<MODE, T>& epi, int32_t* status, cudaStream_t st) {
+  tc::Problem p{};
+  p.m = m, p.n = n, p.k = k, p.batch = d->batch, p.splits = 1, p.chunk = kNsChunk;
+  p.tiles_m = (m + tc::kBM - 1) / tc::kBM, p.tiles_n = (n + kNsTile - 1) / kNsTile;
+  p.symmetric = MODE == kGram || MODE == kPoly;
+  p.status = status;
+  NC_CHECK((tc::make_operand<2, kNsTile>(&p, true, A.p, a_mn, m, k, A.pitch, A.plane, d->batch, 2 * A.plane)));
+  NC_CHECK((tc::make_operand<2, kNsTile>(&p, false, B.p, b_mn, n, k, B.pitch, B.plane, d->batch, 2 * B.plane)));
+  return tc::launch_product<2, kNsTile>(p, epi, st, "Newton-Schulz product launch");
+}
+
+template <typename T>
+nc_status run_tensor(const nc_newton_schulz* d, const T* x, const float* u, const double* part, T* out, float* params,
+                     float decay, float step, char* ws, const NsLayout& L, cudaStream_t st) {
+  const int64_t n = (int64_t)d->rows * d->cols;
+  const int nb = norm_blocks(n), s = d->rows < d->cols ? d->rows : d->cols;
+  const bool tall = d->rows > d->cols;
+  int32_t* status = reinterpret_cast<int32_t*>(ws + L.status);
+  auto planes = [&](size_t o, int rows, int cols) {
+    Planes q;
+    q.p = reinterpret_cast<__half*>(ws + o), q.pitch = plane_pitch(cols), q.plane = (int64_t)rows * q.pitch;
+    return q;
+  };
+  Planes X = planes(L.x, d->rows, d->cols), Y = planes(L.y, d->rows, d->cols);
+  const Planes G = planes(L.gram, s, s), Q = planes(L.poly, s, s);
+  {
+    PdlLaunch l(dim3(nb, d->batch), dim3(kNormThreads), 0, st);
+    if (u)
+      NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, ns_split_kernel<float>, u, n, d->cols, nb, part, (double)d->eps, X));
+    else
+      NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, ns_split_kernel<T>, x, n, d->cols, nb, part, (double)d->eps, X));
+    NC_CHECK(launch_check("ns_split_kernel launch"));
+  }
+  const void* to = params ? static_cast<void*>(params) : static_cast<void*>(out);
+  const size_t size = params ? 4 : sizeof(T);
+  const bool wide = reinterpret_cast<uintptr_t>(to) % 32 == 0 && (size_t)d->cols * size % 32 == 0;
+  for (int k = 0; k < d->steps; ++k) {
+    NsEpilogue<kGram, T> g{};
+    g.src = g.dst = G, g.m = g.n = s, g.mul = kPlaneInv;
+    NC_CHECK(tensor_product(d, X, tall, X, tall, s, s, tall ? d->rows : d->cols, g, status, st));
+    NsEpilogue<kPoly, T> q{};
+    q.src = G, q.dst = Q, q.m = q.n = s, q.mul = d->c * kPlaneInv, q.add = d->b;
+    NC_CHECK(tensor_product(d, G, false, G, false, s, s, s, q, status, st));
+    // rows <= cols: (b A + c A^2) X, X with its own index contiguous; else X (b A + c A^2)
+    const Planes &A = tall ? X : Q, &B = tall ? Q : X;
+    if (k + 1 < d->steps) {
+      NsEpilogue<kUpdate, T> e{};
+      e.src = X, e.dst = Y, e.m = d->rows, e.n = d->cols, e.mul = kPlaneInv, e.add = d->a;
+      NC_CHECK(tensor_product(d, A, false, B, !tall, d->rows, d->cols, s, e, status, st));
+      const Planes t = X;
+      X = Y, Y = t;
+    } else {
+      NsEpilogue<kFinal, T> e{};
+      e.src = X, e.m = d->rows, e.n = d->cols, e.mul = kPlaneInv, e.add = d->a;
+      e.out = out, e.params = params, e.decay = decay, e.step = step, e.wide = wide;
+      NC_CHECK(tensor_product(d, A, false, B, !tall, d->rows, d->cols, s, e, status, st));
+    }
+  }
+  return NC_OK;
+}
+
 // From the source x (or x and momentum) to the orthogonalised matrix; `out` or `params`.
 template <typename T>
 nc_status run(const nc_newton_schulz* d, const T* x, float* momentum, MuonArgs mu, T* out, float* params, float decay,
@@ -213,9 +442,12 @@ nc_status run(const nc_newton_schulz* d, const T* x, float* momentum, MuonArgs m
   const int nb = norm_blocks(n), s = d->rows < d->cols ? d->rows : d->cols;
   {
     PdlLaunch l(dim3(nb, d->batch), dim3(kNormThreads), 0, st);
-    NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, ns_norm_kernel<T>, x, momentum, mu, n, f32(L.u), part));
+    NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, ns_norm_kernel<T>, x, momentum, mu, n, f32(L.u), part,
+                                     reinterpret_cast<int32_t*>(ws + L.status)));
     NC_CHECK(launch_check("ns_norm_kernel launch"));
   }
+  if (on_tensor_cores(d))
+    return run_tensor(d, x, momentum ? f32(L.u) : nullptr, part, out, params, decay, step, ws, L, st);
   float *X = f32(L.x), *Y = f32(L.y);
   {
     PdlLaunch l(dim3(nb, d->batch), dim3(kNormThreads), 0, st);

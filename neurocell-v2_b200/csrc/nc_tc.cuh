@@ -1,0 +1,389 @@
+// nc_tc.cuh -- products of 16-bit matrices on the tensor cores (tcgen05, accumulators in
+// tensor memory), with the caller's epilogue on float32 accumulators in registers.
+//
+// float32 operands come as two float16 planes: x s = hi + lo with hi = fp16(x s) and
+// lo = fp16(x s - hi), s a power of two.  A product takes lo hi + hi lo + hi hi; what is left
+// out (lo lo) and the rounding of lo are 2^-24 and 2^-23 of a factor, so the result is as
+// exact as float32 multiplications, for three 16-bit products (three bfloat16 planes would
+// take six).  bfloat16 operands are one plane and one product.
+//
+// The tensor core adds in float32 but not to nearest, which shows in long sums; with two
+// planes the accumulator is therefore drained every `chunk` k-tiles into float32 registers
+// (added to nearest there) while the other half of tensor memory takes the next chunk.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "nc_common.cuh"
+#include "nc_errors.h"
+
+namespace nc {
+namespace tc {
+
+constexpr int kBM = 128;            // rows of a tile: one tensor-memory lane each
+constexpr int kEpiWarps = 8;        // two per lane quarter, one per half of the columns
+constexpr int kThreads = 32 * (kEpiWarps + 2);
+constexpr int kWaitLimit = 1 << 20; // polls of a bounded wait
+
+// One product of (batched) matrices, D (m, n) = A (m, k) B (n, k)^T.  An operand is stored
+// either with k contiguous, or (a_mn, b_mn) with its own row index contiguous.
+struct Problem {
+  CUtensorMap a, b;
+  int m, n, k;
+  int a_mn, b_mn;
+  int tiles_m, tiles_n, batch, splits;   // splits of k; tiles run over m first
+  int symmetric;                         // D is symmetric: tiles below the diagonal are not computed
+  int chunk;                             // k-tiles per accumulator
+  int bf16;
+  int a_k0, b_k0, b_n0;                  // offsets into the stored operands
+  int32_t* status;                       // set to 1 when a bounded wait gives up
+};
+
+struct Tile {
+  int m0, n0, batch, split;
+  int kt0, kt1;   // k-tiles [kt0, kt1)
+};
+
+template <int PL, int BN>
+struct Config {
+  static constexpr int kBK = PL == 1 ? 64 : 32;
+  static constexpr int kA = PL * kBM * kBK * 2, kB = PL * BN * kBK * 2;
+  static constexpr int kStage = kA + kB;
+  static constexpr int kStages = 192 * 1024 / kStage;
+  static constexpr int kSmem = kStages * kStage + 1024;   // stages start on 1024 bytes
+};
+
+__host__ __device__ inline int problem_tiles(const Problem& p) {
+  const int mn = p.symmetric ? p.tiles_m * (p.tiles_m + 1) / 2 : p.tiles_m * p.tiles_n;
+  return mn * p.batch * p.splits;
+}
+
+template <int PL, int BN>
+__device__ __forceinline__ Tile problem_tile(const Problem& p, int t) {
+  Tile x;
+  int mn;
+  if (p.symmetric) {
+    const int per = p.tiles_m * (p.tiles_m + 1) / 2;
+    mn = t % per;
+    t /= per;
+    int j = 0;   // column j holds rows 0..j
+    while (mn > j) mn -= ++j;
+    x.m0 = mn * kBM, x.n0 = j * BN;
+  } else {
+    const int per = p.tiles_m * p.tiles_n;
+    mn = t % per;
+    t /= per;
+    x.m0 = mn % p.tiles_m * kBM, x.n0 = mn / p.tiles_m * BN;
+  }
+  x.batch = t % p.batch, x.split = t / p.batch;
+  const int kt = (p.k + Config<PL, BN>::kBK - 1) / Config<PL, BN>::kBK;
+  x.kt0 = (int)((int64_t)kt * x.split / p.splits), x.kt1 = (int)((int64_t)kt * (x.split + 1) / p.splits);
+  return x;
+}
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ void bar_init(uint32_t bar, int count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok;
+}
+
+// Bounded wait.  Giving up (here or in another warp of the CTA) sets the abort flag and the
+// caller's status word; every role then leaves its loop.
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* abort, int32_t* status) {
+  for (int i = 0; i < kWaitLimit; ++i) {
+    if (bar_try(bar, parity)) return true;
+    if (*abort) return false;
+  }
+  *abort = 1;
+  *status = 1;
+  return false;
+}
+
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], "
+      "[%2];" ::"r"(dst),
+      "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(0), "r"(c3)
+      : "memory");
+}
+
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(add)
+      : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+
+// 32 columns of this warp's 32 lanes (the wait belongs to the same statement, so that no use
+// of the registers moves above it).
+__device__ __forceinline__ void tmem_load(uint32_t addr, float (&v)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
+        "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]),
+        "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]),
+        "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+      : "r"(addr)
+      : "memory");
+}
+
+// Shared-memory matrix descriptors: start address, leading and stride byte offsets (16-byte
+// units), descriptor version 1, swizzle mode (2: 128 bytes, 4: 64 bytes).
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lead, uint32_t stride, uint32_t swizzle) {
+  return (uint64_t)((addr >> 4) & 0x3fff) | (uint64_t)((lead >> 4) & 0x3fff) << 16 |
+         (uint64_t)((stride >> 4) & 0x3fff) << 32 | (uint64_t)1 << 46 | (uint64_t)swizzle << 61;
+}
+
+// Operand of one plane, 16 values of k from step `ks` on.  k contiguous: rows of kBK values,
+// 8-row groups kBK * 16 bytes apart, swizzled over the row.  Own index contiguous: blocks of
+// 64 of it (`block` bytes apart), each k 128 bytes, 8-k groups 1024 bytes apart.
+template <int BK>
+__device__ __forceinline__ uint64_t operand_desc(uint32_t base, bool mn, uint32_t block, int ks) {
+  if (mn) return smem_desc(base + ks * 2048, block, 1024, 2);
+  return smem_desc(base + ks * 32, 16, BK * 16, BK == 64 ? 2 : 4);
+}
+
+// 16-bit planes of a float32 value that was scaled to float16's range.
+__device__ __forceinline__ void split_f16(float x, uint16_t* hi, uint16_t* lo) {
+  const __half h = __float2half_rn(x);
+  const __half l = __float2half_rn(x - __half2float(h));
+  *hi = __half_as_ushort(h), *lo = __half_as_ushort(l);
+}
+
+// 32-byte global accesses (one full sector per thread).
+__device__ __forceinline__ void store_v8(void* p, const uint32_t (&v)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+__device__ __forceinline__ void load_v8(const void* p, uint32_t (&v)[8]) {
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+               : "l"(p)
+               : "memory");
+}
+
+// The kernel: warps 0..7 epilogue, warp 8 loads, warp 9 multiplies; persistent over tiles.
+// Epi::run(tile, row, col, acc) gets a row's BN / 2 consecutive columns as float32 sums.
+template <int PL, int BN, class Epi>
+__global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_constant__ Problem p, const Epi epi) {
+  using C = Config<PL, BN>;
+  constexpr int BK = C::kBK, HALF = BN / 2;
+  extern __shared__ uint8_t raw[];
+  __shared__ __align__(8) uint64_t bars[2 * C::kStages + 5];
+  __shared__ uint32_t tmem_slot;
+  __shared__ volatile int abort_flag;
+  const uint32_t stages = (smem_addr(raw) + 1023) & ~1023u;
+  const uint32_t bar0 = smem_addr(bars);
+  auto full = [&](int s) { return bar0 + 8 * s; };
+  auto empty = [&](int s) { return bar0 + 8 * (C::kStages + s); };
+  auto acc_full = [&](int b) { return bar0 + 8 * (2 * C::kStages + b); };
+  auto acc_empty = [&](int b) { return bar0 + 8 * (2 * C::kStages + 2 + b); };
+  const uint32_t drain = bar0 + 8 * (2 * C::kStages + 4);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kStages; ++s) bar_init(full(s), 1), bar_init(empty(s), 1);
+    for (int b = 0; b < 2; ++b) bar_init(acc_full(b), 1), bar_init(acc_empty(b), kEpiWarps);
+    bar_init(drain, 1);
+    abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == kEpiWarps + 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_slot)),
+                 "r"(2 * BN)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = tmem_slot;
+  const int tiles = problem_tiles(p);
+  pdl_enter();
+
+  if (warp == kEpiWarps) {
+    if (lane == 0) {
+      int s = 0, issued = 0;
+      uint32_t ph = 1;
+      bool ok = true;
+      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+        const Tile x = problem_tile<PL, BN>(p, t);
+        for (int kt = x.kt0; kt < x.kt1; ++kt) {
+          if (!(ok = bar_wait(empty(s), ph, &abort_flag, p.status))) break;
+          bar_expect(full(s), C::kStage);
+          const uint32_t at = stages + s * C::kStage;
+          const int ka = p.a_k0 + kt * BK, kb = p.b_k0 + kt * BK, nb = p.b_n0 + x.n0;
+          if (p.a_mn) {
+#pragma unroll
+            for (int i = 0; i < kBM / 64; ++i)
+              tma_load(at + i * (C::kA / (kBM / 64)), &p.a, full(s), x.m0 + 64 * i, ka, x.batch);
+          } else {
+            tma_load(at, &p.a, full(s), ka, x.m0, x.batch);
+          }
+          if (p.b_mn) {
+#pragma unroll
+            for (int i = 0; i < BN / 64; ++i)
+              tma_load(at + C::kA + i * (C::kB / (BN / 64)), &p.b, full(s), nb + 64 * i, kb, x.batch);
+          } else {
+            tma_load(at + C::kA, &p.b, full(s), kb, nb, x.batch);
+          }
+          if (issued < C::kStages) ++issued;
+          if (++s == C::kStages) s = 0, ph ^= 1;
+        }
+      }
+      if (!ok) {   // the copies in flight land before the CTA ends
+        for (int i = 0; i < issued; ++i) {
+          if (s-- == 0) s = C::kStages - 1, ph ^= 1;
+          for (int j = 0; j < kWaitLimit && !bar_try(full(s), ph ^ 1); ++j) {
+          }
+        }
+      }
+    }
+  } else if (warp == kEpiWarps + 1) {
+    if (lane == 0) {
+      // accumulator float32; operand types; which operands have their own index contiguous
+      const uint32_t idesc = 1u << 4 | (p.bf16 ? 1u << 7 | 1u << 10 : 0u) | (p.a_mn ? 1u << 15 : 0u) |
+                             (p.b_mn ? 1u << 16 : 0u) | (uint32_t)(BN >> 3) << 17 | (uint32_t)(kBM >> 4) << 24;
+      constexpr uint32_t a_block = C::kA / (kBM / 64), b_block = C::kB / (BN / 64);
+      const uint32_t a_plane = p.a_mn ? a_block / PL : C::kA / PL, b_plane = p.b_mn ? b_block / PL : C::kB / PL;
+      int s = 0, buf = 0;
+      uint32_t ph = 0, aph = 1;
+      bool ok = true;
+      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+        const Tile x = problem_tile<PL, BN>(p, t);
+        for (int c0 = x.kt0; c0 < x.kt1 && ok; c0 += p.chunk) {
+          if (!(ok = bar_wait(acc_empty(buf), aph, &abort_flag, p.status))) break;
+          fence_after();
+          const uint32_t d = tmem + buf * BN;
+          const int c1 = min(c0 + p.chunk, x.kt1);
+          uint32_t add = 0;
+          for (int kt = c0; kt < c1; ++kt) {
+            if (!(ok = bar_wait(full(s), ph, &abort_flag, p.status))) break;
+            fence_after();
+            const uint32_t at = stages + s * C::kStage, bt = at + C::kA;
+            // low parts first, while the accumulator is small
+            constexpr int kProducts = PL == 1 ? 1 : 3;
+#pragma unroll
+            for (int q = 0; q < kProducts; ++q) {
+              const int pa = PL == 1 ? 0 : (q == 0 ? 1 : 0), pb = PL == 1 ? 0 : (q == 1 ? 1 : 0);
+#pragma unroll
+              for (int ks = 0; ks < BK / 16; ++ks) {
+                mma(d, operand_desc<BK>(at + pa * a_plane, p.a_mn, a_block, ks),
+                    operand_desc<BK>(bt + pb * b_plane, p.b_mn, b_block, ks), idesc, add);
+                add = 1;
+              }
+            }
+            mma_commit(empty(s));
+            if (++s == C::kStages) s = 0, ph ^= 1;
+          }
+          if (!ok) break;
+          mma_commit(acc_full(buf));
+          buf ^= 1;
+          if (buf == 0) aph ^= 1;
+        }
+      }
+      // every product has finished before tensor memory is given back
+      mma_commit(drain);
+      for (int j = 0; j < kWaitLimit && !bar_try(drain, 0); ++j) {
+      }
+    }
+    __syncwarp();
+  } else {
+    const int quarter = warp & 3, half = warp >> 2;
+    const uint32_t lanes = tmem + ((uint32_t)(32 * quarter) << 16) + half * HALF;
+    int buf = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+      const Tile x = problem_tile<PL, BN>(p, t);
+      float acc[HALF];
+#pragma unroll
+      for (int i = 0; i < HALF; ++i) acc[i] = 0.f;
+      for (int c0 = x.kt0; c0 < x.kt1; c0 += p.chunk) {
+        ok = bar_wait(acc_full(buf), ph, &abort_flag, p.status);
+        if (!__all_sync(0xffffffffu, ok)) {
+          ok = false;
+          break;
+        }
+        fence_after();
+#pragma unroll
+        for (int i = 0; i < HALF; i += 32) {
+          float v[32];
+          tmem_load(lanes + buf * BN + i, v);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) acc[i + j] += v[j];
+        }
+        fence_before();
+        if (lane == 0) bar_arrive(acc_empty(buf));
+        buf ^= 1;
+        if (buf == 0) ph ^= 1;
+      }
+      if (ok) epi.template run<HALF>(x, x.m0 + 32 * quarter + lane, x.n0 + half * HALF, acc);
+    }
+  }
+  __syncthreads();
+  if (warp == kEpiWarps + 1) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * BN));
+  }
+}
+
+// Tensor map of a stored matrix (inner contiguous, `outer` rows `pitch` elements apart, planes
+// `plane` elements apart, batches `per_batch` apart); box of (box_inner, box_outer) per plane.
+nc_status make_map(CUtensorMap* map, const void* base, bool bf16, int planes, int inner, int outer, int64_t pitch,
+                   int64_t plane, int batch, int64_t per_batch, int box_inner, int box_outer);
+
+int sm_count();
+
+// The two operands' maps: `mn` says that the operand's own index (extent `own`) is contiguous.
+template <int PL, int BN>
+nc_status make_operand(Problem* p, bool is_a, const void* base, bool mn, int own, int k, int64_t pitch, int64_t plane,
+                       int batch, int64_t per_batch) {
+  constexpr int BK = Config<PL, BN>::kBK;
+  (is_a ? p->a_mn : p->b_mn) = mn;
+  const int rows = is_a ? kBM : BN;
+  return mn ? make_map(is_a ? &p->a : &p->b, base, p->bf16, PL, own, k, pitch, plane, batch, per_batch, 64, BK)
+            : make_map(is_a ? &p->a : &p->b, base, p->bf16, PL, k, own, pitch, plane, batch, per_batch, BK, rows);
+}
+
+template <int PL, int BN, class Epi>
+nc_status launch_product(const Problem& p, const Epi& epi, cudaStream_t st, const char* what) {
+  auto k = product_kernel<PL, BN, Epi>;
+  NC_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Config<PL, BN>::kSmem));
+  const int tiles = problem_tiles(p), sms = sm_count();
+  PdlLaunch l(dim3(tiles < sms ? tiles : sms), dim3(kThreads), Config<PL, BN>::kSmem, st);
+  NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, k, p, epi));
+  return launch_check(what);
+}
+
+}  // namespace tc
+}  // namespace nc
