@@ -263,13 +263,17 @@ typedef enum nc_reduction { NC_REDUCE_MEAN = 0, NC_REDUCE_SUM = 1, NC_REDUCE_NON
  * Softmax cross-entropy of a linear readout over a (large) vocabulary, without the
  * (rows, classes) logits in memory: z = features weight^T + bias, and for every row
  * loss = log sum exp z - z[label].
- *   features (rows, dim), weight (classes, dim), bias (classes) or null: row-major, `dtype`
+ *   features (rows, dim), weight (classes, dim), bias (classes) or null: row-major, `dtype`;
+ *   with more than 32 rows and a dim of whole 8s a bfloat16 weight starts on 16 bytes
  *   labels (rows) int32.  A row whose label is ignore_index (which must lie outside
  *   [0, classes)) takes no part: its loss and feature gradient are 0 and its features are
  *   not used, whatever they hold.  Any other label outside [0, classes) makes the loss and
  *   the gradients NaN; nothing is read out of range.
  * A bias of -inf takes its class out; a row with every class taken out has a NaN loss, as
  * has one with a logit of NaN or +inf.  Sums and statistics are held in float32.
+ * Precision with float32 operands and more than 32 rows: as of float32 products, where the
+ * entries of a tensor below 2^-18 of its largest finite one count with an absolute error of
+ * 2^-38 of that one, and dz = p - onehot with one of at most 2^-40 of the largest |g_loss|.
  */
 typedef struct nc_linear_ce {
   int32_t rows, dim, classes;   /* rows may be 0: the loss and the weight's gradients are 0 */
@@ -318,6 +322,13 @@ nc_status nc_stage_from_host(const nc_stage_seg* segs, int32_t nseg, void* strea
 
 /* In-place SGD: params[i] -= lr * grads[i]  (lr read from host scalar). */
 nc_status nc_sgd_update(float* params, const float* grads, int64_t n, float lr, void* stream);
+
+/* Both in one call, on a workspace of nc_linear_ce_workspace_bytes(desc, 1): what the two
+   share is computed once.  lse (rows) is scratch. */
+nc_status nc_linear_ce_value_and_grad(const nc_linear_ce* desc, const void* features, const void* weight,
+                                      const void* bias, const int32_t* labels, float* loss, float* lse,
+                                      void* g_features, void* g_weight, void* g_bias, void* d_ws,
+                                      size_t ws_bytes, void* stream);
 
 /*
  * Newton-Schulz orthogonalisation of `batch` matrices (rows, cols), row-major and packed:

@@ -302,8 +302,6 @@ struct NsEpilogue {
   }
 };
 
-size_t pad256(size_t n) { return (n + 255) / 256 * 256; }
-
 int norm_blocks(int64_t n) { return (int)((n + kNormThreads * kNormPer - 1) / (kNormThreads * kNormPer)); }
 
 // k-tiles (of 32) that one accumulator takes before it is added to the registers.

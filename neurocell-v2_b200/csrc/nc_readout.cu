@@ -51,32 +51,6 @@ __device__ __forceinline__ void store_vec(T* p, const float (&v)[VEC]) {
   }
 }
 
-// Sums v[i] over the lanes.  Each step halves the values a lane keeps while more than one
-// is left, so 64 values take 62 shuffles instead of 320; afterwards a lane holds
-// max(1, N / 32) sums, from value *first on (equal on the lanes that share it).
-template <int N>
-__device__ __forceinline__ void warp_sums(float (&v)[N], int lane, int* first) {
-  int n = N, at = 0;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    if (n > 1) {
-      n >>= 1;
-      const bool up = lane & o;
-#pragma unroll
-      for (int i = 0; i < N / 2; ++i) {
-        if (i < n) {
-          const float send = up ? v[i] : v[i + n], keep = up ? v[i + n] : v[i];
-          v[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
-        }
-      }
-      at += up ? n : 0;
-    } else {
-      v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
-    }
-  }
-  *first = at;
-}
-
 // Logits of the row group [row0, row0 + RN) and the classes [v0, v0 + vb) into
 // z[r * vb + v] (no bias); vb is a multiple of kRowWarps * kRowTile.  A warp takes kRowTile classes at a time, its lanes split the
 // dimension; the group's features are in shared memory, where one 16-byte read serves
@@ -140,15 +114,6 @@ __device__ void group_logits(const CeArgs& a, int row0, int v0, int vb, float* h
   __syncthreads();
 }
 
-// Running (maximum, sum of exp) merges.  A maximum of -inf carries a sum of 0, or NaN when
-// a NaN was seen.
-__device__ __forceinline__ float2 lse_merge(float2 x, float2 y) {
-  const float m = fmaxf(x.x, y.x);
-  const float sx = x.x == -INFINITY ? x.y : x.y * expf(x.x - m);
-  const float sy = y.x == -INFINITY ? y.y : y.y * expf(y.x - m);
-  return make_float2(m, sx + sy);
-}
-
 // grid (class blocks, row groups): the block's (maximum, sum) of each row, and the label's
 // logit where the block holds it.
 template <typename T, int RN, int VEC>
@@ -200,25 +165,7 @@ __global__ void ce_finish_rows_kernel(CeArgs a, int blocks, const float2* __rest
     x = lse_merge(x, y);
   }
   if (lane != 0) return;
-  const int label = a.labels[row];
-  float l = x.x + logf(x.y);
-  if (label < 0 || label >= a.classes) l = NAN;
-  const bool kept = label != a.ignore_index;
-  lse[row] = l;
-  row_loss[row] = kept ? l - zlabel[row] : 0.f;
-}
-
-// Rows that take part, counted by a whole block (every thread gets the count).
-__device__ int count_kept(const CeArgs& a) {
-  __shared__ int total;
-  if (threadIdx.x == 0) total = 0;
-  __syncthreads();
-  int n = 0;
-  for (int i = threadIdx.x; i < a.rows; i += blockDim.x) n += ce_kept(a, i);
-  n = __reduce_add_sync(0xffffffffu, n);
-  if ((threadIdx.x & 31) == 0) atomicAdd(&total, n);
-  __syncthreads();
-  return total;
+  finish_row(a, row, x, zlabel, lse, row_loss);
 }
 
 // One block: the sum or mean of the row losses, in a fixed order.
@@ -384,25 +331,35 @@ RowsPlan rows_plan(const nc_linear_ce* d, int vec) {
   return r;
 }
 
-size_t pad256(size_t n) { return (n + 255) / 256 * 256; }
+// Few rows: the row-group kernels, which read the weight once as it is.  From kRowsMost on
+// the tensor cores.
+constexpr int kRowsMost = 32;
+bool on_tensor_cores(const nc_linear_ce* d) { return d->rows > kRowsMost; }
 
 struct CeLayout {
-  size_t status, part, zlabel, row_loss, df_part, total;
+  size_t status, row_loss, part, zlabel, df_part, tc, total;
 };
 
 CeLayout ce_layout(const nc_linear_ce* d, bool grad) {
   CeLayout L{};
-  if (d->rows == 0) {   // nothing is launched
-    L.total = 256;
-    return L;
-  }
-  const RowsPlan r = rows_plan(d, d->dim % 4 == 0 ? 4 : 1);
   size_t at = 0;
-  L.status = at, at += 256;
-  L.part = at, at += grad ? 0 : pad256((size_t)d->rows * r.blocks * sizeof(float2));
-  L.zlabel = at, at += grad ? 0 : pad256((size_t)d->rows * 4);
-  L.row_loss = at, at += grad ? 0 : pad256((size_t)d->rows * 4);
-  L.df_part = at, at += grad ? pad256((size_t)r.blocks * r.slots * d->rows * d->dim * 4) : 0;
+  auto take = [&](size_t bytes) {
+    const size_t o = at;
+    at += pad256(bytes);
+    return o;
+  };
+  L.status = take(4);
+  if (d->rows > 0) {   // else nothing is launched
+    L.row_loss = take((size_t)d->rows * 4);
+    if (on_tensor_cores(d)) {
+      L.tc = take(ce_tc_bytes(d, grad));
+    } else {
+      const RowsPlan r = rows_plan(d, d->dim % 4 == 0 ? 4 : 1);
+      L.part = take((size_t)d->rows * r.blocks * sizeof(float2));
+      L.zlabel = take((size_t)d->rows * 4);
+      if (grad) L.df_part = take((size_t)r.blocks * r.slots * d->rows * d->dim * 4);
+    }
+  }
   L.total = at;
   return L;
 }
@@ -512,6 +469,75 @@ int vec_of(const nc_linear_ce* d, const void* p, const void* q, const void* out)
   return d->dim % 4 == 0 && at % (d->dtype == NC_BF16 ? 8 : 16) == 0 ? 4 : 1;
 }
 
+// lse and row losses, then the reduced loss.  `grad`: the layout of the workspace.
+nc_status value(const nc_linear_ce* d, const CeArgs& a, bool grad, float* loss, float* lse, char* ws, cudaStream_t st) {
+  const CeLayout L = ce_layout(d, grad);
+  const bool none = d->reduction == NC_REDUCE_NONE;
+  float* row_loss = none ? loss : reinterpret_cast<float*>(ws + L.row_loss);
+  if (on_tensor_cores(d)) {
+    NC_CHECK(ce_tc_value(d, a, grad, lse, row_loss, ws + L.tc, st));
+  } else {
+    const RowsPlan r = rows_plan(d, vec_of(d, a.features, a.weight, nullptr));
+    float2* part = reinterpret_cast<float2*>(ws + L.part);
+    float* zlabel = reinterpret_cast<float*>(ws + L.zlabel);
+    NC_CHECK(rows_value(d->dtype == NC_BF16, a, r, part, zlabel, st));
+    PdlLaunch l(dim3((d->rows + 3) / 4), dim3(128), 0, st);
+    NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, ce_finish_rows_kernel, a, r.blocks, (const float2*)part,
+                                     (const float*)zlabel, lse, row_loss));
+    NC_CHECK(launch_check("ce_finish_rows_kernel launch"));
+  }
+  if (none) return NC_OK;
+  PdlLaunch l(dim3(1), dim3(1024), 0, st);
+  NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, ce_sum_kernel, a, (const float*)row_loss, loss));
+  return launch_check("ce_sum_kernel launch");
+}
+
+nc_status gradients(const nc_linear_ce* d, const CeArgs& a, const CeGrads& g, char* ws, cudaStream_t st) {
+  const CeLayout L = ce_layout(d, true);
+  if (on_tensor_cores(d)) return ce_tc_grad(d, a, g, ws + L.tc, st);
+  const bool bf16 = d->dtype == NC_BF16;
+  const RowsPlan r = rows_plan(d, vec_of(d, a.features, a.weight, g.weight));
+  float* df_part = g.features ? reinterpret_cast<float*>(ws + L.df_part) : nullptr;
+  NC_CHECK(rows_grad(bf16, a, r, g.lse, g.g_loss, g.weight, g.bias, df_part, st));
+  if (!g.features) return NC_OK;
+  const int64_t n = (int64_t)d->rows * d->dim;
+  PdlLaunch l(dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st);
+  const int slots = r.blocks * r.slots;
+  if (bf16)
+    NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, ce_sum_parts_kernel<__nv_bfloat16>, (const float*)df_part, n, slots,
+                                     static_cast<__nv_bfloat16*>(g.features)));
+  else
+    NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, ce_sum_parts_kernel<float>, (const float*)df_part, n, slots,
+                                     static_cast<float*>(g.features)));
+  return launch_check("ce_sum_parts_kernel launch");
+}
+
+nc_status check_inputs(const nc_linear_ce* d, const void* features, const void* weight, const void* bias,
+                       const int32_t* labels, const float* lse) {
+  NC_CHECK(check_elems(d, features, "features"));
+  NC_CHECK(check_elems(d, weight, "weight"));
+  if (bias) NC_CHECK(check_elems(d, bias, "bias"));
+  NC_CHECK(check_ptr(labels, "labels"));
+  return check_ptr(lse, "lse");
+}
+
+nc_status check_grads(const nc_linear_ce* d, const void* g_features, const void* g_weight, const void* g_bias) {
+  if (g_features) NC_CHECK(check_elems(d, g_features, "g_features"));
+  if (g_weight) NC_CHECK(check_elems(d, g_weight, "g_weight"));
+  if (g_bias) NC_CHECK(check_elems(d, g_bias, "g_bias"));
+  return NC_OK;
+}
+
+// No rows: a loss of 0 and gradients of 0.
+nc_status no_rows(const nc_linear_ce* d, float* loss, void* g_weight, void* g_bias, cudaStream_t st) {
+  const size_t size = d->dtype == NC_BF16 ? 2 : 4;
+  if (loss && d->reduction != NC_REDUCE_NONE) NC_CUDA_CHECK(cudaMemsetAsync(loss, 0, 4, st));
+  if (g_weight) NC_CUDA_CHECK(cudaMemsetAsync(g_weight, 0, (size_t)d->classes * d->dim * size, st));
+  if (g_bias) NC_CUDA_CHECK(cudaMemsetAsync(g_bias, 0, (size_t)d->classes * size, st));
+  clear_error();
+  return NC_OK;
+}
+
 }  // namespace
 
 }  // namespace nc
@@ -531,37 +557,13 @@ nc_status nc_linear_ce_forward(const nc_linear_ce* desc, const void* features, c
   NC_CHECK(check_desc(desc));
   NC_CHECK(check_ptr(loss, "loss"));
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (desc->rows == 0) {
-    if (desc->reduction != NC_REDUCE_NONE) NC_CUDA_CHECK(cudaMemsetAsync(loss, 0, 4, st));
-    clear_error();
-    return NC_OK;
-  }
-  NC_CHECK(check_elems(desc, features, "features"));
-  NC_CHECK(check_elems(desc, weight, "weight"));
-  if (bias) NC_CHECK(check_elems(desc, bias, "bias"));
-  NC_CHECK(check_ptr(labels, "labels"));
-  NC_CHECK(check_ptr(lse, "lse"));
-  const CeLayout L = ce_layout(desc, false);
-  NC_CHECK(check_ws(d_ws, ws_bytes, L.total));
+  if (desc->rows == 0) return no_rows(desc, loss, nullptr, nullptr, st);
+  NC_CHECK(check_inputs(desc, features, weight, bias, labels, lse));
+  NC_CHECK(check_ws(d_ws, ws_bytes, ce_layout(desc, false).total));
   char* ws = static_cast<char*>(d_ws);
-  const bool bf16 = desc->dtype == NC_BF16, none = desc->reduction == NC_REDUCE_NONE;
   const CeArgs a = make_args(desc, features, weight, bias, labels);
-  const RowsPlan r = rows_plan(desc, vec_of(desc, features, weight, nullptr));
-  float2* part = reinterpret_cast<float2*>(ws + L.part);
-  float* zlabel = reinterpret_cast<float*>(ws + L.zlabel);
-  float* row_loss = none ? loss : reinterpret_cast<float*>(ws + L.row_loss);
-  NC_CHECK(rows_value(bf16, a, r, part, zlabel, st));
-  {
-    PdlLaunch l(dim3((desc->rows + 3) / 4), dim3(128), 0, st);
-    NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, ce_finish_rows_kernel, a, r.blocks, (const float2*)part,
-                                     (const float*)zlabel, lse, row_loss));
-    NC_CHECK(launch_check("ce_finish_rows_kernel launch"));
-  }
-  if (!none) {
-    PdlLaunch l(dim3(1), dim3(1024), 0, st);
-    NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, ce_sum_kernel, a, (const float*)row_loss, loss));
-    NC_CHECK(launch_check("ce_sum_kernel launch"));
-  }
+  if (on_tensor_cores(desc)) NC_CHECK(ce_tc_prepare(desc, a, false, ws + ce_layout(desc, false).tc, st));
+  NC_CHECK(value(desc, a, false, loss, lse, ws, st));
   clear_error();
   return NC_OK;
 }
@@ -571,45 +573,38 @@ nc_status nc_linear_ce_backward(const nc_linear_ce* desc, const void* features, 
                                 void* g_features, void* g_weight, void* g_bias, void* d_ws, size_t ws_bytes,
                                 void* stream) {
   NC_CHECK(check_desc(desc));
+  NC_CHECK(check_grads(desc, g_features, g_weight, g_bias));
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const size_t size = desc->dtype == NC_BF16 ? 2 : 4;
-  if (g_features) NC_CHECK(check_elems(desc, g_features, "g_features"));
-  if (g_weight) NC_CHECK(check_elems(desc, g_weight, "g_weight"));
-  if (g_bias) NC_CHECK(check_elems(desc, g_bias, "g_bias"));
-  if (desc->rows == 0) {
-    if (g_weight) NC_CUDA_CHECK(cudaMemsetAsync(g_weight, 0, (size_t)desc->classes * desc->dim * size, st));
-    if (g_bias) NC_CUDA_CHECK(cudaMemsetAsync(g_bias, 0, (size_t)desc->classes * size, st));
-    clear_error();
-    return NC_OK;
-  }
-  NC_CHECK(check_elems(desc, features, "features"));
-  NC_CHECK(check_elems(desc, weight, "weight"));
-  if (bias) NC_CHECK(check_elems(desc, bias, "bias"));
-  NC_CHECK(check_ptr(labels, "labels"));
-  NC_CHECK(check_ptr(lse, "lse"));
+  if (desc->rows == 0) return no_rows(desc, nullptr, g_weight, g_bias, st);
+  NC_CHECK(check_inputs(desc, features, weight, bias, labels, lse));
   if (g_loss) NC_CHECK(check_ptr(g_loss, "g_loss"));
-  const CeLayout L = ce_layout(desc, true);
-  NC_CHECK(check_ws(d_ws, ws_bytes, L.total));
+  NC_CHECK(check_ws(d_ws, ws_bytes, ce_layout(desc, true).total));
   char* ws = static_cast<char*>(d_ws);
-  const bool bf16 = desc->dtype == NC_BF16;
   const CeArgs a = make_args(desc, features, weight, bias, labels);
-  const RowsPlan r = rows_plan(desc, vec_of(desc, features, weight, g_weight));
-  if (r.smem_grad > 220 * 1024)
-    return set_error(NC_ERR_UNSUPPORTED, "the readout's gradient takes at most %d rows", 1024);
-  float* df_part = g_features ? reinterpret_cast<float*>(ws + L.df_part) : nullptr;
-  NC_CHECK(rows_grad(bf16, a, r, lse, g_loss, g_weight, g_bias, df_part, st));
-  if (g_features) {
-    const int64_t n = (int64_t)desc->rows * desc->dim;
-    PdlLaunch l(dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st);
-    const int slots = r.blocks * r.slots;
-    if (bf16)
-      NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, ce_sum_parts_kernel<__nv_bfloat16>, (const float*)df_part, n, slots,
-                                       static_cast<__nv_bfloat16*>(g_features)));
-    else
-      NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, ce_sum_parts_kernel<float>, (const float*)df_part, n, slots,
-                                       static_cast<float*>(g_features)));
-    NC_CHECK(launch_check("ce_sum_parts_kernel launch"));
-  }
+  if (on_tensor_cores(desc)) NC_CHECK(ce_tc_prepare(desc, a, true, ws + ce_layout(desc, true).tc, st));
+  const CeGrads g{lse, g_loss, g_features, g_weight, g_bias};
+  NC_CHECK(gradients(desc, a, g, ws, st));
+  clear_error();
+  return NC_OK;
+}
+
+nc_status nc_linear_ce_value_and_grad(const nc_linear_ce* desc, const void* features, const void* weight,
+                                      const void* bias, const int32_t* labels, float* loss, float* lse,
+                                      void* g_features, void* g_weight, void* g_bias, void* d_ws, size_t ws_bytes,
+                                      void* stream) {
+  NC_CHECK(check_desc(desc));
+  NC_CHECK(check_ptr(loss, "loss"));
+  NC_CHECK(check_grads(desc, g_features, g_weight, g_bias));
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (desc->rows == 0) return no_rows(desc, loss, g_weight, g_bias, st);
+  NC_CHECK(check_inputs(desc, features, weight, bias, labels, lse));
+  NC_CHECK(check_ws(d_ws, ws_bytes, ce_layout(desc, true).total));
+  char* ws = static_cast<char*>(d_ws);
+  const CeArgs a = make_args(desc, features, weight, bias, labels);
+  if (on_tensor_cores(desc)) NC_CHECK(ce_tc_prepare(desc, a, true, ws + ce_layout(desc, true).tc, st));
+  NC_CHECK(value(desc, a, true, loss, lse, ws, st));
+  const CeGrads g{lse, nullptr, g_features, g_weight, g_bias};
+  NC_CHECK(gradients(desc, a, g, ws, st));
   clear_error();
   return NC_OK;
 }

@@ -3,6 +3,7 @@
 
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
+#include <math.h>
 #include <stddef.h>
 #include <stdint.h>
 
@@ -22,10 +23,88 @@ struct CeArgs {
   int reduction;
 };
 
+// What the gradient kernels read of the loss's own gradient, and where the results go.
+struct CeGrads {
+  const float* lse;
+  const float* g_loss;
+  void* features;
+  void* weight;
+  void* bias;
+};
+
+// The tensor-core path (nc_readout_tc.cu).  `ws` bytes from ce_tc_bytes; prepare() first.
+size_t ce_tc_bytes(const nc_linear_ce* d, bool grad);
+nc_status ce_tc_prepare(const nc_linear_ce* d, const CeArgs& a, bool grad, char* ws, cudaStream_t st);
+// lse and row losses (rows); reduced by the caller.
+nc_status ce_tc_value(const nc_linear_ce* d, const CeArgs& a, bool grad, float* lse, float* row_loss, char* ws,
+                      cudaStream_t st);
+nc_status ce_tc_grad(const nc_linear_ce* d, const CeArgs& a, const CeGrads& g, char* ws, cudaStream_t st);
+
+inline size_t pad256(size_t n) { return (n + 255) / 256 * 256; }
+
 // A row that takes part: every label but ignore_index.  A label outside [0, classes) takes
 // part with a NaN log-sum-exp, so that its loss and the gradients read NaN.
 __device__ __forceinline__ bool ce_kept(const CeArgs& a, int row) {
   return a.labels[row] != a.ignore_index;
+}
+
+// Running (maximum, sum of exp) merges.  A maximum of -inf carries a sum of 0, or NaN when
+// a NaN was seen.
+__device__ __forceinline__ float2 lse_merge(float2 x, float2 y) {
+  const float m = fmaxf(x.x, y.x);
+  const float sx = x.x == -INFINITY ? x.y : x.y * expf(x.x - m);
+  const float sy = y.x == -INFINITY ? y.y : y.y * expf(y.x - m);
+  return make_float2(m, sx + sy);
+}
+
+// A row's log-sum-exp and loss from the merged pair.  Labels outside the classes, other than
+// ignore_index, make both NaN.
+__device__ __forceinline__ void finish_row(const CeArgs& a, int row, float2 x, const float* zlabel, float* lse,
+                                           float* row_loss) {
+  const int label = a.labels[row];
+  float l = x.x + logf(x.y);
+  if (label < 0 || label >= a.classes) l = NAN;
+  lse[row] = l;
+  row_loss[row] = label == a.ignore_index ? 0.f : l - zlabel[row];
+}
+
+// Rows that take part, counted by a whole block (every thread gets the count).
+__device__ __forceinline__ int count_kept(const CeArgs& a) {
+  __shared__ int total;
+  if (threadIdx.x == 0) total = 0;
+  __syncthreads();
+  int n = 0;
+  for (int i = threadIdx.x; i < a.rows; i += blockDim.x) n += ce_kept(a, i);
+  n = __reduce_add_sync(0xffffffffu, n);
+  if ((threadIdx.x & 31) == 0) atomicAdd(&total, n);
+  __syncthreads();
+  return total;
+}
+
+// Sums v[i] over the lanes.  Each step halves the values a lane keeps while more than one
+// is left, so 64 values take 62 shuffles instead of 320; afterwards a lane holds
+// max(1, N / 32) sums, from value *first on (equal on the lanes that share it).
+template <int N>
+__device__ __forceinline__ void warp_sums(float (&v)[N], int lane, int* first) {
+  int n = N, at = 0;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    if (n > 1) {
+      n >>= 1;
+      const bool up = lane & o;
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i) {
+        if (i < n) {
+          const float send = up ? v[i] : v[i + n], keep = up ? v[i + n] : v[i];
+          v[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+        }
+      }
+      at += up ? n : 0;
+    } else {
+      v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
+    }
+  }
+  *first = at;
 }
 
 __device__ __forceinline__ float to_f32(float x) { return x; }

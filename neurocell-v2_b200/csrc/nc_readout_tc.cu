@@ -1,0 +1,620 @@
+// nc_readout_tc.cu -- the readout's cross-entropy on the tensor cores (nc_tc.cuh).
+//
+//   value:     z tile = features weight^T; the epilogue keeps each row's (maximum, sum of exp)
+//              over its half of the tile's classes, and the label's logit.
+//   gradient:  the classes go by in pieces.  A piece's logits are computed again and their
+//              epilogue writes dz = f_n (exp(z - lse) - onehot) as 16-bit planes, small
+//              enough to stay in L2; two products read them there, dw = dz^T features (whole
+//              for the piece) and df += dz weight (split over the piece's classes, parts
+//              summed in order at the end).
+//
+// float32 operands are two float16 planes each, scaled by a power of two that brings the
+// tensor's largest finite value to [2^13, 2^14): an entry down to 2^-18 of it keeps float32's
+// precision, smaller ones an absolute error of 2^-38 of it.  bfloat16 operands are used as
+// they are, and dz is rounded to bfloat16 (2^-9 of an entry, as the products read it).
+// f_n = g_n / max |g| lies in [-1, 1], so dz needs no more than a fixed scale: 22 bits down
+// to 2^-29, and an absolute error of 2^-40 below.
+#include <math.h>
+
+#include "nc_readout.h"
+#include "nc_tc.cuh"
+
+namespace nc {
+
+namespace {
+
+constexpr int kPrepThreads = 256;
+constexpr int kMaxBlocks = 296;        // blocks of the largest-value pass, per tensor
+constexpr float kDzScale = 32768.f;    // dz planes hold dz 2^15 (|dz| <= 1)
+constexpr int kChunk = 2;              // k-tiles (of 32) per accumulator beside float32 operands
+constexpr size_t kPieceBytes = 56u << 20;   // dz of one piece: it shares the 126 MB L2 with what it multiplies
+
+// Device scalars of a call.
+struct Scales {
+  float w, w_inv, f, f_inv;   // 2^e and 2^-e of weight and features
+  float g;                    // max |g_n|
+};
+
+struct Plan {
+  bool bf16, copy_w;
+  int pitch;                  // of the planes of features and weight
+  int rows_pad;               // rows, whole 128s
+  int classes_pad;            // classes, whole 256s
+  int slots;                  // half tiles of classes
+  int piece, pieces;          // classes per piece (whole 256s)
+  int bn_out;                 // tile width of the gradient products
+  int splits;                 // of df over a piece's classes
+  size_t scales, max_part, w, f, bias, part, zlabel, fac, dz, df_part, db_part, total;
+};
+
+Plan make_plan(const nc_linear_ce* d, bool grad) {
+  Plan p{};
+  p.bf16 = d->dtype == NC_BF16;
+  p.copy_w = !p.bf16 || d->dim % 8 != 0;   // else the weight is read where it is
+  p.pitch = (d->dim + 7) / 8 * 8;
+  p.rows_pad = (d->rows + 127) / 128 * 128;
+  p.classes_pad = (d->classes + 255) / 256 * 256;
+  p.slots = p.classes_pad / 128;
+  const int planes = p.bf16 ? 1 : 2;
+  const int tiles = p.classes_pad / 256;
+  const size_t tile_bytes = (size_t)p.rows_pad * 256 * 2 * planes;
+  int most = (int)(kPieceBytes / tile_bytes);
+  if (most < 1) most = 1;
+  p.pieces = (tiles + most - 1) / most;
+  p.piece = (tiles + p.pieces - 1) / p.pieces * 256;
+  p.pieces = (p.classes_pad + p.piece - 1) / p.piece;   // none is empty
+  p.bn_out = d->dim <= 128 ? 128 : 256;
+  const int out_tiles = p.rows_pad / 128 * ((d->dim + p.bn_out - 1) / p.bn_out);
+  int splits = 148 / out_tiles;
+  if (splits > p.piece / 256) splits = p.piece / 256;
+  p.splits = splits < 1 ? 1 : splits;
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t o = at;
+    at += pad256(bytes);
+    return o;
+  };
+  p.scales = take(sizeof(Scales) + 4);   // and the wait status
+  p.max_part = take(2 * kMaxBlocks * 4);
+  if (p.copy_w) p.w = take((size_t)d->classes * p.pitch * 2 * planes);
+  p.f = take((size_t)d->rows * p.pitch * 2 * planes);
+  p.bias = take((size_t)p.classes_pad * 4);
+  p.part = take((size_t)p.slots * p.rows_pad * sizeof(float2));
+  p.zlabel = take((size_t)d->rows * 4);
+  if (grad) {
+    p.fac = take((size_t)d->rows * 4);
+    p.dz = take((size_t)p.rows_pad * p.piece * 2 * planes);
+    p.df_part = take((size_t)p.splits * d->rows * p.pitch * 4);
+    p.db_part = take((size_t)(p.rows_pad / 32) * p.classes_pad * 4);
+  }
+  p.total = at;
+  return p;
+}
+
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+// ---- preparation ---------------------------------------------------------------------------
+
+// Largest finite magnitude per block: blocks [0, kMaxBlocks) of the weight, the rest of the
+// features' rows that take part.
+__global__ void __launch_bounds__(kPrepThreads) ce_max_kernel(CeArgs a, float* __restrict__ part) {
+  __shared__ float red[kPrepThreads / 32];
+  pdl_enter();
+  const bool of_w = blockIdx.x < kMaxBlocks;
+  const float* x = static_cast<const float*>(of_w ? a.weight : a.features);
+  const int64_t n = (int64_t)(of_w ? a.classes : a.rows) * a.dim;
+  const int64_t step = (int64_t)kMaxBlocks * kPrepThreads, i0 = (blockIdx.x % kMaxBlocks) * kPrepThreads + threadIdx.x;
+  float m = 0.f;
+  auto see = [&](float v) {
+    v = fabsf(v);
+    if (v <= 3.402823466e38f) m = fmaxf(m, v);   // not NaN, not an infinity
+  };
+  if (of_w && n % 4 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0) {
+    const float4* x4 = reinterpret_cast<const float4*>(x);
+#pragma unroll 4
+    for (int64_t i = i0; i < n / 4; i += step) {
+      const float4 v = x4[i];
+      see(v.x), see(v.y), see(v.z), see(v.w);
+    }
+  } else {
+    for (int64_t i = i0; i < n; i += step)
+      if (of_w || ce_kept(a, (int)(i / a.dim))) see(x[i]);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < kPrepThreads / 32; ++i) m = fmaxf(m, red[i]);
+    part[blockIdx.x] = m;
+  }
+}
+
+// Exponent e of the scale: largest value x 2^e in [2^13, 2^14), within what float32 holds.
+__device__ __forceinline__ int scale_exponent(float largest) {
+  if (largest == 0.f) return 0;
+  const int e = 13 - ((int)(__float_as_uint(largest) >> 23) - 127);
+  return min(e, 120);
+}
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+// Eight values of a row as 16-bit planes (or bfloat16, or float32 -> bfloat16-wide copies).
+template <typename T>
+__device__ __forceinline__ void put8(const T* src, int left, bool wide, float scale, bool bf16, uint16_t* out,
+                                     int64_t plane) {
+  float v[8];
+  if (wide && left >= 8) {
+    if constexpr (sizeof(T) == 4) {
+      const float4 a = reinterpret_cast<const float4*>(src)[0], b = reinterpret_cast<const float4*>(src)[1];
+      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
+      const uint4 q = *reinterpret_cast<const uint4*>(src);
+      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < left ? to_f32(src[i]) : 0.f;
+  }
+  uint16_t h[8], l[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (bf16)
+      h[i] = __bfloat16_as_ushort(__float2bfloat16_rn(v[i]));
+    else
+      tc::split_f16(v[i] * scale, &h[i], &l[i]);
+  }
+  *reinterpret_cast<uint4*>(out) =
+      make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+  if (!bf16)
+    *reinterpret_cast<uint4*>(out + plane) =
+        make_uint4(l[0] | l[1] << 16, l[2] | l[3] << 16, l[4] | l[5] << 16, l[6] | l[7] << 16);
+}
+
+// Features, bias and (copy_w) weight in the products' form.  Rows that take no part become
+// zeros; the bias of the classes past the end is -inf.
+template <typename T>
+__global__ void __launch_bounds__(kPrepThreads) ce_planes_kernel(CeArgs a, int copy_w, int pitch, int classes_pad,
+                                                                 int wide_w, int wide_f,
+                                                                 const float* __restrict__ max_part, Scales* scales,
+                                                                 int32_t* status, uint16_t* __restrict__ w,
+                                                                 uint16_t* __restrict__ f, float* __restrict__ bias) {
+  constexpr bool bf16 = sizeof(T) == 2;
+  __shared__ float red[2][kPrepThreads / 32];
+  pdl_enter();
+  float sw = 1.f, sf = 1.f;
+  if constexpr (!bf16) {
+    float m[2] = {0.f, 0.f};
+    for (int k = 0; k < 2; ++k) {
+      for (int i = threadIdx.x; i < kMaxBlocks; i += kPrepThreads) m[k] = fmaxf(m[k], max_part[k * kMaxBlocks + i]);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) m[k] = fmaxf(m[k], __shfl_xor_sync(0xffffffffu, m[k], o));
+      if ((threadIdx.x & 31) == 0) red[k][threadIdx.x >> 5] = m[k];
+    }
+    __syncthreads();
+    for (int k = 0; k < 2; ++k) {
+      m[k] = red[k][0];
+      for (int i = 1; i < kPrepThreads / 32; ++i) m[k] = fmaxf(m[k], red[k][i]);
+    }
+    sw = pow2(scale_exponent(m[0])), sf = pow2(scale_exponent(m[1]));
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    scales->w = sw, scales->f = sf, scales->w_inv = 1.f / sw, scales->f_inv = 1.f / sf;
+    *status = 0;
+  }
+  const int64_t step = (int64_t)gridDim.x * kPrepThreads, i0 = (int64_t)blockIdx.x * kPrepThreads + threadIdx.x;
+  const int per = pitch / 8;
+  const int64_t nf = (int64_t)a.rows * per, nw = copy_w ? (int64_t)a.classes * per : 0;
+  for (int64_t i = i0; i < nf; i += step) {
+    const int row = (int)(i / per), c = (int)(i - (int64_t)row * per) * 8;
+    const T* src = static_cast<const T*>(a.features) + (size_t)row * a.dim + c;
+    put8<T>(src, ce_kept(a, row) ? a.dim - c : 0, wide_f, sf, bf16, f + (size_t)row * pitch + c,
+            (int64_t)a.rows * pitch);
+  }
+  for (int64_t i = i0; i < classes_pad; i += step)
+    bias[i] = i >= a.classes ? -INFINITY : a.bias ? to_f32(static_cast<const T*>(a.bias)[i]) : 0.f;
+#pragma unroll 2
+  for (int64_t i = i0; i < nw; i += step) {
+    const int row = (int)(i / per), c = (int)(i - (int64_t)row * per) * 8;
+    const T* src = static_cast<const T*>(a.weight) + (size_t)row * a.dim + c;
+    put8<T>(src, a.dim - c, wide_w, sw, bf16, w + (size_t)row * pitch + c, (int64_t)a.classes * pitch);
+  }
+}
+
+// ---- value ---------------------------------------------------------------------------------
+
+struct ValueEpilogue {
+  CeArgs a;
+  const Scales* scales;
+  const float* bias;
+  float2* part;      // (slots, rows_pad)
+  float* zlabel;
+  int rows_pad;
+
+  template <int HALF>
+  __device__ __forceinline__ void run(const tc::Tile&, int row, int col, float (&z)[HALF]) const {
+    const float sw = scales->w_inv, sf = scales->f_inv;
+    const int label = row < a.rows ? a.labels[row] - col : -1;
+    float m = -INFINITY, zl = 0.f;
+#pragma unroll
+    for (int j = 0; j < HALF; j += 4) {
+      const float4 b = *reinterpret_cast<const float4*>(bias + col + j);
+      z[j] = z[j] * sw * sf + b.x, z[j + 1] = z[j + 1] * sw * sf + b.y;
+      z[j + 2] = z[j + 2] * sw * sf + b.z, z[j + 3] = z[j + 3] * sw * sf + b.w;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        m = fmaxf(m, z[j + e]);
+        if (j + e == label) zl = z[j + e];
+      }
+    }
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < HALF; ++j) s += z[j] == -INFINITY ? 0.f : __expf(z[j] - m);
+    if (row >= a.rows) return;
+    part[(size_t)(col / HALF) * rows_pad + row] = make_float2(m, s);
+    if (label >= 0 && label < HALF) zlabel[row] = zl;
+  }
+};
+
+// 32 rows per block, a lane each; the warps split the slots and meet in shared memory.
+__global__ void __launch_bounds__(256) ce_finish_kernel(CeArgs a, int slots, int rows_pad,
+                                                        const float2* __restrict__ part,
+                                                        const float* __restrict__ zlabel, float* __restrict__ lse,
+                                                        float* __restrict__ row_loss) {
+  __shared__ float2 sm[8][32];
+  pdl_enter();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.x * 32 + lane;
+  float2 x = make_float2(-INFINITY, 0.f);
+#pragma unroll 4
+  for (int s = warp; s < slots; s += 8) x = lse_merge(x, part[(size_t)s * rows_pad + row]);
+  sm[warp][lane] = x;
+  __syncthreads();
+  if (warp != 0 || row >= a.rows) return;
+  for (int k = 1; k < 8; ++k) x = lse_merge(x, sm[k][lane]);
+  finish_row(a, row, x, zlabel, lse, row_loss);
+}
+
+// ---- gradient ------------------------------------------------------------------------------
+
+// One block: f_n = g_n / max |g| of every row (0 where the row takes no part) and max |g|.
+__global__ void __launch_bounds__(1024) ce_factors_kernel(CeArgs a, const float* __restrict__ g_loss,
+                                                          float* __restrict__ fac, Scales* __restrict__ scales) {
+  __shared__ float red[32];
+  pdl_enter();
+  const int n = count_kept(a);
+  const bool each = a.reduction == NC_REDUCE_NONE && g_loss;
+  const float all = (g_loss && !each ? g_loss[0] : 1.f) / (a.reduction == NC_REDUCE_MEAN ? (float)max(n, 1) : 1.f);
+  float m = fabsf(all);
+  if (each) {
+    m = 0.f;
+    for (int i = threadIdx.x; i < a.rows; i += blockDim.x)
+      if (ce_kept(a, i)) m = fmaxf(m, fabsf(g_loss[i]));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
+    __syncthreads();
+    for (int i = 0; i < 32; ++i) m = fmaxf(m, red[i]);
+  }
+  for (int i = threadIdx.x; i < a.rows; i += blockDim.x)
+    fac[i] = !ce_kept(a, i) || m == 0.f ? 0.f : (each ? g_loss[i] : all) / m;
+  if (threadIdx.x == 0) scales->g = m;
+}
+
+template <bool BF16>
+struct DzEpilogue {
+  CeArgs a;
+  const Scales* scales;
+  const float* bias;
+  const float* lse;
+  const float* fac;
+  uint16_t* dz;        // (planes, rows, piece)
+  float* db_part;      // (rows_pad / 32, classes_pad) or null
+  int v0, piece, classes_pad;
+
+  template <int HALF>
+  __device__ __forceinline__ void run(const tc::Tile&, int row, int col, float (&z)[HALF]) const {
+    const bool in = row < a.rows;
+    const float sw = scales->w_inv, sf = scales->f_inv;
+    const float f = in ? fac[row] : 0.f, l = in ? lse[row] : 0.f;
+    const int label = in ? a.labels[row] - v0 - col : -1;
+#pragma unroll
+    for (int j = 0; j < HALF; j += 4) {
+      const float4 q = *reinterpret_cast<const float4*>(bias + v0 + col + j);
+      const float b[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float p = expf(z[j + e] * sw * sf + b[e] - l) - (j + e == label ? 1.f : 0.f);
+        z[j + e] = f == 0.f ? 0.f : f * p;
+      }
+    }
+    if (in) {
+      uint16_t* out = dz + (size_t)row * piece + col;
+#pragma unroll
+      for (int j = 0; j < HALF; j += 16) {
+        uint32_t h[8], lo[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float x = z[j + 2 * i], y = z[j + 2 * i + 1];
+          if constexpr (BF16) {
+            const __nv_bfloat162 b = __floats2bfloat162_rn(x, y);
+            h[i] = *reinterpret_cast<const uint32_t*>(&b);
+          } else {
+            uint16_t h0, l0, h1, l1;
+            tc::split_f16(x * kDzScale, &h0, &l0);
+            tc::split_f16(y * kDzScale, &h1, &l1);
+            h[i] = h0 | (uint32_t)h1 << 16, lo[i] = l0 | (uint32_t)l1 << 16;
+          }
+        }
+        tc::store_v8(out + j, h);
+        if constexpr (!BF16) tc::store_v8(out + (size_t)a.rows * piece + j, lo);
+      }
+    }
+    if (db_part) {
+      int first;
+      const int lane = threadIdx.x & 31;
+      warp_sums(z, lane, &first);
+      float* o = db_part + (size_t)(row / 32) * classes_pad + v0 + col + first;
+#pragma unroll
+      for (int i = 0; i < HALF / 32; ++i) o[i] = z[i];
+    }
+  }
+};
+
+// dw of a piece, written once.
+template <typename T>
+struct WeightEpilogue {
+  const Scales* scales;
+  T* out;          // of the piece's first class
+  int classes, dim;
+  bool wide;       // rows on 32 bytes
+  template <int HALF>
+  __device__ __forceinline__ void run(const tc::Tile&, int row, int col, float (&v)[HALF]) const {
+    if (row >= classes) return;
+    const float s = scales->f_inv * (sizeof(T) == 4 ? 1.f / kDzScale : 1.f), g = scales->g;
+    T* o = out + (size_t)row * dim + col;
+#pragma unroll
+    for (int j = 0; j < HALF; j += 16) {
+      if (col + j >= dim) break;
+      if (wide && col + j + 16 <= dim) {
+        uint32_t q[8];
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+          for (int e = 0; e < 16; e += 8) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) q[i] = __float_as_uint(v[j + e + i] * s * g);
+            tc::store_v8(o + j + e, q);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const __nv_bfloat162 b = __floats2bfloat162_rn(v[j + 2 * i] * s * g, v[j + 2 * i + 1] * s * g);
+            q[i] = *reinterpret_cast<const uint32_t*>(&b);
+          }
+          tc::store_v8(o + j, q);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (col + j + e < dim) store_as(o + j + e, v[j + e] * s * g);
+      }
+    }
+  }
+};
+
+// df of a piece and split, added to that split's part (one CTA owns an element).
+struct FeatureEpilogue {
+  const Scales* scales;
+  float* part;     // (splits, rows, pitch)
+  int rows, dim, pitch, first;
+  float mul;
+  template <int HALF>
+  __device__ __forceinline__ void run(const tc::Tile& x, int row, int col, float (&v)[HALF]) const {
+    if (row >= rows) return;
+    const float s = scales->w_inv * mul;
+    float* o = part + ((size_t)x.split * rows + row) * pitch + col;
+#pragma unroll
+    for (int j = 0; j < HALF; j += 8) {
+      if (col + j >= dim) break;   // the pitch is whole 8s
+      uint32_t q[8];
+      if (!first) tc::load_v8(o + j, q);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        q[i] = __float_as_uint(v[j + i] * s + (first ? 0.f : __uint_as_float(q[i])));
+      tc::store_v8(o + j, q);
+    }
+  }
+};
+
+template <typename T>
+__global__ void __launch_bounds__(256) ce_features_kernel(const float* __restrict__ part, int splits, int rows, int dim,
+                                                          int pitch, const Scales* __restrict__ scales,
+                                                          T* __restrict__ out) {
+  pdl_enter();
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= (int64_t)rows * dim) return;
+  const int row = (int)(i / dim), c = (int)(i - (int64_t)row * dim);
+  float s = 0.f;
+  for (int k = 0; k < splits; ++k) s += part[((size_t)k * rows + row) * pitch + c];
+  store_as(out + i, s * scales->g);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) ce_bias_kernel(const float* __restrict__ part, int groups, int classes,
+                                                      int classes_pad, const Scales* __restrict__ scales,
+                                                      T* __restrict__ out) {
+  pdl_enter();
+  const int v = blockIdx.x * 256 + threadIdx.x;
+  if (v >= classes) return;
+  float s = 0.f;
+#pragma unroll 8
+  for (int k = 0; k < groups; ++k) s += part[(size_t)k * classes_pad + v];
+  store_as(out + v, s * scales->g);
+}
+
+// ---- launches ------------------------------------------------------------------------------
+
+template <typename T>
+struct Call {
+  static constexpr int PL = sizeof(T) == 2 ? 1 : 2;
+  const nc_linear_ce* d;
+  const CeArgs& a;
+  Plan p;
+  char* ws;
+  cudaStream_t st;
+
+  template <typename U>
+  U* at(size_t o) const {
+    return reinterpret_cast<U*>(ws + o);
+  }
+  Scales* scales() const { return at<Scales>(p.scales); }
+  int32_t* status() const { return reinterpret_cast<int32_t*>(at<Scales>(p.scales) + 1); }
+
+  tc::Problem problem(int m, int n, int k, int bn, int splits) const {
+    tc::Problem q{};
+    q.m = m, q.n = n, q.k = k, q.batch = 1, q.splits = splits, q.bf16 = p.bf16;
+    q.tiles_m = (m + tc::kBM - 1) / tc::kBM, q.tiles_n = (n + bn - 1) / bn;
+    q.chunk = PL == 1 ? 1 << 30 : kChunk;
+    q.status = status();
+    return q;
+  }
+
+  // Operands: rows of features or weight (k = dim contiguous), or with their columns as the
+  // own index and rows as k.
+  template <int BN>
+  nc_status features_op(tc::Problem* q, bool is_a, bool by_column) const {
+    return tc::make_operand<PL, BN>(q, is_a, at<void>(p.f), by_column, by_column ? d->dim : d->rows,
+                                    by_column ? d->rows : d->dim, p.pitch, (int64_t)d->rows * p.pitch, 1,
+                                    (int64_t)PL * d->rows * p.pitch);
+  }
+  template <int BN>
+  nc_status weight_op(tc::Problem* q, bool by_column) const {
+    const void* base = p.copy_w ? at<void>(p.w) : a.weight;
+    const int pitch = p.copy_w ? p.pitch : d->dim;
+    return tc::make_operand<PL, BN>(q, false, base, by_column, by_column ? d->dim : d->classes,
+                                    by_column ? d->classes : d->dim, pitch, (int64_t)d->classes * pitch, 1,
+                                    (int64_t)PL * d->classes * pitch);
+  }
+  template <int BN>
+  nc_status dz_op(tc::Problem* q, bool by_column) const {
+    return tc::make_operand<PL, BN>(q, true, at<void>(p.dz), by_column, by_column ? p.piece : d->rows,
+                                    by_column ? d->rows : p.piece, p.piece, (int64_t)d->rows * p.piece, 1,
+                                    (int64_t)PL * d->rows * p.piece);
+  }
+
+  nc_status prepare() const {
+    if (PL == 2) {
+      PdlLaunch l(dim3(2 * kMaxBlocks), dim3(kPrepThreads), 0, st);
+      NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, ce_max_kernel, a, at<float>(p.max_part)));
+      NC_CHECK(launch_check("ce_max_kernel launch"));
+    }
+    const int64_t items = ((int64_t)d->rows + (p.copy_w ? d->classes : 0)) * (p.pitch / 8);
+    int64_t blocks = (items + kPrepThreads - 1) / kPrepThreads;
+    if (blocks > 148 * 16) blocks = 148 * 16;
+    PdlLaunch l(dim3((unsigned)blocks), dim3(kPrepThreads), 0, st);
+    const int even = d->dim % 8 == 0;
+    NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, ce_planes_kernel<T>, a, (int)p.copy_w, p.pitch, p.classes_pad,
+                                     (int)(even && aligned16(a.weight)), (int)(even && aligned16(a.features)),
+                                     (const float*)at<float>(p.max_part), scales(), status(), at<uint16_t>(p.w),
+                                     at<uint16_t>(p.f), at<float>(p.bias)));
+    return launch_check("ce_planes_kernel launch");
+  }
+
+  nc_status value(float* lse, float* row_loss) const {
+    tc::Problem q = problem(d->rows, d->classes, d->dim, 256, 1);
+    NC_CHECK(features_op<256>(&q, true, false));
+    NC_CHECK(weight_op<256>(&q, false));
+    const ValueEpilogue e{a, scales(), at<float>(p.bias), at<float2>(p.part), at<float>(p.zlabel), p.rows_pad};
+    NC_CHECK((tc::launch_product<PL, 256>(q, e, st, "readout value product launch")));
+    PdlLaunch l(dim3((d->rows + 31) / 32), dim3(256), 0, st);
+    NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, ce_finish_kernel, a, p.slots, p.rows_pad,
+                                     (const float2*)at<float2>(p.part), (const float*)at<float>(p.zlabel), lse,
+                                     row_loss));
+    return launch_check("ce_finish_kernel launch");
+  }
+
+  template <int BN>
+  nc_status piece_products(const CeGrads& g, int v0, int width, int classes) const {
+    if (g.weight) {
+      tc::Problem q = problem(classes, d->dim, d->rows, BN, 1);
+      NC_CHECK(dz_op<BN>(&q, true));
+      NC_CHECK(features_op<BN>(&q, false, true));
+      T* out = static_cast<T*>(g.weight) + (size_t)v0 * d->dim;
+      const bool wide = reinterpret_cast<uintptr_t>(out) % 32 == 0 && (size_t)d->dim * sizeof(T) % 32 == 0;
+      const WeightEpilogue<T> e{scales(), out, classes, d->dim, wide};
+      NC_CHECK((tc::launch_product<PL, BN>(q, e, st, "readout weight gradient launch")));
+    }
+    if (g.features) {
+      tc::Problem q = problem(d->rows, d->dim, width, BN, p.splits);
+      NC_CHECK(dz_op<BN>(&q, false));
+      NC_CHECK(weight_op<BN>(&q, true));
+      q.b_k0 = v0;
+      const FeatureEpilogue e{scales(), at<float>(p.df_part), d->rows, d->dim, p.pitch, v0 == 0,
+                              PL == 1 ? 1.f : 1.f / kDzScale};
+      NC_CHECK((tc::launch_product<PL, BN>(q, e, st, "readout feature gradient launch")));
+    }
+    return NC_OK;
+  }
+
+  nc_status gradients(const CeGrads& g) const {
+    {
+      PdlLaunch l(dim3(1), dim3(1024), 0, st);
+      NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, ce_factors_kernel, a, g.g_loss, at<float>(p.fac), scales()));
+      NC_CHECK(launch_check("ce_factors_kernel launch"));
+    }
+    for (int k = 0; k < p.pieces; ++k) {
+      const int v0 = k * p.piece;
+      // the last piece may be shorter; `width` is whole tiles
+      const int width = p.classes_pad - v0 < p.piece ? p.classes_pad - v0 : p.piece;
+      const int classes = d->classes - v0 < width ? d->classes - v0 : width;
+      tc::Problem q = problem(d->rows, width, d->dim, 256, 1);
+      NC_CHECK(features_op<256>(&q, true, false));
+      NC_CHECK(weight_op<256>(&q, false));
+      q.b_n0 = v0;
+      const DzEpilogue<PL == 1> e{a,     scales(), at<float>(p.bias), g.lse,  at<float>(p.fac), at<uint16_t>(p.dz),
+                                  g.bias ? at<float>(p.db_part) : nullptr, v0, p.piece, p.classes_pad};
+      NC_CHECK((tc::launch_product<PL, 256>(q, e, st, "readout logit gradient launch")));
+      NC_CHECK(p.bn_out == 128 ? piece_products<128>(g, v0, width, classes) : piece_products<256>(g, v0, width, classes));
+    }
+    if (g.features) {
+      const int64_t n = (int64_t)d->rows * d->dim;
+      PdlLaunch l(dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st);
+      NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, ce_features_kernel<T>, (const float*)at<float>(p.df_part), p.splits,
+                                       d->rows, d->dim, p.pitch, (const Scales*)scales(),
+                                       static_cast<T*>(g.features)));
+      NC_CHECK(launch_check("ce_features_kernel launch"));
+    }
+    if (g.bias) {
+      PdlLaunch l(dim3((d->classes + 255) / 256), dim3(256), 0, st);
+      NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, ce_bias_kernel<T>, (const float*)at<float>(p.db_part), p.rows_pad / 32,
+                                       d->classes, p.classes_pad, (const Scales*)scales(), static_cast<T*>(g.bias)));
+      NC_CHECK(launch_check("ce_bias_kernel launch"));
+    }
+    return NC_OK;
+  }
+};
+
+}  // namespace
+
+size_t ce_tc_bytes(const nc_linear_ce* d, bool grad) { return make_plan(d, grad).total; }
+
+#define NC_TC_CALL(GRAD, WHAT)                                                                       \
+  const Plan plan = make_plan(d, GRAD);                                                              \
+  return plan.bf16 ? Call<__nv_bfloat16>{d, a, plan, ws, st}.WHAT : Call<float>{d, a, plan, ws, st}.WHAT
+
+nc_status ce_tc_prepare(const nc_linear_ce* d, const CeArgs& a, bool grad, char* ws, cudaStream_t st) {
+  if (!make_plan(d, grad).copy_w && !aligned16(a.weight))
+    return set_error(NC_ERR_INVALID, "a bfloat16 weight must start on a 16-byte boundary for more than 32 rows");
+  NC_TC_CALL(grad, prepare());
+}
+
+nc_status ce_tc_value(const nc_linear_ce* d, const CeArgs& a, bool grad, float* lse, float* row_loss, char* ws,
+                      cudaStream_t st) {
+  NC_TC_CALL(grad, value(lse, row_loss));
+}
+
+nc_status ce_tc_grad(const nc_linear_ce* d, const CeArgs& a, const CeGrads& g, char* ws, cudaStream_t st) {
+  NC_TC_CALL(true, gradients(g));
+}
+
+}  // namespace nc

@@ -34,6 +34,7 @@ EXPORTED = (
     "nc_vnn_forward_universe", "nc_vnn_backward_universe", "nc_universe_embed_forward",
     "nc_universe_embed_backward", "nc_workspace_status", "nc_dp_reset", "nc_stage_from_host",
     "nc_linear_ce_workspace_bytes", "nc_linear_ce_forward", "nc_linear_ce_backward",
+    "nc_linear_ce_value_and_grad",
     "nc_newton_schulz_workspace_bytes", "nc_orthogonalize", "nc_muon_update",
 )
 NC_DP_MAX_RANKS = 8
@@ -126,6 +127,7 @@ _SIGS = {
     "nc_linear_ce_workspace_bytes": (_sz, [_LP, _i32]),
     "nc_linear_ce_forward": (_i32, [_LP, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "nc_linear_ce_backward": (_i32, [_LP, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "nc_linear_ce_value_and_grad": (_i32, [_LP, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "nc_newton_schulz_workspace_bytes": (_sz, [_NP]),
     "nc_orthogonalize": (_i32, [_NP, _vp, _vp, _vp, _sz, _vp]),
     "nc_muon_update": (_i32, [_NP, _vp, _vp, _vp, _f32, _f32, _i32, _f32, _vp, _sz, _vp]),

@@ -559,7 +559,10 @@ def _linear_ce_args(features, weight, labels, bias, ignore_index, reduction):
     # int64 labels beyond int32 stay out of range instead of wrapping into it
     if labels.dtype == torch.int64:
         labels = labels.clamp(-2 ** 31, 2 ** 31 - 1).to(torch.int32)
-    return (d, features.contiguous(), weight.contiguous(), labels.contiguous(),
+    weight = weight.contiguous()
+    if weight.dtype == torch.bfloat16 and weight.data_ptr() % 16:
+        weight = weight.clone()      # the tensor cores' copies start on 16 bytes
+    return (d, features.contiguous(), weight, labels.contiguous(),
             None if bias is None else bias.contiguous())
 
 
@@ -643,9 +646,20 @@ def linear_softmax_ce_value_and_grad(features: torch.Tensor, weight: torch.Tenso
     those of the losses' sum)."""
     lib = _lib.load()
     d, f, w, lab, b = _linear_ce_args(features, weight, labels, bias, ignore_index, reduction)
-    with _on(f.device):
-        loss, lse = _linear_ce_forward(lib, d, f, w, lab, b)
-        return (loss, *_linear_ce_backward(lib, d, f, w, lab, b, lse, None, True, True, b is not None))
+    dev = f.device
+    none = reduction == "none"
+    loss = torch.empty((d.rows,) if none else (), dtype=torch.float32, device=dev)
+    g_f, g_w, g_b = torch.empty_like(f), torch.empty_like(w), None if b is None else torch.empty_like(b)
+    if none and d.rows == 0:
+        return loss, g_f, g_w.zero_(), None if b is None else g_b.zero_()
+    with _on(dev):
+        ws = _linear_ce_ws(lib, d, 1, dev)
+        lse = torch.empty(d.rows, dtype=torch.float32, device=dev)
+        _lib.check(lib.nc_linear_ce_value_and_grad(ctypes.byref(d), _ptr(f), _ptr(w), _ptr(b), _ptr(lab),
+                                                   _ptr(loss), _ptr(lse), _ptr(g_f), _ptr(g_w), _ptr(g_b),
+                                                   _ptr(ws), ws.numel(), _stream(dev)),
+                   "nc_linear_ce_value_and_grad")
+    return loss, g_f, g_w, g_b
 
 
 # ---------------------------------------------------------------------------------------

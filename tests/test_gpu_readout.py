@@ -8,7 +8,9 @@ Tolerances, elementwise, from the arithmetic (u = 2^-24, one rounding of a float
 * the loss adds the errors of the log-sum-exp and of one logit, and a few roundings.
 * a probability inherits twice the logit error as a relative error, and the rounding of exp
   (2 ulp), of the difference and of its scale: 8 u.  Beside bfloat16 inputs the matrix
-  products read it rounded to bfloat16: 2^-8.
+  products read it rounded to bfloat16: 2^-8.  Beside float32 inputs they read 2^15 dz (dz
+  taken relative to the largest g) as two float16 parts.  float16's smallest step is 2^-24,
+  so whatever dz's size the low part is off by at most half of that, 2^-25 / 2^15 = 2^-40.
 * a gradient is a sum of `rows` (or `classes`) products again; a bfloat16 result is rounded
   once more: 2^-8 relative.
 """
@@ -60,7 +62,7 @@ def _formula(f, w, b, lab, reduction="mean", g_loss=None):
     dz = (p - hot) * g[:, None]
     size = (p + hot) * g.abs()[:, None]
     rel = (2 * ez + 8 * U)[:, None] + (2.0 ** -8 if bf16 else 2.0 ** -21)
-    e_dz = size * rel
+    e_dz = size * rel + (0.0 if bf16 else 2.0 ** -40 * float(g.abs().max()))
     out = 2.0 ** -8 if bf16 else 2 * U
     grads = []
     for exact, a, e, y, k in ((dz @ wd, size, e_dz, wd, classes), (dz.T @ fd, size.T, e_dz.T, fd, rows)):
