@@ -7,6 +7,7 @@
 // singular value s of x goes through s <- a s + b s^3 + c s^5; the singular vectors stay.
 // The norm is summed in float64: the iteration magnifies an error of the scale of X0 up to
 // about a hundred times.
+#include <cooperative_groups.h>
 #include <math.h>
 
 #include "nc_common.cuh"
@@ -66,89 +67,218 @@ __global__ void __launch_bounds__(kNormThreads) ns_norm_kernel(const T* __restri
   if (threadIdx.x == 0) part[(size_t)blockIdx.y * gridDim.x + blockIdx.x] = s;
 }
 
-// X0 of one matrix; every block sums the matrix's parts again, in the same order.
-template <typename T>
-__global__ void __launch_bounds__(kNormThreads) ns_scale_kernel(const T* __restrict__ x, int64_t n, int parts,
-                                                                const double* __restrict__ part, double eps,
-                                                                float* __restrict__ out) {
-  __shared__ double red[kNormThreads / 32];
-  pdl_enter();
-  double s = 0.0;
-  for (int i = threadIdx.x; i < parts; i += kNormThreads) s += part[(size_t)blockIdx.y * parts + i];
-  s = block_sum_f64(s, red);
-  const double inv = 1.0 / (sqrt(s) + eps);
-  const size_t base = (size_t)blockIdx.y * n;
-  const int64_t i0 = (int64_t)blockIdx.x * kNormThreads * kNormPer + threadIdx.x;
-#pragma unroll 4
-  for (int k = 0; k < kNormPer; ++k) {
-    const int64_t i = i0 + (int64_t)k * kNormThreads;
-    if (i >= n) break;
-    out[base + i] = (float)((double)to_f32(x[base + i]) * inv);
-  }
-}
+// ---- short sides up to 64: one cluster per matrix ------------------------------------------
+// The CTAs of a cluster hold slices of the long side in shared memory for all steps, as
+// X[l][i] (i along the short side, padded to S).  A step: every CTA adds up its slice's part
+// of A = X X^T, the cluster sums the parts (each CTA its share of A, read from and written to
+// the others' shared memory), and every CTA updates its slice, Y = A X, X <- a X + b Y + c A Y,
+// which needs no other slice and no A^2.  The momentum, the norm and the final update are in
+// the same launch, so the cost is the two cluster barriers of a step and the FMAs, 3 S^2 per
+// column of a slice.
+constexpr int kSmallThreads = 256;
+constexpr size_t kSmallSmem = 200 * 1024;
 
-// One product of batched matrices, out = alpha A B + beta C: 64 x 64 tiles of float32 in
-// registers (4 x 4 per thread).  Element (i, k) of A is at i * a_i + k * a_k, and so on.
-struct Product {
-  const float *A, *B, *C;
-  float* out;
-  int m, n, k;
-  int64_t a_i, a_k, b_k, b_j, stride_a, stride_b, stride_c;   // C and out: row-major (m, n)
-  float alpha, beta;
+struct SmallArgs {
+  const void* x;
+  float* momentum;
+  float* params;
+  void* out;
+  int rows, cols, slice;    // slice: columns of the long side per CTA, whole 4s
+  int steps;
+  float a, b, c;
+  double eps;
+  MuonArgs mu;
+  float decay, step;
+  int32_t* status;
 };
 
-__global__ void __launch_bounds__(256) ns_product_kernel(Product p) {
-  __shared__ float as[16][64 + 4], bs[16][64 + 4];
-  pdl_enter();
-  const int i0 = blockIdx.y * 64, j0 = blockIdx.x * 64, tid = threadIdx.x;
-  const float* A = p.A + (size_t)blockIdx.z * p.stride_a;
-  const float* B = p.B + (size_t)blockIdx.z * p.stride_b;
-  const int tx = tid & 15, ty = tid >> 4;
-  float acc[4][4] = {};
-  for (int k0 = 0; k0 < p.k; k0 += 16) {
-    __syncthreads();
-    for (int e = tid; e < 16 * 64; e += 256) {
-      // the thread order follows the operand's contiguous direction
-      const int ka = p.a_k == 1 ? e & 15 : e >> 6, ia = p.a_k == 1 ? e >> 4 : e & 63;
-      as[ka][ia] = k0 + ka < p.k && i0 + ia < p.m ? A[(i0 + ia) * p.a_i + (k0 + ka) * p.a_k] : 0.f;
-      const int kb = p.b_k == 1 ? e & 15 : e >> 6, jb = p.b_k == 1 ? e >> 4 : e & 63;
-      bs[kb][jb] = k0 + kb < p.k && j0 + jb < p.n ? B[(k0 + kb) * p.b_k + (j0 + jb) * p.b_j] : 0.f;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < 16; ++k) {
-      float x[4], y[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = as[k][ty * 4 + e], y[e] = bs[k][tx * 4 + e];
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) acc[r][c] = fmaf(x[r], y[c], acc[r][c]);
-    }
-  }
-  const size_t base = (size_t)blockIdx.z * p.stride_c;
-#pragma unroll
-  for (int r = 0; r < 4; ++r)
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const int i = i0 + ty * 4 + r, j = j0 + tx * 4 + c;
-      if (i >= p.m || j >= p.n) continue;
-      const size_t o = base + (size_t)i * p.n + j;
-      p.out[o] = p.alpha * acc[r][c] + (p.C ? p.beta * p.C[o] : 0.f);
-    }
+template <int S>
+__host__ __device__ constexpr size_t small_smem(int slice) {
+  return (size_t)(2 * slice * (S + 4) + 4096 + S * (S + 4)) * 4;
 }
 
-// out = X in the caller's type, or with `params`: p <- decay p - step X.
-template <typename T>
-__global__ void ns_store_kernel(const float* __restrict__ x, int64_t n, T* __restrict__ out, float* __restrict__ params,
-                                float decay, float step) {
+// out[l][i..i+3] for 4 columns l: sum over k of A[k][i] in[l][k].
+template <int S>
+__device__ __forceinline__ void small_product(const float* A, const float* in, int i, float (&acc)[4][4]) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[q][e] = 0.f;
+#pragma unroll 4
+  for (int k = 0; k < S; k += 4) {
+    float m[4][4], v[4][4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) *reinterpret_cast<float4*>(m[e]) = *reinterpret_cast<const float4*>(A + (k + e) * (S + 4) + i);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) *reinterpret_cast<float4*>(v[q]) = *reinterpret_cast<const float4*>(in + q * (S + 4) + k);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[q][r] = fmaf(m[e][r], v[q][e], acc[q][r]);
+  }
+}
+
+template <int S, typename T>
+__global__ void __launch_bounds__(kSmallThreads) ns_small_kernel(SmallArgs p) {
+  namespace cg = cooperative_groups;
+  constexpr int kPitch = S + 4, kPer = S / 4, kCell = kPer * kPer;   // threads of one S x S product
+  constexpr int kGroups = kSmallThreads / kCell;                     // that split the slice's columns
+  extern __shared__ __align__(16) float sm[];
+  __shared__ double red[kSmallThreads / 32], total;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ranks = cluster.num_blocks(), rank = cluster.block_rank(), tid = threadIdx.x;
+  float* X = sm;
+  float* Y = X + p.slice * kPitch;
+  float* part = Y + p.slice * kPitch;   // (kGroups, S, S)
+  float* A = part + 4096;               // (S, pitch)
+  const bool tall = p.rows > p.cols;
+  const int s = tall ? p.cols : p.rows, len = tall ? p.rows : p.cols;
+  const int l0 = rank * p.slice;
+  const size_t base = (size_t)(blockIdx.x / ranks) * p.rows * p.cols;
   pdl_enter();
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= n) return;
-  if (params)
-    params[i] = params[i] * decay - step * x[i];
-  else
-    store_as(out + i, x[i]);
+  if (blockIdx.x == 0 && tid == 0) *p.status = 0;
+
+  // the source in the order of its memory; momentum in passing
+  const T* x = static_cast<const T*>(p.x) + base;
+  double sum = 0.0;
+  for (int e = tid; e < p.slice * S; e += kSmallThreads) {
+    const int l = tall ? e / S : e % p.slice, i = tall ? e % S : e / p.slice;
+    float v = 0.f;
+    if (i < s && l0 + l < len) {
+      const size_t o = tall ? (size_t)(l0 + l) * p.cols + i : (size_t)i * p.cols + l0 + l;
+      v = to_f32(x[o]);
+      if (p.momentum) {
+        const float m = fmaf(p.mu.beta, p.momentum[base + o], v);
+        p.momentum[base + o] = m;
+        v = p.mu.nesterov ? fmaf(p.mu.beta, m, v) : m;
+      }
+    }
+    X[l * kPitch + i] = v;
+    sum += (double)v * v;
+  }
+  sum = block_sum_f64(sum, red);
+  if (tid == 0) total = sum;
+  cluster.sync();
+  double norm = 0.0;
+  for (int r = 0; r < ranks; ++r) norm += *cluster.map_shared_rank(&total, r);
+  const double inv = 1.0 / (sqrt(norm) + p.eps);
+  for (int e = tid; e < p.slice * S; e += kSmallThreads) {
+    const int o = e / S * kPitch + e % S;
+    X[o] = (float)((double)X[o] * inv);
+  }
+  __syncthreads();
+
+  const int cell = tid % kCell, group = tid / kCell;
+  const int ti = cell % kPer * 4, tj = cell / kPer * 4;
+  const int share = S * S / ranks;   // elements of A that this CTA sums
+  for (int step = 0; step < p.steps; ++step) {
+    float acc[4][4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[q][e] = 0.f;
+#pragma unroll 4
+    for (int l = group; l < p.slice; l += kGroups) {
+      float u[4], v[4];
+      *reinterpret_cast<float4*>(u) = *reinterpret_cast<const float4*>(X + l * kPitch + ti);
+      *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(X + l * kPitch + tj);
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[q][e] = fmaf(v[q], u[e], acc[q][e]);
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      *reinterpret_cast<float4*>(part + group * S * S + (tj + q) * S + ti) =
+          make_float4(acc[q][0], acc[q][1], acc[q][2], acc[q][3]);
+    if constexpr (kGroups > 1) {
+      __syncthreads();
+      for (int e = tid; e < S * S; e += kSmallThreads) {
+        float v = part[e];
+#pragma unroll
+        for (int g = 1; g < kGroups; ++g) v += part[g * S * S + e];
+        part[e] = v;
+      }
+    }
+    cluster.sync();
+    for (int e = rank * share + tid; e < (rank + 1) * share; e += kSmallThreads) {
+      float v = 0.f;
+#pragma unroll 8
+      for (int r = 0; r < ranks; ++r) v += cluster.map_shared_rank(part, r)[e];
+      const int o = e / S * kPitch + e % S;
+#pragma unroll 8
+      for (int r = 0; r < ranks; ++r) cluster.map_shared_rank(A, r)[o] = v;
+    }
+    cluster.sync();
+    for (int t = tid; t < p.slice / 4 * kPer; t += kSmallThreads) {
+      const int i = t % kPer * 4, l = t / kPer * 4;
+      small_product<S>(A, X + l * kPitch, i, acc);
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<float4*>(Y + (l + q) * kPitch + i) = make_float4(acc[q][0], acc[q][1], acc[q][2], acc[q][3]);
+    }
+    __syncthreads();
+    for (int t = tid; t < p.slice / 4 * kPer; t += kSmallThreads) {
+      const int i = t % kPer * 4, l = t / kPer * 4;
+      small_product<S>(A, Y + l * kPitch, i, acc);
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int o = (l + q) * kPitch + i + e;
+          X[o] = fmaf(p.a, X[o], fmaf(p.b, Y[o], p.c * acc[q][e]));
+        }
+    }
+    __syncthreads();
+  }
+  T* out = static_cast<T*>(p.out) + base;
+  for (int e = tid; e < p.slice * S; e += kSmallThreads) {
+    const int l = tall ? e / S : e % p.slice, i = tall ? e % S : e / p.slice;
+    if (i >= s || l0 + l >= len) continue;
+    const size_t o = tall ? (size_t)(l0 + l) * p.cols + i : (size_t)i * p.cols + l0 + l;
+    const float v = X[l * kPitch + i];
+    if (p.params)
+      p.params[base + o] = p.params[base + o] * p.decay - p.step * v;
+    else
+      store_as(out + o, v);
+  }
+  cluster.sync();   // no CTA leaves while another may still read its shared memory
+}
+
+// CTAs per cluster and columns per CTA; `fits`: within shared memory.
+struct SmallPlan {
+  int pad, ranks, slice;
+  bool fits;
+};
+
+SmallPlan small_plan(const nc_newton_schulz* d) {
+  const int s = d->rows < d->cols ? d->rows : d->cols, len = d->rows < d->cols ? d->cols : d->rows;
+  SmallPlan r{};
+  r.pad = s <= 16 ? 16 : s <= 32 ? 32 : 64;
+  r.ranks = len > 28 ? 8 : len > 12 ? 4 : len > 4 ? 2 : 1;
+  r.slice = ((len + r.ranks - 1) / r.ranks + 3) / 4 * 4;
+  const size_t need = r.pad == 16 ? small_smem<16>(r.slice) : r.pad == 32 ? small_smem<32>(r.slice) : small_smem<64>(r.slice);
+  r.fits = s <= 64 && need <= kSmallSmem;
+  return r;
+}
+
+template <int S, typename T>
+nc_status launch_small(const SmallArgs& a, const SmallPlan& r, int batch, cudaStream_t st) {
+  auto k = ns_small_kernel<S, T>;
+  const size_t smem = small_smem<S>(r.slice);
+  NC_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = r.ranks, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3(r.ranks * batch), cfg.blockDim = dim3(kSmallThreads);
+  cfg.dynamicSmemBytes = smem, cfg.stream = st, cfg.attrs = attr, cfg.numAttrs = 2;
+  NC_CUDA_CHECK(cudaLaunchKernelEx(&cfg, k, a));
+  return launch_check("ns_small_kernel launch");
 }
 
 // ---- products on the tensor cores --------------------------------------------------------
@@ -308,8 +438,9 @@ int norm_blocks(int64_t n) { return (int)((n + kNormThreads * kNormPer - 1) / (k
 constexpr int kNsChunk = 2;
 constexpr int kNsTile = 128;
 
-// The tensor cores from a short side of 65 on; below, one 64 x 64 float32 tile holds A.
-bool on_tensor_cores(const nc_newton_schulz* d) { return d->rows > 64 && d->cols > 64 && d->steps > 0; }
+// Short sides up to 64 whose slices fit take one cluster per matrix, the others the tensor
+// cores.
+bool on_tensor_cores(const nc_newton_schulz* d) { return !small_plan(d).fits; }
 
 int plane_pitch(int cols) { return (cols + 63) / 64 * 64; }
 
@@ -320,9 +451,7 @@ struct NsLayout {
 NsLayout ns_layout(const nc_newton_schulz* d) {
   NsLayout L{};
   const size_t n = (size_t)d->rows * d->cols, s = d->rows < d->cols ? d->rows : d->cols;
-  // float32 (rows, cols), or two planes of float16 with padded rows
-  const bool tensor = on_tensor_cores(d);
-  const size_t x = tensor ? (size_t)d->rows * plane_pitch(d->cols) : n, g = tensor ? s * plane_pitch((int)s) : s * s;
+  const size_t x = (size_t)d->rows * plane_pitch(d->cols), g = s * plane_pitch((int)s);   // two float16 planes each
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t o = at;
@@ -330,6 +459,10 @@ NsLayout ns_layout(const nc_newton_schulz* d) {
     return o;
   };
   L.status = take(4);
+  if (!on_tensor_cores(d)) {
+    L.total = at;
+    return L;
+  }
   L.part = take((size_t)d->batch * norm_blocks(n) * 8);
   L.u = take(d->batch * n * 4);
   L.x = take(d->batch * x * 4);
@@ -359,10 +492,20 @@ nc_status check_ws(const void* ws, size_t have, size_t need) {
   return NC_OK;
 }
 
-nc_status product(const Product& p, int batch, cudaStream_t st) {
-  PdlLaunch l(dim3((p.n + 63) / 64, (p.m + 63) / 64, batch), dim3(256), 0, st);
-  NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, ns_product_kernel, p));
-  return launch_check("ns_product_kernel launch");
+// No steps: X0 as it is.
+template <typename T>
+__global__ void __launch_bounds__(256) ns_store_kernel(Planes x, int rows, int cols, T* __restrict__ out,
+                                                       float* __restrict__ params, float decay, float step) {
+  pdl_enter();
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= rows * cols) return;
+  const size_t s = (size_t)blockIdx.y * 2 * x.plane + (size_t)(i / cols) * x.pitch + i % cols;
+  const size_t o = (size_t)blockIdx.y * rows * cols + i;
+  const float v = (__half2float(x.p[s]) + __half2float(x.p[x.plane + s])) * kPlaneInv;
+  if (params)
+    params[o] = params[o] * decay - step * v;
+  else
+    store_as(out + o, v);
 }
 
 template <int MODE, typename T>
@@ -400,6 +543,11 @@ nc_status run_tensor(const nc_newton_schulz* d, const T* x, const float* u, cons
       NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, ns_split_kernel<T>, x, n, d->cols, nb, part, (double)d->eps, X));
     NC_CHECK(launch_check("ns_split_kernel launch"));
   }
+  if (d->steps == 0) {
+    PdlLaunch l(dim3((unsigned)((n + 255) / 256), d->batch), dim3(256), 0, st);
+    NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, ns_store_kernel<T>, X, d->rows, d->cols, out, params, decay, step));
+    return launch_check("ns_store_kernel launch");
+  }
   const void* to = params ? static_cast<void*>(params) : static_cast<void*>(out);
   const size_t size = params ? 4 : sizeof(T);
   const bool wide = reinterpret_cast<uintptr_t>(to) % 32 == 0 && (size_t)d->cols * size % 32 == 0;
@@ -434,53 +582,22 @@ nc_status run(const nc_newton_schulz* d, const T* x, float* momentum, MuonArgs m
               float step, void* d_ws, cudaStream_t st) {
   const NsLayout L = ns_layout(d);
   char* ws = static_cast<char*>(d_ws);
-  auto f32 = [&](size_t o) { return reinterpret_cast<float*>(ws + o); };
+  int32_t* status = reinterpret_cast<int32_t*>(ws + L.status);
+  if (!on_tensor_cores(d)) {
+    const SmallPlan r = small_plan(d);
+    const SmallArgs a{x,    momentum, params, out,  d->rows, d->cols, r.slice, d->steps,
+                      d->a, d->b,     d->c,   d->eps, mu,      decay,   step,    status};
+    return r.pad == 16   ? launch_small<16, T>(a, r, d->batch, st)
+           : r.pad == 32 ? launch_small<32, T>(a, r, d->batch, st)
+                         : launch_small<64, T>(a, r, d->batch, st);
+  }
+  float* u = reinterpret_cast<float*>(ws + L.u);
   double* part = reinterpret_cast<double*>(ws + L.part);
   const int64_t n = (int64_t)d->rows * d->cols;
-  const int nb = norm_blocks(n), s = d->rows < d->cols ? d->rows : d->cols;
-  {
-    PdlLaunch l(dim3(nb, d->batch), dim3(kNormThreads), 0, st);
-    NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, ns_norm_kernel<T>, x, momentum, mu, n, f32(L.u), part,
-                                     reinterpret_cast<int32_t*>(ws + L.status)));
-    NC_CHECK(launch_check("ns_norm_kernel launch"));
-  }
-  if (on_tensor_cores(d))
-    return run_tensor(d, x, momentum ? f32(L.u) : nullptr, part, out, params, decay, step, ws, L, st);
-  float *X = f32(L.x), *Y = f32(L.y);
-  {
-    PdlLaunch l(dim3(nb, d->batch), dim3(kNormThreads), 0, st);
-    if (momentum)
-      NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, ns_scale_kernel<float>, (const float*)f32(L.u), n, nb,
-                                       (const double*)part, (double)d->eps, X));
-    else
-      NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, ns_scale_kernel<T>, x, n, nb, (const double*)part, (double)d->eps, X));
-    NC_CHECK(launch_check("ns_scale_kernel launch"));
-  }
-  const bool tall = d->rows > d->cols;
-  const int64_t ss = (int64_t)s * s;
-  for (int k = 0; k < d->steps; ++k) {
-    Product g{};   // Gram matrix of the short side
-    g.A = X, g.B = X, g.out = f32(L.gram), g.m = s, g.n = s, g.k = tall ? d->rows : d->cols;
-    g.a_i = tall ? 1 : d->cols, g.a_k = tall ? d->cols : 1, g.b_k = g.a_k, g.b_j = g.a_i;
-    g.stride_a = g.stride_b = n, g.stride_c = ss, g.alpha = 1.f;
-    NC_CHECK(product(g, d->batch, st));
-    Product q{};   // b A + c A^2
-    q.A = q.B = q.C = f32(L.gram), q.out = f32(L.poly), q.m = q.n = q.k = s;
-    q.a_i = q.b_k = s, q.a_k = q.b_j = 1, q.stride_a = q.stride_b = q.stride_c = ss, q.alpha = d->c, q.beta = d->b;
-    NC_CHECK(product(q, d->batch, st));
-    Product u{};   // a X + (b A + c A^2) X
-    u.m = d->rows, u.n = d->cols, u.k = s, u.C = X, u.out = Y, u.alpha = 1.f, u.beta = d->a, u.stride_c = n;
-    u.A = tall ? X : f32(L.poly), u.B = tall ? f32(L.poly) : X;
-    u.a_i = s, u.a_k = 1, u.b_k = d->cols, u.b_j = 1;
-    u.stride_a = tall ? n : ss, u.stride_b = tall ? ss : n;
-    NC_CHECK(product(u, d->batch, st));
-    float* t = X;
-    X = Y, Y = t;
-  }
-  const int64_t all = n * d->batch;
-  PdlLaunch l(dim3((unsigned)((all + 255) / 256)), dim3(256), 0, st);
-  NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, ns_store_kernel<T>, (const float*)X, all, out, params, decay, step));
-  return launch_check("ns_store_kernel launch");
+  PdlLaunch l(dim3(norm_blocks(n), d->batch), dim3(kNormThreads), 0, st);
+  NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, ns_norm_kernel<T>, x, momentum, mu, n, u, part, status));
+  NC_CHECK(launch_check("ns_norm_kernel launch"));
+  return run_tensor(d, x, momentum ? u : nullptr, part, out, params, decay, step, ws, L, st);
 }
 
 }  // namespace
