@@ -513,12 +513,12 @@ nc_status tensor_product(const nc_newton_schulz* d, const Planes& A, bool a_mn, 
                          int k, const NsEpilogue<MODE, T>& epi, int32_t* status, cudaStream_t st) {
   tc::Problem p{};
   p.m = m, p.n = n, p.k = k, p.batch = d->batch, p.splits = 1, p.chunk = kNsChunk;
-  p.tiles_m = (m + tc::kBM - 1) / tc::kBM, p.tiles_n = (n + kNsTile - 1) / kNsTile;
+  tc::set_tiles<kNsTile, 1>(&p);
   p.symmetric = MODE == kGram || MODE == kPoly;
   p.status = status;
-  NC_CHECK((tc::make_operand<2, kNsTile>(&p, true, A.p, a_mn, m, k, A.pitch, A.plane, d->batch, 2 * A.plane)));
-  NC_CHECK((tc::make_operand<2, kNsTile>(&p, false, B.p, b_mn, n, k, B.pitch, B.plane, d->batch, 2 * B.plane)));
-  return tc::launch_product<2, kNsTile>(p, epi, st, "Newton-Schulz product launch");
+  NC_CHECK((tc::make_operand<2, kNsTile, 1>(&p, true, A.p, a_mn, m, k, A.pitch, A.plane, d->batch, 2 * A.plane)));
+  NC_CHECK((tc::make_operand<2, kNsTile, 1>(&p, false, B.p, b_mn, n, k, B.pitch, B.plane, d->batch, 2 * B.plane)));
+  return tc::launch_product<2, kNsTile, 1>(p, epi, st, "Newton-Schulz product launch");
 }
 
 template <typename T>

@@ -38,11 +38,13 @@ struct Scales {
 struct Plan {
   bool bf16, copy_w;
   int pitch;                  // of the planes of features and weight
-  int rows_pad;               // rows, whole 128s
+  int rows_pad;               // rows, whole 256s
   int classes_pad;            // classes, whole 256s
   int slots;                  // half tiles of classes
   int piece, pieces;          // classes per piece (whole 256s)
-  int bn_out;                 // tile width of the gradient products
+  // CTA pairs on 256 x 256 tiles, or one CTA on 128 x 128 where a side has at most 128: the
+  // logits' products, dw's and df's
+  bool pair, pair_w, pair_f;
   int splits;                 // of df over a piece's classes
   size_t scales, max_part, w, f, bias, part, zlabel, fac, dz, df_part, db_part, total;
 };
@@ -52,9 +54,13 @@ Plan make_plan(const nc_linear_ce* d, bool grad) {
   p.bf16 = d->dtype == NC_BF16;
   p.copy_w = !p.bf16 || d->dim % 8 != 0;   // else the weight is read where it is
   p.pitch = (d->dim + 7) / 8 * 8;
-  p.rows_pad = (d->rows + 127) / 128 * 128;
+  p.rows_pad = (d->rows + 255) / 256 * 256;
   p.classes_pad = (d->classes + 255) / 256 * 256;
-  p.slots = p.classes_pad / 128;
+  p.pair = d->rows > 128;
+  p.pair_w = d->dim > 128;
+  p.pair_f = d->dim > 128 && d->rows > 128;
+  const int tile = p.pair ? 256 : 128;
+  p.slots = (d->classes + tile - 1) / tile * 2;
   const int planes = p.bf16 ? 1 : 2;
   const int tiles = p.classes_pad / 256;
   const size_t tile_bytes = (size_t)p.rows_pad * 256 * 2 * planes;
@@ -63,9 +69,9 @@ Plan make_plan(const nc_linear_ce* d, bool grad) {
   p.pieces = (tiles + most - 1) / most;
   p.piece = (tiles + p.pieces - 1) / p.pieces * 256;
   p.pieces = (p.classes_pad + p.piece - 1) / p.piece;   // none is empty
-  p.bn_out = d->dim <= 128 ? 128 : 256;
-  const int out_tiles = p.rows_pad / 128 * ((d->dim + p.bn_out - 1) / p.bn_out);
-  int splits = 148 / out_tiles;
+  const int out = p.pair_f ? 256 : 128;
+  const int out_tiles = (d->rows + out - 1) / out * ((d->dim + out - 1) / out);
+  int splits = (p.pair_f ? 74 : 148) / out_tiles;
   if (splits > p.piece / 256) splits = p.piece / 256;
   p.splits = splits < 1 ? 1 : splits;
   size_t at = 0;
@@ -470,10 +476,11 @@ struct Call {
   Scales* scales() const { return at<Scales>(p.scales); }
   int32_t* status() const { return reinterpret_cast<int32_t*>(at<Scales>(p.scales) + 1); }
 
-  tc::Problem problem(int m, int n, int k, int bn, int splits) const {
+  template <int BN, int CG>
+  tc::Problem problem(int m, int n, int k, int splits) const {
     tc::Problem q{};
     q.m = m, q.n = n, q.k = k, q.batch = 1, q.splits = splits, q.bf16 = p.bf16;
-    q.tiles_m = (m + tc::kBM - 1) / tc::kBM, q.tiles_n = (n + bn - 1) / bn;
+    tc::set_tiles<BN, CG>(&q);
     q.chunk = PL == 1 ? 1 << 30 : kChunk;
     q.status = status();
     return q;
@@ -481,23 +488,23 @@ struct Call {
 
   // Operands: rows of features or weight (k = dim contiguous), or with their columns as the
   // own index and rows as k.
-  template <int BN>
+  template <int BN, int CG>
   nc_status features_op(tc::Problem* q, bool is_a, bool by_column) const {
-    return tc::make_operand<PL, BN>(q, is_a, at<void>(p.f), by_column, by_column ? d->dim : d->rows,
+    return tc::make_operand<PL, BN, CG>(q, is_a, at<void>(p.f), by_column, by_column ? d->dim : d->rows,
                                     by_column ? d->rows : d->dim, p.pitch, (int64_t)d->rows * p.pitch, 1,
                                     (int64_t)PL * d->rows * p.pitch);
   }
-  template <int BN>
+  template <int BN, int CG>
   nc_status weight_op(tc::Problem* q, bool by_column) const {
     const void* base = p.copy_w ? at<void>(p.w) : a.weight;
     const int pitch = p.copy_w ? p.pitch : d->dim;
-    return tc::make_operand<PL, BN>(q, false, base, by_column, by_column ? d->dim : d->classes,
+    return tc::make_operand<PL, BN, CG>(q, false, base, by_column, by_column ? d->dim : d->classes,
                                     by_column ? d->classes : d->dim, pitch, (int64_t)d->classes * pitch, 1,
                                     (int64_t)PL * d->classes * pitch);
   }
-  template <int BN>
+  template <int BN, int CG>
   nc_status dz_op(tc::Problem* q, bool by_column) const {
-    return tc::make_operand<PL, BN>(q, true, at<void>(p.dz), by_column, by_column ? p.piece : d->rows,
+    return tc::make_operand<PL, BN, CG>(q, true, at<void>(p.dz), by_column, by_column ? p.piece : d->rows,
                                     by_column ? d->rows : p.piece, p.piece, (int64_t)d->rows * p.piece, 1,
                                     (int64_t)PL * d->rows * p.piece);
   }
@@ -520,12 +527,17 @@ struct Call {
     return launch_check("ce_planes_kernel launch");
   }
 
-  nc_status value(float* lse, float* row_loss) const {
-    tc::Problem q = problem(d->rows, d->classes, d->dim, 256, 1);
-    NC_CHECK(features_op<256>(&q, true, false));
-    NC_CHECK(weight_op<256>(&q, false));
+  template <int BN, int CG>
+  nc_status value_product() const {
+    tc::Problem q = problem<BN, CG>(d->rows, d->classes, d->dim, 1);
+    NC_CHECK((features_op<BN, CG>(&q, true, false)));
+    NC_CHECK((weight_op<BN, CG>(&q, false)));
     const ValueEpilogue e{a, scales(), at<float>(p.bias), at<float2>(p.part), at<float>(p.zlabel), p.rows_pad};
-    NC_CHECK((tc::launch_product<PL, 256>(q, e, st, "readout value product launch")));
+    return tc::launch_product<PL, BN, CG>(q, e, st, "readout value product launch");
+  }
+
+  nc_status value(float* lse, float* row_loss) const {
+    NC_CHECK(p.pair ? (value_product<256, 2>()) : (value_product<128, 1>()));
     PdlLaunch l(dim3((d->rows + 31) / 32), dim3(256), 0, st);
     NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, ce_finish_kernel, a, p.slots, p.rows_pad,
                                      (const float2*)at<float2>(p.part), (const float*)at<float>(p.zlabel), lse,
@@ -533,27 +545,37 @@ struct Call {
     return launch_check("ce_finish_kernel launch");
   }
 
-  template <int BN>
-  nc_status piece_products(const CeGrads& g, int v0, int width, int classes) const {
-    if (g.weight) {
-      tc::Problem q = problem(classes, d->dim, d->rows, BN, 1);
-      NC_CHECK(dz_op<BN>(&q, true));
-      NC_CHECK(features_op<BN>(&q, false, true));
-      T* out = static_cast<T*>(g.weight) + (size_t)v0 * d->dim;
-      const bool wide = reinterpret_cast<uintptr_t>(out) % 32 == 0 && (size_t)d->dim * sizeof(T) % 32 == 0;
-      const WeightEpilogue<T> e{scales(), out, classes, d->dim, wide};
-      NC_CHECK((tc::launch_product<PL, BN>(q, e, st, "readout weight gradient launch")));
-    }
-    if (g.features) {
-      tc::Problem q = problem(d->rows, d->dim, width, BN, p.splits);
-      NC_CHECK(dz_op<BN>(&q, false));
-      NC_CHECK(weight_op<BN>(&q, true));
-      q.b_k0 = v0;
-      const FeatureEpilogue e{scales(), at<float>(p.df_part), d->rows, d->dim, p.pitch, v0 == 0,
-                              PL == 1 ? 1.f : 1.f / kDzScale};
-      NC_CHECK((tc::launch_product<PL, BN>(q, e, st, "readout feature gradient launch")));
-    }
-    return NC_OK;
+  template <int BN, int CG>
+  nc_status dz_product(const CeGrads& g, int v0, int width) const {
+    tc::Problem q = problem<BN, CG>(d->rows, width, d->dim, 1);
+    NC_CHECK((features_op<BN, CG>(&q, true, false)));
+    NC_CHECK((weight_op<BN, CG>(&q, false)));
+    q.b_n0 = v0;
+    const DzEpilogue<PL == 1> e{a,     scales(), at<float>(p.bias), g.lse,  at<float>(p.fac), at<uint16_t>(p.dz),
+                                g.bias ? at<float>(p.db_part) : nullptr, v0, p.piece, p.classes_pad};
+    return tc::launch_product<PL, BN, CG>(q, e, st, "readout logit gradient launch");
+  }
+
+  template <int BN, int CG>
+  nc_status weight_product(const CeGrads& g, int v0, int classes) const {
+    tc::Problem q = problem<BN, CG>(classes, d->dim, d->rows, 1);
+    NC_CHECK((dz_op<BN, CG>(&q, true)));
+    NC_CHECK((features_op<BN, CG>(&q, false, true)));
+    T* out = static_cast<T*>(g.weight) + (size_t)v0 * d->dim;
+    const bool wide = reinterpret_cast<uintptr_t>(out) % 32 == 0 && (size_t)d->dim * sizeof(T) % 32 == 0;
+    const WeightEpilogue<T> e{scales(), out, classes, d->dim, wide};
+    return tc::launch_product<PL, BN, CG>(q, e, st, "readout weight gradient launch");
+  }
+
+  template <int BN, int CG>
+  nc_status feature_product(const CeGrads& g, int v0, int width) const {
+    tc::Problem q = problem<BN, CG>(d->rows, d->dim, width, p.splits);
+    NC_CHECK((dz_op<BN, CG>(&q, false)));
+    NC_CHECK((weight_op<BN, CG>(&q, true)));
+    q.b_k0 = v0;
+    const FeatureEpilogue e{scales(), at<float>(p.df_part), d->rows, d->dim, p.pitch, v0 == 0,
+                            PL == 1 ? 1.f : 1.f / kDzScale};
+    return tc::launch_product<PL, BN, CG>(q, e, st, "readout feature gradient launch");
   }
 
   nc_status gradients(const CeGrads& g) const {
@@ -567,14 +589,11 @@ struct Call {
       // the last piece may be shorter; `width` is whole tiles
       const int width = p.classes_pad - v0 < p.piece ? p.classes_pad - v0 : p.piece;
       const int classes = d->classes - v0 < width ? d->classes - v0 : width;
-      tc::Problem q = problem(d->rows, width, d->dim, 256, 1);
-      NC_CHECK(features_op<256>(&q, true, false));
-      NC_CHECK(weight_op<256>(&q, false));
-      q.b_n0 = v0;
-      const DzEpilogue<PL == 1> e{a,     scales(), at<float>(p.bias), g.lse,  at<float>(p.fac), at<uint16_t>(p.dz),
-                                  g.bias ? at<float>(p.db_part) : nullptr, v0, p.piece, p.classes_pad};
-      NC_CHECK((tc::launch_product<PL, 256>(q, e, st, "readout logit gradient launch")));
-      NC_CHECK(p.bn_out == 128 ? piece_products<128>(g, v0, width, classes) : piece_products<256>(g, v0, width, classes));
+      NC_CHECK(p.pair ? (dz_product<256, 2>(g, v0, width)) : (dz_product<128, 1>(g, v0, width)));
+      if (g.weight)
+        NC_CHECK(p.pair_w ? (weight_product<256, 2>(g, v0, classes)) : (weight_product<128, 1>(g, v0, classes)));
+      if (g.features)
+        NC_CHECK(p.pair_f ? (feature_product<256, 2>(g, v0, width)) : (feature_product<128, 1>(g, v0, width)));
     }
     if (g.features) {
       const int64_t n = (int64_t)d->rows * d->dim;
@@ -586,7 +605,7 @@ struct Call {
     }
     if (g.bias) {
       PdlLaunch l(dim3((d->classes + 255) / 256), dim3(256), 0, st);
-      NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, ce_bias_kernel<T>, (const float*)at<float>(p.db_part), p.rows_pad / 32,
+      NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, ce_bias_kernel<T>, (const float*)at<float>(p.db_part), (d->rows + 31) / 32,
                                        d->classes, p.classes_pad, (const Scales*)scales(), static_cast<T*>(g.bias)));
       NC_CHECK(launch_check("ce_bias_kernel launch"));
     }

@@ -23,7 +23,7 @@
 namespace nc {
 namespace tc {
 
-constexpr int kBM = 128;            // rows of a tile: one tensor-memory lane each
+constexpr int kBM = 128;            // rows of a tile per CTA: one tensor-memory lane each
 constexpr int kEpiWarps = 8;        // two per lane quarter, one per half of the columns
 constexpr int kThreads = 32 * (kEpiWarps + 2);
 constexpr int kWaitLimit = 1 << 20; // polls of a bounded wait
@@ -47,10 +47,15 @@ struct Tile {
   int kt0, kt1;   // k-tiles [kt0, kt1)
 };
 
-template <int PL, int BN>
+// CG = 2: two CTAs on two SMs work on one tile of 256 rows.  Each loads its 128 rows of A and
+// half of B; the products read both halves.  Shared memory bounds a product of one CTA (a
+// 128 x 256 tile writes and reads 192 bytes a cycle for 128 that it can take); the pair needs
+// 128.
+template <int PL, int BN, int CG>
 struct Config {
   static constexpr int kBK = PL == 1 ? 64 : 32;
-  static constexpr int kA = PL * kBM * kBK * 2, kB = PL * BN * kBK * 2;
+  static constexpr int kBRows = BN / CG;   // of B in one CTA
+  static constexpr int kA = PL * kBM * kBK * 2, kB = PL * kBRows * kBK * 2;
   static constexpr int kStage = kA + kB;
   static constexpr int kStages = 192 * 1024 / kStage;
   static constexpr int kSmem = kStages * kStage + 1024;   // stages start on 1024 bytes
@@ -61,8 +66,9 @@ __host__ __device__ inline int problem_tiles(const Problem& p) {
   return mn * p.batch * p.splits;
 }
 
-template <int PL, int BN>
-__device__ __forceinline__ Tile problem_tile(const Problem& p, int t) {
+// `rank`: of the CTA in its pair.
+template <int PL, int BN, int CG>
+__device__ __forceinline__ Tile problem_tile(const Problem& p, int t, int rank) {
   Tile x;
   int mn;
   if (p.symmetric) {
@@ -76,10 +82,11 @@ __device__ __forceinline__ Tile problem_tile(const Problem& p, int t) {
     const int per = p.tiles_m * p.tiles_n;
     mn = t % per;
     t /= per;
-    x.m0 = mn % p.tiles_m * kBM, x.n0 = mn / p.tiles_m * BN;
+    x.m0 = mn % p.tiles_m * kBM * CG + rank * kBM, x.n0 = mn / p.tiles_m * BN;
   }
   x.batch = t % p.batch, x.split = t / p.batch;
-  const int kt = (p.k + Config<PL, BN>::kBK - 1) / Config<PL, BN>::kBK;
+  constexpr int BK = Config<PL, BN, CG>::kBK;
+  const int kt = (p.k + BK - 1) / BK;
   x.kt0 = (int)((int64_t)kt * x.split / p.splits), x.kt1 = (int)((int64_t)kt * (x.split + 1) / p.splits);
   return x;
 }
@@ -94,6 +101,23 @@ __device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
 }
 __device__ __forceinline__ void bar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// The same barrier in the pair's first CTA.
+__device__ __forceinline__ uint32_t leader_addr(uint32_t bar) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(bar));
+  return r;
+}
+__device__ __forceinline__ void bar_arrive_leader(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(leader_addr(bar)) : "memory");
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
 }
 __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
   uint32_t ok;
@@ -118,23 +142,65 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
   return false;
 }
 
+// A box into this CTA's shared memory; its bytes count on `bar`, for a pair the first CTA's.
+template <int CG>
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c3) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], "
-      "[%2];" ::"r"(dst),
-      "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(0), "r"(c3)
-      : "memory");
+  if constexpr (CG == 1)
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+        "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(0), "r"(c3)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+        "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(0), "r"(c3)
+        : "memory");
 }
 
+template <int CG>
 __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(add)
-      : "memory");
+  if constexpr (CG == 1)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(add)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(add)
+        : "memory");
 }
+// One arrival on `bar` (of both CTAs of a pair) when the products issued so far are done.
+template <int CG>
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+  if constexpr (CG == 1)
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+  else
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+        "h"((uint16_t)3)
+        : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void tmem_alloc(uint32_t slot, int columns) {
+  if constexpr (CG == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(columns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(columns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+  }
+}
+template <int CG>
+__device__ __forceinline__ void tmem_free(uint32_t tmem, int columns) {
+  if constexpr (CG == 1)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns));
+  else
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns));
 }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -191,12 +257,14 @@ __device__ __forceinline__ void load_v8(const void* p, uint32_t (&v)[8]) {
                : "memory");
 }
 
-// The kernel: warps 0..7 epilogue, warp 8 loads, warp 9 multiplies; persistent over tiles.
-// Epi::run(tile, row, col, acc) gets a row's BN / 2 consecutive columns as float32 sums.
-template <int PL, int BN, class Epi>
+// The kernel: warps 0..7 epilogue, warp 8 loads, warp 9 multiplies (in the first CTA of a
+// pair); persistent over tiles.  Epi::run(tile, row, col, acc) gets a row's BN / 2
+// consecutive columns as float32 sums.
+template <int PL, int BN, int CG, class Epi>
 __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_constant__ Problem p, const Epi epi) {
-  using C = Config<PL, BN>;
+  using C = Config<PL, BN, CG>;
   constexpr int BK = C::kBK, HALF = BN / 2;
+  constexpr uint32_t a_block = C::kA / (kBM / 64), b_block = C::kB / (C::kBRows / 64);
   extern __shared__ uint8_t raw[];
   __shared__ __align__(8) uint64_t bars[2 * C::kStages + 5];
   __shared__ uint32_t tmem_slot;
@@ -209,22 +277,20 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
   auto acc_empty = [&](int b) { return bar0 + 8 * (2 * C::kStages + 2 + b); };
   const uint32_t drain = bar0 + 8 * (2 * C::kStages + 4);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = CG == 1 ? 0 : (int)cluster_rank();
+  const int first = blockIdx.x / CG, stride = gridDim.x / CG;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) bar_init(full(s), 1), bar_init(empty(s), 1);
-    for (int b = 0; b < 2; ++b) bar_init(acc_full(b), 1), bar_init(acc_empty(b), kEpiWarps);
+    for (int b = 0; b < 2; ++b) bar_init(acc_full(b), 1), bar_init(acc_empty(b), kEpiWarps * CG);
     bar_init(drain, 1);
     abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == kEpiWarps + 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_slot)),
-                 "r"(2 * BN)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
-  }
+  if (warp == kEpiWarps + 1) tmem_alloc<CG>(smem_addr(&tmem_slot), 2 * BN);
   fence_before();
   __syncthreads();
+  if constexpr (CG == 2) cluster_sync();
   fence_after();
   const uint32_t tmem = tmem_slot;
   const int tiles = problem_tiles(p);
@@ -235,32 +301,33 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
       int s = 0, issued = 0;
       uint32_t ph = 1;
       bool ok = true;
-      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-        const Tile x = problem_tile<PL, BN>(p, t);
+      for (int t = first; t < tiles && ok; t += stride) {
+        const Tile x = problem_tile<PL, BN, CG>(p, t, rank);
         for (int kt = x.kt0; kt < x.kt1; ++kt) {
           if (!(ok = bar_wait(empty(s), ph, &abort_flag, p.status))) break;
-          bar_expect(full(s), C::kStage);
+          if (rank == 0) bar_expect(full(s), C::kStage * CG);
+          const uint32_t bar = CG == 1 ? full(s) : leader_addr(full(s));
           const uint32_t at = stages + s * C::kStage;
-          const int ka = p.a_k0 + kt * BK, kb = p.b_k0 + kt * BK, nb = p.b_n0 + x.n0;
+          const int ka = p.a_k0 + kt * BK, kb = p.b_k0 + kt * BK, nb = p.b_n0 + x.n0 + rank * C::kBRows;
           if (p.a_mn) {
 #pragma unroll
             for (int i = 0; i < kBM / 64; ++i)
-              tma_load(at + i * (C::kA / (kBM / 64)), &p.a, full(s), x.m0 + 64 * i, ka, x.batch);
+              tma_load<CG>(at + i * a_block, &p.a, bar, x.m0 + 64 * i, ka, x.batch);
           } else {
-            tma_load(at, &p.a, full(s), ka, x.m0, x.batch);
+            tma_load<CG>(at, &p.a, bar, ka, x.m0, x.batch);
           }
           if (p.b_mn) {
 #pragma unroll
-            for (int i = 0; i < BN / 64; ++i)
-              tma_load(at + C::kA + i * (C::kB / (BN / 64)), &p.b, full(s), nb + 64 * i, kb, x.batch);
+            for (int i = 0; i < C::kBRows / 64; ++i)
+              tma_load<CG>(at + C::kA + i * b_block, &p.b, bar, nb + 64 * i, kb, x.batch);
           } else {
-            tma_load(at + C::kA, &p.b, full(s), kb, nb, x.batch);
+            tma_load<CG>(at + C::kA, &p.b, bar, kb, nb, x.batch);
           }
           if (issued < C::kStages) ++issued;
           if (++s == C::kStages) s = 0, ph ^= 1;
         }
       }
-      if (!ok) {   // the copies in flight land before the CTA ends
+      if (!ok && rank == 0) {   // the copies in flight land before the CTA (or the pair) ends
         for (int i = 0; i < issued; ++i) {
           if (s-- == 0) s = C::kStages - 1, ph ^= 1;
           for (int j = 0; j < kWaitLimit && !bar_try(full(s), ph ^ 1); ++j) {
@@ -269,17 +336,16 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
       }
     }
   } else if (warp == kEpiWarps + 1) {
-    if (lane == 0) {
+    if (lane == 0 && rank == 0) {
       // accumulator float32; operand types; which operands have their own index contiguous
       const uint32_t idesc = 1u << 4 | (p.bf16 ? 1u << 7 | 1u << 10 : 0u) | (p.a_mn ? 1u << 15 : 0u) |
-                             (p.b_mn ? 1u << 16 : 0u) | (uint32_t)(BN >> 3) << 17 | (uint32_t)(kBM >> 4) << 24;
-      constexpr uint32_t a_block = C::kA / (kBM / 64), b_block = C::kB / (BN / 64);
+                             (p.b_mn ? 1u << 16 : 0u) | (uint32_t)(BN >> 3) << 17 | (uint32_t)(kBM * CG >> 4) << 24;
       const uint32_t a_plane = p.a_mn ? a_block / PL : C::kA / PL, b_plane = p.b_mn ? b_block / PL : C::kB / PL;
       int s = 0, buf = 0;
       uint32_t ph = 0, aph = 1;
       bool ok = true;
-      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-        const Tile x = problem_tile<PL, BN>(p, t);
+      for (int t = first; t < tiles && ok; t += stride) {
+        const Tile x = problem_tile<PL, BN, CG>(p, t, 0);
         for (int c0 = x.kt0; c0 < x.kt1 && ok; c0 += p.chunk) {
           if (!(ok = bar_wait(acc_empty(buf), aph, &abort_flag, p.status))) break;
           fence_after();
@@ -297,22 +363,22 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
               const int pa = PL == 1 ? 0 : (q == 0 ? 1 : 0), pb = PL == 1 ? 0 : (q == 1 ? 1 : 0);
 #pragma unroll
               for (int ks = 0; ks < BK / 16; ++ks) {
-                mma(d, operand_desc<BK>(at + pa * a_plane, p.a_mn, a_block, ks),
-                    operand_desc<BK>(bt + pb * b_plane, p.b_mn, b_block, ks), idesc, add);
+                mma<CG>(d, operand_desc<BK>(at + pa * a_plane, p.a_mn, a_block, ks),
+                        operand_desc<BK>(bt + pb * b_plane, p.b_mn, b_block, ks), idesc, add);
                 add = 1;
               }
             }
-            mma_commit(empty(s));
+            mma_commit<CG>(empty(s));
             if (++s == C::kStages) s = 0, ph ^= 1;
           }
           if (!ok) break;
-          mma_commit(acc_full(buf));
+          mma_commit<CG>(acc_full(buf));
           buf ^= 1;
           if (buf == 0) aph ^= 1;
         }
       }
       // every product has finished before tensor memory is given back
-      mma_commit(drain);
+      mma_commit<CG>(drain);
       for (int j = 0; j < kWaitLimit && !bar_try(drain, 0); ++j) {
       }
     }
@@ -323,8 +389,8 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
     int buf = 0;
     uint32_t ph = 0;
     bool ok = true;
-    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-      const Tile x = problem_tile<PL, BN>(p, t);
+    for (int t = first; t < tiles && ok; t += stride) {
+      const Tile x = problem_tile<PL, BN, CG>(p, t, rank);
       float acc[HALF];
 #pragma unroll
       for (int i = 0; i < HALF; ++i) acc[i] = 0.f;
@@ -343,7 +409,13 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
           for (int j = 0; j < 32; ++j) acc[i + j] += v[j];
         }
         fence_before();
-        if (lane == 0) bar_arrive(acc_empty(buf));
+        if (lane == 0) {
+          if constexpr (CG == 1)
+            bar_arrive(acc_empty(buf));
+          else
+            bar_arrive_leader(acc_empty(buf));
+        }
+        __syncwarp();
         buf ^= 1;
         if (buf == 0) ph ^= 1;
       }
@@ -351,9 +423,11 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
     }
   }
   __syncthreads();
+  // a pair ends together: each reads the other's shared memory and signals its barriers
+  if constexpr (CG == 2) cluster_sync();
   if (warp == kEpiWarps + 1) {
     fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * BN));
+    tmem_free<CG>(tmem, 2 * BN);
   }
 }
 
@@ -365,23 +439,37 @@ nc_status make_map(CUtensorMap* map, const void* base, bool bf16, int planes, in
 int sm_count();
 
 // The two operands' maps: `mn` says that the operand's own index (extent `own`) is contiguous.
-template <int PL, int BN>
+template <int PL, int BN, int CG>
 nc_status make_operand(Problem* p, bool is_a, const void* base, bool mn, int own, int k, int64_t pitch, int64_t plane,
                        int batch, int64_t per_batch) {
-  constexpr int BK = Config<PL, BN>::kBK;
+  using C = Config<PL, BN, CG>;
   (is_a ? p->a_mn : p->b_mn) = mn;
-  const int rows = is_a ? kBM : BN;
-  return mn ? make_map(is_a ? &p->a : &p->b, base, p->bf16, PL, own, k, pitch, plane, batch, per_batch, 64, BK)
-            : make_map(is_a ? &p->a : &p->b, base, p->bf16, PL, k, own, pitch, plane, batch, per_batch, BK, rows);
+  const int rows = is_a ? kBM : C::kBRows;
+  return mn ? make_map(is_a ? &p->a : &p->b, base, p->bf16, PL, own, k, pitch, plane, batch, per_batch, 64, C::kBK)
+            : make_map(is_a ? &p->a : &p->b, base, p->bf16, PL, k, own, pitch, plane, batch, per_batch, C::kBK, rows);
 }
 
-template <int PL, int BN, class Epi>
+// Tiles that cover (m, n).
+template <int BN, int CG>
+void set_tiles(Problem* p) {
+  p->tiles_m = (p->m + kBM * CG - 1) / (kBM * CG), p->tiles_n = (p->n + BN - 1) / BN;
+}
+
+template <int PL, int BN, int CG, class Epi>
 nc_status launch_product(const Problem& p, const Epi& epi, cudaStream_t st, const char* what) {
-  auto k = product_kernel<PL, BN, Epi>;
-  NC_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Config<PL, BN>::kSmem));
-  const int tiles = problem_tiles(p), sms = sm_count();
-  PdlLaunch l(dim3(tiles < sms ? tiles : sms), dim3(kThreads), Config<PL, BN>::kSmem, st);
-  NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, k, p, epi));
+  auto k = product_kernel<PL, BN, CG, Epi>;
+  constexpr int smem = Config<PL, BN, CG>::kSmem;
+  NC_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  const int tiles = problem_tiles(p), most = sm_count() / CG;
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = CG, attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 1;
+  cfg.gridDim = dim3((tiles < most ? tiles : most) * CG), cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem, cfg.stream = st, cfg.attrs = attr, cfg.numAttrs = CG == 1 ? 1 : 2;
+  NC_CUDA_CHECK(cudaLaunchKernelEx(&cfg, k, p, epi));
   return launch_check(what);
 }
 
