@@ -348,7 +348,11 @@ struct NsEpilogue {
   bool wide;         // rows of out or params start on 32 bytes
 
   template <int HALF>
-  __device__ __forceinline__ void run(const tc::Tile& x, int row, int col, float (&acc)[HALF]) const {
+  __device__ __forceinline__ int begin(const tc::Tile&, int, int, float*) const {
+    return 0;
+  }
+  template <int HALF>
+  __device__ __forceinline__ void run(int, const tc::Tile& x, int row, int col, float (&acc)[HALF]) const {
     if (row >= m) return;
     const size_t base = (size_t)x.batch * 2 * src.plane + (size_t)row * src.pitch;
     const bool mirror = (MODE == kGram || MODE == kPoly) && x.n0 > x.m0;
@@ -408,12 +412,7 @@ struct NsEpilogue {
       } else {
         uint32_t h[8], l[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          uint16_t h0, l0, h1, l1;
-          tc::split_f16(v[2 * i], &h0, &l0);
-          tc::split_f16(v[2 * i + 1], &h1, &l1);
-          h[i] = h0 | (uint32_t)h1 << 16, l[i] = l0 | (uint32_t)l1 << 16;
-        }
+        for (int i = 0; i < 8; ++i) tc::split_f16x2(v[2 * i], v[2 * i + 1], &h[i], &l[i]);
         __half* d = dst.p + base + col + j;
         tc::store_v8(d, h);
         tc::store_v8(d + dst.plane, l);

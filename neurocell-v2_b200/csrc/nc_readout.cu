@@ -474,9 +474,8 @@ nc_status value(const nc_linear_ce* d, const CeArgs& a, bool grad, float* loss, 
   const CeLayout L = ce_layout(d, grad);
   const bool none = d->reduction == NC_REDUCE_NONE;
   float* row_loss = none ? loss : reinterpret_cast<float*>(ws + L.row_loss);
-  if (on_tensor_cores(d)) {
-    NC_CHECK(ce_tc_value(d, a, grad, lse, row_loss, ws + L.tc, st));
-  } else {
+  if (on_tensor_cores(d)) return ce_tc_value(d, a, grad, lse, row_loss, none ? nullptr : loss, ws + L.tc, st);
+  {
     const RowsPlan r = rows_plan(d, vec_of(d, a.features, a.weight, nullptr));
     float2* part = reinterpret_cast<float2*>(ws + L.part);
     float* zlabel = reinterpret_cast<float*>(ws + L.zlabel);
@@ -562,7 +561,7 @@ nc_status nc_linear_ce_forward(const nc_linear_ce* desc, const void* features, c
   NC_CHECK(check_ws(d_ws, ws_bytes, ce_layout(desc, false).total));
   char* ws = static_cast<char*>(d_ws);
   const CeArgs a = make_args(desc, features, weight, bias, labels);
-  if (on_tensor_cores(desc)) NC_CHECK(ce_tc_prepare(desc, a, false, ws + ce_layout(desc, false).tc, st));
+  if (on_tensor_cores(desc)) NC_CHECK(ce_tc_prepare(desc, a, false, nullptr, ws + ce_layout(desc, false).tc, st));
   NC_CHECK(value(desc, a, false, loss, lse, ws, st));
   clear_error();
   return NC_OK;
@@ -581,7 +580,7 @@ nc_status nc_linear_ce_backward(const nc_linear_ce* desc, const void* features, 
   NC_CHECK(check_ws(d_ws, ws_bytes, ce_layout(desc, true).total));
   char* ws = static_cast<char*>(d_ws);
   const CeArgs a = make_args(desc, features, weight, bias, labels);
-  if (on_tensor_cores(desc)) NC_CHECK(ce_tc_prepare(desc, a, true, ws + ce_layout(desc, true).tc, st));
+  if (on_tensor_cores(desc)) NC_CHECK(ce_tc_prepare(desc, a, true, g_loss, ws + ce_layout(desc, true).tc, st));
   const CeGrads g{lse, g_loss, g_features, g_weight, g_bias};
   NC_CHECK(gradients(desc, a, g, ws, st));
   clear_error();
@@ -601,7 +600,7 @@ nc_status nc_linear_ce_value_and_grad(const nc_linear_ce* desc, const void* feat
   NC_CHECK(check_ws(d_ws, ws_bytes, ce_layout(desc, true).total));
   char* ws = static_cast<char*>(d_ws);
   const CeArgs a = make_args(desc, features, weight, bias, labels);
-  if (on_tensor_cores(desc)) NC_CHECK(ce_tc_prepare(desc, a, true, ws + ce_layout(desc, true).tc, st));
+  if (on_tensor_cores(desc)) NC_CHECK(ce_tc_prepare(desc, a, true, nullptr, ws + ce_layout(desc, true).tc, st));
   NC_CHECK(value(desc, a, true, loss, lse, ws, st));
   const CeGrads g{lse, nullptr, g_features, g_weight, g_bias};
   NC_CHECK(gradients(desc, a, g, ws, st));

@@ -34,10 +34,12 @@ struct CeGrads {
 
 // The tensor-core path (nc_readout_tc.cu).  `ws` bytes from ce_tc_bytes; prepare() first.
 size_t ce_tc_bytes(const nc_linear_ce* d, bool grad);
-nc_status ce_tc_prepare(const nc_linear_ce* d, const CeArgs& a, bool grad, char* ws, cudaStream_t st);
-// lse and row losses (rows); reduced by the caller.
-nc_status ce_tc_value(const nc_linear_ce* d, const CeArgs& a, bool grad, float* lse, float* row_loss, char* ws,
-                      cudaStream_t st);
+// `grad`: the workspace is one of a gradient.  g_loss: the loss's own gradient, or null for 1.
+nc_status ce_tc_prepare(const nc_linear_ce* d, const CeArgs& a, bool grad, const float* g_loss, char* ws,
+                        cudaStream_t st);
+// lse and row losses (rows), and their sum or mean into `loss` unless that is null.
+nc_status ce_tc_value(const nc_linear_ce* d, const CeArgs& a, bool grad, float* lse, float* row_loss, float* loss,
+                      char* ws, cudaStream_t st);
 nc_status ce_tc_grad(const nc_linear_ce* d, const CeArgs& a, const CeGrads& g, char* ws, cudaStream_t st);
 
 inline size_t pad256(size_t n) { return (n + 255) / 256 * 256; }

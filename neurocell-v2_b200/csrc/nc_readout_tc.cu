@@ -33,10 +33,12 @@ constexpr size_t kPieceBytes = 56u << 20;   // dz of one piece: it shares the 12
 struct Scales {
   float w, w_inv, f, f_inv;   // 2^e and 2^-e of weight and features
   float g;                    // max |g_n|
+  int kept;                   // rows that take part
+  int blocks_done;            // of the value's last kernel
 };
 
 struct Plan {
-  bool bf16, copy_w;
+  bool grad, bf16, copy_w;
   int pitch;                  // of the planes of features and weight
   int rows_pad;               // rows, whole 256s
   int classes_pad;            // classes, whole 256s
@@ -51,6 +53,7 @@ struct Plan {
 
 Plan make_plan(const nc_linear_ce* d, bool grad) {
   Plan p{};
+  p.grad = grad;
   p.bf16 = d->dtype == NC_BF16;
   p.copy_w = !p.bf16 || d->dim % 8 != 0;   // else the weight is read where it is
   p.pitch = (d->dim + 7) / 8 * 8;
@@ -178,17 +181,48 @@ __device__ __forceinline__ void put8(const T* src, int left, bool wide, float sc
         make_uint4(l[0] | l[1] << 16, l[2] | l[3] << 16, l[4] | l[5] << 16, l[6] | l[7] << 16);
 }
 
-// Features, bias and (copy_w) weight in the products' form.  Rows that take no part become
+// By one block: how many rows take part, f_n = g_n / max |g| of every row (0 where it takes
+// no part) and max |g|.
+__device__ void row_factors(const CeArgs& a, const float* g_loss, float* fac, Scales* scales) {
+  __shared__ float red[kPrepThreads / 32];
+  const int n = count_kept(a);
+  if (threadIdx.x == 0) scales->kept = n;
+  if (!fac) return;
+  const bool each = a.reduction == NC_REDUCE_NONE && g_loss;
+  const float all = (g_loss && !each ? g_loss[0] : 1.f) / (a.reduction == NC_REDUCE_MEAN ? (float)max(n, 1) : 1.f);
+  float m = fabsf(all);
+  if (each) {
+    m = 0.f;
+    for (int i = threadIdx.x; i < a.rows; i += kPrepThreads)
+      if (ce_kept(a, i)) m = fmaxf(m, fabsf(g_loss[i]));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
+    __syncthreads();
+    for (int i = 0; i < kPrepThreads / 32; ++i) m = fmaxf(m, red[i]);
+  }
+  for (int i = threadIdx.x; i < a.rows; i += kPrepThreads)
+    fac[i] = !ce_kept(a, i) || m == 0.f ? 0.f : (each ? g_loss[i] : all) / m;
+  if (threadIdx.x == 0) scales->g = m;
+}
+
+// Features, bias and (copy_w) weight in the products' form; the last block the row factors.  Rows that take no part become
 // zeros; the bias of the classes past the end is -inf.
 template <typename T>
 __global__ void __launch_bounds__(kPrepThreads) ce_planes_kernel(CeArgs a, int copy_w, int pitch, int classes_pad,
                                                                  int wide_w, int wide_f,
                                                                  const float* __restrict__ max_part, Scales* scales,
                                                                  int32_t* status, uint16_t* __restrict__ w,
-                                                                 uint16_t* __restrict__ f, float* __restrict__ bias) {
+                                                                 uint16_t* __restrict__ f, float* __restrict__ bias,
+                                                                 const float* __restrict__ g_loss,
+                                                                 float* __restrict__ fac) {
   constexpr bool bf16 = sizeof(T) == 2;
   __shared__ float red[2][kPrepThreads / 32];
   pdl_enter();
+  if (blockIdx.x == gridDim.x - 1) {
+    row_factors(a, g_loss, fac, scales);
+    return;
+  }
   float sw = 1.f, sf = 1.f;
   if constexpr (!bf16) {
     float m[2] = {0.f, 0.f};
@@ -207,9 +241,10 @@ __global__ void __launch_bounds__(kPrepThreads) ce_planes_kernel(CeArgs a, int c
   }
   if (blockIdx.x == 0 && threadIdx.x == 0) {
     scales->w = sw, scales->f = sf, scales->w_inv = 1.f / sw, scales->f_inv = 1.f / sf;
+    scales->blocks_done = 0;
     *status = 0;
   }
-  const int64_t step = (int64_t)gridDim.x * kPrepThreads, i0 = (int64_t)blockIdx.x * kPrepThreads + threadIdx.x;
+  const int64_t step = (int64_t)(gridDim.x - 1) * kPrepThreads, i0 = (int64_t)blockIdx.x * kPrepThreads + threadIdx.x;
   const int per = pitch / 8;
   const int64_t nf = (int64_t)a.rows * per, nw = copy_w ? (int64_t)a.classes * per : 0;
   for (int64_t i = i0; i < nf; i += step) {
@@ -230,6 +265,30 @@ __global__ void __launch_bounds__(kPrepThreads) ce_planes_kernel(CeArgs a, int c
 
 // ---- value ---------------------------------------------------------------------------------
 
+// 2^t, and e^d.  The hardware's 2^t is good to 2 ulp; exp_near() adds what rounding d log2(e)
+// lost, so that large |d| keep float32's precision.  d is at least -200 (e^d is 0 there).
+__device__ __forceinline__ float exp2_fast(float t) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(t));
+  return r;
+}
+constexpr float kLog2e = 1.4426950408889634f, kLog2eLow = (float)(1.4426950408889634 - (double)1.4426950408889634f);
+__device__ __forceinline__ float exp_fast(float d) { return exp2_fast(d * kLog2e); }
+__device__ __forceinline__ float exp_near(float d) {
+  const float t = d * kLog2e, r = fmaf(d, kLog2eLow, fmaf(d, kLog2e, -t)), e = exp2_fast(t);
+  return fmaf(e, r * 0.69314718f, e);
+}
+
+// The tile's bias into the warp's scratch.
+template <int HALF>
+__device__ __forceinline__ void stage_bias(const float* bias, float* scratch) {
+  const int lane = threadIdx.x & 31;
+  if constexpr (HALF == 128)
+    reinterpret_cast<float4*>(scratch)[lane] = reinterpret_cast<const float4*>(bias)[lane];
+  else
+    reinterpret_cast<float2*>(scratch)[lane] = reinterpret_cast<const float2*>(bias)[lane];
+}
+
 struct ValueEpilogue {
   CeArgs a;
   const Scales* scales;
@@ -238,74 +297,89 @@ struct ValueEpilogue {
   float* zlabel;
   int rows_pad;
 
+  struct State {
+    float sw, sf;
+    int label;            // within the half tile, or out of it
+    const float* bias;
+  };
   template <int HALF>
-  __device__ __forceinline__ void run(const tc::Tile&, int row, int col, float (&z)[HALF]) const {
-    const float sw = scales->w_inv, sf = scales->f_inv;
-    const int label = row < a.rows ? a.labels[row] - col : -1;
-    float m = -INFINITY, zl = 0.f;
+  __device__ __forceinline__ State begin(const tc::Tile&, int row, int col, float* scratch) const {
+    stage_bias<HALF>(bias + col, scratch);
+    return State{scales->w_inv, scales->f_inv, row < a.rows ? a.labels[row] - col : -1, scratch};
+  }
+  template <int HALF>
+  __device__ __forceinline__ void run(const State& st, const tc::Tile&, int row, int col, float (&z)[HALF]) const {
+    float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < HALF; j += 4) {
-      const float4 b = *reinterpret_cast<const float4*>(bias + col + j);
-      z[j] = z[j] * sw * sf + b.x, z[j + 1] = z[j + 1] * sw * sf + b.y;
-      z[j + 2] = z[j + 2] * sw * sf + b.z, z[j + 3] = z[j + 3] * sw * sf + b.w;
+      const float4 q = *reinterpret_cast<const float4*>(st.bias + j);
+      const float b[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        m = fmaxf(m, z[j + e]);
-        if (j + e == label) zl = z[j + e];
+        z[j + e] = fmaf(z[j + e] * st.sw, st.sf, b[e]);
+        m[e] = fmaxf(m[e], z[j + e]);
       }
     }
-    float s = 0.f;
+    const float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), base = top == -INFINITY ? 0.f : top;
+    const bool mine = st.label >= 0 && st.label < HALF;
+    float zl = 0.f;
+    if (__any_sync(0xffffffffu, mine)) {
 #pragma unroll
-    for (int j = 0; j < HALF; ++j) s += z[j] == -INFINITY ? 0.f : __expf(z[j] - m);
+      for (int j = 0; j < HALF; ++j)
+        if (j == st.label) zl = z[j];
+    }
+#pragma unroll
+    for (int j = 0; j < HALF; ++j) s[j & 3] += exp_fast(z[j] - base);
     if (row >= a.rows) return;
-    part[(size_t)(col / HALF) * rows_pad + row] = make_float2(m, s);
-    if (label >= 0 && label < HALF) zlabel[row] = zl;
+    part[(size_t)(col / HALF) * rows_pad + row] = make_float2(top, (s[0] + s[1]) + (s[2] + s[3]));
+    if (mine) zlabel[row] = zl;
   }
 };
 
-// 32 rows per block, a lane each; the warps split the slots and meet in shared memory.
-__global__ void __launch_bounds__(256) ce_finish_kernel(CeArgs a, int slots, int rows_pad,
-                                                        const float2* __restrict__ part,
-                                                        const float* __restrict__ zlabel, float* __restrict__ lse,
-                                                        float* __restrict__ row_loss) {
-  __shared__ float2 sm[8][32];
+// 32 rows per block, a lane each; the warps split the slots and meet in shared memory.  The
+// last block to finish adds up the row losses (in order, whichever block that is), except
+// with NC_REDUCE_NONE.
+__global__ void __launch_bounds__(1024) ce_finish_kernel(CeArgs a, int slots, int rows_pad,
+                                                         const float2* __restrict__ part,
+                                                         const float* __restrict__ zlabel, Scales* scales,
+                                                         float* __restrict__ lse, float* __restrict__ row_loss,
+                                                         float* __restrict__ loss) {
+  __shared__ float2 sm[32][32];
+  __shared__ double red[32];
+  __shared__ bool last;
   pdl_enter();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.x * 32 + lane;
   float2 x = make_float2(-INFINITY, 0.f);
 #pragma unroll 4
-  for (int s = warp; s < slots; s += 8) x = lse_merge(x, part[(size_t)s * rows_pad + row]);
+  for (int s = warp; s < slots; s += 32) x = lse_merge(x, part[(size_t)s * rows_pad + row]);
   sm[warp][lane] = x;
   __syncthreads();
-  if (warp != 0 || row >= a.rows) return;
-  for (int k = 1; k < 8; ++k) x = lse_merge(x, sm[k][lane]);
-  finish_row(a, row, x, zlabel, lse, row_loss);
+  x = sm[lane][warp];   // a warp per row now
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    x = lse_merge(x, make_float2(__shfl_xor_sync(0xffffffffu, x.x, o), __shfl_xor_sync(0xffffffffu, x.y, o)));
+  if (lane == 0 && blockIdx.x * 32 + warp < a.rows) finish_row(a, blockIdx.x * 32 + warp, x, zlabel, lse, row_loss);
+  if (!loss) return;
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) last = atomicAdd(&scales->blocks_done, 1) == (int)gridDim.x - 1;
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  double s = 0.0;
+  for (int i = threadIdx.x; i < a.rows; i += 1024) s += *((volatile const float*)row_loss + i);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if (lane == 0) red[warp] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double t = 0.0;
+    for (int i = 0; i < 32; ++i) t += red[i];
+    loss[0] = (float)(a.reduction == NC_REDUCE_MEAN ? t / (double)max(scales->kept, 1) : t);
+  }
 }
 
 // ---- gradient ------------------------------------------------------------------------------
-
-// One block: f_n = g_n / max |g| of every row (0 where the row takes no part) and max |g|.
-__global__ void __launch_bounds__(1024) ce_factors_kernel(CeArgs a, const float* __restrict__ g_loss,
-                                                          float* __restrict__ fac, Scales* __restrict__ scales) {
-  __shared__ float red[32];
-  pdl_enter();
-  const int n = count_kept(a);
-  const bool each = a.reduction == NC_REDUCE_NONE && g_loss;
-  const float all = (g_loss && !each ? g_loss[0] : 1.f) / (a.reduction == NC_REDUCE_MEAN ? (float)max(n, 1) : 1.f);
-  float m = fabsf(all);
-  if (each) {
-    m = 0.f;
-    for (int i = threadIdx.x; i < a.rows; i += blockDim.x)
-      if (ce_kept(a, i)) m = fmaxf(m, fabsf(g_loss[i]));
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
-    __syncthreads();
-    for (int i = 0; i < 32; ++i) m = fmaxf(m, red[i]);
-  }
-  for (int i = threadIdx.x; i < a.rows; i += blockDim.x)
-    fac[i] = !ce_kept(a, i) || m == 0.f ? 0.f : (each ? g_loss[i] : all) / m;
-  if (threadIdx.x == 0) scales->g = m;
-}
 
 template <bool BF16>
 struct DzEpilogue {
@@ -318,23 +392,40 @@ struct DzEpilogue {
   float* db_part;      // (rows_pad / 32, classes_pad) or null
   int v0, piece, classes_pad;
 
+  struct State {
+    float sw, sf, f, lse;
+    int label;
+    const float* bias;
+  };
   template <int HALF>
-  __device__ __forceinline__ void run(const tc::Tile&, int row, int col, float (&z)[HALF]) const {
+  __device__ __forceinline__ State begin(const tc::Tile&, int row, int col, float* scratch) const {
+    stage_bias<HALF>(bias + v0 + col, scratch);
     const bool in = row < a.rows;
-    const float sw = scales->w_inv, sf = scales->f_inv;
-    const float f = in ? fac[row] : 0.f, l = in ? lse[row] : 0.f;
-    const int label = in ? a.labels[row] - v0 - col : -1;
+    float f = in ? fac[row] : 0.f, l = in ? lse[row] : 0.f;
+    if (f == 0.f)
+      l = INFINITY;          // p = 0
+    else if (!(l > -INFINITY))
+      f = NAN, l = 0.f;      // a bad label, no class left, or NaN among the logits
+    return State{scales->w_inv, scales->f_inv, f, l, in ? a.labels[row] - v0 - col : -1, scratch};
+  }
+  template <int HALF>
+  __device__ __forceinline__ void run(const State& st, const tc::Tile&, int row, int col, float (&z)[HALF]) const {
 #pragma unroll
     for (int j = 0; j < HALF; j += 4) {
-      const float4 q = *reinterpret_cast<const float4*>(bias + v0 + col + j);
+      const float4 q = *reinterpret_cast<const float4*>(st.bias + j);
       const float b[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float p = expf(z[j + e] * sw * sf + b[e] - l) - (j + e == label ? 1.f : 0.f);
-        z[j + e] = f == 0.f ? 0.f : f * p;
+        const float d = fmaxf(fmaf(z[j + e] * st.sw, st.sf, b[e]) - st.lse, -200.f);
+        z[j + e] = st.f * (BF16 ? exp_fast(d) : exp_near(d));
       }
     }
-    if (in) {
+    if (__any_sync(0xffffffffu, st.label >= 0 && st.label < HALF)) {
+#pragma unroll
+      for (int j = 0; j < HALF; ++j)
+        if (j == st.label) z[j] -= st.f;
+    }
+    if (row < a.rows) {
       uint16_t* out = dz + (size_t)row * piece + col;
 #pragma unroll
       for (int j = 0; j < HALF; j += 16) {
@@ -346,10 +437,7 @@ struct DzEpilogue {
             const __nv_bfloat162 b = __floats2bfloat162_rn(x, y);
             h[i] = *reinterpret_cast<const uint32_t*>(&b);
           } else {
-            uint16_t h0, l0, h1, l1;
-            tc::split_f16(x * kDzScale, &h0, &l0);
-            tc::split_f16(y * kDzScale, &h1, &l1);
-            h[i] = h0 | (uint32_t)h1 << 16, lo[i] = l0 | (uint32_t)l1 << 16;
+            tc::split_f16x2(x * kDzScale, y * kDzScale, &h[i], &lo[i]);
           }
         }
         tc::store_v8(out + j, h);
@@ -375,9 +463,13 @@ struct WeightEpilogue {
   int classes, dim;
   bool wide;       // rows on 32 bytes
   template <int HALF>
-  __device__ __forceinline__ void run(const tc::Tile&, int row, int col, float (&v)[HALF]) const {
+  __device__ __forceinline__ float2 begin(const tc::Tile&, int, int, float*) const {
+    return make_float2(scales->f_inv * (sizeof(T) == 4 ? 1.f / kDzScale : 1.f), scales->g);
+  }
+  template <int HALF>
+  __device__ __forceinline__ void run(float2 st, const tc::Tile&, int row, int col, float (&v)[HALF]) const {
     if (row >= classes) return;
-    const float s = scales->f_inv * (sizeof(T) == 4 ? 1.f / kDzScale : 1.f), g = scales->g;
+    const float s = st.x, g = st.y;
     T* o = out + (size_t)row * dim + col;
 #pragma unroll
     for (int j = 0; j < HALF; j += 16) {
@@ -415,9 +507,12 @@ struct FeatureEpilogue {
   int rows, dim, pitch, first;
   float mul;
   template <int HALF>
-  __device__ __forceinline__ void run(const tc::Tile& x, int row, int col, float (&v)[HALF]) const {
+  __device__ __forceinline__ float begin(const tc::Tile&, int, int, float*) const {
+    return scales->w_inv * mul;
+  }
+  template <int HALF>
+  __device__ __forceinline__ void run(float s, const tc::Tile& x, int row, int col, float (&v)[HALF]) const {
     if (row >= rows) return;
-    const float s = scales->w_inv * mul;
     float* o = part + ((size_t)x.split * rows + row) * pitch + col;
 #pragma unroll
     for (int j = 0; j < HALF; j += 8) {
@@ -509,7 +604,7 @@ struct Call {
                                     (int64_t)PL * d->rows * p.piece);
   }
 
-  nc_status prepare() const {
+  nc_status prepare(const float* g_loss) const {
     if (PL == 2) {
       PdlLaunch l(dim3(2 * kMaxBlocks), dim3(kPrepThreads), 0, st);
       NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, ce_max_kernel, a, at<float>(p.max_part)));
@@ -518,12 +613,13 @@ struct Call {
     const int64_t items = ((int64_t)d->rows + (p.copy_w ? d->classes : 0)) * (p.pitch / 8);
     int64_t blocks = (items + kPrepThreads - 1) / kPrepThreads;
     if (blocks > 148 * 16) blocks = 148 * 16;
-    PdlLaunch l(dim3((unsigned)blocks), dim3(kPrepThreads), 0, st);
+    PdlLaunch l(dim3((unsigned)blocks + 1), dim3(kPrepThreads), 0, st);
     const int even = d->dim % 8 == 0;
     NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, ce_planes_kernel<T>, a, (int)p.copy_w, p.pitch, p.classes_pad,
                                      (int)(even && aligned16(a.weight)), (int)(even && aligned16(a.features)),
                                      (const float*)at<float>(p.max_part), scales(), status(), at<uint16_t>(p.w),
-                                     at<uint16_t>(p.f), at<float>(p.bias)));
+                                     at<uint16_t>(p.f), at<float>(p.bias), g_loss,
+                                     p.grad ? at<float>(p.fac) : nullptr));
     return launch_check("ce_planes_kernel launch");
   }
 
@@ -536,12 +632,12 @@ struct Call {
     return tc::launch_product<PL, BN, CG>(q, e, st, "readout value product launch");
   }
 
-  nc_status value(float* lse, float* row_loss) const {
+  nc_status value(float* lse, float* row_loss, float* loss) const {
     NC_CHECK(p.pair ? (value_product<256, 2>()) : (value_product<128, 1>()));
-    PdlLaunch l(dim3((d->rows + 31) / 32), dim3(256), 0, st);
+    PdlLaunch l(dim3((d->rows + 31) / 32), dim3(1024), 0, st);
     NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, ce_finish_kernel, a, p.slots, p.rows_pad,
-                                     (const float2*)at<float2>(p.part), (const float*)at<float>(p.zlabel), lse,
-                                     row_loss));
+                                     (const float2*)at<float2>(p.part), (const float*)at<float>(p.zlabel), scales(),
+                                     lse, row_loss, loss));
     return launch_check("ce_finish_kernel launch");
   }
 
@@ -579,11 +675,6 @@ struct Call {
   }
 
   nc_status gradients(const CeGrads& g) const {
-    {
-      PdlLaunch l(dim3(1), dim3(1024), 0, st);
-      NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, ce_factors_kernel, a, g.g_loss, at<float>(p.fac), scales()));
-      NC_CHECK(launch_check("ce_factors_kernel launch"));
-    }
     for (int k = 0; k < p.pieces; ++k) {
       const int v0 = k * p.piece;
       // the last piece may be shorter; `width` is whole tiles
@@ -621,15 +712,16 @@ size_t ce_tc_bytes(const nc_linear_ce* d, bool grad) { return make_plan(d, grad)
   const Plan plan = make_plan(d, GRAD);                                                              \
   return plan.bf16 ? Call<__nv_bfloat16>{d, a, plan, ws, st}.WHAT : Call<float>{d, a, plan, ws, st}.WHAT
 
-nc_status ce_tc_prepare(const nc_linear_ce* d, const CeArgs& a, bool grad, char* ws, cudaStream_t st) {
+nc_status ce_tc_prepare(const nc_linear_ce* d, const CeArgs& a, bool grad, const float* g_loss, char* ws,
+                        cudaStream_t st) {
   if (!make_plan(d, grad).copy_w && !aligned16(a.weight))
     return set_error(NC_ERR_INVALID, "a bfloat16 weight must start on a 16-byte boundary for more than 32 rows");
-  NC_TC_CALL(grad, prepare());
+  NC_TC_CALL(grad, prepare(g_loss));
 }
 
-nc_status ce_tc_value(const nc_linear_ce* d, const CeArgs& a, bool grad, float* lse, float* row_loss, char* ws,
-                      cudaStream_t st) {
-  NC_TC_CALL(grad, value(lse, row_loss));
+nc_status ce_tc_value(const nc_linear_ce* d, const CeArgs& a, bool grad, float* lse, float* row_loss, float* loss,
+                      char* ws, cudaStream_t st) {
+  NC_TC_CALL(grad, value(lse, row_loss, loss));
 }
 
 nc_status ce_tc_grad(const nc_linear_ce* d, const CeArgs& a, const CeGrads& g, char* ws, cudaStream_t st) {

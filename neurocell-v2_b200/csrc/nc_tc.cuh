@@ -244,6 +244,14 @@ __device__ __forceinline__ void split_f16(float x, uint16_t* hi, uint16_t* lo) {
   *hi = __half_as_ushort(h), *lo = __half_as_ushort(l);
 }
 
+// Two of them, packed.
+__device__ __forceinline__ void split_f16x2(float x, float y, uint32_t* hi, uint32_t* lo) {
+  const __half2 h = __floats2half2_rn(x, y);
+  const float2 b = __half22float2(h);
+  const __half2 l = __floats2half2_rn(x - b.x, y - b.y);
+  *hi = *reinterpret_cast<const uint32_t*>(&h), *lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+
 // 32-byte global accesses (one full sector per thread).
 __device__ __forceinline__ void store_v8(void* p, const uint32_t (&v)[8]) {
   asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
@@ -259,7 +267,8 @@ __device__ __forceinline__ void load_v8(const void* p, uint32_t (&v)[8]) {
 
 // The kernel: warps 0..7 epilogue, warp 8 loads, warp 9 multiplies (in the first CTA of a
 // pair); persistent over tiles.  Epi::run(tile, row, col, acc) gets a row's BN / 2
-// consecutive columns as float32 sums.
+// consecutive columns as float32 sums; Epi::begin(tile, row, col, scratch) runs before the
+// wait for them and returns what run() takes along (scratch: BN / 2 floats of the warp).
 template <int PL, int BN, int CG, class Epi>
 __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_constant__ Problem p, const Epi epi) {
   using C = Config<PL, BN, CG>;
@@ -267,6 +276,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
   constexpr uint32_t a_block = C::kA / (kBM / 64), b_block = C::kB / (C::kBRows / 64);
   extern __shared__ uint8_t raw[];
   __shared__ __align__(8) uint64_t bars[2 * C::kStages + 5];
+  __shared__ __align__(16) float scratch[kEpiWarps][HALF];
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag;
   const uint32_t stages = (smem_addr(raw) + 1023) & ~1023u;
@@ -391,6 +401,10 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
     bool ok = true;
     for (int t = first; t < tiles && ok; t += stride) {
       const Tile x = problem_tile<PL, BN, CG>(p, t, rank);
+      const int row = x.m0 + 32 * quarter + lane, col = x.n0 + half * HALF;
+      __syncwarp();   // the last tile's readers of scratch are done
+      const auto state = epi.template begin<HALF>(x, row, col, scratch[warp]);
+      __syncwarp();
       float acc[HALF];
 #pragma unroll
       for (int i = 0; i < HALF; ++i) acc[i] = 0.f;
@@ -406,7 +420,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
           float v[32];
           tmem_load(lanes + buf * BN + i, v);
 #pragma unroll
-          for (int j = 0; j < 32; ++j) acc[i + j] += v[j];
+          for (int j = 0; j < 32; ++j) acc[i + j] = PL == 1 ? v[j] : acc[i + j] + v[j];   // one plane, one chunk
         }
         fence_before();
         if (lane == 0) {
@@ -419,7 +433,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
         buf ^= 1;
         if (buf == 0) ph ^= 1;
       }
-      if (ok) epi.template run<HALF>(x, x.m0 + 32 * quarter + lane, x.n0 + half * HALF, acc);
+      if (ok) epi.template run<HALF>(state, x, row, col, acc);
     }
   }
   __syncthreads();
