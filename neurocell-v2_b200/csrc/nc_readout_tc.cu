@@ -26,8 +26,9 @@ namespace {
 constexpr int kPrepThreads = 256;
 constexpr int kMaxBlocks = 296;        // blocks of the largest-value pass, per tensor
 constexpr float kDzScale = 32768.f;    // dz planes hold dz 2^15 (|dz| <= 1)
-constexpr int kChunk = 2;              // k-tiles (of 32) per accumulator beside float32 operands
-constexpr size_t kPieceBytes = 56u << 20;   // dz of one piece: it shares the 126 MB L2 with what it multiplies
+constexpr int kChunk = 6;              // k-tiles (of 32) per accumulator beside float32 operands
+constexpr size_t kPieceBytes = 160u << 20;  // most that dz of one piece takes
+constexpr int kMaxSplits = 16;
 
 // Device scalars of a call.
 struct Scales {
@@ -51,6 +52,38 @@ struct Plan {
   size_t scales, max_part, w, f, bias, part, zlabel, fac, dz, df_part, db_part, total;
 };
 
+// Pieces and splits by a count of k-tiles on the busiest SM (or pair): a product takes
+// ceil(tiles / SMs) times its k-tiles, so a piece is good where its tiles fill whole rounds.
+// 2048 x 512 x 32768 in float32: five pieces of 26 tiles of 256 classes, which fit L2, leave a
+// third of the pairs idle in dw and take 949 us; see DESIGN for what the choice here takes.
+void choose_pieces(const nc_linear_ce* d, int planes, Plan* p) {
+  auto ceil_div = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
+  const int sms = 148, bk = planes == 1 ? 64 : 32;
+  const int tiles = p->classes_pad / 256;
+  const size_t tile_bytes = (size_t)p->rows_pad * 256 * 2 * planes;
+  int64_t most = (int64_t)(kPieceBytes / tile_bytes);
+  if (most < 1) most = 1;
+  const int64_t fewest = ceil_div(tiles, most);
+  // products: tiles per 256 classes, and how many run at a time
+  const int64_t dz_tiles = p->pair ? ceil_div(d->rows, 256) : ceil_div(d->rows, 128) * 2, dz_at = p->pair ? sms / 2 : sms;
+  const int64_t w_tiles = p->pair_w ? ceil_div(d->dim, 256) : ceil_div(d->dim, 128) * 2, w_at = p->pair_w ? sms / 2 : sms;
+  const int f_side = p->pair_f ? 256 : 128;
+  const int64_t f_tiles = ceil_div(d->rows, f_side) * ceil_div(d->dim, f_side), f_at = p->pair_f ? sms / 2 : sms;
+  const int64_t launch = 12;   // k-tiles that a launch's start and end are worth
+  int64_t best = INT64_MAX;
+  for (int64_t pieces = fewest; pieces < fewest + 4 && pieces <= tiles; ++pieces) {
+    const int64_t t = ceil_div(tiles, pieces);
+    const int64_t one = ceil_div(t * dz_tiles, dz_at) * ceil_div(d->dim, bk) + ceil_div(t * w_tiles, w_at) * ceil_div(d->rows, bk) +
+                        3 * launch;
+    for (int splits = 1; splits <= kMaxSplits && splits <= t; ++splits) {
+      // each split adds a pass over df's parts: about 4 k-tiles
+      const int64_t all = (one + ceil_div(f_tiles * splits, f_at) * ceil_div(t * (256 / bk), splits)) * ceil_div(tiles, t) + 4 * splits;
+      if (all < best) best = all, p->piece = (int)t * 256, p->splits = splits;
+    }
+  }
+  p->pieces = (int)ceil_div(tiles, p->piece / 256);
+}
+
 Plan make_plan(const nc_linear_ce* d, bool grad) {
   Plan p{};
   p.grad = grad;
@@ -65,18 +98,7 @@ Plan make_plan(const nc_linear_ce* d, bool grad) {
   const int tile = p.pair ? 256 : 128;
   p.slots = (d->classes + tile - 1) / tile * 2;
   const int planes = p.bf16 ? 1 : 2;
-  const int tiles = p.classes_pad / 256;
-  const size_t tile_bytes = (size_t)p.rows_pad * 256 * 2 * planes;
-  int most = (int)(kPieceBytes / tile_bytes);
-  if (most < 1) most = 1;
-  p.pieces = (tiles + most - 1) / most;
-  p.piece = (tiles + p.pieces - 1) / p.pieces * 256;
-  p.pieces = (p.classes_pad + p.piece - 1) / p.piece;   // none is empty
-  const int out = p.pair_f ? 256 : 128;
-  const int out_tiles = (d->rows + out - 1) / out * ((d->dim + out - 1) / out);
-  int splits = (p.pair_f ? 74 : 148) / out_tiles;
-  if (splits > p.piece / 256) splits = p.piece / 256;
-  p.splits = splits < 1 ? 1 : splits;
+  choose_pieces(d, planes, &p);
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t o = at;
