@@ -433,8 +433,8 @@ struct NsEpilogue {
 
 int norm_blocks(int64_t n) { return (int)((n + kNormThreads * kNormPer - 1) / (kNormThreads * kNormPer)); }
 
-// k-tiles (of 32) that one accumulator takes before it is added to the registers.
-constexpr int kNsChunk = 2;
+// k-tiles (of 64) that one accumulator takes before it is added to the registers.
+constexpr int kNsChunk = 1;
 constexpr int kNsTile = 128;
 
 // Short sides up to 64 whose slices fit take one cluster per matrix, the others the tensor

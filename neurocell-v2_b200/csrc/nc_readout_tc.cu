@@ -26,7 +26,7 @@ namespace {
 constexpr int kPrepThreads = 256;
 constexpr int kMaxBlocks = 296;        // blocks of the largest-value pass, per tensor
 constexpr float kDzScale = 32768.f;    // dz planes hold dz 2^15 (|dz| <= 1)
-constexpr int kChunk = 6;              // k-tiles (of 32) per accumulator beside float32 operands
+constexpr int kChunk = 3;              // k-tiles (of 64) per accumulator beside float32 operands
 constexpr size_t kPieceBytes = 160u << 20;  // most that dz of one piece takes
 constexpr int kMaxSplits = 16;
 
@@ -58,7 +58,7 @@ struct Plan {
 // third of the pairs idle in dw and take 949 us; see DESIGN for what the choice here takes.
 void choose_pieces(const nc_linear_ce* d, int planes, Plan* p) {
   auto ceil_div = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
-  const int sms = 148, bk = planes == 1 ? 64 : 32;
+  const int sms = 148, bk = 64;
   const int tiles = p->classes_pad / 256;
   const size_t tile_bytes = (size_t)p->rows_pad * 256 * 2 * planes;
   int64_t most = (int64_t)(kPieceBytes / tile_bytes);

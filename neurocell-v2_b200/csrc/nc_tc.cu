@@ -31,7 +31,7 @@ nc_status make_map(CUtensorMap* map, const void* base, bool bf16, int planes, in
   const CUresult r =
       fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base),
          dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-         box_inner == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
     return set_error(NC_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d) for %d x %d, pitch %lld", (int)r, outer, inner,

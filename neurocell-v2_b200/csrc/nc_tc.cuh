@@ -53,7 +53,7 @@ struct Tile {
 // 128.
 template <int PL, int BN, int CG>
 struct Config {
-  static constexpr int kBK = PL == 1 ? 64 : 32;
+  static constexpr int kBK = 64;   // one swizzled row of 128 bytes (rows of 64 took the copies 6 % longer)
   static constexpr int kBRows = BN / CG;   // of B in one CTA
   static constexpr int kA = PL * kBM * kBK * 2, kB = PL * kBRows * kBK * 2;
   static constexpr int kStage = kA + kB;
@@ -222,19 +222,18 @@ __device__ __forceinline__ void tmem_load(uint32_t addr, float (&v)[32]) {
 }
 
 // Shared-memory matrix descriptors: start address, leading and stride byte offsets (16-byte
-// units), descriptor version 1, swizzle mode (2: 128 bytes, 4: 64 bytes).
+// units), descriptor version 1, swizzle mode (2: 128 bytes).
 __device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lead, uint32_t stride, uint32_t swizzle) {
   return (uint64_t)((addr >> 4) & 0x3fff) | (uint64_t)((lead >> 4) & 0x3fff) << 16 |
          (uint64_t)((stride >> 4) & 0x3fff) << 32 | (uint64_t)1 << 46 | (uint64_t)swizzle << 61;
 }
 
-// Operand of one plane, 16 values of k from step `ks` on.  k contiguous: rows of kBK values,
-// 8-row groups kBK * 16 bytes apart, swizzled over the row.  Own index contiguous: blocks of
-// 64 of it (`block` bytes apart), each k 128 bytes, 8-k groups 1024 bytes apart.
-template <int BK>
+// Operand of one plane, 16 values of k from step `ks` on, rows of 128 bytes swizzled over 8.
+// k contiguous: 8-row groups 1024 bytes apart.  Own index contiguous: blocks of 64 of it
+// (`block` bytes apart), each k 128 bytes, 8-k groups 1024 bytes apart.
 __device__ __forceinline__ uint64_t operand_desc(uint32_t base, bool mn, uint32_t block, int ks) {
   if (mn) return smem_desc(base + ks * 2048, block, 1024, 2);
-  return smem_desc(base + ks * 32, 16, BK * 16, BK == 64 ? 2 : 4);
+  return smem_desc(base + ks * 32, 16, 1024, 2);
 }
 
 // 16-bit planes of a float32 value that was scaled to float16's range.
@@ -265,184 +264,217 @@ __device__ __forceinline__ void load_v8(const void* p, uint32_t (&v)[8]) {
                : "memory");
 }
 
-// The kernel: warps 0..7 epilogue, warp 8 loads, warp 9 multiplies (in the first CTA of a
-// pair); persistent over tiles.  Epi::run(tile, row, col, acc) gets a row's BN / 2
-// consecutive columns as float32 sums; Epi::begin(tile, row, col, scratch) runs before the
-// wait for them and returns what run() takes along (scratch: BN / 2 floats of the warp).
+// What a CTA's warps share beside the stages.
+template <int PL, int BN, int CG>
+struct Shared {
+  uint64_t bars[2 * Config<PL, BN, CG>::kStages + 5];
+  uint32_t tmem_slot;
+  int abort;
+};
+
+// One warp's view of the pipeline: the loading warp fills stages, the multiplying warp (of a
+// pair's first CTA) turns them into accumulators, the epilogue warps collect those.  Each
+// role keeps its own place; the places advance over tiles and over products alike.
+template <int PL, int BN, int CG>
+struct Engine {
+  using C = Config<PL, BN, CG>;
+  static constexpr int BK = C::kBK, HALF = BN / 2;
+  static constexpr uint32_t a_block = C::kA / (kBM / 64), b_block = C::kB / (C::kBRows / 64);
+
+  uint32_t stages, bar0, tmem;
+  volatile int* abort;
+  int32_t* status;
+  int rank;
+  int s = 0, buf = 0, issued = 0;
+  uint32_t ph, aph = 1;
+  bool ok = true;
+
+  __device__ __forceinline__ uint32_t full(int i) const { return bar0 + 8 * i; }
+  __device__ __forceinline__ uint32_t empty(int i) const { return bar0 + 8 * (C::kStages + i); }
+  __device__ __forceinline__ uint32_t acc_full(int i) const { return bar0 + 8 * (2 * C::kStages + i); }
+  __device__ __forceinline__ uint32_t acc_empty(int i) const { return bar0 + 8 * (2 * C::kStages + 2 + i); }
+  __device__ __forceinline__ uint32_t drain() const { return bar0 + 8 * (2 * C::kStages + 4); }
+
+  // By the whole CTA, before it reads anything that an earlier kernel wrote.
+  __device__ __forceinline__ Engine(uint8_t* raw, Shared<PL, BN, CG>* sh, int32_t* status_word) {
+    stages = (smem_addr(raw) + 1023) & ~1023u;
+    bar0 = smem_addr(sh->bars);
+    abort = &sh->abort;
+    status = status_word;
+    rank = CG == 1 ? 0 : (int)cluster_rank();
+    const int warp = threadIdx.x >> 5;
+    ph = warp == kEpiWarps;   // the loader starts on empty stages
+    if (threadIdx.x == 0) {
+      for (int i = 0; i < C::kStages; ++i) bar_init(full(i), 1), bar_init(empty(i), 1);
+      for (int i = 0; i < 2; ++i) bar_init(acc_full(i), 1), bar_init(acc_empty(i), kEpiWarps * CG);
+      bar_init(drain(), 1);
+      sh->abort = 0;
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == kEpiWarps + 1) tmem_alloc<CG>(smem_addr(&sh->tmem_slot), 2 * BN);
+    fence_before();
+    __syncthreads();
+    if constexpr (CG == 2) cluster_sync();
+    fence_after();
+    tmem = sh->tmem_slot;
+  }
+
+  // One thread of the loading warp: the k-tiles of a tile.
+  __device__ __forceinline__ void load(const Problem& p, const CUtensorMap* a, const CUtensorMap* b, const Tile& x) {
+    for (int kt = x.kt0; kt < x.kt1 && ok; ++kt) {
+      if (!(ok = bar_wait(empty(s), ph, abort, status))) return;
+      if (rank == 0) bar_expect(full(s), C::kStage * CG);
+      const uint32_t bar = CG == 1 ? full(s) : leader_addr(full(s));
+      const uint32_t at = stages + s * C::kStage;
+      const int ka = p.a_k0 + kt * BK, kb = p.b_k0 + kt * BK, nb = p.b_n0 + x.n0 + rank * C::kBRows;
+      if (p.a_mn) {
+#pragma unroll
+        for (int i = 0; i < kBM / 64; ++i) tma_load<CG>(at + i * a_block, a, bar, x.m0 + 64 * i, ka, x.batch);
+      } else {
+        tma_load<CG>(at, a, bar, ka, x.m0, x.batch);
+      }
+      if (p.b_mn) {
+#pragma unroll
+        for (int i = 0; i < C::kBRows / 64; ++i)
+          tma_load<CG>(at + C::kA + i * b_block, b, bar, nb + 64 * i, kb, x.batch);
+      } else {
+        tma_load<CG>(at + C::kA, b, bar, kb, nb, x.batch);
+      }
+      if (issued < C::kStages) ++issued;
+      if (++s == C::kStages) s = 0, ph ^= 1;
+    }
+  }
+
+  // One thread of the multiplying warp.
+  __device__ __forceinline__ void multiply(const Problem& p, const Tile& x) {
+    // accumulator float32; operand types; which operands have their own index contiguous
+    const uint32_t idesc = 1u << 4 | (p.bf16 ? 1u << 7 | 1u << 10 : 0u) | (p.a_mn ? 1u << 15 : 0u) |
+                           (p.b_mn ? 1u << 16 : 0u) | (uint32_t)(BN >> 3) << 17 | (uint32_t)(kBM * CG >> 4) << 24;
+    const uint32_t a_plane = p.a_mn ? a_block / PL : C::kA / PL, b_plane = p.b_mn ? b_block / PL : C::kB / PL;
+    for (int c0 = x.kt0; c0 < x.kt1 && ok; c0 += p.chunk) {
+      if (!(ok = bar_wait(acc_empty(buf), aph, abort, status))) return;
+      fence_after();
+      const uint32_t d = tmem + buf * BN;
+      const int c1 = min(c0 + p.chunk, x.kt1);
+      uint32_t add = 0;
+      for (int kt = c0; kt < c1; ++kt) {
+        if (!(ok = bar_wait(full(s), ph, abort, status))) return;
+        fence_after();
+        const uint32_t at = stages + s * C::kStage, bt = at + C::kA;
+        // low parts first, while the accumulator is small
+        constexpr int kProducts = PL == 1 ? 1 : 3;
+#pragma unroll
+        for (int q = 0; q < kProducts; ++q) {
+          const int pa = PL == 1 ? 0 : (q == 0 ? 1 : 0), pb = PL == 1 ? 0 : (q == 1 ? 1 : 0);
+#pragma unroll
+          for (int ks = 0; ks < BK / 16; ++ks) {
+            mma<CG>(d, operand_desc(at + pa * a_plane, p.a_mn, a_block, ks),
+                    operand_desc(bt + pb * b_plane, p.b_mn, b_block, ks), idesc, add);
+            add = 1;
+          }
+        }
+        mma_commit<CG>(empty(s));
+        if (++s == C::kStages) s = 0, ph ^= 1;
+      }
+      mma_commit<CG>(acc_full(buf));
+      buf ^= 1;
+      if (buf == 0) aph ^= 1;
+    }
+  }
+
+  // An epilogue warp: the sums of its 32 rows and HALF columns.
+  __device__ __forceinline__ void collect(const Problem& p, const Tile& x, float (&acc)[HALF]) {
+    const int warp = threadIdx.x >> 5;
+    const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + (warp >> 2) * HALF;
+#pragma unroll
+    for (int i = 0; i < HALF; ++i) acc[i] = 0.f;
+    for (int c0 = x.kt0; c0 < x.kt1; c0 += p.chunk) {
+      if (!__all_sync(0xffffffffu, ok && bar_wait(acc_full(buf), ph, abort, status))) {
+        ok = false;
+        return;
+      }
+      fence_after();
+#pragma unroll
+      for (int i = 0; i < HALF; i += 32) {
+        float v[32];
+        tmem_load(lanes + buf * BN + i, v);
+#pragma unroll
+        for (int j = 0; j < 32; ++j) acc[i + j] = PL == 1 ? v[j] : acc[i + j] + v[j];   // one plane, one chunk
+      }
+      fence_before();
+      if ((threadIdx.x & 31) == 0) {
+        if constexpr (CG == 1)
+          bar_arrive(acc_empty(buf));
+        else
+          bar_arrive_leader(acc_empty(buf));
+      }
+      __syncwarp();
+      buf ^= 1;
+      if (buf == 0) ph ^= 1;
+    }
+  }
+
+  // At the end, by the whole CTA.
+  __device__ __forceinline__ void finish() {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (warp == kEpiWarps && lane == 0 && !ok && rank == 0) {
+      // the copies in flight land before the CTA (or the pair) ends
+      for (int i = 0; i < issued; ++i) {
+        if (s-- == 0) s = C::kStages - 1, ph ^= 1;
+        for (int j = 0; j < kWaitLimit && !bar_try(full(s), ph ^ 1); ++j) {
+        }
+      }
+    }
+    if (warp == kEpiWarps + 1 && lane == 0 && rank == 0) {
+      // every product has finished before tensor memory is given back
+      mma_commit<CG>(drain());
+      for (int j = 0; j < kWaitLimit && !bar_try(drain(), 0); ++j) {
+      }
+    }
+    __syncthreads();
+    // a pair ends together: each reads the other's shared memory and signals its barriers
+    if constexpr (CG == 2) cluster_sync();
+    if (warp == kEpiWarps + 1) {
+      fence_after();
+      tmem_free<CG>(tmem, 2 * BN);
+    }
+  }
+};
+
+// The kernel of one product: warps 0..7 epilogue, warp 8 loads, warp 9 multiplies; persistent
+// over tiles.  Epi::run(state, tile, row, col, acc) gets a row's BN / 2 consecutive columns as
+// float32 sums; Epi::begin(tile, row, col, scratch) runs before the wait for them and returns
+// the state (scratch: BN / 2 floats of the warp).
 template <int PL, int BN, int CG, class Epi>
 __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_constant__ Problem p, const Epi epi) {
-  using C = Config<PL, BN, CG>;
-  constexpr int BK = C::kBK, HALF = BN / 2;
-  constexpr uint32_t a_block = C::kA / (kBM / 64), b_block = C::kB / (C::kBRows / 64);
+  using E = Engine<PL, BN, CG>;
   extern __shared__ uint8_t raw[];
-  __shared__ __align__(8) uint64_t bars[2 * C::kStages + 5];
-  __shared__ __align__(16) float scratch[kEpiWarps][HALF];
-  __shared__ uint32_t tmem_slot;
-  __shared__ volatile int abort_flag;
-  const uint32_t stages = (smem_addr(raw) + 1023) & ~1023u;
-  const uint32_t bar0 = smem_addr(bars);
-  auto full = [&](int s) { return bar0 + 8 * s; };
-  auto empty = [&](int s) { return bar0 + 8 * (C::kStages + s); };
-  auto acc_full = [&](int b) { return bar0 + 8 * (2 * C::kStages + b); };
-  auto acc_empty = [&](int b) { return bar0 + 8 * (2 * C::kStages + 2 + b); };
-  const uint32_t drain = bar0 + 8 * (2 * C::kStages + 4);
+  __shared__ __align__(16) float scratch[kEpiWarps][E::HALF];
+  __shared__ Shared<PL, BN, CG> sh;
+  E e(raw, &sh, p.status);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = CG == 1 ? 0 : (int)cluster_rank();
-  const int first = blockIdx.x / CG, stride = gridDim.x / CG;
-
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < C::kStages; ++s) bar_init(full(s), 1), bar_init(empty(s), 1);
-    for (int b = 0; b < 2; ++b) bar_init(acc_full(b), 1), bar_init(acc_empty(b), kEpiWarps * CG);
-    bar_init(drain, 1);
-    abort_flag = 0;
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
-  if (warp == kEpiWarps + 1) tmem_alloc<CG>(smem_addr(&tmem_slot), 2 * BN);
-  fence_before();
-  __syncthreads();
-  if constexpr (CG == 2) cluster_sync();
-  fence_after();
-  const uint32_t tmem = tmem_slot;
-  const int tiles = problem_tiles(p);
+  const int first = blockIdx.x / CG, stride = gridDim.x / CG, tiles = problem_tiles(p);
   pdl_enter();
-
   if (warp == kEpiWarps) {
-    if (lane == 0) {
-      int s = 0, issued = 0;
-      uint32_t ph = 1;
-      bool ok = true;
-      for (int t = first; t < tiles && ok; t += stride) {
-        const Tile x = problem_tile<PL, BN, CG>(p, t, rank);
-        for (int kt = x.kt0; kt < x.kt1; ++kt) {
-          if (!(ok = bar_wait(empty(s), ph, &abort_flag, p.status))) break;
-          if (rank == 0) bar_expect(full(s), C::kStage * CG);
-          const uint32_t bar = CG == 1 ? full(s) : leader_addr(full(s));
-          const uint32_t at = stages + s * C::kStage;
-          const int ka = p.a_k0 + kt * BK, kb = p.b_k0 + kt * BK, nb = p.b_n0 + x.n0 + rank * C::kBRows;
-          if (p.a_mn) {
-#pragma unroll
-            for (int i = 0; i < kBM / 64; ++i)
-              tma_load<CG>(at + i * a_block, &p.a, bar, x.m0 + 64 * i, ka, x.batch);
-          } else {
-            tma_load<CG>(at, &p.a, bar, ka, x.m0, x.batch);
-          }
-          if (p.b_mn) {
-#pragma unroll
-            for (int i = 0; i < C::kBRows / 64; ++i)
-              tma_load<CG>(at + C::kA + i * b_block, &p.b, bar, nb + 64 * i, kb, x.batch);
-          } else {
-            tma_load<CG>(at + C::kA, &p.b, bar, kb, nb, x.batch);
-          }
-          if (issued < C::kStages) ++issued;
-          if (++s == C::kStages) s = 0, ph ^= 1;
-        }
-      }
-      if (!ok && rank == 0) {   // the copies in flight land before the CTA (or the pair) ends
-        for (int i = 0; i < issued; ++i) {
-          if (s-- == 0) s = C::kStages - 1, ph ^= 1;
-          for (int j = 0; j < kWaitLimit && !bar_try(full(s), ph ^ 1); ++j) {
-          }
-        }
-      }
-    }
+    if (lane == 0)
+      for (int t = first; t < tiles && e.ok; t += stride) e.load(p, &p.a, &p.b, problem_tile<PL, BN, CG>(p, t, e.rank));
   } else if (warp == kEpiWarps + 1) {
-    if (lane == 0 && rank == 0) {
-      // accumulator float32; operand types; which operands have their own index contiguous
-      const uint32_t idesc = 1u << 4 | (p.bf16 ? 1u << 7 | 1u << 10 : 0u) | (p.a_mn ? 1u << 15 : 0u) |
-                             (p.b_mn ? 1u << 16 : 0u) | (uint32_t)(BN >> 3) << 17 | (uint32_t)(kBM * CG >> 4) << 24;
-      const uint32_t a_plane = p.a_mn ? a_block / PL : C::kA / PL, b_plane = p.b_mn ? b_block / PL : C::kB / PL;
-      int s = 0, buf = 0;
-      uint32_t ph = 0, aph = 1;
-      bool ok = true;
-      for (int t = first; t < tiles && ok; t += stride) {
-        const Tile x = problem_tile<PL, BN, CG>(p, t, 0);
-        for (int c0 = x.kt0; c0 < x.kt1 && ok; c0 += p.chunk) {
-          if (!(ok = bar_wait(acc_empty(buf), aph, &abort_flag, p.status))) break;
-          fence_after();
-          const uint32_t d = tmem + buf * BN;
-          const int c1 = min(c0 + p.chunk, x.kt1);
-          uint32_t add = 0;
-          for (int kt = c0; kt < c1; ++kt) {
-            if (!(ok = bar_wait(full(s), ph, &abort_flag, p.status))) break;
-            fence_after();
-            const uint32_t at = stages + s * C::kStage, bt = at + C::kA;
-            // low parts first, while the accumulator is small
-            constexpr int kProducts = PL == 1 ? 1 : 3;
-#pragma unroll
-            for (int q = 0; q < kProducts; ++q) {
-              const int pa = PL == 1 ? 0 : (q == 0 ? 1 : 0), pb = PL == 1 ? 0 : (q == 1 ? 1 : 0);
-#pragma unroll
-              for (int ks = 0; ks < BK / 16; ++ks) {
-                mma<CG>(d, operand_desc<BK>(at + pa * a_plane, p.a_mn, a_block, ks),
-                        operand_desc<BK>(bt + pb * b_plane, p.b_mn, b_block, ks), idesc, add);
-                add = 1;
-              }
-            }
-            mma_commit<CG>(empty(s));
-            if (++s == C::kStages) s = 0, ph ^= 1;
-          }
-          if (!ok) break;
-          mma_commit<CG>(acc_full(buf));
-          buf ^= 1;
-          if (buf == 0) aph ^= 1;
-        }
-      }
-      // every product has finished before tensor memory is given back
-      mma_commit<CG>(drain);
-      for (int j = 0; j < kWaitLimit && !bar_try(drain, 0); ++j) {
-      }
-    }
-    __syncwarp();
+    if (lane == 0 && e.rank == 0)
+      for (int t = first; t < tiles && e.ok; t += stride) e.multiply(p, problem_tile<PL, BN, CG>(p, t, 0));
   } else {
-    const int quarter = warp & 3, half = warp >> 2;
-    const uint32_t lanes = tmem + ((uint32_t)(32 * quarter) << 16) + half * HALF;
-    int buf = 0;
-    uint32_t ph = 0;
-    bool ok = true;
-    for (int t = first; t < tiles && ok; t += stride) {
-      const Tile x = problem_tile<PL, BN, CG>(p, t, rank);
-      const int row = x.m0 + 32 * quarter + lane, col = x.n0 + half * HALF;
+    for (int t = first; t < tiles && e.ok; t += stride) {
+      const Tile x = problem_tile<PL, BN, CG>(p, t, e.rank);
+      const int row = x.m0 + 32 * (warp & 3) + lane, col = x.n0 + (warp >> 2) * E::HALF;
       __syncwarp();   // the last tile's readers of scratch are done
-      const auto state = epi.template begin<HALF>(x, row, col, scratch[warp]);
+      const auto state = epi.template begin<E::HALF>(x, row, col, scratch[warp]);
       __syncwarp();
-      float acc[HALF];
-#pragma unroll
-      for (int i = 0; i < HALF; ++i) acc[i] = 0.f;
-      for (int c0 = x.kt0; c0 < x.kt1; c0 += p.chunk) {
-        ok = bar_wait(acc_full(buf), ph, &abort_flag, p.status);
-        if (!__all_sync(0xffffffffu, ok)) {
-          ok = false;
-          break;
-        }
-        fence_after();
-#pragma unroll
-        for (int i = 0; i < HALF; i += 32) {
-          float v[32];
-          tmem_load(lanes + buf * BN + i, v);
-#pragma unroll
-          for (int j = 0; j < 32; ++j) acc[i + j] = PL == 1 ? v[j] : acc[i + j] + v[j];   // one plane, one chunk
-        }
-        fence_before();
-        if (lane == 0) {
-          if constexpr (CG == 1)
-            bar_arrive(acc_empty(buf));
-          else
-            bar_arrive_leader(acc_empty(buf));
-        }
-        __syncwarp();
-        buf ^= 1;
-        if (buf == 0) ph ^= 1;
-      }
-      if (ok) epi.template run<HALF>(state, x, row, col, acc);
+      float acc[E::HALF];
+      e.collect(p, x, acc);
+      if (e.ok) epi.template run<E::HALF>(state, x, row, col, acc);
     }
   }
-  __syncthreads();
-  // a pair ends together: each reads the other's shared memory and signals its barriers
-  if constexpr (CG == 2) cluster_sync();
-  if (warp == kEpiWarps + 1) {
-    fence_after();
-    tmem_free<CG>(tmem, 2 * BN);
-  }
+  __syncwarp();
+  e.finish();
 }
 
 // Tensor map of a stored matrix (inner contiguous, `outer` rows `pitch` elements apart, planes
