@@ -19,9 +19,6 @@ namespace nc {
 
 namespace {
 
-constexpr int kNormThreads = 256;
-constexpr int kNormPer = 16;   // elements a thread of the momentum / norm pass takes
-
 struct MuonArgs {
   float beta;
   int nesterov;
@@ -35,36 +32,6 @@ __device__ __forceinline__ double block_sum_f64(double v, double* red) {
   double t = 0.0;
   for (int i = 0; i < (int)(blockDim.x >> 5); ++i) t += red[i];
   return t;
-}
-
-// grid (blocks, batch).  Sum of squares of x per block; with `momentum`: m = beta m + x,
-// and the sum is of u = x + beta m (nesterov) or m, written to `u`.
-template <typename T>
-__global__ void __launch_bounds__(kNormThreads) ns_norm_kernel(const T* __restrict__ x, float* __restrict__ momentum,
-                                                               MuonArgs mu, int64_t n, float* __restrict__ u,
-                                                               double* __restrict__ part,
-                                                               int32_t* __restrict__ status) {
-  __shared__ double red[kNormThreads / 32];
-  pdl_enter();
-  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *status = 0;
-  const size_t base = (size_t)blockIdx.y * n;
-  const int64_t i0 = (int64_t)blockIdx.x * kNormThreads * kNormPer + threadIdx.x;
-  double s = 0.0;
-#pragma unroll 4
-  for (int k = 0; k < kNormPer; ++k) {
-    const int64_t i = i0 + (int64_t)k * kNormThreads;
-    if (i >= n) break;
-    float v = to_f32(x[base + i]);
-    if (momentum) {
-      const float m = fmaf(mu.beta, momentum[base + i], v);
-      momentum[base + i] = m;
-      v = mu.nesterov ? fmaf(mu.beta, m, v) : m;
-      u[base + i] = v;
-    }
-    s += (double)v * v;
-  }
-  s = block_sum_f64(s, red);
-  if (threadIdx.x == 0) part[(size_t)blockIdx.y * gridDim.x + blockIdx.x] = s;
 }
 
 // ---- short sides up to 64: one cluster per matrix ------------------------------------------
@@ -281,11 +248,19 @@ nc_status launch_small(const SmallArgs& a, const SmallPlan& r, int batch, cudaSt
   return launch_check("ns_small_kernel launch");
 }
 
-// ---- products on the tensor cores --------------------------------------------------------
-// X, A = X X^T and b A + c A^2 are kept as two float16 planes each (nc_tc.cuh), scaled by
+// ---- longer short sides: products on the tensor cores --------------------------------------
+// X, A = X X^T and Q = b A + c A^2 are kept as two float16 planes each (nc_tc.cuh), scaled by
 // 2^12: |entries| stay below 16 while the singular values do, and an entry of 2^-26 still has
 // its 11 bits in the high plane.
+//
+// All steps are one cooperative launch: a product of such sizes takes a few microseconds, and
+// a launch, its set-up of tensor memory and its first loads as much again.  Between products
+// the grid meets (cooperative_groups); the symmetric ones compute the tiles on and above the
+// diagonal and store them twice; a product with fewer tiles than SMs is split along k, its
+// float32 parts summed in order by the whole grid.
 constexpr float kPlaneScale = 4096.f, kPlaneInv = 1.f / 4096.f;
+constexpr int kTile = 128;   // square tiles: at most sizes the number of tiles matters more than a tile's rate
+using NsEngine = tc::Engine<2, kTile, 1>;
 
 struct Planes {   // (batch, plane, rows, pitch)
   __half* p;
@@ -293,34 +268,40 @@ struct Planes {   // (batch, plane, rows, pitch)
   int64_t plane;
 };
 
-// X0 of one matrix as planes.
-template <typename T>
-__global__ void __launch_bounds__(kNormThreads) ns_split_kernel(const T* __restrict__ x, int64_t n, int cols, int parts,
-                                                                const double* __restrict__ part, double eps,
-                                                                Planes out) {
-  __shared__ double red[kNormThreads / 32];
-  pdl_enter();
-  double s = 0.0;
-  for (int i = threadIdx.x; i < parts; i += kNormThreads) s += part[(size_t)blockIdx.y * parts + i];
-  s = block_sum_f64(s, red);
-  const double inv = 1.0 / (sqrt(s) + eps);
-  const size_t base = (size_t)blockIdx.y * n;
-  __half* hi = out.p + (size_t)blockIdx.y * 2 * out.plane;
-  const int64_t i0 = (int64_t)blockIdx.x * kNormThreads * kNormPer + threadIdx.x;
-#pragma unroll 4
-  for (int k = 0; k < kNormPer; ++k) {
-    const int64_t i = i0 + (int64_t)k * kNormThreads;
-    if (i >= n) break;
-    const int r = (int)i / cols, c = (int)i - r * cols;
-    uint16_t h, l;
-    tc::split_f16((float)((double)to_f32(x[base + i]) * inv) * kPlaneScale, &h, &l);
-    const size_t o = (size_t)r * out.pitch + c;
-    hi[o] = __ushort_as_half(h);
-    hi[out.plane + o] = __ushort_as_half(l);
-  }
-}
+enum NsProduct { kGram, kPoly, kUpdate };
 
-enum NsMode { kGram, kPoly, kUpdate, kFinal };
+// The elements a thread of an element-wise phase takes; a unit is a CTA's.
+constexpr int kUnit = tc::kThreads * 4;
+
+struct NsArgs {
+  CUtensorMap by_k[2], by_row[2];   // X and its next value, both ways (short side as the own index)
+  CUtensorMap gram, poly;
+  Planes X[2], G, Q;
+  const void* x;
+  float* momentum;
+  float* params;
+  void* out;
+  double* norms;    // (batch, units) parts of the squared norms
+  float4* parts;    // of split products
+  int batch, rows, cols, steps, units;
+  int splits[3];
+  int vec;          // cols and the addresses allow 4 elements at a time
+  int wide;         // rows of the result start on 32 bytes
+  float a, b, c;
+  double eps;
+  MuonArgs mu;
+  float decay, step;
+  int32_t* status;
+};
+
+// u of an element: x itself, or from the updated momentum.
+template <typename T>
+__device__ __forceinline__ float source(const NsArgs& p, size_t o) {
+  const float x = to_f32(static_cast<const T*>(p.x)[o]);
+  if (!p.momentum) return x;
+  const float m = p.momentum[o];
+  return p.mu.nesterov ? fmaf(p.mu.beta, m, x) : m;
+}
 
 // 16 values of both planes, added up (still scaled).
 __device__ __forceinline__ void load_planes(const Planes& s, size_t o, float (&v)[16]) {
@@ -335,107 +316,258 @@ __device__ __forceinline__ void load_planes(const Planes& s, size_t o, float (&v
   }
 }
 
-// Epilogue of the three products of a step, on scaled values:
-//   gram: A = acc;  poly: b A + c acc;  update: a X + acc;  final: the same, to the caller
-template <int MODE, typename T>
-struct NsEpilogue {
-  Planes src, dst;   // same shape: A for poly, X for update
-  int m, n;
-  float mul, add;    // value = mul acc + add src
-  T* out;            // final: the result (rows, cols), or
-  float* params;     // params <- decay params - step result
-  float decay, step;
-  bool wide;         // rows of out or params start on 32 bytes
-
-  template <int HALF>
-  __device__ __forceinline__ int begin(const tc::Tile&, int, int, float*) const {
-    return 0;
+// 16 columns of the transposed store: lanes hold consecutive rows; pairs of lanes exchange so
+// that each stores two rows of one column at a time.
+__device__ __forceinline__ void store_mirrored(__half* p, int64_t pitch, int row, int col, int m, int n,
+                                               const uint32_t (&v)[8]) {
+  const bool odd = row & 1;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t other = __shfl_xor_sync(0xffffffffu, v[i], 1);
+    const uint32_t two = odd ? __byte_perm(other, v[i], 0x7632) : __byte_perm(v[i], other, 0x5410);
+    const int c = col + 2 * i + odd;
+    // the row next to an odd last one is padding
+    if (c < n && (row & ~1) < m) *reinterpret_cast<uint32_t*>(p + c * pitch + (row & ~1)) = two;
   }
-  template <int HALF>
-  __device__ __forceinline__ void run(int, const tc::Tile& x, int row, int col, float (&acc)[HALF]) const {
-    if (row >= m) return;
-    const size_t base = (size_t)x.batch * 2 * src.plane + (size_t)row * src.pitch;
-    const bool mirror = (MODE == kGram || MODE == kPoly) && x.n0 > x.m0;
+}
+
+// Result of a product on scaled values: value = mul acc + add src, to planes (and mirrored), or
+// (out) unscaled to the caller.
+template <typename T>
+__device__ __forceinline__ void ns_store(const NsArgs& p, NsProduct product, int k, bool last, const tc::Tile& x, int row,
+                                         int col, float (&acc)[64]) {
+  const Planes& src = product == kUpdate ? p.X[k & 1] : p.G;
+  const Planes& dst = product == kGram ? p.G : product == kPoly ? p.Q : p.X[(k + 1) & 1];
+  const int s = min(p.rows, p.cols), m = product == kUpdate ? p.rows : s, n = product == kUpdate ? p.cols : s;
+  const float mul = product == kPoly ? p.c * kPlaneInv : kPlaneInv, add = product == kPoly ? p.b : p.a;
+  const bool mirror = product != kUpdate && x.n0 > x.m0;
+  const size_t base = (size_t)x.batch * 2 * dst.plane + (size_t)row * dst.pitch;
 #pragma unroll
-    for (int j = 0; j < HALF; j += 16) {
-      if (col + j >= n) break;
-      float v[16];
-      if constexpr (MODE == kGram) {
+  for (int j = 0; j < 64; j += 16) {
+    if (col + j >= n) break;
+    float v[16];
+    if (product == kGram || row >= m) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) v[e] = acc[j + e] * mul;
-      } else {
-        load_planes(src, base + col + j, v);
+      for (int e = 0; e < 16; ++e) v[e] = acc[j + e] * mul;
+    } else {
+      load_planes(src, base + col + j, v);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) v[e] = fmaf(acc[j + e], mul, v[e] * add);
+      for (int e = 0; e < 16; ++e) v[e] = fmaf(acc[j + e], mul, v[e] * add);
+    }
+    if (!last) {
+      uint32_t h[8], l[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) tc::split_f16x2(v[2 * i], v[2 * i + 1], &h[i], &l[i]);
+      if (row < m) {
+        tc::store_v8(dst.p + base + col + j, h);
+        tc::store_v8(dst.p + base + dst.plane + col + j, l);
       }
-      if constexpr (MODE == kFinal) {
-        const size_t o = ((size_t)x.batch * m + row) * n + col + j;
+      if (mirror) {
+        __half* t = dst.p + (size_t)x.batch * 2 * dst.plane;
+        store_mirrored(t, dst.pitch, row, col + j, m, n, h);
+        store_mirrored(t + dst.plane, dst.pitch, row, col + j, m, n, l);
+      }
+      continue;
+    }
+    if (row >= m) continue;
+    const size_t o = ((size_t)x.batch * m + row) * n + col + j;
+    T* out = static_cast<T*>(p.out);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) v[e] *= kPlaneInv;
-        if (params) {
-          if (wide && col + j + 16 <= n) {
+    for (int e = 0; e < 16; ++e) v[e] *= kPlaneInv;
+    if (p.wide && col + j + 16 <= n) {
+      uint32_t q[8];
 #pragma unroll
-            for (int e = 0; e < 16; e += 8) {
-              uint32_t q[8];
-              tc::load_v8(params + o + e, q);
+      for (int e = 0; e < 16; e += 8) {
+        if (p.params) {
+          tc::load_v8(p.params + o + e, q);
 #pragma unroll
-              for (int i = 0; i < 8; ++i) q[i] = __float_as_uint(__uint_as_float(q[i]) * decay - step * v[e + i]);
-              tc::store_v8(params + o + e, q);
-            }
-          } else {
+          for (int i = 0; i < 8; ++i) q[i] = __float_as_uint(__uint_as_float(q[i]) * p.decay - p.step * v[e + i]);
+          tc::store_v8(p.params + o + e, q);
+        } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e)
-              if (col + j + e < n) params[o + e] = params[o + e] * decay - step * v[e];
-          }
-        } else if (wide && col + j + 16 <= n) {
-          uint32_t q[8];
-          if constexpr (sizeof(T) == 4) {
-#pragma unroll
-            for (int e = 0; e < 16; e += 8) {
-#pragma unroll
-              for (int i = 0; i < 8; ++i) q[i] = __float_as_uint(v[e + i]);
-              tc::store_v8(out + o + e, q);
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-              q[i] = *reinterpret_cast<const uint32_t*>(&b);
-            }
-            tc::store_v8(out + o, q);
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (col + j + e < n) store_as(out + o + e, v[e]);
+          for (int i = 0; i < 8; ++i) q[i] = __float_as_uint(v[e + i]);
+          tc::store_v8(out + o + e, q);
         }
-      } else {
-        uint32_t h[8], l[8];
+      }
+      if constexpr (sizeof(T) == 2) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) tc::split_f16x2(v[2 * i], v[2 * i + 1], &h[i], &l[i]);
-        __half* d = dst.p + base + col + j;
-        tc::store_v8(d, h);
-        tc::store_v8(d + dst.plane, l);
-        if (mirror) {   // lanes hold consecutive rows: the transposed store is contiguous over them
-          __half* t = dst.p + (size_t)x.batch * 2 * dst.plane + row;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            if (col + j + i >= n) break;
-            const size_t o = (size_t)(col + j + i) * dst.pitch;
-            t[o] = __ushort_as_half((uint16_t)(h[i / 2] >> (16 * (i & 1))));
-            t[o + dst.plane] = __ushort_as_half((uint16_t)(l[i / 2] >> (16 * (i & 1))));
-          }
+        for (int i = 0; i < 8; ++i) {
+          const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+          q[i] = *reinterpret_cast<const uint32_t*>(&b);
         }
+        tc::store_v8(out + o, q);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        if (col + j + e >= n) break;
+        if (p.params)
+          p.params[o + e] = p.params[o + e] * p.decay - p.step * v[e];
+        else
+          store_as(out + o + e, v[e]);
       }
     }
   }
-};
+}
 
-int norm_blocks(int64_t n) { return (int)((n + kNormThreads * kNormPer - 1) / (kNormThreads * kNormPer)); }
+template <typename T>
+__global__ void __launch_bounds__(tc::kThreads, 1) ns_kernel(const __grid_constant__ NsArgs p) {
+  extern __shared__ uint8_t raw[];
+  __shared__ tc::Shared<2, kTile, 1> sh;
+  __shared__ double red[tc::kThreads / 32];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (blockIdx.x == 0 && tid == 0) *p.status = 0;
+  NsEngine e(raw, &sh, p.status);
+  cooperative_groups::grid_group grid = cooperative_groups::this_grid();
+  // Everything stored so far is there for every CTA's loads, plain ones and tensor copies.
+  auto meet = [&] {
+    __threadfence();
+    asm volatile("fence.proxy.async;" ::: "memory");
+    grid.sync();
+    asm volatile("fence.proxy.async;" ::: "memory");
+  };
+  const int64_t n = (int64_t)p.rows * p.cols;
 
-// k-tiles (of 64) that one accumulator takes before it is added to the registers.
-constexpr int kNsChunk = 1;
-constexpr int kNsTile = 128;
+  // momentum, and the parts of the squared norms
+  for (int64_t w = blockIdx.x; w < (int64_t)p.batch * p.units; w += gridDim.x) {
+    const int b = (int)(w / p.units);
+    const int64_t i = (w - (int64_t)b * p.units) * kUnit;
+    double sum = 0.0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t at = i + j * tc::kThreads + tid;
+      if (at >= n) break;
+      const size_t o = (size_t)b * n + at;
+      if (p.momentum) p.momentum[o] = fmaf(p.mu.beta, p.momentum[o], to_f32(static_cast<const T*>(p.x)[o]));
+      const float u = source<T>(p, o);
+      sum += (double)u * u;
+    }
+    __syncthreads();   // red of the last unit has been read
+    sum = block_sum_f64(sum, red);
+    if (tid == 0) p.norms[w] = sum;
+  }
+  meet();
+  // X0 as planes; each CTA adds up the parts of the matrices it meets, in order
+  int have = -1;
+  double inv = 0.0;
+  for (int64_t w = blockIdx.x; w < (int64_t)p.batch * p.units; w += gridDim.x) {
+    const int b = (int)(w / p.units);
+    const int64_t i = (w - (int64_t)b * p.units) * kUnit;
+    if (b != have) {
+      double sum = 0.0;
+      for (int j = tid; j < p.units; j += tc::kThreads) sum += p.norms[(int64_t)b * p.units + j];
+      __syncthreads();
+      sum = block_sum_f64(sum, red);
+      inv = 1.0 / (sqrt(sum) + p.eps);
+      have = b;
+    }
+    __half* hi = p.X[0].p + (size_t)b * 2 * p.X[0].plane;
+    if (p.vec) {
+      const int64_t at = i + 4 * tid;
+      if (at < n) {
+        const int r = (int)at / p.cols, c = (int)at - r * p.cols;
+        float v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = (float)((double)source<T>(p, (size_t)b * n + at + j) * inv) * kPlaneScale;
+        uint32_t h[2], l[2];
+        tc::split_f16x2(v[0], v[1], &h[0], &l[0]);
+        tc::split_f16x2(v[2], v[3], &h[1], &l[1]);
+        const size_t o = (size_t)r * p.X[0].pitch + c;
+        *reinterpret_cast<uint2*>(hi + o) = make_uint2(h[0], h[1]);
+        *reinterpret_cast<uint2*>(hi + p.X[0].plane + o) = make_uint2(l[0], l[1]);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int64_t at = i + j * tc::kThreads + tid;
+        if (at >= n) break;
+        const int r = (int)at / p.cols, c = (int)at - r * p.cols;
+        uint32_t h, l;
+        tc::split_f16x2((float)((double)source<T>(p, (size_t)b * n + at) * inv) * kPlaneScale, 0.f, &h, &l);
+        const size_t o = (size_t)r * p.X[0].pitch + c;
+        hi[o] = __ushort_as_half((uint16_t)h), hi[p.X[0].plane + o] = __ushort_as_half((uint16_t)l);
+      }
+    }
+  }
+  meet();
+
+  const bool tall = p.rows > p.cols;
+  const int s = tall ? p.cols : p.rows, len = tall ? p.rows : p.cols;
+  for (int k = 0; k < p.steps; ++k) {
+    const CUtensorMap *xk = &p.by_k[k & 1], *xr = &p.by_row[k & 1];
+#pragma unroll 1
+    for (int f = kGram; f <= kUpdate; ++f) {
+      // gram: the short side's rows of X against themselves; poly: A A; update: Q X, or X Q
+      tc::Problem q;
+      q.m = f == kUpdate ? p.rows : s, q.n = f == kUpdate ? p.cols : s, q.k = f == kGram ? len : s;
+      q.a_mn = f == kGram && tall, q.b_mn = f == kGram ? tall : f == kUpdate && !tall;
+      q.tiles_m = (q.m + kTile - 1) / kTile, q.tiles_n = (q.n + kTile - 1) / kTile;
+      q.batch = p.batch, q.splits = p.splits[f], q.symmetric = f != kUpdate, q.chunk = 1, q.bf16 = 0;
+      q.a_k0 = q.b_k0 = q.b_n0 = 0;
+      const CUtensorMap* ma = f == kGram ? (tall ? xr : xk) : f == kPoly ? &p.gram : tall ? xk : &p.poly;
+      const CUtensorMap* mb = f == kGram ? (tall ? xr : xk) : f == kPoly ? &p.gram : tall ? &p.poly : xr;
+      const bool last = f == kUpdate && k + 1 == p.steps;
+      const int tiles = tc::problem_tiles(q);
+      if (warp == tc::kEpiWarps) {
+        if (lane == 0)
+          for (int t = blockIdx.x; t < tiles && e.ok; t += gridDim.x) e.load(q, ma, mb, tc::problem_tile<2, kTile, 1>(q, t, 0));
+      } else if (warp == tc::kEpiWarps + 1) {
+        if (lane == 0)
+          for (int t = blockIdx.x; t < tiles && e.ok; t += gridDim.x) e.multiply(q, tc::problem_tile<2, kTile, 1>(q, t, 0));
+      } else {
+        for (int t = blockIdx.x; t < tiles && e.ok; t += gridDim.x) {
+          const tc::Tile x = tc::problem_tile<2, kTile, 1>(q, t, 0);
+          float acc[64];
+          e.collect(q, x, acc);
+          if (!e.ok) break;
+          if (q.splits > 1) {
+            float4* o = p.parts + ((size_t)t * tc::kEpiWarps + warp) * 16 * 32 + lane;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) o[j * 32] = make_float4(acc[4 * j], acc[4 * j + 1], acc[4 * j + 2], acc[4 * j + 3]);
+          } else {
+            ns_store<T>(p, (NsProduct)f, k, last, x, x.m0 + 32 * (warp & 3) + lane, x.n0 + (warp >> 2) * 64, acc);
+          }
+        }
+      }
+      __syncwarp();
+      meet();
+      if (q.splits == 1) continue;
+      // the parts of a tile are tiles / splits apart; a warp sums its 32 rows and 64 columns
+      const int whole = tiles / q.splits;
+      if (warp < tc::kEpiWarps) {
+        for (int w = blockIdx.x * tc::kEpiWarps + warp; w < whole * tc::kEpiWarps; w += gridDim.x * tc::kEpiWarps) {
+          const int t = w / tc::kEpiWarps, part = w % tc::kEpiWarps;
+          const tc::Tile x = tc::problem_tile<2, kTile, 1>(q, t, 0);
+          float acc[64];
+#pragma unroll
+          for (int j = 0; j < 64; ++j) acc[j] = 0.f;
+          for (int g = 0; g < q.splits; ++g) {
+            const float4* o = p.parts + ((size_t)(t + g * whole) * tc::kEpiWarps + part) * 16 * 32 + lane;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const float4 v = o[j * 32];
+              acc[4 * j] += v.x, acc[4 * j + 1] += v.y, acc[4 * j + 2] += v.z, acc[4 * j + 3] += v.w;
+            }
+          }
+          ns_store<T>(p, (NsProduct)f, k, last, x, x.m0 + 32 * (part & 3) + lane, x.n0 + (part >> 2) * 64, acc);
+        }
+      }
+      meet();
+    }
+  }
+  if (p.steps == 0) {   // X0 as it is
+    for (int64_t w = blockIdx.x * (int64_t)tc::kThreads + tid; w < n * p.batch; w += (int64_t)gridDim.x * tc::kThreads) {
+      const int64_t b = w / n, i = w - b * n;
+      const size_t o = (size_t)b * 2 * p.X[0].plane + (size_t)(i / p.cols) * p.X[0].pitch + i % p.cols;
+      const float v = (__half2float(p.X[0].p[o]) + __half2float(p.X[0].p[p.X[0].plane + o])) * kPlaneInv;
+      if (p.params)
+        p.params[w] = p.params[w] * p.decay - p.step * v;
+      else
+        store_as(static_cast<T*>(p.out) + w, v);
+    }
+  }
+  e.finish();
+}
 
 // Short sides up to 64 whose slices fit take one cluster per matrix, the others the tensor
 // cores.
@@ -443,8 +575,24 @@ bool on_tensor_cores(const nc_newton_schulz* d) { return !small_plan(d).fits; }
 
 int plane_pitch(int cols) { return (cols + 63) / 64 * 64; }
 
+// Tiles of a product and its splits along k: as many as shorten the longest SM's k-tiles by
+// more than the sum costs (about 3 k-tiles' time for the extra meeting, and the parts' traffic).
+int choose_splits(int64_t tiles, int k, int sms) {
+  auto ceil_div = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
+  const int64_t kt = ceil_div(k, NsEngine::BK);
+  int64_t best = ceil_div(tiles, sms) * kt;
+  int splits = 1;
+  for (int s = 2; s <= 32 && s <= kt; ++s) {
+    const int64_t cost = ceil_div(tiles * s, sms) * ceil_div(kt, s) + 3 + s / 4;
+    if (cost < best) best = cost, splits = s;
+  }
+  return splits;
+}
+
 struct NsLayout {
-  size_t status, part, u, x, y, gram, poly, total;
+  size_t status, norms, x, y, gram, poly, parts, total;
+  int units, splits[3];
+  int64_t tiles;   // of the largest product, splits included
 };
 
 NsLayout ns_layout(const nc_newton_schulz* d) {
@@ -462,12 +610,23 @@ NsLayout ns_layout(const nc_newton_schulz* d) {
     L.total = at;
     return L;
   }
-  L.part = take((size_t)d->batch * norm_blocks(n) * 8);
-  L.u = take(d->batch * n * 4);
+  const int64_t side = (s + kTile - 1) / kTile, triangle = side * (side + 1) / 2 * d->batch;
+  const int64_t all = (int64_t)((d->rows + kTile - 1) / kTile) * ((d->cols + kTile - 1) / kTile) * d->batch;
+  const int64_t count[3] = {triangle, triangle, all};
+  const int depth[3] = {d->rows < d->cols ? d->cols : d->rows, (int)s, (int)s};
+  int64_t parts = 0;
+  for (int f = 0; f < 3; ++f) {
+    L.splits[f] = choose_splits(count[f], depth[f], 148);
+    if (count[f] * L.splits[f] > L.tiles) L.tiles = count[f] * L.splits[f];
+    if (L.splits[f] > 1 && count[f] * L.splits[f] > parts) parts = count[f] * L.splits[f];
+  }
+  L.units = (int)((n + kUnit - 1) / kUnit);
+  L.norms = take((size_t)d->batch * L.units * 8);
   L.x = take(d->batch * x * 4);
   L.y = take(d->batch * x * 4);
   L.gram = take(d->batch * g * 4);
   L.poly = take(d->batch * g * 4);
+  L.parts = take((size_t)parts * kTile * kTile * 4);
   L.total = at;
   return L;
 }
@@ -491,88 +650,55 @@ nc_status check_ws(const void* ws, size_t have, size_t need) {
   return NC_OK;
 }
 
-// No steps: X0 as it is.
 template <typename T>
-__global__ void __launch_bounds__(256) ns_store_kernel(Planes x, int rows, int cols, T* __restrict__ out,
-                                                       float* __restrict__ params, float decay, float step) {
-  pdl_enter();
-  const int i = blockIdx.x * 256 + threadIdx.x;
-  if (i >= rows * cols) return;
-  const size_t s = (size_t)blockIdx.y * 2 * x.plane + (size_t)(i / cols) * x.pitch + i % cols;
-  const size_t o = (size_t)blockIdx.y * rows * cols + i;
-  const float v = (__half2float(x.p[s]) + __half2float(x.p[x.plane + s])) * kPlaneInv;
-  if (params)
-    params[o] = params[o] * decay - step * v;
-  else
-    store_as(out + o, v);
-}
-
-template <int MODE, typename T>
-nc_status tensor_product(const nc_newton_schulz* d, const Planes& A, bool a_mn, const Planes& B, bool b_mn, int m, int n,
-                         int k, const NsEpilogue<MODE, T>& epi, int32_t* status, cudaStream_t st) {
-  tc::Problem p{};
-  p.m = m, p.n = n, p.k = k, p.batch = d->batch, p.splits = 1, p.chunk = kNsChunk;
-  tc::set_tiles<kNsTile, 1>(&p);
-  p.symmetric = MODE == kGram || MODE == kPoly;
-  p.status = status;
-  NC_CHECK((tc::make_operand<2, kNsTile, 1>(&p, true, A.p, a_mn, m, k, A.pitch, A.plane, d->batch, 2 * A.plane)));
-  NC_CHECK((tc::make_operand<2, kNsTile, 1>(&p, false, B.p, b_mn, n, k, B.pitch, B.plane, d->batch, 2 * B.plane)));
-  return tc::launch_product<2, kNsTile, 1>(p, epi, st, "Newton-Schulz product launch");
-}
-
-template <typename T>
-nc_status run_tensor(const nc_newton_schulz* d, const T* x, const float* u, const double* part, T* out, float* params,
+nc_status run_tensor(const nc_newton_schulz* d, const T* x, float* momentum, MuonArgs mu, T* out, float* params,
                      float decay, float step, char* ws, const NsLayout& L, cudaStream_t st) {
-  const int64_t n = (int64_t)d->rows * d->cols;
-  const int nb = norm_blocks(n), s = d->rows < d->cols ? d->rows : d->cols;
-  const bool tall = d->rows > d->cols;
-  int32_t* status = reinterpret_cast<int32_t*>(ws + L.status);
+  const int s = d->rows < d->cols ? d->rows : d->cols;
   auto planes = [&](size_t o, int rows, int cols) {
     Planes q;
     q.p = reinterpret_cast<__half*>(ws + o), q.pitch = plane_pitch(cols), q.plane = (int64_t)rows * q.pitch;
     return q;
   };
-  Planes X = planes(L.x, d->rows, d->cols), Y = planes(L.y, d->rows, d->cols);
-  const Planes G = planes(L.gram, s, s), Q = planes(L.poly, s, s);
-  {
-    PdlLaunch l(dim3(nb, d->batch), dim3(kNormThreads), 0, st);
-    if (u)
-      NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, ns_split_kernel<float>, u, n, d->cols, nb, part, (double)d->eps, X));
-    else
-      NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, ns_split_kernel<T>, x, n, d->cols, nb, part, (double)d->eps, X));
-    NC_CHECK(launch_check("ns_split_kernel launch"));
+  NsArgs a{};
+  a.X[0] = planes(L.x, d->rows, d->cols), a.X[1] = planes(L.y, d->rows, d->cols);
+  a.G = planes(L.gram, s, s), a.Q = planes(L.poly, s, s);
+  // operands as (own index, k) with k contiguous, or the other way round; every box has 128 of
+  // the own index or 64 of it
+  auto map = [&](CUtensorMap* m, const Planes& q, int rows, int cols, bool by_k) {
+    return tc::make_map(m, q.p, false, 2, cols, rows, q.pitch, q.plane, d->batch, 2 * q.plane, 64,
+                        by_k ? kTile : NsEngine::BK);
+  };
+  for (int i = 0; i < 2; ++i) {
+    NC_CHECK(map(&a.by_k[i], a.X[i], d->rows, d->cols, true));
+    NC_CHECK(map(&a.by_row[i], a.X[i], d->rows, d->cols, false));
   }
-  if (d->steps == 0) {
-    PdlLaunch l(dim3((unsigned)((n + 255) / 256), d->batch), dim3(256), 0, st);
-    NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, ns_store_kernel<T>, X, d->rows, d->cols, out, params, decay, step));
-    return launch_check("ns_store_kernel launch");
-  }
+  NC_CHECK(map(&a.gram, a.G, s, s, true));
+  NC_CHECK(map(&a.poly, a.Q, s, s, true));
+  a.x = x, a.momentum = momentum, a.params = params, a.out = out;
+  a.norms = reinterpret_cast<double*>(ws + L.norms), a.parts = reinterpret_cast<float4*>(ws + L.parts);
+  a.batch = d->batch, a.rows = d->rows, a.cols = d->cols, a.steps = d->steps, a.units = L.units;
+  for (int f = 0; f < 3; ++f) a.splits[f] = L.splits[f];
+  a.vec = d->cols % 4 == 0;
   const void* to = params ? static_cast<void*>(params) : static_cast<void*>(out);
   const size_t size = params ? 4 : sizeof(T);
-  const bool wide = reinterpret_cast<uintptr_t>(to) % 32 == 0 && (size_t)d->cols * size % 32 == 0;
-  for (int k = 0; k < d->steps; ++k) {
-    NsEpilogue<kGram, T> g{};
-    g.src = g.dst = G, g.m = g.n = s, g.mul = kPlaneInv;
-    NC_CHECK(tensor_product(d, X, tall, X, tall, s, s, tall ? d->rows : d->cols, g, status, st));
-    NsEpilogue<kPoly, T> q{};
-    q.src = G, q.dst = Q, q.m = q.n = s, q.mul = d->c * kPlaneInv, q.add = d->b;
-    NC_CHECK(tensor_product(d, G, false, G, false, s, s, s, q, status, st));
-    // rows <= cols: (b A + c A^2) X, X with its own index contiguous; else X (b A + c A^2)
-    const Planes &A = tall ? X : Q, &B = tall ? Q : X;
-    if (k + 1 < d->steps) {
-      NsEpilogue<kUpdate, T> e{};
-      e.src = X, e.dst = Y, e.m = d->rows, e.n = d->cols, e.mul = kPlaneInv, e.add = d->a;
-      NC_CHECK(tensor_product(d, A, false, B, !tall, d->rows, d->cols, s, e, status, st));
-      const Planes t = X;
-      X = Y, Y = t;
-    } else {
-      NsEpilogue<kFinal, T> e{};
-      e.src = X, e.m = d->rows, e.n = d->cols, e.mul = kPlaneInv, e.add = d->a;
-      e.out = out, e.params = params, e.decay = decay, e.step = step, e.wide = wide;
-      NC_CHECK(tensor_product(d, A, false, B, !tall, d->rows, d->cols, s, e, status, st));
-    }
-  }
-  return NC_OK;
+  a.wide = reinterpret_cast<uintptr_t>(to) % 32 == 0 && (size_t)d->cols * size % 32 == 0;
+  a.a = d->a, a.b = d->b, a.c = d->c, a.eps = d->eps, a.mu = mu, a.decay = decay, a.step = step;
+  a.status = reinterpret_cast<int32_t*>(ws + L.status);
+  auto k = ns_kernel<T>;
+  constexpr int smem = NsEngine::C::kSmem;
+  NC_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  // as many CTAs as any phase keeps busy
+  int64_t blocks = (int64_t)d->batch * L.units;
+  if (L.tiles > blocks) blocks = L.tiles;
+  if (blocks > tc::sm_count()) blocks = tc::sm_count();
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeCooperative;
+  attr[0].val.cooperative = 1;
+  cfg.gridDim = dim3((unsigned)blocks), cfg.blockDim = dim3(tc::kThreads);
+  cfg.dynamicSmemBytes = smem, cfg.stream = st, cfg.attrs = attr, cfg.numAttrs = 1;
+  NC_CUDA_CHECK(cudaLaunchKernelEx(&cfg, k, a));
+  return launch_check("ns_kernel launch");
 }
 
 // From the source x (or x and momentum) to the orthogonalised matrix; `out` or `params`.
@@ -590,13 +716,7 @@ nc_status run(const nc_newton_schulz* d, const T* x, float* momentum, MuonArgs m
            : r.pad == 32 ? launch_small<32, T>(a, r, d->batch, st)
                          : launch_small<64, T>(a, r, d->batch, st);
   }
-  float* u = reinterpret_cast<float*>(ws + L.u);
-  double* part = reinterpret_cast<double*>(ws + L.part);
-  const int64_t n = (int64_t)d->rows * d->cols;
-  PdlLaunch l(dim3(norm_blocks(n), d->batch), dim3(kNormThreads), 0, st);
-  NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, ns_norm_kernel<T>, x, momentum, mu, n, u, part, status));
-  NC_CHECK(launch_check("ns_norm_kernel launch"));
-  return run_tensor(d, x, momentum ? u : nullptr, part, out, params, decay, step, ws, L, st);
+  return run_tensor(d, x, momentum, mu, out, params, decay, step, ws, L, st);
 }
 
 }  // namespace
