@@ -260,6 +260,7 @@ nc_status launch_small(const SmallArgs& a, const SmallPlan& r, int batch, cudaSt
 // float32 parts summed in order by the whole grid.
 constexpr float kPlaneScale = 4096.f, kPlaneInv = 1.f / 4096.f;
 constexpr int kTile = 128;   // square tiles: at most sizes the number of tiles matters more than a tile's rate
+constexpr int kNsChunk = 1;  // k-tiles (of 64) per accumulator: Gram sums of one sign show the additions' truncation
 using NsEngine = tc::Engine<2, kTile, 1>;
 
 struct Planes {   // (batch, plane, rows, pitch)
@@ -270,8 +271,7 @@ struct Planes {   // (batch, plane, rows, pitch)
 
 enum NsProduct { kGram, kPoly, kUpdate };
 
-// The elements a thread of an element-wise phase takes; a unit is a CTA's.
-constexpr int kUnit = tc::kThreads * 4;
+constexpr int kCluster = 8;
 
 struct NsArgs {
   CUtensorMap by_k[2], by_row[2];   // X and its next value, both ways (short side as the own index)
@@ -281,12 +281,11 @@ struct NsArgs {
   float* momentum;
   float* params;
   void* out;
-  double* norms;    // (batch, units) parts of the squared norms
+  double* norms;    // (batch, CTAs) parts of the squared norms
   float4* parts;    // of split products
-  int batch, rows, cols, steps, units;
+  int64_t parts_each;   // of one matrix, where clusters work on one each
+  int batch, rows, cols, steps;
   int splits[3];
-  int vec;          // cols and the addresses allow 4 elements at a time
-  int wide;         // rows of the result start on 32 bytes
   float a, b, c;
   double eps;
   MuonArgs mu;
@@ -303,114 +302,127 @@ __device__ __forceinline__ float source(const NsArgs& p, size_t o) {
   return p.mu.nesterov ? fmaf(p.mu.beta, m, x) : m;
 }
 
-// 16 values of both planes, added up (still scaled).
-__device__ __forceinline__ void load_planes(const Planes& s, size_t o, float (&v)[16]) {
-  uint32_t h[8], l[8];
-  tc::load_v8(s.p + o, h);
-  tc::load_v8(s.p + s.plane + o, l);
+// The transposed store of 32 rows (a lane each) and 64 columns: through the warp's patch, as 64
+// rows of 64 bytes.  `rows`, `cols`: how many of them exist; what lies behind a row's end is
+// padding.
+__device__ __forceinline__ void store_mirrored(uint8_t* patch, __half* p, int64_t pitch, int rows, int cols,
+                                               const uint32_t (&v)[32]) {
+  const int lane = threadIdx.x & 31, odd = lane & 1;
+  __syncwarp();
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float2 a = __half22float2(*reinterpret_cast<__half2*>(&h[i]));
-    const float2 b = __half22float2(*reinterpret_cast<__half2*>(&l[i]));
-    v[2 * i] = a.x + b.x, v[2 * i + 1] = a.y + b.y;
-  }
-}
-
-// 16 columns of the transposed store: lanes hold consecutive rows; pairs of lanes exchange so
-// that each stores two rows of one column at a time.
-__device__ __forceinline__ void store_mirrored(__half* p, int64_t pitch, int row, int col, int m, int n,
-                                               const uint32_t (&v)[8]) {
-  const bool odd = row & 1;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < 32; ++i) {
+    // pairs of lanes exchange: an even one gets both rows of column 2 i, an odd one of 2 i + 1
     const uint32_t other = __shfl_xor_sync(0xffffffffu, v[i], 1);
     const uint32_t two = odd ? __byte_perm(other, v[i], 0x7632) : __byte_perm(v[i], other, 0x5410);
-    const int c = col + 2 * i + odd;
-    // the row next to an odd last one is padding
-    if (c < n && (row & ~1) < m) *reinterpret_cast<uint32_t*>(p + c * pitch + (row & ~1)) = two;
+    *reinterpret_cast<uint32_t*>(patch + (2 * i + odd) * 64 + (lane >> 1) * 4) = two;
+  }
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int c = i * 8 + (lane >> 2), q = lane & 3;
+    if (c < cols && 8 * q < rows)
+      *reinterpret_cast<uint4*>(p + c * pitch + 8 * q) = *reinterpret_cast<const uint4*>(patch + c * 64 + 16 * q);
   }
 }
 
-// Result of a product on scaled values: value = mul acc + add src, to planes (and mirrored), or
-// (out) unscaled to the caller.
+// acc += add times a row's 64 values of one plane, in 16-byte pieces at `at(i)`.
+template <typename At>
+__device__ __forceinline__ void add_row(At at, float add, float (&acc)[64]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint4 w = *reinterpret_cast<const uint4*>(at(i));
+    const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&x[e]));
+      acc[8 * i + 2 * e] = fmaf(add, f.x, acc[8 * i + 2 * e]);
+      acc[8 * i + 2 * e + 1] = fmaf(add, f.y, acc[8 * i + 2 * e + 1]);
+    }
+  }
+}
+
+// acc += add times 32 rows and 64 columns of both planes in global memory.
+__device__ __forceinline__ void add_planes(uint8_t* patch, const Planes& s, size_t at, int rows, int cols, float add,
+                                           float (&acc)[64]) {
+  const int lane = threadIdx.x & 31, q = lane & 7;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    uint4 v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = i * 4 + (lane >> 3);
+      v[i] = r < rows && 8 * q < cols ? *reinterpret_cast<const uint4*>(s.p + k * s.plane + at + (size_t)r * s.pitch + 8 * q)
+                                      : make_uint4(0, 0, 0, 0);
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) *tc::patch_at(patch, i * 4 + (lane >> 3), q) = v[i];
+    __syncwarp();
+    add_row([&](int i) { return tc::patch_at(patch, lane, i); }, add, acc);
+  }
+}
+
+// Result of a product for 32 rows from row0 on and 64 columns from col on, on scaled values:
+// mul acc + add (A or X), to planes (and mirrored), or (last) unscaled to the caller.  `prior`:
+// the tile of A or X in shared memory (Engine::extra), or null to take it from global memory.
 template <typename T>
-__device__ __forceinline__ void ns_store(const NsArgs& p, NsProduct product, int k, bool last, const tc::Tile& x, int row,
-                                         int col, float (&acc)[64]) {
-  const Planes& src = product == kUpdate ? p.X[k & 1] : p.G;
+__device__ __forceinline__ void ns_store(const NsArgs& p, NsProduct product, int k, bool last, const tc::Tile& x,
+                                         int row0, int col, uint8_t* patch, const uint8_t* prior, float (&acc)[64]) {
   const Planes& dst = product == kGram ? p.G : product == kPoly ? p.Q : p.X[(k + 1) & 1];
   const int s = min(p.rows, p.cols), m = product == kUpdate ? p.rows : s, n = product == kUpdate ? p.cols : s;
-  const float mul = product == kPoly ? p.c * kPlaneInv : kPlaneInv, add = product == kPoly ? p.b : p.a;
-  const bool mirror = product != kUpdate && x.n0 > x.m0;
-  const size_t base = (size_t)x.batch * 2 * dst.plane + (size_t)row * dst.pitch;
+  const int lane = threadIdx.x & 31, rows = min(32, m - row0), cols = min(64, n - col);
+  const size_t at = (size_t)x.batch * 2 * dst.plane + (size_t)row0 * dst.pitch + col;
+  const float mul = product == kPoly ? p.c * kPlaneInv : kPlaneInv;
 #pragma unroll
-  for (int j = 0; j < 64; j += 16) {
-    if (col + j >= n) break;
-    float v[16];
-    if (product == kGram || row >= m) {
+  for (int j = 0; j < 64; ++j) acc[j] *= mul;
+  const float add = product == kPoly ? p.b : p.a;
+  if (product != kGram && prior) {
+    const int r = row0 - x.m0 + lane;
+    const uint8_t* half = prior + (col - x.n0) / 64 * (NsEngine::C::kStage / 2) + r * 128;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) v[e] = acc[j + e] * mul;
-    } else {
-      load_planes(src, base + col + j, v);
+    for (int k2 = 0; k2 < 2; ++k2)
+      add_row([&](int i) { return half + k2 * (kTile * 128) + ((i ^ (r & 7)) << 4); }, add, acc);
+  } else if (product != kGram) {
+    add_planes(patch, product == kPoly ? p.G : p.X[k & 1], at, rows, cols, add, acc);
+  }
+  if (row0 >= m || col >= n) return;   // the same for the whole warp
+  if (!last) {
+    uint32_t h[32], l[32];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) v[e] = fmaf(acc[j + e], mul, v[e] * add);
+    for (int i = 0; i < 32; ++i) tc::split_f16x2(acc[2 * i], acc[2 * i + 1], &h[i], &l[i]);
+    uint16_t* d = reinterpret_cast<uint16_t*>(dst.p);
+    tc::patch_store(patch, h, d + at, dst.pitch, rows, (cols + 7) / 8);
+    tc::patch_store(patch, l, d + dst.plane + at, dst.pitch, rows, (cols + 7) / 8);
+    if (product != kUpdate && x.n0 > x.m0) {
+      __half* t = dst.p + (size_t)x.batch * 2 * dst.plane + (size_t)col * dst.pitch + row0;
+      store_mirrored(patch, t, dst.pitch, rows, cols, h);
+      store_mirrored(patch, t + dst.plane, dst.pitch, rows, cols, l);
     }
-    if (!last) {
-      uint32_t h[8], l[8];
+    return;
+  }
+  // 32 columns at a time, a row per access
+  float* f = reinterpret_cast<float*>(patch);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) tc::split_f16x2(v[2 * i], v[2 * i + 1], &h[i], &l[i]);
-      if (row < m) {
-        tc::store_v8(dst.p + base + col + j, h);
-        tc::store_v8(dst.p + base + dst.plane + col + j, l);
-      }
-      if (mirror) {
-        __half* t = dst.p + (size_t)x.batch * 2 * dst.plane;
-        store_mirrored(t, dst.pitch, row, col + j, m, n, h);
-        store_mirrored(t + dst.plane, dst.pitch, row, col + j, m, n, l);
-      }
-      continue;
-    }
-    if (row >= m) continue;
-    const size_t o = ((size_t)x.batch * m + row) * n + col + j;
-    T* out = static_cast<T*>(p.out);
+  for (int g = 0; g < 2; ++g) {
+    __syncwarp();
 #pragma unroll
-    for (int e = 0; e < 16; ++e) v[e] *= kPlaneInv;
-    if (p.wide && col + j + 16 <= n) {
-      uint32_t q[8];
-#pragma unroll
-      for (int e = 0; e < 16; e += 8) {
-        if (p.params) {
-          tc::load_v8(p.params + o + e, q);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) q[i] = __float_as_uint(__uint_as_float(q[i]) * p.decay - p.step * v[e + i]);
-          tc::store_v8(p.params + o + e, q);
-        } else if constexpr (sizeof(T) == 4) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) q[i] = __float_as_uint(v[e + i]);
-          tc::store_v8(out + o + e, q);
-        }
-      }
-      if constexpr (sizeof(T) == 2) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-          q[i] = *reinterpret_cast<const uint32_t*>(&b);
-        }
-        tc::store_v8(out + o, q);
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        if (col + j + e >= n) break;
+    for (int j = 0; j < 32; ++j) f[lane * 32 + (j ^ lane)] = acc[32 * g + j] * kPlaneInv;
+    __syncwarp();
+    if (32 * g + lane < cols) {
+      const size_t o = ((size_t)x.batch * m + row0) * n + col + 32 * g + lane;
+#pragma unroll 8
+      for (int r = 0; r < rows; ++r) {
+        const float v = f[r * 32 + (lane ^ r)];
         if (p.params)
-          p.params[o + e] = p.params[o + e] * p.decay - p.step * v[e];
+          p.params[o + (size_t)r * n] = p.params[o + (size_t)r * n] * p.decay - p.step * v;
         else
-          store_as(out + o + e, v[e]);
+          store_as(static_cast<T*>(p.out) + o + (size_t)r * n, v);
       }
     }
   }
 }
 
-template <typename T>
+template <typename T, bool CLUSTER>
 __global__ void __launch_bounds__(tc::kThreads, 1) ns_kernel(const __grid_constant__ NsArgs p) {
   extern __shared__ uint8_t raw[];
   __shared__ tc::Shared<2, kTile, 1> sh;
@@ -418,75 +430,64 @@ __global__ void __launch_bounds__(tc::kThreads, 1) ns_kernel(const __grid_consta
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (blockIdx.x == 0 && tid == 0) *p.status = 0;
   NsEngine e(raw, &sh, p.status);
-  cooperative_groups::grid_group grid = cooperative_groups::this_grid();
+  // The CTAs that work together: the whole grid on all matrices, or a cluster on one.
+  const int size = CLUSTER ? kCluster : gridDim.x, rank = CLUSTER ? (int)tc::cluster_rank() : blockIdx.x;
+  const int b0 = CLUSTER ? blockIdx.x / kCluster : 0, batch = CLUSTER ? 1 : p.batch;
   // Everything stored so far is there for every CTA's loads, plain ones and tensor copies.
   auto meet = [&] {
     __threadfence();
     asm volatile("fence.proxy.async;" ::: "memory");
-    grid.sync();
+    if constexpr (CLUSTER)
+      tc::cluster_sync();
+    else
+      cooperative_groups::this_grid().sync();
     asm volatile("fence.proxy.async;" ::: "memory");
   };
+  auto tile = [&](const tc::Problem& q, int t) {
+    tc::Tile x = tc::problem_tile<2, kTile, 1>(q, t, 0);
+    x.batch += b0;
+    return x;
+  };
+  float4* const parts = p.parts + (size_t)b0 * p.parts_each;
   const int64_t n = (int64_t)p.rows * p.cols;
 
-  // momentum, and the parts of the squared norms
-  for (int64_t w = blockIdx.x; w < (int64_t)p.batch * p.units; w += gridDim.x) {
-    const int b = (int)(w / p.units);
-    const int64_t i = (w - (int64_t)b * p.units) * kUnit;
+  // momentum, and each CTA's part of the squared norms
+  for (int b = b0; b < b0 + batch; ++b) {
+    const size_t o = (size_t)b * n;
     double sum = 0.0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t at = i + j * tc::kThreads + tid;
-      if (at >= n) break;
-      const size_t o = (size_t)b * n + at;
-      if (p.momentum) p.momentum[o] = fmaf(p.mu.beta, p.momentum[o], to_f32(static_cast<const T*>(p.x)[o]));
-      const float u = source<T>(p, o);
+#pragma unroll 4
+    for (int64_t i = (int64_t)rank * tc::kThreads + tid; i < n; i += (int64_t)size * tc::kThreads) {
+      if (p.momentum) p.momentum[o + i] = fmaf(p.mu.beta, p.momentum[o + i], to_f32(static_cast<const T*>(p.x)[o + i]));
+      const float u = source<T>(p, o + i);
       sum += (double)u * u;
     }
-    __syncthreads();   // red of the last unit has been read
+    __syncthreads();   // red of the last matrix has been read
     sum = block_sum_f64(sum, red);
-    if (tid == 0) p.norms[w] = sum;
+    if (tid == 0) p.norms[(size_t)b * size + rank] = sum;
   }
   meet();
-  // X0 as planes; each CTA adds up the parts of the matrices it meets, in order
-  int have = -1;
-  double inv = 0.0;
-  for (int64_t w = blockIdx.x; w < (int64_t)p.batch * p.units; w += gridDim.x) {
-    const int b = (int)(w / p.units);
-    const int64_t i = (w - (int64_t)b * p.units) * kUnit;
-    if (b != have) {
-      double sum = 0.0;
-      for (int j = tid; j < p.units; j += tc::kThreads) sum += p.norms[(int64_t)b * p.units + j];
-      __syncthreads();
-      sum = block_sum_f64(sum, red);
-      inv = 1.0 / (sqrt(sum) + p.eps);
-      have = b;
-    }
+  // X0 as planes; every CTA adds up a matrix's parts, in order
+  for (int b = b0; b < b0 + batch; ++b) {
+    double sum = 0.0;
+    for (int j = tid; j < size; j += tc::kThreads) sum += p.norms[(size_t)b * size + j];
+    __syncthreads();
+    sum = block_sum_f64(sum, red);
+    const double inv = 1.0 / (sqrt(sum) + p.eps);
     __half* hi = p.X[0].p + (size_t)b * 2 * p.X[0].plane;
-    if (p.vec) {
-      const int64_t at = i + 4 * tid;
-      if (at < n) {
-        const int r = (int)at / p.cols, c = (int)at - r * p.cols;
-        float v[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = (float)((double)source<T>(p, (size_t)b * n + at + j) * inv) * kPlaneScale;
-        uint32_t h[2], l[2];
-        tc::split_f16x2(v[0], v[1], &h[0], &l[0]);
-        tc::split_f16x2(v[2], v[3], &h[1], &l[1]);
-        const size_t o = (size_t)r * p.X[0].pitch + c;
-        *reinterpret_cast<uint2*>(hi + o) = make_uint2(h[0], h[1]);
-        *reinterpret_cast<uint2*>(hi + p.X[0].plane + o) = make_uint2(l[0], l[1]);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int64_t at = i + j * tc::kThreads + tid;
-        if (at >= n) break;
-        const int r = (int)at / p.cols, c = (int)at - r * p.cols;
-        uint32_t h, l;
-        tc::split_f16x2((float)((double)source<T>(p, (size_t)b * n + at) * inv) * kPlaneScale, 0.f, &h, &l);
-        const size_t o = (size_t)r * p.X[0].pitch + c;
-        hi[o] = __ushort_as_half((uint16_t)h), hi[p.X[0].plane + o] = __ushort_as_half((uint16_t)l);
-      }
+    const size_t from = (size_t)b * n;
+    const int pairs = (p.cols + 1) / 2;   // two columns at a time
+    const int64_t all = (int64_t)p.rows * pairs;
+#pragma unroll 4
+    for (int64_t i = (int64_t)rank * tc::kThreads + tid; i < all; i += (int64_t)size * tc::kThreads) {
+      const int r = (int)((uint32_t)i / (uint32_t)pairs), c = 2 * ((int)i - r * pairs);
+      const size_t at = from + (size_t)r * p.cols + c;
+      const float v = (float)((double)source<T>(p, at) * inv) * kPlaneScale;
+      const float w = c + 1 < p.cols ? (float)((double)source<T>(p, at + 1) * inv) * kPlaneScale : 0.f;
+      uint32_t h, l;
+      tc::split_f16x2(v, w, &h, &l);
+      const size_t to = (size_t)r * p.X[0].pitch + c;
+      *reinterpret_cast<uint32_t*>(hi + to) = h;
+      *reinterpret_cast<uint32_t*>(hi + p.X[0].plane + to) = l;
     }
   }
   meet();
@@ -502,30 +503,41 @@ __global__ void __launch_bounds__(tc::kThreads, 1) ns_kernel(const __grid_consta
       q.m = f == kUpdate ? p.rows : s, q.n = f == kUpdate ? p.cols : s, q.k = f == kGram ? len : s;
       q.a_mn = f == kGram && tall, q.b_mn = f == kGram ? tall : f == kUpdate && !tall;
       q.tiles_m = (q.m + kTile - 1) / kTile, q.tiles_n = (q.n + kTile - 1) / kTile;
-      q.batch = p.batch, q.splits = p.splits[f], q.symmetric = f != kUpdate, q.chunk = 1, q.bf16 = 0;
+      q.batch = batch, q.splits = p.splits[f], q.symmetric = f != kUpdate, q.chunk = kNsChunk, q.bf16 = 0;
       q.a_k0 = q.b_k0 = q.b_n0 = 0;
       const CUtensorMap* ma = f == kGram ? (tall ? xr : xk) : f == kPoly ? &p.gram : tall ? xk : &p.poly;
       const CUtensorMap* mb = f == kGram ? (tall ? xr : xk) : f == kPoly ? &p.gram : tall ? &p.poly : xr;
       const bool last = f == kUpdate && k + 1 == p.steps;
       const int tiles = tc::problem_tiles(q);
+      const bool extra = f != kGram && q.splits == 1;
       if (warp == tc::kEpiWarps) {
-        if (lane == 0)
-          for (int t = blockIdx.x; t < tiles && e.ok; t += gridDim.x) e.load(q, ma, mb, tc::problem_tile<2, kTile, 1>(q, t, 0));
+        if (lane == 0) {
+          for (int t = rank; t < tiles && e.ok; t += size) {
+            const tc::Tile x = tile(q, t);
+            e.load(q, ma, mb, x);
+            if (extra) e.load_extra(f == kPoly ? &p.gram : xk, x);
+          }
+        }
       } else if (warp == tc::kEpiWarps + 1) {
-        if (lane == 0)
-          for (int t = blockIdx.x; t < tiles && e.ok; t += gridDim.x) e.multiply(q, tc::problem_tile<2, kTile, 1>(q, t, 0));
+        for (int t = rank; t < tiles && e.ok; t += size) {
+          e.multiply(q, tile(q, t));
+          if (extra) e.skip_extra();
+        }
       } else {
-        for (int t = blockIdx.x; t < tiles && e.ok; t += gridDim.x) {
-          const tc::Tile x = tc::problem_tile<2, kTile, 1>(q, t, 0);
+        for (int t = rank; t < tiles && e.ok; t += size) {
+          const tc::Tile x = tile(q, t);
           float acc[64];
           e.collect(q, x, acc);
           if (!e.ok) break;
           if (q.splits > 1) {
-            float4* o = p.parts + ((size_t)t * tc::kEpiWarps + warp) * 16 * 32 + lane;
+            float4* o = parts + ((size_t)t * tc::kEpiWarps + warp) * 16 * 32 + lane;
 #pragma unroll
             for (int j = 0; j < 16; ++j) o[j * 32] = make_float4(acc[4 * j], acc[4 * j + 1], acc[4 * j + 2], acc[4 * j + 3]);
           } else {
-            ns_store<T>(p, (NsProduct)f, k, last, x, x.m0 + 32 * (warp & 3) + lane, x.n0 + (warp >> 2) * 64, acc);
+            const uint8_t* prior = extra ? e.extra() : nullptr;
+            if (!e.ok) break;
+            ns_store<T>(p, (NsProduct)f, k, last, x, x.m0 + 32 * (warp & 3), x.n0 + (warp >> 2) * 64, e.patch, prior, acc);
+            if (extra) e.extra_done();
           }
         }
       }
@@ -535,28 +547,28 @@ __global__ void __launch_bounds__(tc::kThreads, 1) ns_kernel(const __grid_consta
       // the parts of a tile are tiles / splits apart; a warp sums its 32 rows and 64 columns
       const int whole = tiles / q.splits;
       if (warp < tc::kEpiWarps) {
-        for (int w = blockIdx.x * tc::kEpiWarps + warp; w < whole * tc::kEpiWarps; w += gridDim.x * tc::kEpiWarps) {
+        for (int w = rank * tc::kEpiWarps + warp; w < whole * tc::kEpiWarps; w += size * tc::kEpiWarps) {
           const int t = w / tc::kEpiWarps, part = w % tc::kEpiWarps;
-          const tc::Tile x = tc::problem_tile<2, kTile, 1>(q, t, 0);
+          const tc::Tile x = tile(q, t);
           float acc[64];
 #pragma unroll
           for (int j = 0; j < 64; ++j) acc[j] = 0.f;
           for (int g = 0; g < q.splits; ++g) {
-            const float4* o = p.parts + ((size_t)(t + g * whole) * tc::kEpiWarps + part) * 16 * 32 + lane;
+            const float4* o = parts + ((size_t)(t + g * whole) * tc::kEpiWarps + part) * 16 * 32 + lane;
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
               const float4 v = o[j * 32];
               acc[4 * j] += v.x, acc[4 * j + 1] += v.y, acc[4 * j + 2] += v.z, acc[4 * j + 3] += v.w;
             }
           }
-          ns_store<T>(p, (NsProduct)f, k, last, x, x.m0 + 32 * (part & 3) + lane, x.n0 + (part >> 2) * 64, acc);
+          ns_store<T>(p, (NsProduct)f, k, last, x, x.m0 + 32 * (part & 3), x.n0 + (part >> 2) * 64, e.patch, nullptr, acc);
         }
       }
       meet();
     }
   }
   if (p.steps == 0) {   // X0 as it is
-    for (int64_t w = blockIdx.x * (int64_t)tc::kThreads + tid; w < n * p.batch; w += (int64_t)gridDim.x * tc::kThreads) {
+    for (int64_t w = b0 * n + rank * (int64_t)tc::kThreads + tid; w < n * (b0 + batch); w += (int64_t)size * tc::kThreads) {
       const int64_t b = w / n, i = w - b * n;
       const size_t o = (size_t)b * 2 * p.X[0].plane + (size_t)(i / p.cols) * p.X[0].pitch + i % p.cols;
       const float v = (__half2float(p.X[0].p[o]) + __half2float(p.X[0].p[p.X[0].plane + o])) * kPlaneInv;
@@ -591,8 +603,9 @@ int choose_splits(int64_t tiles, int k, int sms) {
 
 struct NsLayout {
   size_t status, norms, x, y, gram, poly, parts, total;
-  int units, splits[3];
-  int64_t tiles;   // of the largest product, splits included
+  bool cluster;
+  int splits[3], blocks;
+  int64_t parts_each;
 };
 
 NsLayout ns_layout(const nc_newton_schulz* d) {
@@ -610,23 +623,32 @@ NsLayout ns_layout(const nc_newton_schulz* d) {
     L.total = at;
     return L;
   }
-  const int64_t side = (s + kTile - 1) / kTile, triangle = side * (side + 1) / 2 * d->batch;
-  const int64_t all = (int64_t)((d->rows + kTile - 1) / kTile) * ((d->cols + kTile - 1) / kTile) * d->batch;
+  const int64_t side = (s + kTile - 1) / kTile, triangle = side * (side + 1) / 2;
+  const int64_t all = (int64_t)((d->rows + kTile - 1) / kTile) * ((d->cols + kTile - 1) / kTile);
   const int64_t count[3] = {triangle, triangle, all};
   const int depth[3] = {d->rows < d->cols ? d->cols : d->rows, (int)s, (int)s};
-  int64_t parts = 0;
+  // A cluster's barrier takes a tenth of the grid's; worth it where a cluster's CTAs have a
+  // tile each, or where the matrices fill the SMs
+  L.cluster = all <= kCluster || (int64_t)d->batch * kCluster >= 2 * 148;
+  const int64_t matrices = L.cluster ? 1 : d->batch;
+  int64_t most = 1, parts = 0;
   for (int f = 0; f < 3; ++f) {
-    L.splits[f] = choose_splits(count[f], depth[f], 148);
-    if (count[f] * L.splits[f] > L.tiles) L.tiles = count[f] * L.splits[f];
-    if (L.splits[f] > 1 && count[f] * L.splits[f] > parts) parts = count[f] * L.splits[f];
+    const int64_t tiles = count[f] * matrices;
+    L.splits[f] = choose_splits(tiles, depth[f], L.cluster ? kCluster : 148);
+    if (tiles * L.splits[f] > most) most = tiles * L.splits[f];
+    if (L.splits[f] > 1 && tiles * L.splits[f] > parts) parts = tiles * L.splits[f];
   }
-  L.units = (int)((n + kUnit - 1) / kUnit);
-  L.norms = take((size_t)d->batch * L.units * 8);
+  L.parts_each = parts * kTile * kTile / 4;
+  // as many CTAs as any product keeps busy, or as share the element-wise passes well
+  int64_t blocks = (int64_t)(d->batch * n / (tc::kThreads * 8));
+  if (most > blocks) blocks = most;
+  L.blocks = L.cluster ? kCluster * d->batch : (int)(blocks < 148 ? blocks : 148);
+  L.norms = take((size_t)d->batch * L.blocks * 8);
   L.x = take(d->batch * x * 4);
   L.y = take(d->batch * x * 4);
   L.gram = take(d->batch * g * 4);
   L.poly = take(d->batch * g * 4);
-  L.parts = take((size_t)parts * kTile * kTile * 4);
+  L.parts = take((size_t)L.parts_each * (L.cluster ? d->batch : 1) * 16);
   L.total = at;
   return L;
 }
@@ -676,26 +698,24 @@ nc_status run_tensor(const nc_newton_schulz* d, const T* x, float* momentum, Muo
   NC_CHECK(map(&a.poly, a.Q, s, s, true));
   a.x = x, a.momentum = momentum, a.params = params, a.out = out;
   a.norms = reinterpret_cast<double*>(ws + L.norms), a.parts = reinterpret_cast<float4*>(ws + L.parts);
-  a.batch = d->batch, a.rows = d->rows, a.cols = d->cols, a.steps = d->steps, a.units = L.units;
+  a.parts_each = L.parts_each;
+  a.batch = d->batch, a.rows = d->rows, a.cols = d->cols, a.steps = d->steps;
   for (int f = 0; f < 3; ++f) a.splits[f] = L.splits[f];
-  a.vec = d->cols % 4 == 0;
-  const void* to = params ? static_cast<void*>(params) : static_cast<void*>(out);
-  const size_t size = params ? 4 : sizeof(T);
-  a.wide = reinterpret_cast<uintptr_t>(to) % 32 == 0 && (size_t)d->cols * size % 32 == 0;
   a.a = d->a, a.b = d->b, a.c = d->c, a.eps = d->eps, a.mu = mu, a.decay = decay, a.step = step;
   a.status = reinterpret_cast<int32_t*>(ws + L.status);
-  auto k = ns_kernel<T>;
+  auto k = L.cluster ? ns_kernel<T, true> : ns_kernel<T, false>;
   constexpr int smem = NsEngine::C::kSmem;
   NC_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  // as many CTAs as any phase keeps busy
-  int64_t blocks = (int64_t)d->batch * L.units;
-  if (L.tiles > blocks) blocks = L.tiles;
-  if (blocks > tc::sm_count()) blocks = tc::sm_count();
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeCooperative;
-  attr[0].val.cooperative = 1;
-  cfg.gridDim = dim3((unsigned)blocks), cfg.blockDim = dim3(tc::kThreads);
+  if (L.cluster) {
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = kCluster, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+  } else {
+    attr[0].id = cudaLaunchAttributeCooperative;
+    attr[0].val.cooperative = 1;
+  }
+  cfg.gridDim = dim3((unsigned)L.blocks), cfg.blockDim = dim3(tc::kThreads);
   cfg.dynamicSmemBytes = smem, cfg.stream = st, cfg.attrs = attr, cfg.numAttrs = 1;
   NC_CUDA_CHECK(cudaLaunchKernelEx(&cfg, k, a));
   return launch_check("ns_kernel launch");

@@ -325,9 +325,9 @@ struct ValueEpilogue {
     const float* bias;
   };
   template <int HALF>
-  __device__ __forceinline__ State begin(const tc::Tile&, int row, int col, float* scratch) const {
-    stage_bias<HALF>(bias + col, scratch);
-    return State{scales->w_inv, scales->f_inv, row < a.rows ? a.labels[row] - col : -1, scratch};
+  __device__ __forceinline__ State begin(const tc::Tile&, int row, int col, uint8_t* patch) const {
+    stage_bias<HALF>(bias + col, reinterpret_cast<float*>(patch));
+    return State{scales->w_inv, scales->f_inv, row < a.rows ? a.labels[row] - col : -1, reinterpret_cast<const float*>(patch)};
   }
   template <int HALF>
   __device__ __forceinline__ void run(const State& st, const tc::Tile&, int row, int col, float (&z)[HALF]) const {
@@ -417,24 +417,24 @@ struct DzEpilogue {
   struct State {
     float sw, sf, f, lse;
     int label;
-    const float* bias;
+    uint8_t* patch;   // the bias first
   };
   template <int HALF>
-  __device__ __forceinline__ State begin(const tc::Tile&, int row, int col, float* scratch) const {
-    stage_bias<HALF>(bias + v0 + col, scratch);
+  __device__ __forceinline__ State begin(const tc::Tile&, int row, int col, uint8_t* patch) const {
+    stage_bias<HALF>(bias + v0 + col, reinterpret_cast<float*>(patch));
     const bool in = row < a.rows;
     float f = in ? fac[row] : 0.f, l = in ? lse[row] : 0.f;
     if (f == 0.f)
       l = INFINITY;          // p = 0
     else if (!(l > -INFINITY))
       f = NAN, l = 0.f;      // a bad label, no class left, or NaN among the logits
-    return State{scales->w_inv, scales->f_inv, f, l, in ? a.labels[row] - v0 - col : -1, scratch};
+    return State{scales->w_inv, scales->f_inv, f, l, in ? a.labels[row] - v0 - col : -1, patch};
   }
   template <int HALF>
   __device__ __forceinline__ void run(const State& st, const tc::Tile&, int row, int col, float (&z)[HALF]) const {
 #pragma unroll
     for (int j = 0; j < HALF; j += 4) {
-      const float4 q = *reinterpret_cast<const float4*>(st.bias + j);
+      const float4 q = *reinterpret_cast<const float4*>(st.patch + 4 * j);
       const float b[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -447,28 +447,30 @@ struct DzEpilogue {
       for (int j = 0; j < HALF; ++j)
         if (j == st.label) z[j] -= st.f;
     }
-    if (row < a.rows) {
-      uint16_t* out = dz + (size_t)row * piece + col;
+    const int lane = threadIdx.x & 31, rows = min(32, a.rows - (row - lane));
+    uint16_t* out = dz + (size_t)(row - lane) * piece + col;
 #pragma unroll
-      for (int j = 0; j < HALF; j += 16) {
-        uint32_t h[8], lo[8];
+    for (int j = 0; j < HALF; j += 64) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+      for (int k = 0; k < (BF16 ? 1 : 2); ++k) {   // a plane at a time
+        uint32_t v[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
           const float x = z[j + 2 * i], y = z[j + 2 * i + 1];
           if constexpr (BF16) {
             const __nv_bfloat162 b = __floats2bfloat162_rn(x, y);
-            h[i] = *reinterpret_cast<const uint32_t*>(&b);
+            v[i] = *reinterpret_cast<const uint32_t*>(&b);
           } else {
-            tc::split_f16x2(x * kDzScale, y * kDzScale, &h[i], &lo[i]);
+            uint32_t h, lo;
+            tc::split_f16x2(x * kDzScale, y * kDzScale, &h, &lo);
+            v[i] = k == 0 ? h : lo;
           }
         }
-        tc::store_v8(out + j, h);
-        if constexpr (!BF16) tc::store_v8(out + (size_t)a.rows * piece + j, lo);
+        tc::patch_store(st.patch, v, out + (size_t)k * a.rows * piece + j, piece, rows, 8);
       }
     }
     if (db_part) {
       int first;
-      const int lane = threadIdx.x & 31;
       warp_sums(z, lane, &first);
       float* o = db_part + (size_t)(row / 32) * classes_pad + v0 + col + first;
 #pragma unroll
@@ -485,7 +487,7 @@ struct WeightEpilogue {
   int classes, dim;
   bool wide;       // rows on 32 bytes
   template <int HALF>
-  __device__ __forceinline__ float2 begin(const tc::Tile&, int, int, float*) const {
+  __device__ __forceinline__ float2 begin(const tc::Tile&, int, int, uint8_t*) const {
     return make_float2(scales->f_inv * (sizeof(T) == 4 ? 1.f / kDzScale : 1.f), scales->g);
   }
   template <int HALF>
@@ -529,7 +531,7 @@ struct FeatureEpilogue {
   int rows, dim, pitch, first;
   float mul;
   template <int HALF>
-  __device__ __forceinline__ float begin(const tc::Tile&, int, int, float*) const {
+  __device__ __forceinline__ float begin(const tc::Tile&, int, int, uint8_t*) const {
     return scales->w_inv * mul;
   }
   template <int HALF>

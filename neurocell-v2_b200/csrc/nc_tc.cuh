@@ -26,6 +26,7 @@ namespace tc {
 constexpr int kBM = 128;            // rows of a tile per CTA: one tensor-memory lane each
 constexpr int kEpiWarps = 8;        // two per lane quarter, one per half of the columns
 constexpr int kThreads = 32 * (kEpiWarps + 2);
+constexpr int kPatch = 4096;        // bytes of shared memory of an epilogue warp: 32 rows of 128 bytes
 constexpr int kWaitLimit = 1 << 20; // polls of a bounded wait
 
 // One product of (batched) matrices, D (m, n) = A (m, k) B (n, k)^T.  An operand is stored
@@ -58,7 +59,7 @@ struct Config {
   static constexpr int kA = PL * kBM * kBK * 2, kB = PL * kBRows * kBK * 2;
   static constexpr int kStage = kA + kB;
   static constexpr int kStages = 192 * 1024 / kStage;
-  static constexpr int kSmem = kStages * kStage + 1024;   // stages start on 1024 bytes
+  static constexpr int kSmem = kStages * kStage + kEpiWarps * kPatch + 1024;   // stages start on 1024 bytes
 };
 
 __host__ __device__ inline int problem_tiles(const Problem& p) {
@@ -221,19 +222,22 @@ __device__ __forceinline__ void tmem_load(uint32_t addr, float (&v)[32]) {
       : "memory");
 }
 
-// Shared-memory matrix descriptors: start address, leading and stride byte offsets (16-byte
-// units), descriptor version 1, swizzle mode (2: 128 bytes).
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lead, uint32_t stride, uint32_t swizzle) {
-  return (uint64_t)((addr >> 4) & 0x3fff) | (uint64_t)((lead >> 4) & 0x3fff) << 16 |
-         (uint64_t)((stride >> 4) & 0x3fff) << 32 | (uint64_t)1 << 46 | (uint64_t)swizzle << 61;
+// Shared-memory matrix descriptors: in the low word the start address and the leading byte
+// offset, in the high word the stride byte offset (16-byte units), descriptor version 1 and
+// the swizzle mode (2: rows of 128 bytes).  k contiguous: 8-row groups 1024 bytes apart, 16
+// values of k 32 bytes.  Own index contiguous: blocks of 64 of it `block` bytes apart, each k
+// 128 bytes, 8-k groups 1024 bytes apart, 16 values of k 2048 bytes.
+constexpr uint32_t kDescHigh = 1024 >> 4 | 1u << 14 | 2u << 29;
+__device__ __forceinline__ uint32_t desc_low(uint32_t addr, bool mn, uint32_t block) {
+  return (addr & 0x3ffff) >> 4 | (mn ? block >> 4 : 1u) << 16;   // a cluster address holds the CTA above
 }
+__device__ __forceinline__ uint64_t desc(uint32_t low) { return (uint64_t)kDescHigh << 32 | low; }
 
-// Operand of one plane, 16 values of k from step `ks` on, rows of 128 bytes swizzled over 8.
-// k contiguous: 8-row groups 1024 bytes apart.  Own index contiguous: blocks of 64 of it
-// (`block` bytes apart), each k 128 bytes, 8-k groups 1024 bytes apart.
-__device__ __forceinline__ uint64_t operand_desc(uint32_t base, bool mn, uint32_t block, int ks) {
-  if (mn) return smem_desc(base + ks * 2048, block, 1024, 2);
-  return smem_desc(base + ks * 32, 16, 1024, 2);
+// One lane of a whole warp (always the same one).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p;
 }
 
 // 16-bit planes of a float32 value that was scaled to float16's range.
@@ -249,6 +253,30 @@ __device__ __forceinline__ void split_f16x2(float x, float y, uint32_t* hi, uint
   const float2 b = __half22float2(h);
   const __half2 l = __floats2half2_rn(x - b.x, y - b.y);
   *hi = *reinterpret_cast<const uint32_t*>(&h), *lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+
+// An epilogue thread holds a row, so that its own global accesses would touch 32 rows at a
+// time (a 128-byte line each: they took most of an epilogue).  The warp's patch of shared
+// memory turns them: 16-byte piece q of row r lies at r * 128 + (q ^ (r & 7)) * 16, which
+// is free of bank conflicts by rows and by pieces.
+__device__ __forceinline__ uint4* patch_at(uint8_t* patch, int r, int q) {
+  return reinterpret_cast<uint4*>(patch + r * 128 + ((q ^ (r & 7)) << 4));
+}
+
+// Rows [0, rows) of 64 16-bit values, one per lane in `v` (32 words), to p + row * pitch; the
+// first 8 * pieces values of each.  p and pitch on 16 bytes.
+__device__ __forceinline__ void patch_store(uint8_t* patch, const uint32_t* v, uint16_t* p, int64_t pitch, int rows,
+                                            int pieces) {
+  const int lane = threadIdx.x & 31, q = lane & 7;
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) *patch_at(patch, lane, i) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = i * 4 + (lane >> 3);
+    if (r < rows && q < pieces) *reinterpret_cast<uint4*>(p + r * pitch + 8 * q) = *patch_at(patch, r, q);
+  }
 }
 
 // 32-byte global accesses (one full sector per thread).
@@ -269,7 +297,7 @@ template <int PL, int BN, int CG>
 struct Shared {
   uint64_t bars[2 * Config<PL, BN, CG>::kStages + 5];
   uint32_t tmem_slot;
-  int abort;
+  int abort, extra_readers[Config<PL, BN, CG>::kStages];
 };
 
 // One warp's view of the pipeline: the loading warp fills stages, the multiplying warp (of a
@@ -282,11 +310,15 @@ struct Engine {
   static constexpr uint32_t a_block = C::kA / (kBM / 64), b_block = C::kB / (C::kBRows / 64);
 
   uint32_t stages, bar0, tmem;
+  uint8_t *base, *patch;   // of the stages, and of this epilogue warp
+  int* extra_readers;
   volatile int* abort;
   int32_t* status;
   int rank;
-  int s = 0, buf = 0, issued = 0;
-  uint32_t ph, aph = 1;
+  // stage and its phase (loader and multiplier), accumulator and its phase (multiplier; the
+  // epilogue's is ph), the epilogue's own stage for extra()
+  int s = 0, buf = 0, issued = 0, es = 0;
+  uint32_t ph, aph = 1, eph = 0;
   bool ok = true;
 
   __device__ __forceinline__ uint32_t full(int i) const { return bar0 + 8 * i; }
@@ -298,6 +330,9 @@ struct Engine {
   // By the whole CTA, before it reads anything that an earlier kernel wrote.
   __device__ __forceinline__ Engine(uint8_t* raw, Shared<PL, BN, CG>* sh, int32_t* status_word) {
     stages = (smem_addr(raw) + 1023) & ~1023u;
+    base = raw + (stages - smem_addr(raw));
+    patch = base + C::kStages * C::kStage + (threadIdx.x >> 5) * kPatch;
+    extra_readers = sh->extra_readers;
     bar0 = smem_addr(sh->bars);
     abort = &sh->abort;
     status = status_word;
@@ -308,6 +343,7 @@ struct Engine {
       for (int i = 0; i < C::kStages; ++i) bar_init(full(i), 1), bar_init(empty(i), 1);
       for (int i = 0; i < 2; ++i) bar_init(acc_full(i), 1), bar_init(acc_empty(i), kEpiWarps * CG);
       bar_init(drain(), 1);
+      for (int i = 0; i < C::kStages; ++i) sh->extra_readers[i] = 0;
       sh->abort = 0;
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -345,38 +381,59 @@ struct Engine {
     }
   }
 
-  // One thread of the multiplying warp.
+  // One more stage behind a tile's k-tiles: BN columns (from x.n0 on) of kBM rows of a stored
+  // matrix, both planes, that the epilogue wants (BN = 128, two planes: exactly a stage).  The
+  // multiplying warp steps over it, the epilogue takes it with extra() and extra_done().
+  __device__ __forceinline__ void load_extra(const CUtensorMap* m, const Tile& x) {
+    static_assert(C::kStage == 2 * PL * kBM * 128 && CG == 1, "an extra tile fills a stage");
+    if (!ok || !(ok = bar_wait(empty(s), ph, abort, status))) return;
+    bar_expect(full(s), C::kStage);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      tma_load<CG>(stages + s * C::kStage + i * (C::kStage / 2), m, full(s), x.n0 + 64 * i, x.m0, x.batch);
+    if (issued < C::kStages) ++issued;
+    if (++s == C::kStages) s = 0, ph ^= 1;
+  }
+  __device__ __forceinline__ void skip_extra() {
+    if (++s == C::kStages) s = 0, ph ^= 1;
+  }
+
+  // The multiplying warp, whole: what it computes is the same on all lanes and stays in
+  // uniform registers, and one lane issues (issuing from a lane's own branch cost about 150
+  // cycles a product, more than a 128-wide one takes).
   __device__ __forceinline__ void multiply(const Problem& p, const Tile& x) {
     // accumulator float32; operand types; which operands have their own index contiguous
     const uint32_t idesc = 1u << 4 | (p.bf16 ? 1u << 7 | 1u << 10 : 0u) | (p.a_mn ? 1u << 15 : 0u) |
                            (p.b_mn ? 1u << 16 : 0u) | (uint32_t)(BN >> 3) << 17 | (uint32_t)(kBM * CG >> 4) << 24;
-    const uint32_t a_plane = p.a_mn ? a_block / PL : C::kA / PL, b_plane = p.b_mn ? b_block / PL : C::kB / PL;
-    for (int c0 = x.kt0; c0 < x.kt1 && ok; c0 += p.chunk) {
+    const uint32_t a_plane = (p.a_mn ? a_block / PL : C::kA / PL) >> 4, b_plane = (p.b_mn ? b_block / PL : C::kB / PL) >> 4;
+    const uint32_t a_step = p.a_mn ? 2048 >> 4 : 32 >> 4, b_step = p.b_mn ? 2048 >> 4 : 32 >> 4;
+    const uint32_t a0 = desc_low(stages, p.a_mn, a_block), b0 = desc_low(stages + C::kA, p.b_mn, b_block);
+    for (int c0 = x.kt0; c0 < x.kt1; c0 += p.chunk) {
       if (!(ok = bar_wait(acc_empty(buf), aph, abort, status))) return;
       fence_after();
       const uint32_t d = tmem + buf * BN;
       const int c1 = min(c0 + p.chunk, x.kt1);
-      uint32_t add = 0;
       for (int kt = c0; kt < c1; ++kt) {
         if (!(ok = bar_wait(full(s), ph, abort, status))) return;
         fence_after();
-        const uint32_t at = stages + s * C::kStage, bt = at + C::kA;
-        // low parts first, while the accumulator is small
-        constexpr int kProducts = PL == 1 ? 1 : 3;
+        const uint32_t a = a0 + s * (C::kStage >> 4), b = b0 + s * (C::kStage >> 4);
+        if (elect_one()) {
+          // low parts first, while the accumulator is small
+          constexpr int kProducts = PL == 1 ? 1 : 3;
 #pragma unroll
-        for (int q = 0; q < kProducts; ++q) {
-          const int pa = PL == 1 ? 0 : (q == 0 ? 1 : 0), pb = PL == 1 ? 0 : (q == 1 ? 1 : 0);
+          for (int q = 0; q < kProducts; ++q) {
+            const int pa = PL == 1 ? 0 : (q == 0 ? 1 : 0), pb = PL == 1 ? 0 : (q == 1 ? 1 : 0);
 #pragma unroll
-          for (int ks = 0; ks < BK / 16; ++ks) {
-            mma<CG>(d, operand_desc(at + pa * a_plane, p.a_mn, a_block, ks),
-                    operand_desc(bt + pb * b_plane, p.b_mn, b_block, ks), idesc, add);
-            add = 1;
+            for (int ks = 0; ks < BK / 16; ++ks)
+              mma<CG>(d, desc(a + pa * a_plane + ks * a_step), desc(b + pb * b_plane + ks * b_step), idesc,
+                      kt > c0 || q > 0 || ks > 0);
           }
+          mma_commit<CG>(empty(s));
+          if (kt + 1 == c1) mma_commit<CG>(acc_full(buf));
         }
-        mma_commit<CG>(empty(s));
+        __syncwarp();
         if (++s == C::kStages) s = 0, ph ^= 1;
       }
-      mma_commit<CG>(acc_full(buf));
       buf ^= 1;
       if (buf == 0) aph ^= 1;
     }
@@ -412,6 +469,26 @@ struct Engine {
       buf ^= 1;
       if (buf == 0) ph ^= 1;
     }
+    for (es += x.kt1 - x.kt0; es >= C::kStages; es -= C::kStages) eph ^= 1;
+  }
+
+  // An epilogue warp, after collect(): the extra stage (null after an abort), whose half i holds
+  // 64 columns: plane, row, 128 bytes in 16-byte pieces q ^ (row & 7).  Every epilogue warp calls
+  // extra_done() when it has read its part.
+  __device__ __forceinline__ uint8_t* extra() {
+    if (!__all_sync(0xffffffffu, ok && bar_wait(full(es), eph, abort, status))) {
+      ok = false;
+      return nullptr;
+    }
+    return base + es * C::kStage;
+  }
+  __device__ __forceinline__ void extra_done() {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) {
+      __threadfence_block();
+      if (atomicAdd(extra_readers + es, 1) % kEpiWarps == kEpiWarps - 1) bar_arrive(empty(es));
+    }
+    if (++es == C::kStages) es = 0, eph ^= 1;
   }
 
   // At the end, by the whole CTA.
@@ -425,9 +502,9 @@ struct Engine {
         }
       }
     }
-    if (warp == kEpiWarps + 1 && lane == 0 && rank == 0) {
+    if (warp == kEpiWarps + 1 && rank == 0) {
       // every product has finished before tensor memory is given back
-      mma_commit<CG>(drain());
+      if (elect_one()) mma_commit<CG>(drain());
       for (int j = 0; j < kWaitLimit && !bar_try(drain(), 0); ++j) {
       }
     }
@@ -443,13 +520,12 @@ struct Engine {
 
 // The kernel of one product: warps 0..7 epilogue, warp 8 loads, warp 9 multiplies; persistent
 // over tiles.  Epi::run(state, tile, row, col, acc) gets a row's BN / 2 consecutive columns as
-// float32 sums; Epi::begin(tile, row, col, scratch) runs before the wait for them and returns
-// the state (scratch: BN / 2 floats of the warp).
+// float32 sums; Epi::begin(tile, row, col, patch) runs before the wait for them and returns the
+// state.
 template <int PL, int BN, int CG, class Epi>
 __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_constant__ Problem p, const Epi epi) {
   using E = Engine<PL, BN, CG>;
   extern __shared__ uint8_t raw[];
-  __shared__ __align__(16) float scratch[kEpiWarps][E::HALF];
   __shared__ Shared<PL, BN, CG> sh;
   E e(raw, &sh, p.status);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -459,14 +535,14 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
     if (lane == 0)
       for (int t = first; t < tiles && e.ok; t += stride) e.load(p, &p.a, &p.b, problem_tile<PL, BN, CG>(p, t, e.rank));
   } else if (warp == kEpiWarps + 1) {
-    if (lane == 0 && e.rank == 0)
+    if (e.rank == 0)
       for (int t = first; t < tiles && e.ok; t += stride) e.multiply(p, problem_tile<PL, BN, CG>(p, t, 0));
   } else {
     for (int t = first; t < tiles && e.ok; t += stride) {
       const Tile x = problem_tile<PL, BN, CG>(p, t, e.rank);
       const int row = x.m0 + 32 * (warp & 3) + lane, col = x.n0 + (warp >> 2) * E::HALF;
-      __syncwarp();   // the last tile's readers of scratch are done
-      const auto state = epi.template begin<E::HALF>(x, row, col, scratch[warp]);
+      __syncwarp();   // the last tile's readers of the patch are done
+      const auto state = epi.template begin<E::HALF>(x, row, col, e.patch);
       __syncwarp();
       float acc[E::HALF];
       e.collect(p, x, acc);
