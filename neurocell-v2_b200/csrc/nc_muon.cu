@@ -261,7 +261,9 @@ nc_status launch_small(const SmallArgs& a, const SmallPlan& r, int batch, cudaSt
 constexpr float kPlaneScale = 4096.f, kPlaneInv = 1.f / 4096.f;
 constexpr int kTile = 128;   // square tiles: at most sizes the number of tiles matters more than a tile's rate
 constexpr int kNsChunk = 1;  // k-tiles (of 64) per accumulator: Gram sums of one sign show the additions' truncation
-using NsEngine = tc::Engine<2, kTile, 1>;
+using NsEngine = tc::Engine<2, kTile, 1, 16>;
+constexpr int kNsCols = NsEngine::COLS, kNsWarps = NsEngine::kEpiWarps, kNsThreads = NsEngine::C::kThreads;
+static_assert(kNsCols == 32, "an epilogue thread takes 32 columns");
 
 struct Planes {   // (batch, plane, rows, pitch)
   __half* p;
@@ -302,15 +304,15 @@ __device__ __forceinline__ float source(const NsArgs& p, size_t o) {
   return p.mu.nesterov ? fmaf(p.mu.beta, m, x) : m;
 }
 
-// The transposed store of 32 rows (a lane each) and 64 columns: through the warp's patch, as 64
+// The transposed store of 32 rows (a lane each) and 32 columns: through the warp's patch, as 32
 // rows of 64 bytes.  `rows`, `cols`: how many of them exist; what lies behind a row's end is
 // padding.
 __device__ __forceinline__ void store_mirrored(uint8_t* patch, __half* p, int64_t pitch, int rows, int cols,
-                                               const uint32_t (&v)[32]) {
+                                               const uint32_t (&v)[16]) {
   const int lane = threadIdx.x & 31, odd = lane & 1;
   __syncwarp();
 #pragma unroll
-  for (int i = 0; i < 32; ++i) {
+  for (int i = 0; i < 16; ++i) {
     // pairs of lanes exchange: an even one gets both rows of column 2 i, an odd one of 2 i + 1
     const uint32_t other = __shfl_xor_sync(0xffffffffu, v[i], 1);
     const uint32_t two = odd ? __byte_perm(other, v[i], 0x7632) : __byte_perm(v[i], other, 0x5410);
@@ -318,18 +320,18 @@ __device__ __forceinline__ void store_mirrored(uint8_t* patch, __half* p, int64_
   }
   __syncwarp();
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < 4; ++i) {
     const int c = i * 8 + (lane >> 2), q = lane & 3;
     if (c < cols && 8 * q < rows)
       *reinterpret_cast<uint4*>(p + c * pitch + 8 * q) = *reinterpret_cast<const uint4*>(patch + c * 64 + 16 * q);
   }
 }
 
-// acc += add times a row's 64 values of one plane, in 16-byte pieces at `at(i)`.
+// acc += add times a row's 32 values of one plane, in 16-byte pieces at `at(i)`.
 template <typename At>
-__device__ __forceinline__ void add_row(At at, float add, float (&acc)[64]) {
+__device__ __forceinline__ void add_row(At at, float add, float (&acc)[32]) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < 4; ++i) {
     const uint4 w = *reinterpret_cast<const uint4*>(at(i));
     const uint32_t x[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
@@ -341,58 +343,59 @@ __device__ __forceinline__ void add_row(At at, float add, float (&acc)[64]) {
   }
 }
 
-// acc += add times 32 rows and 64 columns of both planes in global memory.
+// acc += add times 32 rows and 32 columns of both planes in global memory.
 __device__ __forceinline__ void add_planes(uint8_t* patch, const Planes& s, size_t at, int rows, int cols, float add,
-                                           float (&acc)[64]) {
-  const int lane = threadIdx.x & 31, q = lane & 7;
+                                           float (&acc)[32]) {
+  const int lane = threadIdx.x & 31, q = lane & 3;
+  uint4 v[2][4];
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = i * 8 + (lane >> 2);
+      v[k][i] = r < rows && 8 * q < cols ? *reinterpret_cast<const uint4*>(s.p + k * s.plane + at + (size_t)r * s.pitch + 8 * q)
+                                         : make_uint4(0, 0, 0, 0);
+    }
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
-    uint4 v[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int r = i * 4 + (lane >> 3);
-      v[i] = r < rows && 8 * q < cols ? *reinterpret_cast<const uint4*>(s.p + k * s.plane + at + (size_t)r * s.pitch + 8 * q)
-                                      : make_uint4(0, 0, 0, 0);
-    }
     __syncwarp();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) *tc::patch_at(patch, i * 4 + (lane >> 3), q) = v[i];
+    for (int i = 0; i < 4; ++i) *tc::patch_at<32>(patch, i * 8 + (lane >> 2), q) = v[k][i];
     __syncwarp();
-    add_row([&](int i) { return tc::patch_at(patch, lane, i); }, add, acc);
+    add_row([&](int i) { return tc::patch_at<32>(patch, lane, i); }, add, acc);
   }
 }
 
-// Result of a product for 32 rows from row0 on and 64 columns from col on, on scaled values:
+// Result of a product for 32 rows from row0 on and 32 columns from col on, on scaled values:
 // mul acc + add (A or X), to planes (and mirrored), or (last) unscaled to the caller.  `prior`:
 // the tile of A or X in shared memory (Engine::extra), or null to take it from global memory.
 template <typename T>
 __device__ __forceinline__ void ns_store(const NsArgs& p, NsProduct product, int k, bool last, const tc::Tile& x,
-                                         int row0, int col, uint8_t* patch, const uint8_t* prior, float (&acc)[64]) {
+                                         int row0, int col, uint8_t* patch, const uint8_t* prior, float (&acc)[32]) {
   const Planes& dst = product == kGram ? p.G : product == kPoly ? p.Q : p.X[(k + 1) & 1];
   const int s = min(p.rows, p.cols), m = product == kUpdate ? p.rows : s, n = product == kUpdate ? p.cols : s;
-  const int lane = threadIdx.x & 31, rows = min(32, m - row0), cols = min(64, n - col);
+  const int lane = threadIdx.x & 31, rows = min(32, m - row0), cols = min(32, n - col);
   const size_t at = (size_t)x.batch * 2 * dst.plane + (size_t)row0 * dst.pitch + col;
-  const float mul = product == kPoly ? p.c * kPlaneInv : kPlaneInv;
+  const float mul = product == kPoly ? p.c * kPlaneInv : kPlaneInv, add = product == kPoly ? p.b : p.a;
+  if (rows <= 0 || cols <= 0) return;   // the same for the whole warp
 #pragma unroll
-  for (int j = 0; j < 64; ++j) acc[j] *= mul;
-  const float add = product == kPoly ? p.b : p.a;
+  for (int j = 0; j < 32; ++j) acc[j] *= mul;
   if (product != kGram && prior) {
-    const int r = row0 - x.m0 + lane;
-    const uint8_t* half = prior + (col - x.n0) / 64 * (NsEngine::C::kStage / 2) + r * 128;
+    const int r = row0 - x.m0 + lane, c = col - x.n0;
+    const uint8_t* half = prior + c / 64 * (NsEngine::C::kStage / 2) + r * 128;
 #pragma unroll
-    for (int k2 = 0; k2 < 2; ++k2)
-      add_row([&](int i) { return half + k2 * (kTile * 128) + ((i ^ (r & 7)) << 4); }, add, acc);
+    for (int h = 0; h < 2; ++h)
+      add_row([&](int i) { return half + h * (kTile * 128) + (((c % 64 / 8 + i) ^ (r & 7)) << 4); }, add, acc);
   } else if (product != kGram) {
     add_planes(patch, product == kPoly ? p.G : p.X[k & 1], at, rows, cols, add, acc);
   }
-  if (row0 >= m || col >= n) return;   // the same for the whole warp
   if (!last) {
-    uint32_t h[32], l[32];
+    uint32_t h[16], l[16];
 #pragma unroll
-    for (int i = 0; i < 32; ++i) tc::split_f16x2(acc[2 * i], acc[2 * i + 1], &h[i], &l[i]);
-    uint16_t* d = reinterpret_cast<uint16_t*>(dst.p);
-    tc::patch_store(patch, h, d + at, dst.pitch, rows, (cols + 7) / 8);
-    tc::patch_store(patch, l, d + dst.plane + at, dst.pitch, rows, (cols + 7) / 8);
+    for (int i = 0; i < 16; ++i) tc::split_f16x2(acc[2 * i], acc[2 * i + 1], &h[i], &l[i]);
+    uint16_t* d = reinterpret_cast<uint16_t*>(dst.p) + at;
+    tc::patch_store<32>(patch, h, d, dst.pitch, rows, (cols + 7) / 8);
+    tc::patch_store<32>(patch, l, d + dst.plane, dst.pitch, rows, (cols + 7) / 8);
     if (product != kUpdate && x.n0 > x.m0) {
       __half* t = dst.p + (size_t)x.batch * 2 * dst.plane + (size_t)col * dst.pitch + row0;
       store_mirrored(patch, t, dst.pitch, rows, cols, h);
@@ -400,19 +403,20 @@ __device__ __forceinline__ void ns_store(const NsArgs& p, NsProduct product, int
     }
     return;
   }
-  // 32 columns at a time, a row per access
+  // 16 columns at a time, two rows per access
   float* f = reinterpret_cast<float*>(patch);
 #pragma unroll
   for (int g = 0; g < 2; ++g) {
     __syncwarp();
 #pragma unroll
-    for (int j = 0; j < 32; ++j) f[lane * 32 + (j ^ lane)] = acc[32 * g + j] * kPlaneInv;
+    for (int j = 0; j < 16; ++j) f[lane * 16 + (j ^ (lane & 15))] = acc[16 * g + j] * kPlaneInv;
     __syncwarp();
-    if (32 * g + lane < cols) {
-      const size_t o = ((size_t)x.batch * m + row0) * n + col + 32 * g + lane;
+    const int c = lane & 15;
+    if (16 * g + c < cols) {
+      const size_t o = ((size_t)x.batch * m + row0) * n + col + 16 * g + c;
 #pragma unroll 8
-      for (int r = 0; r < rows; ++r) {
-        const float v = f[r * 32 + (lane ^ r)];
+      for (int r = lane >> 4; r < rows; r += 2) {
+        const float v = f[r * 16 + (c ^ (r & 15))];
         if (p.params)
           p.params[o + (size_t)r * n] = p.params[o + (size_t)r * n] * p.decay - p.step * v;
         else
@@ -423,10 +427,10 @@ __device__ __forceinline__ void ns_store(const NsArgs& p, NsProduct product, int
 }
 
 template <typename T, bool CLUSTER>
-__global__ void __launch_bounds__(tc::kThreads, 1) ns_kernel(const __grid_constant__ NsArgs p) {
+__global__ void __launch_bounds__(kNsThreads, 1) ns_kernel(const __grid_constant__ NsArgs p) {
   extern __shared__ uint8_t raw[];
-  __shared__ tc::Shared<2, kTile, 1> sh;
-  __shared__ double red[tc::kThreads / 32];
+  __shared__ tc::Shared<2, kTile, 1, kNsWarps> sh;
+  __shared__ double red[kNsThreads / 32];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (blockIdx.x == 0 && tid == 0) *p.status = 0;
   NsEngine e(raw, &sh, p.status);
@@ -444,7 +448,7 @@ __global__ void __launch_bounds__(tc::kThreads, 1) ns_kernel(const __grid_consta
     asm volatile("fence.proxy.async;" ::: "memory");
   };
   auto tile = [&](const tc::Problem& q, int t) {
-    tc::Tile x = tc::problem_tile<2, kTile, 1>(q, t, 0);
+    tc::Tile x = tc::problem_tile<kTile, 1>(q, t, 0);
     x.batch += b0;
     return x;
   };
@@ -456,7 +460,7 @@ __global__ void __launch_bounds__(tc::kThreads, 1) ns_kernel(const __grid_consta
     const size_t o = (size_t)b * n;
     double sum = 0.0;
 #pragma unroll 4
-    for (int64_t i = (int64_t)rank * tc::kThreads + tid; i < n; i += (int64_t)size * tc::kThreads) {
+    for (int64_t i = (int64_t)rank * kNsThreads + tid; i < n; i += (int64_t)size * kNsThreads) {
       if (p.momentum) p.momentum[o + i] = fmaf(p.mu.beta, p.momentum[o + i], to_f32(static_cast<const T*>(p.x)[o + i]));
       const float u = source<T>(p, o + i);
       sum += (double)u * u;
@@ -469,7 +473,7 @@ __global__ void __launch_bounds__(tc::kThreads, 1) ns_kernel(const __grid_consta
   // X0 as planes; every CTA adds up a matrix's parts, in order
   for (int b = b0; b < b0 + batch; ++b) {
     double sum = 0.0;
-    for (int j = tid; j < size; j += tc::kThreads) sum += p.norms[(size_t)b * size + j];
+    for (int j = tid; j < size; j += kNsThreads) sum += p.norms[(size_t)b * size + j];
     __syncthreads();
     sum = block_sum_f64(sum, red);
     const double inv = 1.0 / (sqrt(sum) + p.eps);
@@ -478,7 +482,7 @@ __global__ void __launch_bounds__(tc::kThreads, 1) ns_kernel(const __grid_consta
     const int pairs = (p.cols + 1) / 2;   // two columns at a time
     const int64_t all = (int64_t)p.rows * pairs;
 #pragma unroll 4
-    for (int64_t i = (int64_t)rank * tc::kThreads + tid; i < all; i += (int64_t)size * tc::kThreads) {
+    for (int64_t i = (int64_t)rank * kNsThreads + tid; i < all; i += (int64_t)size * kNsThreads) {
       const int r = (int)((uint32_t)i / (uint32_t)pairs), c = 2 * ((int)i - r * pairs);
       const size_t at = from + (size_t)r * p.cols + c;
       const float v = (float)((double)source<T>(p, at) * inv) * kPlaneScale;
@@ -510,7 +514,7 @@ __global__ void __launch_bounds__(tc::kThreads, 1) ns_kernel(const __grid_consta
       const bool last = f == kUpdate && k + 1 == p.steps;
       const int tiles = tc::problem_tiles(q);
       const bool extra = f != kGram && q.splits == 1;
-      if (warp == tc::kEpiWarps) {
+      if (warp == kNsWarps) {
         if (lane == 0) {
           for (int t = rank; t < tiles && e.ok; t += size) {
             const tc::Tile x = tile(q, t);
@@ -518,7 +522,7 @@ __global__ void __launch_bounds__(tc::kThreads, 1) ns_kernel(const __grid_consta
             if (extra) e.load_extra(f == kPoly ? &p.gram : xk, x);
           }
         }
-      } else if (warp == tc::kEpiWarps + 1) {
+      } else if (warp == kNsWarps + 1) {
         for (int t = rank; t < tiles && e.ok; t += size) {
           e.multiply(q, tile(q, t));
           if (extra) e.skip_extra();
@@ -526,17 +530,19 @@ __global__ void __launch_bounds__(tc::kThreads, 1) ns_kernel(const __grid_consta
       } else {
         for (int t = rank; t < tiles && e.ok; t += size) {
           const tc::Tile x = tile(q, t);
-          float acc[64];
+          float acc[kNsCols];
           e.collect(q, x, acc);
           if (!e.ok) break;
           if (q.splits > 1) {
-            float4* o = parts + ((size_t)t * tc::kEpiWarps + warp) * 16 * 32 + lane;
+            float4* o = parts + ((size_t)t * kNsWarps + warp) * (kNsCols * 8) + lane;
 #pragma unroll
-            for (int j = 0; j < 16; ++j) o[j * 32] = make_float4(acc[4 * j], acc[4 * j + 1], acc[4 * j + 2], acc[4 * j + 3]);
+            for (int j = 0; j < kNsCols / 4; ++j)
+              o[j * 32] = make_float4(acc[4 * j], acc[4 * j + 1], acc[4 * j + 2], acc[4 * j + 3]);
           } else {
             const uint8_t* prior = extra ? e.extra() : nullptr;
             if (!e.ok) break;
-            ns_store<T>(p, (NsProduct)f, k, last, x, x.m0 + 32 * (warp & 3), x.n0 + (warp >> 2) * 64, e.patch, prior, acc);
+            ns_store<T>(p, (NsProduct)f, k, last, x, x.m0 + 32 * (warp & 3), x.n0 + (warp >> 2) * kNsCols, e.patch, prior,
+                        acc);
             if (extra) e.extra_done();
           }
         }
@@ -544,31 +550,32 @@ __global__ void __launch_bounds__(tc::kThreads, 1) ns_kernel(const __grid_consta
       __syncwarp();
       meet();
       if (q.splits == 1) continue;
-      // the parts of a tile are tiles / splits apart; a warp sums its 32 rows and 64 columns
+      // the parts of a tile are tiles / splits apart; a warp sums its 32 rows and columns
       const int whole = tiles / q.splits;
-      if (warp < tc::kEpiWarps) {
-        for (int w = rank * tc::kEpiWarps + warp; w < whole * tc::kEpiWarps; w += size * tc::kEpiWarps) {
-          const int t = w / tc::kEpiWarps, part = w % tc::kEpiWarps;
+      if (warp < kNsWarps) {
+        for (int w = rank * kNsWarps + warp; w < whole * kNsWarps; w += size * kNsWarps) {
+          const int t = w / kNsWarps, part = w % kNsWarps;
           const tc::Tile x = tile(q, t);
-          float acc[64];
+          float acc[kNsCols];
 #pragma unroll
-          for (int j = 0; j < 64; ++j) acc[j] = 0.f;
+          for (int j = 0; j < kNsCols; ++j) acc[j] = 0.f;
           for (int g = 0; g < q.splits; ++g) {
-            const float4* o = parts + ((size_t)(t + g * whole) * tc::kEpiWarps + part) * 16 * 32 + lane;
+            const float4* o = parts + ((size_t)(t + g * whole) * kNsWarps + part) * (kNsCols * 8) + lane;
+            float4 v[kNsCols / 4];
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              const float4 v = o[j * 32];
-              acc[4 * j] += v.x, acc[4 * j + 1] += v.y, acc[4 * j + 2] += v.z, acc[4 * j + 3] += v.w;
-            }
+            for (int j = 0; j < kNsCols / 4; ++j) v[j] = __ldcg(o + j * 32);
+#pragma unroll
+            for (int j = 0; j < kNsCols / 4; ++j)
+              acc[4 * j] += v[j].x, acc[4 * j + 1] += v[j].y, acc[4 * j + 2] += v[j].z, acc[4 * j + 3] += v[j].w;
           }
-          ns_store<T>(p, (NsProduct)f, k, last, x, x.m0 + 32 * (part & 3), x.n0 + (part >> 2) * 64, e.patch, nullptr, acc);
+          ns_store<T>(p, (NsProduct)f, k, last, x, x.m0 + 32 * (part & 3), x.n0 + (part >> 2) * kNsCols, e.patch, nullptr, acc);
         }
       }
       meet();
     }
   }
   if (p.steps == 0) {   // X0 as it is
-    for (int64_t w = b0 * n + rank * (int64_t)tc::kThreads + tid; w < n * (b0 + batch); w += (int64_t)size * tc::kThreads) {
+    for (int64_t w = b0 * n + rank * (int64_t)kNsThreads + tid; w < n * (b0 + batch); w += (int64_t)size * kNsThreads) {
       const int64_t b = w / n, i = w - b * n;
       const size_t o = (size_t)b * 2 * p.X[0].plane + (size_t)(i / p.cols) * p.X[0].pitch + i % p.cols;
       const float v = (__half2float(p.X[0].p[o]) + __half2float(p.X[0].p[p.X[0].plane + o])) * kPlaneInv;
@@ -588,14 +595,14 @@ bool on_tensor_cores(const nc_newton_schulz* d) { return !small_plan(d).fits; }
 int plane_pitch(int cols) { return (cols + 63) / 64 * 64; }
 
 // Tiles of a product and its splits along k: as many as shorten the longest SM's k-tiles by
-// more than the sum costs (about 3 k-tiles' time for the extra meeting, and the parts' traffic).
+// more than the sum costs (an extra meeting and a pass over the parts, about 8 k-tiles' time).
 int choose_splits(int64_t tiles, int k, int sms) {
   auto ceil_div = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
   const int64_t kt = ceil_div(k, NsEngine::BK);
   int64_t best = ceil_div(tiles, sms) * kt;
   int splits = 1;
   for (int s = 2; s <= 32 && s <= kt; ++s) {
-    const int64_t cost = ceil_div(tiles * s, sms) * ceil_div(kt, s) + 3 + s / 4;
+    const int64_t cost = ceil_div(tiles * s, sms) * ceil_div(kt, s) + 8 + s / 4;
     if (cost < best) best = cost, splits = s;
   }
   return splits;
@@ -640,7 +647,7 @@ NsLayout ns_layout(const nc_newton_schulz* d) {
   }
   L.parts_each = parts * kTile * kTile / 4;
   // as many CTAs as any product keeps busy, or as share the element-wise passes well
-  int64_t blocks = (int64_t)(d->batch * n / (tc::kThreads * 8));
+  int64_t blocks = (int64_t)(d->batch * n / (kNsThreads * 8));
   if (most > blocks) blocks = most;
   L.blocks = L.cluster ? kCluster * d->batch : (int)(blocks < 148 ? blocks : 148);
   L.norms = take((size_t)d->batch * L.blocks * 8);
@@ -715,7 +722,7 @@ nc_status run_tensor(const nc_newton_schulz* d, const T* x, float* momentum, Muo
     attr[0].id = cudaLaunchAttributeCooperative;
     attr[0].val.cooperative = 1;
   }
-  cfg.gridDim = dim3((unsigned)L.blocks), cfg.blockDim = dim3(tc::kThreads);
+  cfg.gridDim = dim3((unsigned)L.blocks), cfg.blockDim = dim3(kNsThreads);
   cfg.dynamicSmemBytes = smem, cfg.stream = st, cfg.attrs = attr, cfg.numAttrs = 1;
   NC_CUDA_CHECK(cudaLaunchKernelEx(&cfg, k, a));
   return launch_check("ns_kernel launch");

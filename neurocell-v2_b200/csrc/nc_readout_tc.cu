@@ -302,10 +302,10 @@ __device__ __forceinline__ float exp_near(float d) {
 }
 
 // The tile's bias into the warp's scratch.
-template <int HALF>
+template <int COLS>
 __device__ __forceinline__ void stage_bias(const float* bias, float* scratch) {
   const int lane = threadIdx.x & 31;
-  if constexpr (HALF == 128)
+  if constexpr (COLS == 128)
     reinterpret_cast<float4*>(scratch)[lane] = reinterpret_cast<const float4*>(bias)[lane];
   else
     reinterpret_cast<float2*>(scratch)[lane] = reinterpret_cast<const float2*>(bias)[lane];
@@ -324,16 +324,16 @@ struct ValueEpilogue {
     int label;            // within the half tile, or out of it
     const float* bias;
   };
-  template <int HALF>
+  template <int COLS>
   __device__ __forceinline__ State begin(const tc::Tile&, int row, int col, uint8_t* patch) const {
-    stage_bias<HALF>(bias + col, reinterpret_cast<float*>(patch));
+    stage_bias<COLS>(bias + col, reinterpret_cast<float*>(patch));
     return State{scales->w_inv, scales->f_inv, row < a.rows ? a.labels[row] - col : -1, reinterpret_cast<const float*>(patch)};
   }
-  template <int HALF>
-  __device__ __forceinline__ void run(const State& st, const tc::Tile&, int row, int col, float (&z)[HALF]) const {
+  template <int COLS>
+  __device__ __forceinline__ void run(const State& st, const tc::Tile&, int row, int col, float (&z)[COLS]) const {
     float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int j = 0; j < HALF; j += 4) {
+    for (int j = 0; j < COLS; j += 4) {
       const float4 q = *reinterpret_cast<const float4*>(st.bias + j);
       const float b[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
@@ -343,17 +343,17 @@ struct ValueEpilogue {
       }
     }
     const float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), base = top == -INFINITY ? 0.f : top;
-    const bool mine = st.label >= 0 && st.label < HALF;
+    const bool mine = st.label >= 0 && st.label < COLS;
     float zl = 0.f;
     if (__any_sync(0xffffffffu, mine)) {
 #pragma unroll
-      for (int j = 0; j < HALF; ++j)
+      for (int j = 0; j < COLS; ++j)
         if (j == st.label) zl = z[j];
     }
 #pragma unroll
-    for (int j = 0; j < HALF; ++j) s[j & 3] += exp_fast(z[j] - base);
+    for (int j = 0; j < COLS; ++j) s[j & 3] += exp_fast(z[j] - base);
     if (row >= a.rows) return;
-    part[(size_t)(col / HALF) * rows_pad + row] = make_float2(top, (s[0] + s[1]) + (s[2] + s[3]));
+    part[(size_t)(col / COLS) * rows_pad + row] = make_float2(top, (s[0] + s[1]) + (s[2] + s[3]));
     if (mine) zlabel[row] = zl;
   }
 };
@@ -419,9 +419,9 @@ struct DzEpilogue {
     int label;
     uint8_t* patch;   // the bias first
   };
-  template <int HALF>
+  template <int COLS>
   __device__ __forceinline__ State begin(const tc::Tile&, int row, int col, uint8_t* patch) const {
-    stage_bias<HALF>(bias + v0 + col, reinterpret_cast<float*>(patch));
+    stage_bias<COLS>(bias + v0 + col, reinterpret_cast<float*>(patch));
     const bool in = row < a.rows;
     float f = in ? fac[row] : 0.f, l = in ? lse[row] : 0.f;
     if (f == 0.f)
@@ -430,10 +430,10 @@ struct DzEpilogue {
       f = NAN, l = 0.f;      // a bad label, no class left, or NaN among the logits
     return State{scales->w_inv, scales->f_inv, f, l, in ? a.labels[row] - v0 - col : -1, patch};
   }
-  template <int HALF>
-  __device__ __forceinline__ void run(const State& st, const tc::Tile&, int row, int col, float (&z)[HALF]) const {
+  template <int COLS>
+  __device__ __forceinline__ void run(const State& st, const tc::Tile&, int row, int col, float (&z)[COLS]) const {
 #pragma unroll
-    for (int j = 0; j < HALF; j += 4) {
+    for (int j = 0; j < COLS; j += 4) {
       const float4 q = *reinterpret_cast<const float4*>(st.patch + 4 * j);
       const float b[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
@@ -442,15 +442,15 @@ struct DzEpilogue {
         z[j + e] = st.f * (BF16 ? exp_fast(d) : exp_near(d));
       }
     }
-    if (__any_sync(0xffffffffu, st.label >= 0 && st.label < HALF)) {
+    if (__any_sync(0xffffffffu, st.label >= 0 && st.label < COLS)) {
 #pragma unroll
-      for (int j = 0; j < HALF; ++j)
+      for (int j = 0; j < COLS; ++j)
         if (j == st.label) z[j] -= st.f;
     }
     const int lane = threadIdx.x & 31, rows = min(32, a.rows - (row - lane));
     uint16_t* out = dz + (size_t)(row - lane) * piece + col;
 #pragma unroll
-    for (int j = 0; j < HALF; j += 64) {
+    for (int j = 0; j < COLS; j += 64) {
 #pragma unroll
       for (int k = 0; k < (BF16 ? 1 : 2); ++k) {   // a plane at a time
         uint32_t v[32];
@@ -466,7 +466,7 @@ struct DzEpilogue {
             v[i] = k == 0 ? h : lo;
           }
         }
-        tc::patch_store(st.patch, v, out + (size_t)k * a.rows * piece + j, piece, rows, 8);
+        tc::patch_store<64>(st.patch, v, out + (size_t)k * a.rows * piece + j, piece, rows, 8);
       }
     }
     if (db_part) {
@@ -474,7 +474,7 @@ struct DzEpilogue {
       warp_sums(z, lane, &first);
       float* o = db_part + (size_t)(row / 32) * classes_pad + v0 + col + first;
 #pragma unroll
-      for (int i = 0; i < HALF / 32; ++i) o[i] = z[i];
+      for (int i = 0; i < COLS / 32; ++i) o[i] = z[i];
     }
   }
 };
@@ -486,17 +486,17 @@ struct WeightEpilogue {
   T* out;          // of the piece's first class
   int classes, dim;
   bool wide;       // rows on 32 bytes
-  template <int HALF>
+  template <int COLS>
   __device__ __forceinline__ float2 begin(const tc::Tile&, int, int, uint8_t*) const {
     return make_float2(scales->f_inv * (sizeof(T) == 4 ? 1.f / kDzScale : 1.f), scales->g);
   }
-  template <int HALF>
-  __device__ __forceinline__ void run(float2 st, const tc::Tile&, int row, int col, float (&v)[HALF]) const {
+  template <int COLS>
+  __device__ __forceinline__ void run(float2 st, const tc::Tile&, int row, int col, float (&v)[COLS]) const {
     if (row >= classes) return;
     const float s = st.x, g = st.y;
     T* o = out + (size_t)row * dim + col;
 #pragma unroll
-    for (int j = 0; j < HALF; j += 16) {
+    for (int j = 0; j < COLS; j += 16) {
       if (col + j >= dim) break;
       if (wide && col + j + 16 <= dim) {
         uint32_t q[8];
@@ -530,16 +530,16 @@ struct FeatureEpilogue {
   float* part;     // (splits, rows, pitch)
   int rows, dim, pitch, first;
   float mul;
-  template <int HALF>
+  template <int COLS>
   __device__ __forceinline__ float begin(const tc::Tile&, int, int, uint8_t*) const {
     return scales->w_inv * mul;
   }
-  template <int HALF>
-  __device__ __forceinline__ void run(float s, const tc::Tile& x, int row, int col, float (&v)[HALF]) const {
+  template <int COLS>
+  __device__ __forceinline__ void run(float s, const tc::Tile& x, int row, int col, float (&v)[COLS]) const {
     if (row >= rows) return;
     float* o = part + ((size_t)x.split * rows + row) * pitch + col;
 #pragma unroll
-    for (int j = 0; j < HALF; j += 8) {
+    for (int j = 0; j < COLS; j += 8) {
       if (col + j >= dim) break;   // the pitch is whole 8s
       uint32_t q[8];
       if (!first) tc::load_v8(o + j, q);
@@ -595,7 +595,7 @@ struct Call {
   Scales* scales() const { return at<Scales>(p.scales); }
   int32_t* status() const { return reinterpret_cast<int32_t*>(at<Scales>(p.scales) + 1); }
 
-  template <int BN, int CG>
+  template <int BN, int CG, int EW>
   tc::Problem problem(int m, int n, int k, int splits) const {
     tc::Problem q{};
     q.m = m, q.n = n, q.k = k, q.batch = 1, q.splits = splits, q.bf16 = p.bf16;
@@ -607,23 +607,23 @@ struct Call {
 
   // Operands: rows of features or weight (k = dim contiguous), or with their columns as the
   // own index and rows as k.
-  template <int BN, int CG>
+  template <int BN, int CG, int EW>
   nc_status features_op(tc::Problem* q, bool is_a, bool by_column) const {
-    return tc::make_operand<PL, BN, CG>(q, is_a, at<void>(p.f), by_column, by_column ? d->dim : d->rows,
+    return tc::make_operand<PL, BN, CG, EW>(q, is_a, at<void>(p.f), by_column, by_column ? d->dim : d->rows,
                                     by_column ? d->rows : d->dim, p.pitch, (int64_t)d->rows * p.pitch, 1,
                                     (int64_t)PL * d->rows * p.pitch);
   }
-  template <int BN, int CG>
+  template <int BN, int CG, int EW>
   nc_status weight_op(tc::Problem* q, bool by_column) const {
     const void* base = p.copy_w ? at<void>(p.w) : a.weight;
     const int pitch = p.copy_w ? p.pitch : d->dim;
-    return tc::make_operand<PL, BN, CG>(q, false, base, by_column, by_column ? d->dim : d->classes,
+    return tc::make_operand<PL, BN, CG, EW>(q, false, base, by_column, by_column ? d->dim : d->classes,
                                     by_column ? d->classes : d->dim, pitch, (int64_t)d->classes * pitch, 1,
                                     (int64_t)PL * d->classes * pitch);
   }
-  template <int BN, int CG>
+  template <int BN, int CG, int EW>
   nc_status dz_op(tc::Problem* q, bool by_column) const {
-    return tc::make_operand<PL, BN, CG>(q, true, at<void>(p.dz), by_column, by_column ? p.piece : d->rows,
+    return tc::make_operand<PL, BN, CG, EW>(q, true, at<void>(p.dz), by_column, by_column ? p.piece : d->rows,
                                     by_column ? d->rows : p.piece, p.piece, (int64_t)d->rows * p.piece, 1,
                                     (int64_t)PL * d->rows * p.piece);
   }
@@ -647,17 +647,17 @@ struct Call {
     return launch_check("ce_planes_kernel launch");
   }
 
-  template <int BN, int CG>
+  template <int BN, int CG, int EW>
   nc_status value_product() const {
-    tc::Problem q = problem<BN, CG>(d->rows, d->classes, d->dim, 1);
-    NC_CHECK((features_op<BN, CG>(&q, true, false)));
-    NC_CHECK((weight_op<BN, CG>(&q, false)));
+    tc::Problem q = problem<BN, CG, EW>(d->rows, d->classes, d->dim, 1);
+    NC_CHECK((features_op<BN, CG, EW>(&q, true, false)));
+    NC_CHECK((weight_op<BN, CG, EW>(&q, false)));
     const ValueEpilogue e{a, scales(), at<float>(p.bias), at<float2>(p.part), at<float>(p.zlabel), p.rows_pad};
-    return tc::launch_product<PL, BN, CG>(q, e, st, "readout value product launch");
+    return tc::launch_product<PL, BN, CG, EW>(q, e, st, "readout value product launch");
   }
 
   nc_status value(float* lse, float* row_loss, float* loss) const {
-    NC_CHECK(p.pair ? (value_product<256, 2>()) : (value_product<128, 1>()));
+    NC_CHECK(p.pair ? (value_product<256, 2, 8>()) : (value_product<128, 1, 8>()));
     PdlLaunch l(dim3((d->rows + 31) / 32), dim3(1024), 0, st);
     NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, ce_finish_kernel, a, p.slots, p.rows_pad,
                                      (const float2*)at<float2>(p.part), (const float*)at<float>(p.zlabel), scales(),
@@ -665,37 +665,37 @@ struct Call {
     return launch_check("ce_finish_kernel launch");
   }
 
-  template <int BN, int CG>
+  template <int BN, int CG, int EW>
   nc_status dz_product(const CeGrads& g, int v0, int width) const {
-    tc::Problem q = problem<BN, CG>(d->rows, width, d->dim, 1);
-    NC_CHECK((features_op<BN, CG>(&q, true, false)));
-    NC_CHECK((weight_op<BN, CG>(&q, false)));
+    tc::Problem q = problem<BN, CG, EW>(d->rows, width, d->dim, 1);
+    NC_CHECK((features_op<BN, CG, EW>(&q, true, false)));
+    NC_CHECK((weight_op<BN, CG, EW>(&q, false)));
     q.b_n0 = v0;
     const DzEpilogue<PL == 1> e{a,     scales(), at<float>(p.bias), g.lse,  at<float>(p.fac), at<uint16_t>(p.dz),
                                 g.bias ? at<float>(p.db_part) : nullptr, v0, p.piece, p.classes_pad};
-    return tc::launch_product<PL, BN, CG>(q, e, st, "readout logit gradient launch");
+    return tc::launch_product<PL, BN, CG, EW>(q, e, st, "readout logit gradient launch");
   }
 
-  template <int BN, int CG>
+  template <int BN, int CG, int EW>
   nc_status weight_product(const CeGrads& g, int v0, int classes) const {
-    tc::Problem q = problem<BN, CG>(classes, d->dim, d->rows, 1);
-    NC_CHECK((dz_op<BN, CG>(&q, true)));
-    NC_CHECK((features_op<BN, CG>(&q, false, true)));
+    tc::Problem q = problem<BN, CG, EW>(classes, d->dim, d->rows, 1);
+    NC_CHECK((dz_op<BN, CG, EW>(&q, true)));
+    NC_CHECK((features_op<BN, CG, EW>(&q, false, true)));
     T* out = static_cast<T*>(g.weight) + (size_t)v0 * d->dim;
     const bool wide = reinterpret_cast<uintptr_t>(out) % 32 == 0 && (size_t)d->dim * sizeof(T) % 32 == 0;
     const WeightEpilogue<T> e{scales(), out, classes, d->dim, wide};
-    return tc::launch_product<PL, BN, CG>(q, e, st, "readout weight gradient launch");
+    return tc::launch_product<PL, BN, CG, EW>(q, e, st, "readout weight gradient launch");
   }
 
-  template <int BN, int CG>
+  template <int BN, int CG, int EW>
   nc_status feature_product(const CeGrads& g, int v0, int width) const {
-    tc::Problem q = problem<BN, CG>(d->rows, d->dim, width, p.splits);
-    NC_CHECK((dz_op<BN, CG>(&q, false)));
-    NC_CHECK((weight_op<BN, CG>(&q, true)));
+    tc::Problem q = problem<BN, CG, EW>(d->rows, d->dim, width, p.splits);
+    NC_CHECK((dz_op<BN, CG, EW>(&q, false)));
+    NC_CHECK((weight_op<BN, CG, EW>(&q, true)));
     q.b_k0 = v0;
     const FeatureEpilogue e{scales(), at<float>(p.df_part), d->rows, d->dim, p.pitch, v0 == 0,
                             PL == 1 ? 1.f : 1.f / kDzScale};
-    return tc::launch_product<PL, BN, CG>(q, e, st, "readout feature gradient launch");
+    return tc::launch_product<PL, BN, CG, EW>(q, e, st, "readout feature gradient launch");
   }
 
   nc_status gradients(const CeGrads& g) const {
@@ -704,11 +704,11 @@ struct Call {
       // the last piece may be shorter; `width` is whole tiles
       const int width = p.classes_pad - v0 < p.piece ? p.classes_pad - v0 : p.piece;
       const int classes = d->classes - v0 < width ? d->classes - v0 : width;
-      NC_CHECK(p.pair ? (dz_product<256, 2>(g, v0, width)) : (dz_product<128, 1>(g, v0, width)));
+      NC_CHECK(p.pair ? (dz_product<256, 2, 8>(g, v0, width)) : (dz_product<128, 1, 8>(g, v0, width)));
       if (g.weight)
-        NC_CHECK(p.pair_w ? (weight_product<256, 2>(g, v0, classes)) : (weight_product<128, 1>(g, v0, classes)));
+        NC_CHECK(p.pair_w ? (weight_product<256, 2, 8>(g, v0, classes)) : (weight_product<128, 1, 8>(g, v0, classes)));
       if (g.features)
-        NC_CHECK(p.pair_f ? (feature_product<256, 2>(g, v0, width)) : (feature_product<128, 1>(g, v0, width)));
+        NC_CHECK(p.pair_f ? (feature_product<256, 2, 8>(g, v0, width)) : (feature_product<128, 1, 8>(g, v0, width)));
     }
     if (g.features) {
       const int64_t n = (int64_t)d->rows * d->dim;

@@ -24,9 +24,7 @@ namespace nc {
 namespace tc {
 
 constexpr int kBM = 128;            // rows of a tile per CTA: one tensor-memory lane each
-constexpr int kEpiWarps = 8;        // two per lane quarter, one per half of the columns
-constexpr int kThreads = 32 * (kEpiWarps + 2);
-constexpr int kPatch = 4096;        // bytes of shared memory of an epilogue warp: 32 rows of 128 bytes
+constexpr int kBK = 64;             // k of a stage: a swizzled row of 128 bytes (rows of 64 took products 6 % longer)
 constexpr int kWaitLimit = 1 << 20; // polls of a bounded wait
 
 // One product of (batched) matrices, D (m, n) = A (m, k) B (n, k)^T.  An operand is stored
@@ -52,14 +50,19 @@ struct Tile {
 // half of B; the products read both halves.  Shared memory bounds a product of one CTA (a
 // 128 x 256 tile writes and reads 192 bytes a cycle for 128 that it can take); the pair needs
 // 128.
-template <int PL, int BN, int CG>
+//
+// EW epilogue warps (the first of the CTA), EW / 4 side by side on the columns of each lane quarter.
+template <int PL, int BN, int CG, int EW>
 struct Config {
-  static constexpr int kBK = 64;   // one swizzled row of 128 bytes (rows of 64 took the copies 6 % longer)
   static constexpr int kBRows = BN / CG;   // of B in one CTA
   static constexpr int kA = PL * kBM * kBK * 2, kB = PL * kBRows * kBK * 2;
+  static constexpr int kCols = BN * 4 / EW;               // of an epilogue thread
+  static constexpr int kPiece = kCols < 64 ? kCols : 64;  // 16-bit values of a row in a warp's patch
+  static constexpr int kPatch = 32 * kPiece * 2;
+  static constexpr int kThreads = 32 * (EW + 2);
   static constexpr int kStage = kA + kB;
   static constexpr int kStages = 192 * 1024 / kStage;
-  static constexpr int kSmem = kStages * kStage + kEpiWarps * kPatch + 1024;   // stages start on 1024 bytes
+  static constexpr int kSmem = kStages * kStage + EW * kPatch + 1024;   // stages start on 1024 bytes
 };
 
 __host__ __device__ inline int problem_tiles(const Problem& p) {
@@ -68,7 +71,7 @@ __host__ __device__ inline int problem_tiles(const Problem& p) {
 }
 
 // `rank`: of the CTA in its pair.
-template <int PL, int BN, int CG>
+template <int BN, int CG>
 __device__ __forceinline__ Tile problem_tile(const Problem& p, int t, int rank) {
   Tile x;
   int mn;
@@ -86,8 +89,7 @@ __device__ __forceinline__ Tile problem_tile(const Problem& p, int t, int rank) 
     x.m0 = mn % p.tiles_m * kBM * CG + rank * kBM, x.n0 = mn / p.tiles_m * BN;
   }
   x.batch = t % p.batch, x.split = t / p.batch;
-  constexpr int BK = Config<PL, BN, CG>::kBK;
-  const int kt = (p.k + BK - 1) / BK;
+  const int kt = (p.k + kBK - 1) / kBK;
   x.kt0 = (int)((int64_t)kt * x.split / p.splits), x.kt1 = (int)((int64_t)kt * (x.split + 1) / p.splits);
   return x;
 }
@@ -257,25 +259,30 @@ __device__ __forceinline__ void split_f16x2(float x, float y, uint32_t* hi, uint
 
 // An epilogue thread holds a row, so that its own global accesses would touch 32 rows at a
 // time (a 128-byte line each: they took most of an epilogue).  The warp's patch of shared
-// memory turns them: 16-byte piece q of row r lies at r * 128 + (q ^ (r & 7)) * 16, which
-// is free of bank conflicts by rows and by pieces.
+// memory, 32 rows of W 16-bit values, turns them: the 16-byte pieces of a row are placed so
+// that neither the rows of a piece nor the pieces of a row meet in a bank.
+template <int W>
 __device__ __forceinline__ uint4* patch_at(uint8_t* patch, int r, int q) {
-  return reinterpret_cast<uint4*>(patch + r * 128 + ((q ^ (r & 7)) << 4));
+  const int turn = W == 64 ? r & 7 : r >> 1 & 3;
+  return reinterpret_cast<uint4*>(patch + r * 2 * W + ((q ^ turn) << 4));
 }
 
-// Rows [0, rows) of 64 16-bit values, one per lane in `v` (32 words), to p + row * pitch; the
+// Rows [0, rows) of W 16-bit values, one per lane in `v` (W / 2 words), to p + row * pitch; the
 // first 8 * pieces values of each.  p and pitch on 16 bytes.
+template <int W>
 __device__ __forceinline__ void patch_store(uint8_t* patch, const uint32_t* v, uint16_t* p, int64_t pitch, int rows,
                                             int pieces) {
-  const int lane = threadIdx.x & 31, q = lane & 7;
+  constexpr int kPer = W / 8;   // lanes a row
+  const int lane = threadIdx.x & 31, q = lane % kPer;
   __syncwarp();
 #pragma unroll
-  for (int i = 0; i < 8; ++i) *patch_at(patch, lane, i) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+  for (int i = 0; i < kPer; ++i)
+    *patch_at<W>(patch, lane, i) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
   __syncwarp();
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int r = i * 4 + (lane >> 3);
-    if (r < rows && q < pieces) *reinterpret_cast<uint4*>(p + r * pitch + 8 * q) = *patch_at(patch, r, q);
+  for (int i = 0; i < kPer; ++i) {
+    const int r = i * (32 / kPer) + lane / kPer;
+    if (r < rows && q < pieces) *reinterpret_cast<uint4*>(p + r * pitch + 8 * q) = *patch_at<W>(patch, r, q);
   }
 }
 
@@ -293,20 +300,20 @@ __device__ __forceinline__ void load_v8(const void* p, uint32_t (&v)[8]) {
 }
 
 // What a CTA's warps share beside the stages.
-template <int PL, int BN, int CG>
+template <int PL, int BN, int CG, int EW>
 struct Shared {
-  uint64_t bars[2 * Config<PL, BN, CG>::kStages + 5];
+  uint64_t bars[2 * Config<PL, BN, CG, EW>::kStages + 5];
   uint32_t tmem_slot;
-  int abort, extra_readers[Config<PL, BN, CG>::kStages];
+  int abort, extra_readers[Config<PL, BN, CG, EW>::kStages];
 };
 
 // One warp's view of the pipeline: the loading warp fills stages, the multiplying warp (of a
 // pair's first CTA) turns them into accumulators, the epilogue warps collect those.  Each
 // role keeps its own place; the places advance over tiles and over products alike.
-template <int PL, int BN, int CG>
+template <int PL, int BN, int CG, int EW>
 struct Engine {
-  using C = Config<PL, BN, CG>;
-  static constexpr int BK = C::kBK, HALF = BN / 2;
+  using C = Config<PL, BN, CG, EW>;
+  static constexpr int BK = kBK, COLS = C::kCols, kEpiWarps = EW;
   static constexpr uint32_t a_block = C::kA / (kBM / 64), b_block = C::kB / (C::kBRows / 64);
 
   uint32_t stages, bar0, tmem;
@@ -328,10 +335,10 @@ struct Engine {
   __device__ __forceinline__ uint32_t drain() const { return bar0 + 8 * (2 * C::kStages + 4); }
 
   // By the whole CTA, before it reads anything that an earlier kernel wrote.
-  __device__ __forceinline__ Engine(uint8_t* raw, Shared<PL, BN, CG>* sh, int32_t* status_word) {
+  __device__ __forceinline__ Engine(uint8_t* raw, Shared<PL, BN, CG, EW>* sh, int32_t* status_word) {
     stages = (smem_addr(raw) + 1023) & ~1023u;
     base = raw + (stages - smem_addr(raw));
-    patch = base + C::kStages * C::kStage + (threadIdx.x >> 5) * kPatch;
+    patch = base + C::kStages * C::kStage + (threadIdx.x >> 5) * C::kPatch;
     extra_readers = sh->extra_readers;
     bar0 = smem_addr(sh->bars);
     abort = &sh->abort;
@@ -439,12 +446,12 @@ struct Engine {
     }
   }
 
-  // An epilogue warp: the sums of its 32 rows and HALF columns.
-  __device__ __forceinline__ void collect(const Problem& p, const Tile& x, float (&acc)[HALF]) {
+  // An epilogue warp: the sums of its 32 rows and COLS columns.
+  __device__ __forceinline__ void collect(const Problem& p, const Tile& x, float (&acc)[COLS]) {
     const int warp = threadIdx.x >> 5;
-    const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + (warp >> 2) * HALF;
+    const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + (warp >> 2) * COLS;
 #pragma unroll
-    for (int i = 0; i < HALF; ++i) acc[i] = 0.f;
+    for (int i = 0; i < COLS; ++i) acc[i] = 0.f;
     for (int c0 = x.kt0; c0 < x.kt1; c0 += p.chunk) {
       if (!__all_sync(0xffffffffu, ok && bar_wait(acc_full(buf), ph, abort, status))) {
         ok = false;
@@ -452,7 +459,7 @@ struct Engine {
       }
       fence_after();
 #pragma unroll
-      for (int i = 0; i < HALF; i += 32) {
+      for (int i = 0; i < COLS; i += 32) {
         float v[32];
         tmem_load(lanes + buf * BN + i, v);
 #pragma unroll
@@ -518,35 +525,35 @@ struct Engine {
   }
 };
 
-// The kernel of one product: warps 0..7 epilogue, warp 8 loads, warp 9 multiplies; persistent
-// over tiles.  Epi::run(state, tile, row, col, acc) gets a row's BN / 2 consecutive columns as
+// The kernel of one product: the first EW warps epilogue, the next loads, the last multiplies;
+// persistent over tiles.  Epi::run(state, tile, row, col, acc) gets COLS consecutive columns of a row as
 // float32 sums; Epi::begin(tile, row, col, patch) runs before the wait for them and returns the
 // state.
-template <int PL, int BN, int CG, class Epi>
-__global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_constant__ Problem p, const Epi epi) {
-  using E = Engine<PL, BN, CG>;
+template <int PL, int BN, int CG, int EW, class Epi>
+__global__ void __launch_bounds__(32 * (EW + 2), 1) product_kernel(const __grid_constant__ Problem p, const Epi epi) {
+  using E = Engine<PL, BN, CG, EW>;
   extern __shared__ uint8_t raw[];
-  __shared__ Shared<PL, BN, CG> sh;
+  __shared__ Shared<PL, BN, CG, EW> sh;
   E e(raw, &sh, p.status);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int first = blockIdx.x / CG, stride = gridDim.x / CG, tiles = problem_tiles(p);
   pdl_enter();
-  if (warp == kEpiWarps) {
+  if (warp == EW) {
     if (lane == 0)
-      for (int t = first; t < tiles && e.ok; t += stride) e.load(p, &p.a, &p.b, problem_tile<PL, BN, CG>(p, t, e.rank));
-  } else if (warp == kEpiWarps + 1) {
+      for (int t = first; t < tiles && e.ok; t += stride) e.load(p, &p.a, &p.b, problem_tile<BN, CG>(p, t, e.rank));
+  } else if (warp == EW + 1) {
     if (e.rank == 0)
-      for (int t = first; t < tiles && e.ok; t += stride) e.multiply(p, problem_tile<PL, BN, CG>(p, t, 0));
+      for (int t = first; t < tiles && e.ok; t += stride) e.multiply(p, problem_tile<BN, CG>(p, t, 0));
   } else {
     for (int t = first; t < tiles && e.ok; t += stride) {
-      const Tile x = problem_tile<PL, BN, CG>(p, t, e.rank);
-      const int row = x.m0 + 32 * (warp & 3) + lane, col = x.n0 + (warp >> 2) * E::HALF;
+      const Tile x = problem_tile<BN, CG>(p, t, e.rank);
+      const int row = x.m0 + 32 * (warp & 3) + lane, col = x.n0 + (warp >> 2) * E::COLS;
       __syncwarp();   // the last tile's readers of the patch are done
-      const auto state = epi.template begin<E::HALF>(x, row, col, e.patch);
+      const auto state = epi.template begin<E::COLS>(x, row, col, e.patch);
       __syncwarp();
-      float acc[E::HALF];
+      float acc[E::COLS];
       e.collect(p, x, acc);
-      if (e.ok) epi.template run<E::HALF>(state, x, row, col, acc);
+      if (e.ok) epi.template run<E::COLS>(state, x, row, col, acc);
     }
   }
   __syncwarp();
@@ -561,14 +568,14 @@ nc_status make_map(CUtensorMap* map, const void* base, bool bf16, int planes, in
 int sm_count();
 
 // The two operands' maps: `mn` says that the operand's own index (extent `own`) is contiguous.
-template <int PL, int BN, int CG>
+template <int PL, int BN, int CG, int EW>
 nc_status make_operand(Problem* p, bool is_a, const void* base, bool mn, int own, int k, int64_t pitch, int64_t plane,
                        int batch, int64_t per_batch) {
-  using C = Config<PL, BN, CG>;
+  using C = Config<PL, BN, CG, EW>;
   (is_a ? p->a_mn : p->b_mn) = mn;
   const int rows = is_a ? kBM : C::kBRows;
-  return mn ? make_map(is_a ? &p->a : &p->b, base, p->bf16, PL, own, k, pitch, plane, batch, per_batch, 64, C::kBK)
-            : make_map(is_a ? &p->a : &p->b, base, p->bf16, PL, k, own, pitch, plane, batch, per_batch, C::kBK, rows);
+  return mn ? make_map(is_a ? &p->a : &p->b, base, p->bf16, PL, own, k, pitch, plane, batch, per_batch, 64, kBK)
+            : make_map(is_a ? &p->a : &p->b, base, p->bf16, PL, k, own, pitch, plane, batch, per_batch, kBK, rows);
 }
 
 // Tiles that cover (m, n).
@@ -577,10 +584,10 @@ void set_tiles(Problem* p) {
   p->tiles_m = (p->m + kBM * CG - 1) / (kBM * CG), p->tiles_n = (p->n + BN - 1) / BN;
 }
 
-template <int PL, int BN, int CG, class Epi>
+template <int PL, int BN, int CG, int EW, class Epi>
 nc_status launch_product(const Problem& p, const Epi& epi, cudaStream_t st, const char* what) {
-  auto k = product_kernel<PL, BN, CG, Epi>;
-  constexpr int smem = Config<PL, BN, CG>::kSmem;
+  auto k = product_kernel<PL, BN, CG, EW, Epi>;
+  constexpr int smem = Config<PL, BN, CG, EW>::kSmem;
   NC_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   const int tiles = problem_tiles(p), most = sm_count() / CG;
   cudaLaunchConfig_t cfg{};
@@ -589,7 +596,7 @@ nc_status launch_product(const Problem& p, const Epi& epi, cudaStream_t st, cons
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
   attr[1].val.clusterDim.x = CG, attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 1;
-  cfg.gridDim = dim3((tiles < most ? tiles : most) * CG), cfg.blockDim = dim3(kThreads);
+  cfg.gridDim = dim3((tiles < most ? tiles : most) * CG), cfg.blockDim = dim3(32 * (EW + 2));
   cfg.dynamicSmemBytes = smem, cfg.stream = st, cfg.attrs = attr, cfg.numAttrs = CG == 1 ? 1 : 2;
   NC_CUDA_CHECK(cudaLaunchKernelEx(&cfg, k, p, epi));
   return launch_check(what);
