@@ -390,16 +390,22 @@ __device__ __forceinline__ void ns_store(const NsArgs& p, NsProduct product, int
     add_planes(patch, product == kPoly ? p.G : p.X[k & 1], at, rows, cols, add, acc);
   }
   if (!last) {
-    uint32_t h[16], l[16];
+    __half* d = dst.p + at;
+    __half* t = dst.p + (size_t)x.batch * 2 * dst.plane + (size_t)col * dst.pitch + row0;
+    const bool mirror = product != kUpdate && x.n0 > x.m0;
+#pragma unroll 1
+    for (int h = 0; h < 2; ++h) {   // a plane, and what it leaves for the next
+      uint32_t v[16];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) tc::split_f16x2(acc[2 * i], acc[2 * i + 1], &h[i], &l[i]);
-    uint16_t* d = reinterpret_cast<uint16_t*>(dst.p) + at;
-    tc::patch_store<32>(patch, h, d, dst.pitch, rows, (cols + 7) / 8);
-    tc::patch_store<32>(patch, l, d + dst.plane, dst.pitch, rows, (cols + 7) / 8);
-    if (product != kUpdate && x.n0 > x.m0) {
-      __half* t = dst.p + (size_t)x.batch * 2 * dst.plane + (size_t)col * dst.pitch + row0;
-      store_mirrored(patch, t, dst.pitch, rows, cols, h);
-      store_mirrored(patch, t + dst.plane, dst.pitch, rows, cols, l);
+      for (int i = 0; i < 16; ++i) {
+        const __half2 w = __floats2half2_rn(acc[2 * i], acc[2 * i + 1]);
+        const float2 b = __half22float2(w);
+        acc[2 * i] -= b.x, acc[2 * i + 1] -= b.y;
+        v[i] = *reinterpret_cast<const uint32_t*>(&w);
+      }
+      tc::patch_store<32>(patch, v, reinterpret_cast<uint16_t*>(d), dst.pitch, rows, (cols + 7) / 8);
+      if (mirror) store_mirrored(patch, t, dst.pitch, rows, cols, v);
+      d += dst.plane, t += dst.plane;
     }
     return;
   }
@@ -426,9 +432,25 @@ __device__ __forceinline__ void ns_store(const NsArgs& p, NsProduct product, int
   }
 }
 
+// Product f of a step on `batch` matrices.  gram: the short side's rows of X against themselves;
+// poly: A A; update: Q X, or X Q.
+__device__ __forceinline__ tc::Problem ns_problem(const NsArgs& p, int f, int batch) {
+  const bool tall = p.rows > p.cols;
+  const int s = tall ? p.cols : p.rows, len = tall ? p.rows : p.cols;
+  tc::Problem q;
+  q.m = f == kUpdate ? p.rows : s, q.n = f == kUpdate ? p.cols : s, q.k = f == kGram ? len : s;
+  q.a_mn = f == kGram && tall, q.b_mn = f == kGram ? tall : f == kUpdate && !tall;
+  q.tiles_m = (q.m + kTile - 1) / kTile, q.tiles_n = (q.n + kTile - 1) / kTile;
+  q.batch = batch, q.splits = p.splits[f], q.symmetric = f != kUpdate, q.chunk = kNsChunk, q.bf16 = 0;
+  q.a_k0 = q.b_k0 = q.b_n0 = 0;
+  return q;
+}
+// Whether the result is added to a tile that comes through the pipeline.
+__device__ __forceinline__ bool wants_prior(const tc::Problem& q, int f) { return f != kGram && q.splits == 1; }
+
 template <typename T, bool CLUSTER>
 __global__ void __launch_bounds__(kNsThreads, 1) ns_kernel(const __grid_constant__ NsArgs p) {
-  extern __shared__ uint8_t raw[];
+  extern __shared__ __align__(1024) uint8_t raw[];
   __shared__ tc::Shared<2, kTile, 1, kNsWarps> sh;
   __shared__ double red[kNsThreads / 32];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -496,82 +518,92 @@ __global__ void __launch_bounds__(kNsThreads, 1) ns_kernel(const __grid_constant
   }
   meet();
 
-  const bool tall = p.rows > p.cols;
-  const int s = tall ? p.cols : p.rows, len = tall ? p.rows : p.cols;
-  for (int k = 0; k < p.steps; ++k) {
-    const CUtensorMap *xk = &p.by_k[k & 1], *xr = &p.by_row[k & 1];
+  // The roles go through the products each in a loop of its own: what one of them keeps does
+  // not cost the others registers (a spilled value comes back from L2 after every meeting).
+  if (warp == kNsWarps) {
+    for (int k = 0; k < p.steps; ++k) {
 #pragma unroll 1
-    for (int f = kGram; f <= kUpdate; ++f) {
-      // gram: the short side's rows of X against themselves; poly: A A; update: Q X, or X Q
-      tc::Problem q;
-      q.m = f == kUpdate ? p.rows : s, q.n = f == kUpdate ? p.cols : s, q.k = f == kGram ? len : s;
-      q.a_mn = f == kGram && tall, q.b_mn = f == kGram ? tall : f == kUpdate && !tall;
-      q.tiles_m = (q.m + kTile - 1) / kTile, q.tiles_n = (q.n + kTile - 1) / kTile;
-      q.batch = batch, q.splits = p.splits[f], q.symmetric = f != kUpdate, q.chunk = kNsChunk, q.bf16 = 0;
-      q.a_k0 = q.b_k0 = q.b_n0 = 0;
-      const CUtensorMap* ma = f == kGram ? (tall ? xr : xk) : f == kPoly ? &p.gram : tall ? xk : &p.poly;
-      const CUtensorMap* mb = f == kGram ? (tall ? xr : xk) : f == kPoly ? &p.gram : tall ? &p.poly : xr;
-      const bool last = f == kUpdate && k + 1 == p.steps;
-      const int tiles = tc::problem_tiles(q);
-      const bool extra = f != kGram && q.splits == 1;
-      if (warp == kNsWarps) {
+      for (int f = kGram; f <= kUpdate; ++f) {
+        const tc::Problem q = ns_problem(p, f, batch);
+        const bool tall = p.rows > p.cols;
+        const CUtensorMap *xk = &p.by_k[k & 1], *xr = &p.by_row[k & 1];
+        const CUtensorMap* ma = f == kGram ? (tall ? xr : xk) : f == kPoly ? &p.gram : tall ? xk : &p.poly;
+        const CUtensorMap* mb = f == kGram ? (tall ? xr : xk) : f == kPoly ? &p.gram : tall ? &p.poly : xr;
+        const int tiles = tc::problem_tiles(q);
         if (lane == 0) {
           for (int t = rank; t < tiles && e.ok; t += size) {
             const tc::Tile x = tile(q, t);
             e.load(q, ma, mb, x);
-            if (extra) e.load_extra(f == kPoly ? &p.gram : xk, x);
+            if (wants_prior(q, f)) e.load_extra(f == kPoly ? &p.gram : xk, x);
           }
         }
-      } else if (warp == kNsWarps + 1) {
+        __syncwarp();
+        meet();
+        if (q.splits > 1) meet();
+      }
+    }
+  } else if (warp == kNsWarps + 1) {
+    for (int k = 0; k < p.steps; ++k) {
+#pragma unroll 1
+      for (int f = kGram; f <= kUpdate; ++f) {
+        const tc::Problem q = ns_problem(p, f, batch);
+        const int tiles = tc::problem_tiles(q);
         for (int t = rank; t < tiles && e.ok; t += size) {
           e.multiply(q, tile(q, t));
-          if (extra) e.skip_extra();
+          if (wants_prior(q, f)) e.skip_extra();
         }
-      } else {
-        for (int t = rank; t < tiles && e.ok; t += size) {
-          const tc::Tile x = tile(q, t);
-          float acc[kNsCols];
-          e.collect(q, x, acc);
-          if (!e.ok) break;
-          if (q.splits > 1) {
-            float4* o = parts + ((size_t)t * kNsWarps + warp) * (kNsCols * 8) + lane;
+        meet();
+        if (q.splits > 1) meet();
+      }
+    }
+  } else {
+    for (int k = 0; k < p.steps; ++k) {
+#pragma unroll 1
+      for (int f = kGram; f <= kUpdate; ++f) {
+        const tc::Problem q = ns_problem(p, f, batch);
+        const bool last = f == kUpdate && k + 1 == p.steps;
+        const int tiles = tc::problem_tiles(q), whole = tiles / q.splits;
+        // The tiles of this CTA; then, where a product was split, a second pass in which each
+        // warp of the group adds up the parts of 32 rows and columns (`whole` tiles apart).
+        for (int pass = 0; pass < (q.splits > 1 ? 2 : 1); ++pass) {
+          const int unit = pass == 0 ? rank : rank * kNsWarps + warp, units = pass == 0 ? tiles : whole * kNsWarps;
+          for (int w = unit; w < units && e.ok; w += pass == 0 ? size : size * kNsWarps) {
+            const int t = pass == 0 ? w : w / kNsWarps, part = pass == 0 ? warp : w % kNsWarps;
+            const tc::Tile x = tile(q, t);
+            float acc[kNsCols];
+            const uint8_t* prior = nullptr;
+            if (pass == 0) {
+              e.collect(q, x, acc);
+              if (!e.ok) break;
+              if (q.splits > 1) {
+                float4* o = parts + ((size_t)t * kNsWarps + warp) * (kNsCols * 8) + lane;
 #pragma unroll
-            for (int j = 0; j < kNsCols / 4; ++j)
-              o[j * 32] = make_float4(acc[4 * j], acc[4 * j + 1], acc[4 * j + 2], acc[4 * j + 3]);
-          } else {
-            const uint8_t* prior = extra ? e.extra() : nullptr;
-            if (!e.ok) break;
-            ns_store<T>(p, (NsProduct)f, k, last, x, x.m0 + 32 * (warp & 3), x.n0 + (warp >> 2) * kNsCols, e.patch, prior,
+                for (int j = 0; j < kNsCols / 4; ++j)
+                  o[j * 32] = make_float4(acc[4 * j], acc[4 * j + 1], acc[4 * j + 2], acc[4 * j + 3]);
+                continue;
+              }
+              if (wants_prior(q, f)) prior = e.extra();
+              if (!e.ok) break;
+            } else {
+#pragma unroll
+              for (int j = 0; j < kNsCols; ++j) acc[j] = 0.f;
+              for (int g = 0; g < q.splits; ++g) {
+                const float4* o = parts + ((size_t)(t + g * whole) * kNsWarps + part) * (kNsCols * 8) + lane;
+                float4 v[kNsCols / 4];
+#pragma unroll
+                for (int j = 0; j < kNsCols / 4; ++j) v[j] = __ldcg(o + j * 32);
+#pragma unroll
+                for (int j = 0; j < kNsCols / 4; ++j)
+                  acc[4 * j] += v[j].x, acc[4 * j + 1] += v[j].y, acc[4 * j + 2] += v[j].z, acc[4 * j + 3] += v[j].w;
+              }
+            }
+            ns_store<T>(p, (NsProduct)f, k, last, x, x.m0 + 32 * (part & 3), x.n0 + (part >> 2) * kNsCols, e.patch, prior,
                         acc);
-            if (extra) e.extra_done();
+            if (prior) e.extra_done();
           }
+          meet();
         }
       }
-      __syncwarp();
-      meet();
-      if (q.splits == 1) continue;
-      // the parts of a tile are tiles / splits apart; a warp sums its 32 rows and columns
-      const int whole = tiles / q.splits;
-      if (warp < kNsWarps) {
-        for (int w = rank * kNsWarps + warp; w < whole * kNsWarps; w += size * kNsWarps) {
-          const int t = w / kNsWarps, part = w % kNsWarps;
-          const tc::Tile x = tile(q, t);
-          float acc[kNsCols];
-#pragma unroll
-          for (int j = 0; j < kNsCols; ++j) acc[j] = 0.f;
-          for (int g = 0; g < q.splits; ++g) {
-            const float4* o = parts + ((size_t)(t + g * whole) * kNsWarps + part) * (kNsCols * 8) + lane;
-            float4 v[kNsCols / 4];
-#pragma unroll
-            for (int j = 0; j < kNsCols / 4; ++j) v[j] = __ldcg(o + j * 32);
-#pragma unroll
-            for (int j = 0; j < kNsCols / 4; ++j)
-              acc[4 * j] += v[j].x, acc[4 * j + 1] += v[j].y, acc[4 * j + 2] += v[j].z, acc[4 * j + 3] += v[j].w;
-          }
-          ns_store<T>(p, (NsProduct)f, k, last, x, x.m0 + 32 * (part & 3), x.n0 + (part >> 2) * kNsCols, e.patch, nullptr, acc);
-        }
-      }
-      meet();
     }
   }
   if (p.steps == 0) {   // X0 as it is

@@ -62,7 +62,7 @@ struct Config {
   static constexpr int kThreads = 32 * (EW + 2);
   static constexpr int kStage = kA + kB;
   static constexpr int kStages = 192 * 1024 / kStage;
-  static constexpr int kSmem = kStages * kStage + EW * kPatch + 1024;   // stages start on 1024 bytes
+  static constexpr int kSmem = kStages * kStage + EW * kPatch;   // the stages first, on 1024 bytes
 };
 
 __host__ __device__ inline int problem_tiles(const Problem& p) {
@@ -334,10 +334,11 @@ struct Engine {
   __device__ __forceinline__ uint32_t acc_empty(int i) const { return bar0 + 8 * (2 * C::kStages + 2 + i); }
   __device__ __forceinline__ uint32_t drain() const { return bar0 + 8 * (2 * C::kStages + 4); }
 
-  // By the whole CTA, before it reads anything that an earlier kernel wrote.
+  // By the whole CTA, before it reads anything that an earlier kernel wrote.  `raw`: the dynamic
+  // shared memory, on 1024 bytes.
   __device__ __forceinline__ Engine(uint8_t* raw, Shared<PL, BN, CG, EW>* sh, int32_t* status_word) {
-    stages = (smem_addr(raw) + 1023) & ~1023u;
-    base = raw + (stages - smem_addr(raw));
+    stages = smem_addr(raw);
+    base = raw;
     patch = base + C::kStages * C::kStage + (threadIdx.x >> 5) * C::kPatch;
     extra_readers = sh->extra_readers;
     bar0 = smem_addr(sh->bars);
@@ -532,7 +533,7 @@ struct Engine {
 template <int PL, int BN, int CG, int EW, class Epi>
 __global__ void __launch_bounds__(32 * (EW + 2), 1) product_kernel(const __grid_constant__ Problem p, const Epi epi) {
   using E = Engine<PL, BN, CG, EW>;
-  extern __shared__ uint8_t raw[];
+  extern __shared__ __align__(1024) uint8_t raw[];
   __shared__ Shared<PL, BN, CG, EW> sh;
   E e(raw, &sh, p.status);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
