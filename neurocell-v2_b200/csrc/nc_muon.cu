@@ -259,11 +259,14 @@ nc_status launch_small(const SmallArgs& a, const SmallPlan& r, int batch, cudaSt
 // diagonal and store them twice; a product with fewer tiles than SMs is split along k, its
 // float32 parts summed in order by the whole grid.
 constexpr float kPlaneScale = 4096.f, kPlaneInv = 1.f / 4096.f;
-constexpr int kTile = 128;   // square tiles: at most sizes the number of tiles matters more than a tile's rate
 constexpr int kNsChunk = 1;  // k-tiles (of 64) per accumulator: Gram sums of one sign show the additions' truncation
-using NsEngine = tc::Engine<2, kTile, 1, 16>;
-constexpr int kNsCols = NsEngine::COLS, kNsWarps = NsEngine::kEpiWarps, kNsThreads = NsEngine::C::kThreads;
-static_assert(kNsCols == 32, "an epilogue thread takes 32 columns");
+constexpr int kNsCols = 32;  // columns of an epilogue thread
+// Where matrices have many tiles: pairs of CTAs on 256 x 128 (a product reads and writes 120 KB
+// of a CTA's shared memory per k-tile, 160 KB as one CTA's 128 x 128), the whole grid on all
+// matrices.  Where they have few: 128 x 64 and a cluster of 8 on each matrix.
+template <bool CLUSTER>
+using NsEngine = tc::Engine<2, CLUSTER ? 64 : 128, CLUSTER ? 1 : 2, CLUSTER ? 8 : 16>;
+static_assert(NsEngine<true>::COLS == kNsCols && NsEngine<false>::COLS == kNsCols, "the epilogue is written for 32");
 
 struct Planes {   // (batch, plane, rows, pitch)
   __half* p;
@@ -276,8 +279,8 @@ enum NsProduct { kGram, kPoly, kUpdate };
 constexpr int kCluster = 8;
 
 struct NsArgs {
-  CUtensorMap by_k[2], by_row[2];   // X and its next value, both ways (short side as the own index)
-  CUtensorMap gram, poly;
+  // X and its next value, A and Q as operands a and b: with k contiguous, or by rows of k
+  CUtensorMap k_a[2], k_b[2], rows_a[2], rows_b[2], gram_a, gram_b, poly_a, poly_b;
   Planes X[2], G, Q;
   const void* x;
   float* momentum;
@@ -288,21 +291,13 @@ struct NsArgs {
   int64_t parts_each;   // of one matrix, where clusters work on one each
   int batch, rows, cols, steps;
   int splits[3];
+  int vec;              // cols are whole 4s and the tensors start on 16 bytes
   float a, b, c;
   double eps;
   MuonArgs mu;
   float decay, step;
   int32_t* status;
 };
-
-// u of an element: x itself, or from the updated momentum.
-template <typename T>
-__device__ __forceinline__ float source(const NsArgs& p, size_t o) {
-  const float x = to_f32(static_cast<const T*>(p.x)[o]);
-  if (!p.momentum) return x;
-  const float m = p.momentum[o];
-  return p.mu.nesterov ? fmaf(p.mu.beta, m, x) : m;
-}
 
 // The transposed store of 32 rows (a lane each) and 32 columns: through the warp's patch, as 32
 // rows of 64 bytes.  `rows`, `cols`: how many of them exist; what lies behind a row's end is
@@ -368,7 +363,7 @@ __device__ __forceinline__ void add_planes(uint8_t* patch, const Planes& s, size
 
 // Result of a product for 32 rows from row0 on and 32 columns from col on, on scaled values:
 // mul acc + add (A or X), to planes (and mirrored), or (last) unscaled to the caller.  `prior`:
-// the tile of A or X in shared memory (Engine::extra), or null to take it from global memory.
+// 64 columns of A or X in shared memory (Engine::extra), or null to take them from global memory.
 template <typename T>
 __device__ __forceinline__ void ns_store(const NsArgs& p, NsProduct product, int k, bool last, const tc::Tile& x,
                                          int row0, int col, uint8_t* patch, const uint8_t* prior, float (&acc)[32]) {
@@ -377,22 +372,24 @@ __device__ __forceinline__ void ns_store(const NsArgs& p, NsProduct product, int
   const int lane = threadIdx.x & 31, rows = min(32, m - row0), cols = min(32, n - col);
   const size_t at = (size_t)x.batch * 2 * dst.plane + (size_t)row0 * dst.pitch + col;
   const float mul = product == kPoly ? p.c * kPlaneInv : kPlaneInv, add = product == kPoly ? p.b : p.a;
-  if (rows <= 0 || cols <= 0) return;   // the same for the whole warp
+  // Symmetric results: the 128 rows of this CTA against its columns.  Left of the diagonal's
+  // square another tile's mirror image fills in (one writer, so the bits do not depend on which
+  // comes last); right of it this one's goes there.
+  const bool beside = product != kUpdate && col < x.m0, mirror = product != kUpdate && col >= x.m0 + tc::kBM;
+  if (rows <= 0 || cols <= 0 || beside) return;   // the same for the whole warp
 #pragma unroll
   for (int j = 0; j < 32; ++j) acc[j] *= mul;
   if (product != kGram && prior) {
-    const int r = row0 - x.m0 + lane, c = col - x.n0;
-    const uint8_t* half = prior + c / 64 * (NsEngine::C::kStage / 2) + r * 128;
+    const int r = row0 - x.m0 + lane, c = (col - x.n0) % 64 / 8;
 #pragma unroll
     for (int h = 0; h < 2; ++h)
-      add_row([&](int i) { return half + h * (kTile * 128) + (((c % 64 / 8 + i) ^ (r & 7)) << 4); }, add, acc);
+      add_row([&](int i) { return prior + h * (tc::kBM * 128) + r * 128 + (((c + i) ^ (r & 7)) << 4); }, add, acc);
   } else if (product != kGram) {
     add_planes(patch, product == kPoly ? p.G : p.X[k & 1], at, rows, cols, add, acc);
   }
   if (!last) {
     __half* d = dst.p + at;
     __half* t = dst.p + (size_t)x.batch * 2 * dst.plane + (size_t)col * dst.pitch + row0;
-    const bool mirror = product != kUpdate && x.n0 > x.m0;
 #pragma unroll 1
     for (int h = 0; h < 2; ++h) {   // a plane, and what it leaves for the next
       uint32_t v[16];
@@ -434,13 +431,14 @@ __device__ __forceinline__ void ns_store(const NsArgs& p, NsProduct product, int
 
 // Product f of a step on `batch` matrices.  gram: the short side's rows of X against themselves;
 // poly: A A; update: Q X, or X Q.
+template <bool CLUSTER>
 __device__ __forceinline__ tc::Problem ns_problem(const NsArgs& p, int f, int batch) {
   const bool tall = p.rows > p.cols;
   const int s = tall ? p.cols : p.rows, len = tall ? p.rows : p.cols;
   tc::Problem q;
   q.m = f == kUpdate ? p.rows : s, q.n = f == kUpdate ? p.cols : s, q.k = f == kGram ? len : s;
   q.a_mn = f == kGram && tall, q.b_mn = f == kGram ? tall : f == kUpdate && !tall;
-  q.tiles_m = (q.m + kTile - 1) / kTile, q.tiles_n = (q.n + kTile - 1) / kTile;
+  tc::set_tiles<CLUSTER ? 64 : 128, CLUSTER ? 1 : 2>(&q);
   q.batch = batch, q.splits = p.splits[f], q.symmetric = f != kUpdate, q.chunk = kNsChunk, q.bf16 = 0;
   q.a_k0 = q.b_k0 = q.b_n0 = 0;
   return q;
@@ -448,14 +446,42 @@ __device__ __forceinline__ tc::Problem ns_problem(const NsArgs& p, int f, int ba
 // Whether the result is added to a tile that comes through the pipeline.
 __device__ __forceinline__ bool wants_prior(const tc::Problem& q, int f) { return f != kGram && q.splits == 1; }
 
+// Four consecutive elements, or as many as `left`.
+template <typename T>
+__device__ __forceinline__ void load4(const T* p, bool vec, int left, float (&v)[4]) {
+  if (vec) {
+    if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(p);
+    } else {
+      const uint2 q = *reinterpret_cast<const uint2*>(p);
+      v[0] = __uint_as_float(q.x << 16), v[1] = __uint_as_float(q.x & 0xffff0000u);
+      v[2] = __uint_as_float(q.y << 16), v[3] = __uint_as_float(q.y & 0xffff0000u);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = j < left ? to_f32(p[j]) : 0.f;
+  }
+}
+__device__ __forceinline__ void store4(float* p, bool vec, int left, const float (&v)[4]) {
+  if (vec) {
+    *reinterpret_cast<float4*>(p) = *reinterpret_cast<const float4*>(v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < left) p[j] = v[j];
+  }
+}
+
 template <typename T, bool CLUSTER>
-__global__ void __launch_bounds__(kNsThreads, 1) ns_kernel(const __grid_constant__ NsArgs p) {
+__global__ void __launch_bounds__(NsEngine<CLUSTER>::C::kThreads, 1) ns_kernel(const __grid_constant__ NsArgs p) {
+  using E = NsEngine<CLUSTER>;
+  constexpr int kWarps = E::kEpiWarps, kThreads = E::C::kThreads, kCg = CLUSTER ? 1 : 2, kBN = CLUSTER ? 64 : 128;
   extern __shared__ __align__(1024) uint8_t raw[];
-  __shared__ tc::Shared<2, kTile, 1, kNsWarps> sh;
-  __shared__ double red[kNsThreads / 32];
+  __shared__ tc::Shared<2, kBN, kCg, kWarps> sh;
+  __shared__ double red[kThreads / 32];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (blockIdx.x == 0 && tid == 0) *p.status = 0;
-  NsEngine e(raw, &sh, p.status);
+  E e(raw, &sh, p.status);
   // The CTAs that work together: the whole grid on all matrices, or a cluster on one.
   const int size = CLUSTER ? kCluster : gridDim.x, rank = CLUSTER ? (int)tc::cluster_rank() : blockIdx.x;
   const int b0 = CLUSTER ? blockIdx.x / kCluster : 0, batch = CLUSTER ? 1 : p.batch;
@@ -469,23 +495,37 @@ __global__ void __launch_bounds__(kNsThreads, 1) ns_kernel(const __grid_constant
       cooperative_groups::this_grid().sync();
     asm volatile("fence.proxy.async;" ::: "memory");
   };
-  auto tile = [&](const tc::Problem& q, int t) {
-    tc::Tile x = tc::problem_tile<kTile, 1>(q, t, 0);
+  auto tile = [&](const tc::Problem& q, int t, int in_pair) {
+    tc::Tile x = tc::problem_tile<kBN, kCg>(q, t, in_pair);
     x.batch += b0;
     return x;
   };
-  float4* const parts = p.parts + (size_t)b0 * p.parts_each;
   const int64_t n = (int64_t)p.rows * p.cols;
+  const int quads = (p.cols + 3) / 4;   // four columns at a time
+  const int64_t all = (int64_t)p.rows * quads;
 
   // momentum, and each CTA's part of the squared norms
   for (int b = b0; b < b0 + batch; ++b) {
-    const size_t o = (size_t)b * n;
     double sum = 0.0;
-#pragma unroll 4
-    for (int64_t i = (int64_t)rank * kNsThreads + tid; i < n; i += (int64_t)size * kNsThreads) {
-      if (p.momentum) p.momentum[o + i] = fmaf(p.mu.beta, p.momentum[o + i], to_f32(static_cast<const T*>(p.x)[o + i]));
-      const float u = source<T>(p, o + i);
-      sum += (double)u * u;
+#pragma unroll 2
+    for (int64_t i = (int64_t)rank * kThreads + tid; i < all; i += (int64_t)size * kThreads) {
+      const int r = (int)((uint32_t)i / (uint32_t)quads), c = 4 * ((int)i - r * quads), left = p.cols - c;
+      const size_t o = (size_t)b * n + (size_t)r * p.cols + c;
+      float u[4];
+      load4(static_cast<const T*>(p.x) + o, p.vec, left, u);
+      if (p.momentum) {
+        float m[4];
+        load4(p.momentum + o, p.vec, left, m);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) m[j] = fmaf(p.mu.beta, m[j], u[j]);
+        store4(p.momentum + o, p.vec, left, m);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) u[j] = p.mu.nesterov ? fmaf(p.mu.beta, m[j], u[j]) : m[j];
+      }
+      double s = 0.0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s += (double)u[j] * u[j];
+      sum += s;
     }
     __syncthreads();   // red of the last matrix has been read
     sum = block_sum_f64(sum, red);
@@ -495,46 +535,52 @@ __global__ void __launch_bounds__(kNsThreads, 1) ns_kernel(const __grid_constant
   // X0 as planes; every CTA adds up a matrix's parts, in order
   for (int b = b0; b < b0 + batch; ++b) {
     double sum = 0.0;
-    for (int j = tid; j < size; j += kNsThreads) sum += p.norms[(size_t)b * size + j];
+    for (int j = tid; j < size; j += kThreads) sum += p.norms[(size_t)b * size + j];
     __syncthreads();
     sum = block_sum_f64(sum, red);
     const double inv = 1.0 / (sqrt(sum) + p.eps);
     __half* hi = p.X[0].p + (size_t)b * 2 * p.X[0].plane;
-    const size_t from = (size_t)b * n;
-    const int pairs = (p.cols + 1) / 2;   // two columns at a time
-    const int64_t all = (int64_t)p.rows * pairs;
-#pragma unroll 4
-    for (int64_t i = (int64_t)rank * kNsThreads + tid; i < all; i += (int64_t)size * kNsThreads) {
-      const int r = (int)((uint32_t)i / (uint32_t)pairs), c = 2 * ((int)i - r * pairs);
-      const size_t at = from + (size_t)r * p.cols + c;
-      const float v = (float)((double)source<T>(p, at) * inv) * kPlaneScale;
-      const float w = c + 1 < p.cols ? (float)((double)source<T>(p, at + 1) * inv) * kPlaneScale : 0.f;
-      uint32_t h, l;
-      tc::split_f16x2(v, w, &h, &l);
-      const size_t to = (size_t)r * p.X[0].pitch + c;
-      *reinterpret_cast<uint32_t*>(hi + to) = h;
-      *reinterpret_cast<uint32_t*>(hi + p.X[0].plane + to) = l;
+#pragma unroll 2
+    for (int64_t i = (int64_t)rank * kThreads + tid; i < all; i += (int64_t)size * kThreads) {
+      const int r = (int)((uint32_t)i / (uint32_t)quads), c = 4 * ((int)i - r * quads), left = p.cols - c;
+      const size_t o = (size_t)b * n + (size_t)r * p.cols + c;
+      float u[4];
+      load4(static_cast<const T*>(p.x) + o, p.vec, left, u);
+      if (p.momentum) {
+        float m[4];
+        load4(p.momentum + o, p.vec, left, m);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) u[j] = p.mu.nesterov ? fmaf(p.mu.beta, m[j], u[j]) : m[j];
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) u[j] = (float)((double)u[j] * inv) * kPlaneScale;
+      uint32_t h[2], l[2];
+      tc::split_f16x2(u[0], u[1], &h[0], &l[0]);
+      tc::split_f16x2(u[2], u[3], &h[1], &l[1]);
+      __half* to = hi + (size_t)r * p.X[0].pitch + c;   // the padding behind a row takes the rest
+      *reinterpret_cast<uint2*>(to) = make_uint2(h[0], h[1]);
+      *reinterpret_cast<uint2*>(to + p.X[0].plane) = make_uint2(l[0], l[1]);
     }
   }
   meet();
 
-  // The roles go through the products each in a loop of its own: what one of them keeps does
-  // not cost the others registers (a spilled value comes back from L2 after every meeting).
-  if (warp == kNsWarps) {
+  // The roles go through the products each in a loop of its own.
+  const int first = rank / kCg, stride = size / kCg;
+  if (warp == kWarps) {
     for (int k = 0; k < p.steps; ++k) {
 #pragma unroll 1
       for (int f = kGram; f <= kUpdate; ++f) {
-        const tc::Problem q = ns_problem(p, f, batch);
+        const tc::Problem q = ns_problem<CLUSTER>(p, f, batch);
         const bool tall = p.rows > p.cols;
-        const CUtensorMap *xk = &p.by_k[k & 1], *xr = &p.by_row[k & 1];
-        const CUtensorMap* ma = f == kGram ? (tall ? xr : xk) : f == kPoly ? &p.gram : tall ? xk : &p.poly;
-        const CUtensorMap* mb = f == kGram ? (tall ? xr : xk) : f == kPoly ? &p.gram : tall ? &p.poly : xr;
+        const int w = k & 1;
+        const CUtensorMap* ma = f == kGram ? (tall ? &p.rows_a[w] : &p.k_a[w]) : f == kPoly ? &p.gram_a : tall ? &p.k_a[w] : &p.poly_a;
+        const CUtensorMap* mb = f == kGram ? (tall ? &p.rows_b[w] : &p.k_b[w]) : f == kPoly ? &p.gram_b : tall ? &p.poly_b : &p.rows_b[w];
         const int tiles = tc::problem_tiles(q);
         if (lane == 0) {
-          for (int t = rank; t < tiles && e.ok; t += size) {
-            const tc::Tile x = tile(q, t);
+          for (int t = first; t < tiles && e.ok; t += stride) {
+            const tc::Tile x = tile(q, t, e.rank);
             e.load(q, ma, mb, x);
-            if (wants_prior(q, f)) e.load_extra(f == kPoly ? &p.gram : xk, x);
+            if (wants_prior(q, f)) e.load_extra(f == kPoly ? &p.gram_a : &p.k_a[w], x);
           }
         }
         __syncwarp();
@@ -542,41 +588,47 @@ __global__ void __launch_bounds__(kNsThreads, 1) ns_kernel(const __grid_constant
         if (q.splits > 1) meet();
       }
     }
-  } else if (warp == kNsWarps + 1) {
+  } else if (warp == kWarps + 1) {
     for (int k = 0; k < p.steps; ++k) {
 #pragma unroll 1
       for (int f = kGram; f <= kUpdate; ++f) {
-        const tc::Problem q = ns_problem(p, f, batch);
+        const tc::Problem q = ns_problem<CLUSTER>(p, f, batch);
         const int tiles = tc::problem_tiles(q);
-        for (int t = rank; t < tiles && e.ok; t += size) {
-          e.multiply(q, tile(q, t));
-          if (wants_prior(q, f)) e.skip_extra();
+        if (e.rank == 0) {
+          for (int t = first; t < tiles && e.ok; t += stride) {
+            e.multiply(q, tile(q, t, 0));
+            if (wants_prior(q, f)) e.skip_extra();
+          }
         }
         meet();
         if (q.splits > 1) meet();
       }
     }
   } else {
+    float4* const parts = p.parts + (size_t)b0 * p.parts_each;
     for (int k = 0; k < p.steps; ++k) {
 #pragma unroll 1
       for (int f = kGram; f <= kUpdate; ++f) {
-        const tc::Problem q = ns_problem(p, f, batch);
+        const tc::Problem q = ns_problem<CLUSTER>(p, f, batch);
         const bool last = f == kUpdate && k + 1 == p.steps;
+        // A tile's work as kCg * kWarps warps' shares.  The tiles of this CTA; then, where a product
+        // was split, a second pass in which each warp of the group adds up a share's parts, which
+        // are `whole` tiles apart.
         const int tiles = tc::problem_tiles(q), whole = tiles / q.splits;
-        // The tiles of this CTA; then, where a product was split, a second pass in which each
-        // warp of the group adds up the parts of 32 rows and columns (`whole` tiles apart).
+        constexpr int kShares = kCg * kWarps;
         for (int pass = 0; pass < (q.splits > 1 ? 2 : 1); ++pass) {
-          const int unit = pass == 0 ? rank : rank * kNsWarps + warp, units = pass == 0 ? tiles : whole * kNsWarps;
-          for (int w = unit; w < units && e.ok; w += pass == 0 ? size : size * kNsWarps) {
-            const int t = pass == 0 ? w : w / kNsWarps, part = pass == 0 ? warp : w % kNsWarps;
-            const tc::Tile x = tile(q, t);
+          const int begin = pass == 0 ? first : rank * kWarps + warp, end = pass == 0 ? tiles : whole * kShares;
+          for (int w = begin; w < end && e.ok; w += pass == 0 ? stride : size * kWarps) {
+            const int t = pass == 0 ? w : w / kShares, share = pass == 0 ? e.rank * kWarps + warp : w % kShares;
+            const tc::Tile x = tile(q, t, share / kWarps);
+            const int part = share % kWarps;
             float acc[kNsCols];
             const uint8_t* prior = nullptr;
             if (pass == 0) {
               e.collect(q, x, acc);
               if (!e.ok) break;
               if (q.splits > 1) {
-                float4* o = parts + ((size_t)t * kNsWarps + warp) * (kNsCols * 8) + lane;
+                float4* o = parts + ((size_t)t * kShares + share) * (kNsCols * 8) + lane;
 #pragma unroll
                 for (int j = 0; j < kNsCols / 4; ++j)
                   o[j * 32] = make_float4(acc[4 * j], acc[4 * j + 1], acc[4 * j + 2], acc[4 * j + 3]);
@@ -588,7 +640,7 @@ __global__ void __launch_bounds__(kNsThreads, 1) ns_kernel(const __grid_constant
 #pragma unroll
               for (int j = 0; j < kNsCols; ++j) acc[j] = 0.f;
               for (int g = 0; g < q.splits; ++g) {
-                const float4* o = parts + ((size_t)(t + g * whole) * kNsWarps + part) * (kNsCols * 8) + lane;
+                const float4* o = parts + ((size_t)(t + g * whole) * kShares + share) * (kNsCols * 8) + lane;
                 float4 v[kNsCols / 4];
 #pragma unroll
                 for (int j = 0; j < kNsCols / 4; ++j) v[j] = __ldcg(o + j * 32);
@@ -607,7 +659,7 @@ __global__ void __launch_bounds__(kNsThreads, 1) ns_kernel(const __grid_constant
     }
   }
   if (p.steps == 0) {   // X0 as it is
-    for (int64_t w = b0 * n + rank * (int64_t)kNsThreads + tid; w < n * (b0 + batch); w += (int64_t)size * kNsThreads) {
+    for (int64_t w = b0 * n + rank * (int64_t)kThreads + tid; w < n * (b0 + batch); w += (int64_t)size * kThreads) {
       const int64_t b = w / n, i = w - b * n;
       const size_t o = (size_t)b * 2 * p.X[0].plane + (size_t)(i / p.cols) * p.X[0].pitch + i % p.cols;
       const float v = (__half2float(p.X[0].p[o]) + __half2float(p.X[0].p[p.X[0].plane + o])) * kPlaneInv;
@@ -626,15 +678,15 @@ bool on_tensor_cores(const nc_newton_schulz* d) { return !small_plan(d).fits; }
 
 int plane_pitch(int cols) { return (cols + 63) / 64 * 64; }
 
-// Tiles of a product and its splits along k: as many as shorten the longest SM's k-tiles by
-// more than the sum costs (an extra meeting and a pass over the parts, about 8 k-tiles' time).
-int choose_splits(int64_t tiles, int k, int sms) {
+// Splits of a product along k: as many as shorten the k-tiles of the busiest of `at_once` workers
+// by more than the sum costs (an extra meeting and a pass over the parts, about 8 k-tiles' time).
+int choose_splits(int64_t tiles, int k, int at_once) {
   auto ceil_div = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
-  const int64_t kt = ceil_div(k, NsEngine::BK);
-  int64_t best = ceil_div(tiles, sms) * kt;
+  const int64_t kt = ceil_div(k, tc::kBK);
+  int64_t best = ceil_div(tiles, at_once) * kt;
   int splits = 1;
   for (int s = 2; s <= 32 && s <= kt; ++s) {
-    const int64_t cost = ceil_div(tiles * s, sms) * ceil_div(kt, s) + 8 + s / 4;
+    const int64_t cost = ceil_div(tiles * s, at_once) * ceil_div(kt, s) + 8 + s / 4;
     if (cost < best) best = cost, splits = s;
   }
   return splits;
@@ -662,25 +714,34 @@ NsLayout ns_layout(const nc_newton_schulz* d) {
     L.total = at;
     return L;
   }
-  const int64_t side = (s + kTile - 1) / kTile, triangle = side * (side + 1) / 2;
-  const int64_t all = (int64_t)((d->rows + kTile - 1) / kTile) * ((d->cols + kTile - 1) / kTile);
-  const int64_t count[3] = {triangle, triangle, all};
+  // A cluster's barrier takes a tenth of the grid's; worth it where its CTAs have a tile each, or
+  // where the matrices fill the SMs
+  const auto tiles_of = [&](int64_t m, int64_t k, int high, int wide) {
+    return ((m + high - 1) / high) * ((k + wide - 1) / wide);
+  };
+  L.cluster = tiles_of(d->rows, d->cols, 128, 64) <= kCluster || (int64_t)d->batch * kCluster >= 2 * 148;
+  tc::Problem q{};
+  q.m = q.n = (int)s, q.batch = L.cluster ? 1 : d->batch, q.splits = 1, q.symmetric = 1;
+  if (L.cluster)
+    tc::set_tiles<64, 1>(&q);
+  else
+    tc::set_tiles<128, 2>(&q);
+  const int64_t triangle = tc::problem_tiles(q);
+  const int64_t whole = L.cluster ? tiles_of(d->rows, d->cols, 128, 64) : tiles_of(d->rows, d->cols, 256, 128) * d->batch;
+  const int64_t count[3] = {triangle, triangle, whole};
   const int depth[3] = {d->rows < d->cols ? d->cols : d->rows, (int)s, (int)s};
-  // A cluster's barrier takes a tenth of the grid's; worth it where a cluster's CTAs have a
-  // tile each, or where the matrices fill the SMs
-  L.cluster = all <= kCluster || (int64_t)d->batch * kCluster >= 2 * 148;
-  const int64_t matrices = L.cluster ? 1 : d->batch;
+  const int ctas = L.cluster ? 1 : 2, tile = ctas * 128 * (L.cluster ? 64 : 128);
   int64_t most = 1, parts = 0;
   for (int f = 0; f < 3; ++f) {
-    const int64_t tiles = count[f] * matrices;
-    L.splits[f] = choose_splits(tiles, depth[f], L.cluster ? kCluster : 148);
-    if (tiles * L.splits[f] > most) most = tiles * L.splits[f];
-    if (L.splits[f] > 1 && tiles * L.splits[f] > parts) parts = tiles * L.splits[f];
+    L.splits[f] = choose_splits(count[f], depth[f], L.cluster ? kCluster : 148 / 2);
+    const int64_t all = count[f] * L.splits[f];
+    if (all > most) most = all;
+    if (L.splits[f] > 1 && all > parts) parts = all;
   }
-  L.parts_each = parts * kTile * kTile / 4;
+  L.parts_each = parts * tile / 4;
   // as many CTAs as any product keeps busy, or as share the element-wise passes well
-  int64_t blocks = (int64_t)(d->batch * n / (kNsThreads * 8));
-  if (most > blocks) blocks = most;
+  int64_t blocks = (int64_t)(d->batch * n / 4096 + 1) / 2 * 2;
+  if (most * ctas > blocks) blocks = most * ctas;
   L.blocks = L.cluster ? kCluster * d->batch : (int)(blocks < 148 ? blocks : 148);
   L.norms = take((size_t)d->batch * L.blocks * 8);
   L.x = take(d->batch * x * 4);
@@ -723,39 +784,42 @@ nc_status run_tensor(const nc_newton_schulz* d, const T* x, float* momentum, Muo
   NsArgs a{};
   a.X[0] = planes(L.x, d->rows, d->cols), a.X[1] = planes(L.y, d->rows, d->cols);
   a.G = planes(L.gram, s, s), a.Q = planes(L.poly, s, s);
-  // operands as (own index, k) with k contiguous, or the other way round; every box has 128 of
-  // the own index or 64 of it
-  auto map = [&](CUtensorMap* m, const Planes& q, int rows, int cols, bool by_k) {
-    return tc::make_map(m, q.p, false, 2, cols, rows, q.pitch, q.plane, d->batch, 2 * q.plane, 64,
-                        by_k ? kTile : NsEngine::BK);
+  // operands with k contiguous (a box has as many of the own index as a CTA's tile), or by rows of
+  // k (boxes of 64 by 64)
+  const int a_rows = 128, b_rows = 64;   // of a CTA, in either engine
+  auto map = [&](CUtensorMap* m, const Planes& q, int rows, int cols, int box) {
+    return tc::make_map(m, q.p, false, 2, cols, rows, q.pitch, q.plane, d->batch, 2 * q.plane, 64, box);
   };
   for (int i = 0; i < 2; ++i) {
-    NC_CHECK(map(&a.by_k[i], a.X[i], d->rows, d->cols, true));
-    NC_CHECK(map(&a.by_row[i], a.X[i], d->rows, d->cols, false));
+    NC_CHECK(map(&a.k_a[i], a.X[i], d->rows, d->cols, a_rows));
+    NC_CHECK(map(&a.k_b[i], a.X[i], d->rows, d->cols, b_rows));
+    NC_CHECK(map(&a.rows_a[i], a.X[i], d->rows, d->cols, tc::kBK));
+    a.rows_b[i] = a.rows_a[i];
   }
-  NC_CHECK(map(&a.gram, a.G, s, s, true));
-  NC_CHECK(map(&a.poly, a.Q, s, s, true));
+  NC_CHECK(map(&a.gram_a, a.G, s, s, a_rows));
+  NC_CHECK(map(&a.gram_b, a.G, s, s, b_rows));
+  NC_CHECK(map(&a.poly_a, a.Q, s, s, a_rows));
+  NC_CHECK(map(&a.poly_b, a.Q, s, s, b_rows));
   a.x = x, a.momentum = momentum, a.params = params, a.out = out;
   a.norms = reinterpret_cast<double*>(ws + L.norms), a.parts = reinterpret_cast<float4*>(ws + L.parts);
   a.parts_each = L.parts_each;
   a.batch = d->batch, a.rows = d->rows, a.cols = d->cols, a.steps = d->steps;
   for (int f = 0; f < 3; ++f) a.splits[f] = L.splits[f];
+  a.vec = d->cols % 4 == 0 && (reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(momentum)) % 16 == 0;
   a.a = d->a, a.b = d->b, a.c = d->c, a.eps = d->eps, a.mu = mu, a.decay = decay, a.step = step;
   a.status = reinterpret_cast<int32_t*>(ws + L.status);
   auto k = L.cluster ? ns_kernel<T, true> : ns_kernel<T, false>;
-  constexpr int smem = NsEngine::C::kSmem;
+  const int smem = L.cluster ? NsEngine<true>::C::kSmem : NsEngine<false>::C::kSmem;
   NC_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   cudaLaunchConfig_t cfg{};
-  cudaLaunchAttribute attr[1];
-  if (L.cluster) {
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = kCluster, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
-  } else {
-    attr[0].id = cudaLaunchAttributeCooperative;
-    attr[0].val.cooperative = 1;
-  }
-  cfg.gridDim = dim3((unsigned)L.blocks), cfg.blockDim = dim3(kNsThreads);
-  cfg.dynamicSmemBytes = smem, cfg.stream = st, cfg.attrs = attr, cfg.numAttrs = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = L.cluster ? kCluster : 2, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeCooperative;
+  attr[1].val.cooperative = 1;
+  cfg.gridDim = dim3((unsigned)L.blocks);
+  cfg.blockDim = dim3(L.cluster ? NsEngine<true>::C::kThreads : NsEngine<false>::C::kThreads);
+  cfg.dynamicSmemBytes = smem, cfg.stream = st, cfg.attrs = attr, cfg.numAttrs = L.cluster ? 1 : 2;
   NC_CUDA_CHECK(cudaLaunchKernelEx(&cfg, k, a));
   return launch_check("ns_kernel launch");
 }

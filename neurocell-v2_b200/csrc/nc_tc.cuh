@@ -34,7 +34,7 @@ struct Problem {
   int m, n, k;
   int a_mn, b_mn;
   int tiles_m, tiles_n, batch, splits;   // splits of k; tiles run over m first
-  int symmetric;                         // D is symmetric: tiles below the diagonal are not computed
+  int symmetric;                         // D is symmetric: tiles below the diagonal are left out
   int chunk;                             // k-tiles per accumulator
   int bf16;
   int a_k0, b_k0, b_n0;                  // offsets into the stored operands
@@ -60,13 +60,16 @@ struct Config {
   static constexpr int kPiece = kCols < 64 ? kCols : 64;  // 16-bit values of a row in a warp's patch
   static constexpr int kPatch = 32 * kPiece * 2;
   static constexpr int kThreads = 32 * (EW + 2);
+  static constexpr int kExtras = (BN + 63) / 64;          // stages of an extra tile (load_extra)
   static constexpr int kStage = kA + kB;
   static constexpr int kStages = 192 * 1024 / kStage;
   static constexpr int kSmem = kStages * kStage + EW * kPatch;   // the stages first, on 1024 bytes
 };
 
+// A symmetric D wants tiles twice as high as wide: those with column index j >= 2 i then hold
+// all on and above the diagonal, row i of them tiles_n - 2 i.
 __host__ __device__ inline int problem_tiles(const Problem& p) {
-  const int mn = p.symmetric ? p.tiles_m * (p.tiles_m + 1) / 2 : p.tiles_m * p.tiles_n;
+  const int mn = p.symmetric ? p.tiles_m * (p.tiles_n - p.tiles_m + 1) : p.tiles_m * p.tiles_n;
   return mn * p.batch * p.splits;
 }
 
@@ -76,12 +79,12 @@ __device__ __forceinline__ Tile problem_tile(const Problem& p, int t, int rank) 
   Tile x;
   int mn;
   if (p.symmetric) {
-    const int per = p.tiles_m * (p.tiles_m + 1) / 2;
+    const int per = p.tiles_m * (p.tiles_n - p.tiles_m + 1);
     mn = t % per;
     t /= per;
-    int j = 0;   // column j holds rows 0..j
-    while (mn > j) mn -= ++j;
-    x.m0 = mn * kBM, x.n0 = j * BN;
+    int i = 0;
+    for (; mn >= p.tiles_n - 2 * i; ++i) mn -= p.tiles_n - 2 * i;
+    x.m0 = i * kBM * CG + rank * kBM, x.n0 = (2 * i + mn) * BN;
   } else {
     const int per = p.tiles_m * p.tiles_n;
     mn = t % per;
@@ -105,14 +108,14 @@ __device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
 __device__ __forceinline__ void bar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-// The same barrier in the pair's first CTA.
-__device__ __forceinline__ uint32_t leader_addr(uint32_t bar) {
+// The same barrier in another CTA of the cluster.
+__device__ __forceinline__ uint32_t remote_addr(uint32_t bar, uint32_t cta) {
   uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(bar));
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(bar), "r"(cta));
   return r;
 }
-__device__ __forceinline__ void bar_arrive_leader(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(leader_addr(bar)) : "memory");
+__device__ __forceinline__ void bar_arrive_remote(uint32_t bar, uint32_t cta) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(remote_addr(bar, cta)) : "memory");
 }
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -177,15 +180,16 @@ __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t
         "l"(a), "l"(b), "r"(idesc), "r"(add)
         : "memory");
 }
-// One arrival on `bar` (of both CTAs of a pair) when the products issued so far are done.
+// One arrival on `bar` (in both CTAs of the pair that starts with CTA `lead`) when the products
+// issued so far are done.
 template <int CG>
-__device__ __forceinline__ void mma_commit(uint32_t bar) {
+__device__ __forceinline__ void mma_commit(uint32_t bar, uint32_t lead) {
   if constexpr (CG == 1)
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
   else
     asm volatile(
         "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
-        "h"((uint16_t)3)
+        "h"((uint16_t)(3u << lead))
         : "memory");
 }
 template <int CG>
@@ -302,9 +306,9 @@ __device__ __forceinline__ void load_v8(const void* p, uint32_t (&v)[8]) {
 // What a CTA's warps share beside the stages.
 template <int PL, int BN, int CG, int EW>
 struct Shared {
-  uint64_t bars[2 * Config<PL, BN, CG, EW>::kStages + 5];
+  uint64_t bars[2 * Config<PL, BN, CG, EW>::kStages + 5 + Config<PL, BN, CG, EW>::kExtras];
   uint32_t tmem_slot;
-  int abort, extra_readers[Config<PL, BN, CG, EW>::kStages];
+  int abort, extra_readers[Config<PL, BN, CG, EW>::kExtras];
 };
 
 // One warp's view of the pipeline: the loading warp fills stages, the multiplying warp (of a
@@ -315,16 +319,18 @@ struct Engine {
   using C = Config<PL, BN, CG, EW>;
   static constexpr int BK = kBK, COLS = C::kCols, kEpiWarps = EW;
   static constexpr uint32_t a_block = C::kA / (kBM / 64), b_block = C::kB / (C::kBRows / 64);
+  static_assert(C::kBRows >= 64, "operands by columns come in blocks of 64");
 
   uint32_t stages, bar0, tmem;
   uint8_t *base, *patch;   // of the stages, and of this epilogue warp
   int* extra_readers;
   volatile int* abort;
   int32_t* status;
-  int rank;
+  int rank;        // in the pair
+  uint32_t lead;   // the pair's first CTA in the cluster
   // stage and its phase (loader and multiplier), accumulator and its phase (multiplier; the
-  // epilogue's is ph), the epilogue's own stage for extra()
-  int s = 0, buf = 0, issued = 0, es = 0;
+  // epilogue's is ph); the epilogue's own stage and the phase of extra tiles
+  int s = 0, buf = 0, issued = 0, extras = 0, es = 0;
   uint32_t ph, aph = 1, eph = 0;
   bool ok = true;
 
@@ -333,6 +339,7 @@ struct Engine {
   __device__ __forceinline__ uint32_t acc_full(int i) const { return bar0 + 8 * (2 * C::kStages + i); }
   __device__ __forceinline__ uint32_t acc_empty(int i) const { return bar0 + 8 * (2 * C::kStages + 2 + i); }
   __device__ __forceinline__ uint32_t drain() const { return bar0 + 8 * (2 * C::kStages + 4); }
+  __device__ __forceinline__ uint32_t extra_full(int i) const { return bar0 + 8 * (2 * C::kStages + 5 + i); }
 
   // By the whole CTA, before it reads anything that an earlier kernel wrote.  `raw`: the dynamic
   // shared memory, on 1024 bytes.
@@ -344,14 +351,15 @@ struct Engine {
     bar0 = smem_addr(sh->bars);
     abort = &sh->abort;
     status = status_word;
-    rank = CG == 1 ? 0 : (int)cluster_rank();
+    const uint32_t cta = CG == 1 ? 0 : cluster_rank();
+    rank = cta & 1, lead = cta & ~1u;
     const int warp = threadIdx.x >> 5;
     ph = warp == kEpiWarps;   // the loader starts on empty stages
     if (threadIdx.x == 0) {
       for (int i = 0; i < C::kStages; ++i) bar_init(full(i), 1), bar_init(empty(i), 1);
       for (int i = 0; i < 2; ++i) bar_init(acc_full(i), 1), bar_init(acc_empty(i), kEpiWarps * CG);
       bar_init(drain(), 1);
-      for (int i = 0; i < C::kStages; ++i) sh->extra_readers[i] = 0;
+      for (int i = 0; i < C::kExtras; ++i) bar_init(extra_full(i), 1), sh->extra_readers[i] = 0;
       sh->abort = 0;
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -368,7 +376,7 @@ struct Engine {
     for (int kt = x.kt0; kt < x.kt1 && ok; ++kt) {
       if (!(ok = bar_wait(empty(s), ph, abort, status))) return;
       if (rank == 0) bar_expect(full(s), C::kStage * CG);
-      const uint32_t bar = CG == 1 ? full(s) : leader_addr(full(s));
+      const uint32_t bar = CG == 1 ? full(s) : remote_addr(full(s), lead);
       const uint32_t at = stages + s * C::kStage;
       const int ka = p.a_k0 + kt * BK, kb = p.b_k0 + kt * BK, nb = p.b_n0 + x.n0 + rank * C::kBRows;
       if (p.a_mn) {
@@ -389,21 +397,28 @@ struct Engine {
     }
   }
 
-  // One more stage behind a tile's k-tiles: BN columns (from x.n0 on) of kBM rows of a stored
-  // matrix, both planes, that the epilogue wants (BN = 128, two planes: exactly a stage).  The
-  // multiplying warp steps over it, the epilogue takes it with extra() and extra_done().
+  // Behind a tile's k-tiles, what the epilogue wants of a stored matrix: this CTA's rows of the
+  // tile, both planes, a stage for every 64 columns.  It lands in this CTA (of a pair too) on
+  // barriers of its own; the multiplying warp steps over it with skip_extra(), the epilogue
+  // takes it with extra() and extra_done().
   __device__ __forceinline__ void load_extra(const CUtensorMap* m, const Tile& x) {
-    static_assert(C::kStage == 2 * PL * kBM * 128 && CG == 1, "an extra tile fills a stage");
-    if (!ok || !(ok = bar_wait(empty(s), ph, abort, status))) return;
-    bar_expect(full(s), C::kStage);
+    constexpr int bytes = PL * kBM * 128;
+    static_assert(bytes <= C::kStage, "64 columns fit a stage");
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      tma_load<CG>(stages + s * C::kStage + i * (C::kStage / 2), m, full(s), x.n0 + 64 * i, x.m0, x.batch);
-    if (issued < C::kStages) ++issued;
-    if (++s == C::kStages) s = 0, ph ^= 1;
+    for (int i = 0; i < C::kExtras; ++i) {
+      if (!ok || !(ok = bar_wait(empty(s), ph, abort, status))) return;
+      bar_expect(extra_full(i), bytes);
+      tma_load<1>(stages + s * C::kStage, m, extra_full(i), x.n0 + 64 * i, x.m0, x.batch);
+      if (rank == 0) bar_arrive(full(s));   // keeps the stage's phases in step
+      if (issued < C::kStages) ++issued;
+      if (++s == C::kStages) s = 0, ph ^= 1;
+    }
+    ++extras;
   }
   __device__ __forceinline__ void skip_extra() {
-    if (++s == C::kStages) s = 0, ph ^= 1;
+#pragma unroll
+    for (int i = 0; i < C::kExtras; ++i)
+      if (++s == C::kStages) s = 0, ph ^= 1;
   }
 
   // The multiplying warp, whole: what it computes is the same on all lanes and stays in
@@ -436,8 +451,8 @@ struct Engine {
               mma<CG>(d, desc(a + pa * a_plane + ks * a_step), desc(b + pb * b_plane + ks * b_step), idesc,
                       kt > c0 || q > 0 || ks > 0);
           }
-          mma_commit<CG>(empty(s));
-          if (kt + 1 == c1) mma_commit<CG>(acc_full(buf));
+          mma_commit<CG>(empty(s), lead);
+          if (kt + 1 == c1) mma_commit<CG>(acc_full(buf), lead);
         }
         __syncwarp();
         if (++s == C::kStages) s = 0, ph ^= 1;
@@ -471,48 +486,57 @@ struct Engine {
         if constexpr (CG == 1)
           bar_arrive(acc_empty(buf));
         else
-          bar_arrive_leader(acc_empty(buf));
+          bar_arrive_remote(acc_empty(buf), lead);
       }
       __syncwarp();
       buf ^= 1;
       if (buf == 0) ph ^= 1;
     }
-    for (es += x.kt1 - x.kt0; es >= C::kStages; es -= C::kStages) eph ^= 1;
+    es = (es + x.kt1 - x.kt0) % C::kStages;
   }
 
-  // An epilogue warp, after collect(): the extra stage (null after an abort), whose half i holds
-  // 64 columns: plane, row, 128 bytes in 16-byte pieces q ^ (row & 7).  Every epilogue warp calls
-  // extra_done() when it has read its part.
-  __device__ __forceinline__ uint8_t* extra() {
-    if (!__all_sync(0xffffffffu, ok && bar_wait(full(es), eph, abort, status))) {
+  // An epilogue warp, after collect(): the stage of its columns' 64 (null after an abort): plane,
+  // row, 128 bytes in 16-byte pieces q ^ (row & 7).  Every epilogue warp calls extra_done() when it
+  // has read its part; the last of a stage's readers frees it.
+  __device__ __forceinline__ const uint8_t* extra() {
+    const int i = (threadIdx.x >> 7) * COLS / 64;
+    if (!__all_sync(0xffffffffu, ok && bar_wait(extra_full(i), eph, abort, status))) {
       ok = false;
       return nullptr;
     }
-    return base + es * C::kStage;
+    const int at = es + i;
+    return base + (at >= C::kStages ? at - C::kStages : at) * C::kStage;
   }
   __device__ __forceinline__ void extra_done() {
+    const int i = (threadIdx.x >> 7) * COLS / 64, at = es + i;
     __syncwarp();
     if ((threadIdx.x & 31) == 0) {
       __threadfence_block();
-      if (atomicAdd(extra_readers + es, 1) % kEpiWarps == kEpiWarps - 1) bar_arrive(empty(es));
+      constexpr int readers = EW / C::kExtras;
+      if (atomicAdd(extra_readers + i, 1) % readers == readers - 1) bar_arrive(empty(at >= C::kStages ? at - C::kStages : at));
     }
-    if (++es == C::kStages) es = 0, eph ^= 1;
+    eph ^= 1;
+    es += C::kExtras;
+    if (es >= C::kStages) es -= C::kStages;
   }
 
   // At the end, by the whole CTA.
   __device__ __forceinline__ void finish() {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (warp == kEpiWarps && lane == 0 && !ok && rank == 0) {
+    if (warp == kEpiWarps && lane == 0 && (!ok || *abort)) {
       // the copies in flight land before the CTA (or the pair) ends
-      for (int i = 0; i < issued; ++i) {
+      for (int i = 0; i < issued && rank == 0; ++i) {
         if (s-- == 0) s = C::kStages - 1, ph ^= 1;
         for (int j = 0; j < kWaitLimit && !bar_try(full(s), ph ^ 1); ++j) {
         }
       }
+      for (int i = 0; i < C::kExtras && extras > 0; ++i)
+        for (int j = 0; j < kWaitLimit && !bar_try(extra_full(i), (extras - 1) & 1); ++j) {
+        }
     }
     if (warp == kEpiWarps + 1 && rank == 0) {
       // every product has finished before tensor memory is given back
-      if (elect_one()) mma_commit<CG>(drain());
+      if (elect_one()) mma_commit<CG>(drain(), lead);
       for (int j = 0; j < kWaitLimit && !bar_try(drain(), 0); ++j) {
       }
     }
@@ -581,7 +605,7 @@ nc_status make_operand(Problem* p, bool is_a, const void* base, bool mn, int own
 
 // Tiles that cover (m, n).
 template <int BN, int CG>
-void set_tiles(Problem* p) {
+__host__ __device__ inline void set_tiles(Problem* p) {
   p->tiles_m = (p->m + kBM * CG - 1) / (kBM * CG), p->tiles_n = (p->n + BN - 1) / BN;
 }
 
