@@ -261,11 +261,15 @@ nc_status launch_small(const SmallArgs& a, const SmallPlan& r, int batch, cudaSt
 constexpr float kPlaneScale = 4096.f, kPlaneInv = 1.f / 4096.f;
 constexpr int kNsChunk = 1;  // k-tiles (of 64) per accumulator: Gram sums of one sign show the additions' truncation
 constexpr int kNsCols = 32;  // columns of an epilogue thread
-// Where matrices have many tiles: pairs of CTAs on 256 x 128 (a product reads and writes 120 KB
-// of a CTA's shared memory per k-tile, 160 KB as one CTA's 128 x 128), the whole grid on all
-// matrices.  Where they have few: 128 x 64 and a cluster of 8 on each matrix.
+// Where matrices have many tiles: 128 x 128, the whole grid on all matrices (pairs of CTAs on
+// 256 x 128 took 146 cycles for a product of 16 k that one CTA does in 115 on its half).  Where
+// they have few: 128 x 64 and a cluster of 8 on each matrix.
 template <bool CLUSTER>
-using NsEngine = tc::Engine<2, CLUSTER ? 64 : 128, CLUSTER ? 1 : 2, CLUSTER ? 8 : 16>;
+struct NsTile {
+  static constexpr int kBN = CLUSTER ? 64 : 128, kWarps = CLUSTER ? 8 : 16;
+};
+template <bool CLUSTER>
+using NsEngine = tc::Engine<2, NsTile<CLUSTER>::kBN, 1, NsTile<CLUSTER>::kWarps>;
 static_assert(NsEngine<true>::COLS == kNsCols && NsEngine<false>::COLS == kNsCols, "the epilogue is written for 32");
 
 struct Planes {   // (batch, plane, rows, pitch)
@@ -372,11 +376,9 @@ __device__ __forceinline__ void ns_store(const NsArgs& p, NsProduct product, int
   const int lane = threadIdx.x & 31, rows = min(32, m - row0), cols = min(32, n - col);
   const size_t at = (size_t)x.batch * 2 * dst.plane + (size_t)row0 * dst.pitch + col;
   const float mul = product == kPoly ? p.c * kPlaneInv : kPlaneInv, add = product == kPoly ? p.b : p.a;
-  // Symmetric results: the 128 rows of this CTA against its columns.  Left of the diagonal's
-  // square another tile's mirror image fills in (one writer, so the bits do not depend on which
-  // comes last); right of it this one's goes there.
-  const bool beside = product != kUpdate && col < x.m0, mirror = product != kUpdate && col >= x.m0 + tc::kBM;
-  if (rows <= 0 || cols <= 0 || beside) return;   // the same for the whole warp
+  // symmetric results: what lies right of the diagonal's square goes left of it too
+  const bool mirror = product != kUpdate && col >= x.m0 + tc::kBM;
+  if (rows <= 0 || cols <= 0) return;   // the same for the whole warp
 #pragma unroll
   for (int j = 0; j < 32; ++j) acc[j] *= mul;
   if (product != kGram && prior) {
@@ -438,7 +440,7 @@ __device__ __forceinline__ tc::Problem ns_problem(const NsArgs& p, int f, int ba
   tc::Problem q;
   q.m = f == kUpdate ? p.rows : s, q.n = f == kUpdate ? p.cols : s, q.k = f == kGram ? len : s;
   q.a_mn = f == kGram && tall, q.b_mn = f == kGram ? tall : f == kUpdate && !tall;
-  tc::set_tiles<CLUSTER ? 64 : 128, CLUSTER ? 1 : 2>(&q);
+  tc::set_tiles<NsTile<CLUSTER>::kBN, 1>(&q);
   q.batch = batch, q.splits = p.splits[f], q.symmetric = f != kUpdate, q.chunk = kNsChunk, q.bf16 = 0;
   q.a_k0 = q.b_k0 = q.b_n0 = 0;
   return q;
@@ -475,9 +477,9 @@ __device__ __forceinline__ void store4(float* p, bool vec, int left, const float
 template <typename T, bool CLUSTER>
 __global__ void __launch_bounds__(NsEngine<CLUSTER>::C::kThreads, 1) ns_kernel(const __grid_constant__ NsArgs p) {
   using E = NsEngine<CLUSTER>;
-  constexpr int kWarps = E::kEpiWarps, kThreads = E::C::kThreads, kCg = CLUSTER ? 1 : 2, kBN = CLUSTER ? 64 : 128;
+  constexpr int kWarps = E::kEpiWarps, kThreads = E::C::kThreads, kBN = NsTile<CLUSTER>::kBN;
   extern __shared__ __align__(1024) uint8_t raw[];
-  __shared__ tc::Shared<2, kBN, kCg, kWarps> sh;
+  __shared__ tc::Shared<2, kBN, 1, kWarps> sh;
   __shared__ double red[kThreads / 32];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (blockIdx.x == 0 && tid == 0) *p.status = 0;
@@ -495,8 +497,8 @@ __global__ void __launch_bounds__(NsEngine<CLUSTER>::C::kThreads, 1) ns_kernel(c
       cooperative_groups::this_grid().sync();
     asm volatile("fence.proxy.async;" ::: "memory");
   };
-  auto tile = [&](const tc::Problem& q, int t, int in_pair) {
-    tc::Tile x = tc::problem_tile<kBN, kCg>(q, t, in_pair);
+  auto tile = [&](const tc::Problem& q, int t) {
+    tc::Tile x = tc::problem_tile<kBN, 1>(q, t, 0);
     x.batch += b0;
     return x;
   };
@@ -565,7 +567,6 @@ __global__ void __launch_bounds__(NsEngine<CLUSTER>::C::kThreads, 1) ns_kernel(c
   meet();
 
   // The roles go through the products each in a loop of its own.
-  const int first = rank / kCg, stride = size / kCg;
   if (warp == kWarps) {
     for (int k = 0; k < p.steps; ++k) {
 #pragma unroll 1
@@ -575,10 +576,10 @@ __global__ void __launch_bounds__(NsEngine<CLUSTER>::C::kThreads, 1) ns_kernel(c
         const int w = k & 1;
         const CUtensorMap* ma = f == kGram ? (tall ? &p.rows_a[w] : &p.k_a[w]) : f == kPoly ? &p.gram_a : tall ? &p.k_a[w] : &p.poly_a;
         const CUtensorMap* mb = f == kGram ? (tall ? &p.rows_b[w] : &p.k_b[w]) : f == kPoly ? &p.gram_b : tall ? &p.poly_b : &p.rows_b[w];
-        const int tiles = tc::problem_tiles(q);
+        const int tiles = tc::problem_tiles<kBN, 1>(q);
         if (lane == 0) {
-          for (int t = first; t < tiles && e.ok; t += stride) {
-            const tc::Tile x = tile(q, t, e.rank);
+          for (int t = rank; t < tiles && e.ok; t += size) {
+            const tc::Tile x = tile(q, t);
             e.load(q, ma, mb, x);
             if (wants_prior(q, f)) e.load_extra(f == kPoly ? &p.gram_a : &p.k_a[w], x);
           }
@@ -593,12 +594,10 @@ __global__ void __launch_bounds__(NsEngine<CLUSTER>::C::kThreads, 1) ns_kernel(c
 #pragma unroll 1
       for (int f = kGram; f <= kUpdate; ++f) {
         const tc::Problem q = ns_problem<CLUSTER>(p, f, batch);
-        const int tiles = tc::problem_tiles(q);
-        if (e.rank == 0) {
-          for (int t = first; t < tiles && e.ok; t += stride) {
-            e.multiply(q, tile(q, t, 0));
-            if (wants_prior(q, f)) e.skip_extra();
-          }
+        const int tiles = tc::problem_tiles<kBN, 1>(q);
+        for (int t = rank; t < tiles && e.ok; t += size) {
+          e.multiply(q, tile(q, t));
+          if (wants_prior(q, f)) e.skip_extra();
         }
         meet();
         if (q.splits > 1) meet();
@@ -611,24 +610,21 @@ __global__ void __launch_bounds__(NsEngine<CLUSTER>::C::kThreads, 1) ns_kernel(c
       for (int f = kGram; f <= kUpdate; ++f) {
         const tc::Problem q = ns_problem<CLUSTER>(p, f, batch);
         const bool last = f == kUpdate && k + 1 == p.steps;
-        // A tile's work as kCg * kWarps warps' shares.  The tiles of this CTA; then, where a product
-        // was split, a second pass in which each warp of the group adds up a share's parts, which
-        // are `whole` tiles apart.
-        const int tiles = tc::problem_tiles(q), whole = tiles / q.splits;
-        constexpr int kShares = kCg * kWarps;
+        // The tiles of this CTA; then, where a product was split, a second pass in which each warp
+        // of the group adds up the parts of one warp's rows and columns, `whole` tiles apart.
+        const int tiles = tc::problem_tiles<kBN, 1>(q), whole = tiles / q.splits;
         for (int pass = 0; pass < (q.splits > 1 ? 2 : 1); ++pass) {
-          const int begin = pass == 0 ? first : rank * kWarps + warp, end = pass == 0 ? tiles : whole * kShares;
-          for (int w = begin; w < end && e.ok; w += pass == 0 ? stride : size * kWarps) {
-            const int t = pass == 0 ? w : w / kShares, share = pass == 0 ? e.rank * kWarps + warp : w % kShares;
-            const tc::Tile x = tile(q, t, share / kWarps);
-            const int part = share % kWarps;
+          const int begin = pass == 0 ? rank : rank * kWarps + warp, end = pass == 0 ? tiles : whole * kWarps;
+          for (int w = begin; w < end && e.ok; w += pass == 0 ? size : size * kWarps) {
+            const int t = pass == 0 ? w : w / kWarps, part = pass == 0 ? warp : w % kWarps;
+            const tc::Tile x = tile(q, t);
             float acc[kNsCols];
             const uint8_t* prior = nullptr;
             if (pass == 0) {
               e.collect(q, x, acc);
               if (!e.ok) break;
               if (q.splits > 1) {
-                float4* o = parts + ((size_t)t * kShares + share) * (kNsCols * 8) + lane;
+                float4* o = parts + ((size_t)t * kWarps + warp) * (kNsCols * 8) + lane;
 #pragma unroll
                 for (int j = 0; j < kNsCols / 4; ++j)
                   o[j * 32] = make_float4(acc[4 * j], acc[4 * j + 1], acc[4 * j + 2], acc[4 * j + 3]);
@@ -640,7 +636,7 @@ __global__ void __launch_bounds__(NsEngine<CLUSTER>::C::kThreads, 1) ns_kernel(c
 #pragma unroll
               for (int j = 0; j < kNsCols; ++j) acc[j] = 0.f;
               for (int g = 0; g < q.splits; ++g) {
-                const float4* o = parts + ((size_t)(t + g * whole) * kShares + share) * (kNsCols * 8) + lane;
+                const float4* o = parts + ((size_t)(t + g * whole) * kWarps + part) * (kNsCols * 8) + lane;
                 float4 v[kNsCols / 4];
 #pragma unroll
                 for (int j = 0; j < kNsCols / 4; ++j) v[j] = __ldcg(o + j * 32);
@@ -716,32 +712,30 @@ NsLayout ns_layout(const nc_newton_schulz* d) {
   }
   // A cluster's barrier takes a tenth of the grid's; worth it where its CTAs have a tile each, or
   // where the matrices fill the SMs
-  const auto tiles_of = [&](int64_t m, int64_t k, int high, int wide) {
-    return ((m + high - 1) / high) * ((k + wide - 1) / wide);
-  };
-  L.cluster = tiles_of(d->rows, d->cols, 128, 64) <= kCluster || (int64_t)d->batch * kCluster >= 2 * 148;
+  const auto tiles_of = [](int64_t m, int64_t n, int wide) { return ((m + 127) / 128) * ((n + wide - 1) / wide); };
+  L.cluster = tiles_of(d->rows, d->cols, 64) <= kCluster || (int64_t)d->batch * kCluster >= 2 * 148;
   tc::Problem q{};
   q.m = q.n = (int)s, q.batch = L.cluster ? 1 : d->batch, q.splits = 1, q.symmetric = 1;
   if (L.cluster)
     tc::set_tiles<64, 1>(&q);
   else
-    tc::set_tiles<128, 2>(&q);
-  const int64_t triangle = tc::problem_tiles(q);
-  const int64_t whole = L.cluster ? tiles_of(d->rows, d->cols, 128, 64) : tiles_of(d->rows, d->cols, 256, 128) * d->batch;
+    tc::set_tiles<128, 1>(&q);
+  const int64_t triangle = L.cluster ? tc::problem_tiles<64, 1>(q) : tc::problem_tiles<128, 1>(q);
+  const int64_t whole = tiles_of(d->rows, d->cols, L.cluster ? 64 : 128) * q.batch;
   const int64_t count[3] = {triangle, triangle, whole};
   const int depth[3] = {d->rows < d->cols ? d->cols : d->rows, (int)s, (int)s};
-  const int ctas = L.cluster ? 1 : 2, tile = ctas * 128 * (L.cluster ? 64 : 128);
+  const int tile = 128 * (L.cluster ? 64 : 128);
   int64_t most = 1, parts = 0;
   for (int f = 0; f < 3; ++f) {
-    L.splits[f] = choose_splits(count[f], depth[f], L.cluster ? kCluster : 148 / 2);
+    L.splits[f] = choose_splits(count[f], depth[f], L.cluster ? kCluster : 148);
     const int64_t all = count[f] * L.splits[f];
     if (all > most) most = all;
     if (L.splits[f] > 1 && all > parts) parts = all;
   }
   L.parts_each = parts * tile / 4;
   // as many CTAs as any product keeps busy, or as share the element-wise passes well
-  int64_t blocks = (int64_t)(d->batch * n / 4096 + 1) / 2 * 2;
-  if (most * ctas > blocks) blocks = most * ctas;
+  int64_t blocks = (int64_t)(d->batch * n / 4096);
+  if (most > blocks) blocks = most;
   L.blocks = L.cluster ? kCluster * d->batch : (int)(blocks < 148 ? blocks : 148);
   L.norms = take((size_t)d->batch * L.blocks * 8);
   L.x = take(d->batch * x * 4);
@@ -786,7 +780,7 @@ nc_status run_tensor(const nc_newton_schulz* d, const T* x, float* momentum, Muo
   a.G = planes(L.gram, s, s), a.Q = planes(L.poly, s, s);
   // operands with k contiguous (a box has as many of the own index as a CTA's tile), or by rows of
   // k (boxes of 64 by 64)
-  const int a_rows = 128, b_rows = 64;   // of a CTA, in either engine
+  const int a_rows = 128, b_rows = L.cluster ? 64 : 128;
   auto map = [&](CUtensorMap* m, const Planes& q, int rows, int cols, int box) {
     return tc::make_map(m, q.p, false, 2, cols, rows, q.pitch, q.plane, d->batch, 2 * q.plane, 64, box);
   };
@@ -812,14 +806,17 @@ nc_status run_tensor(const nc_newton_schulz* d, const T* x, float* momentum, Muo
   const int smem = L.cluster ? NsEngine<true>::C::kSmem : NsEngine<false>::C::kSmem;
   NC_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   cudaLaunchConfig_t cfg{};
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = L.cluster ? kCluster : 2, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeCooperative;
-  attr[1].val.cooperative = 1;
+  cudaLaunchAttribute attr[1];
+  if (L.cluster) {
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = kCluster, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+  } else {
+    attr[0].id = cudaLaunchAttributeCooperative;
+    attr[0].val.cooperative = 1;
+  }
   cfg.gridDim = dim3((unsigned)L.blocks);
   cfg.blockDim = dim3(L.cluster ? NsEngine<true>::C::kThreads : NsEngine<false>::C::kThreads);
-  cfg.dynamicSmemBytes = smem, cfg.stream = st, cfg.attrs = attr, cfg.numAttrs = L.cluster ? 1 : 2;
+  cfg.dynamicSmemBytes = smem, cfg.stream = st, cfg.attrs = attr, cfg.numAttrs = 1;
   NC_CUDA_CHECK(cudaLaunchKernelEx(&cfg, k, a));
   return launch_check("ns_kernel launch");
 }

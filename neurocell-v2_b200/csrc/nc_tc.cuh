@@ -25,6 +25,10 @@ namespace tc {
 
 constexpr int kBM = 128;            // rows of a tile per CTA: one tensor-memory lane each
 constexpr int kBK = 64;             // k of a stage: a swizzled row of 128 bytes (rows of 64 took products 6 % longer)
+// The tensor core adds toward zero: where a chunk's terms share a sign (the diagonal of a Gram
+// matrix) the sum of a k-tile comes out short by about 2^-22 of itself.  Given back, the
+// orthogonalised 96 x 4000 matrix is off by 1.3e-6 instead of 1.7e-6.
+constexpr float kRestore = 1.f + 2.3841858e-7f;
 constexpr int kWaitLimit = 1 << 20; // polls of a bounded wait
 
 // One product of (batched) matrices, D (m, n) = A (m, k) B (n, k)^T.  An operand is stored
@@ -60,17 +64,24 @@ struct Config {
   static constexpr int kPiece = kCols < 64 ? kCols : 64;  // 16-bit values of a row in a warp's patch
   static constexpr int kPatch = 32 * kPiece * 2;
   static constexpr int kThreads = 32 * (EW + 2);
+  // Accumulators in turn: all that 512 columns of tensor memory hold, up to 4.  A drain takes
+  // about 2000 cycles from the last product to the freed accumulator (of a pair), more than a
+  // k-tile's products on a narrow tile.
+  static constexpr int kAccs = BN >= 256 ? 2 : 4;
   static constexpr int kExtras = (BN + 63) / 64;          // stages of an extra tile (load_extra)
   static constexpr int kStage = kA + kB;
   static constexpr int kStages = 192 * 1024 / kStage;
   static constexpr int kSmem = kStages * kStage + EW * kPatch;   // the stages first, on 1024 bytes
 };
 
-// A symmetric D wants tiles twice as high as wide: those with column index j >= 2 i then hold
-// all on and above the diagonal, row i of them tiles_n - 2 i.
+// Symmetric D, tiles `high` times as high as wide: those with column index j >= high i hold all
+// on and above the diagonal, row i of them tiles_n - high i.
+__host__ __device__ inline int symmetric_tiles(const Problem& p, int high) {
+  return p.tiles_m * p.tiles_n - high * (p.tiles_m * (p.tiles_m - 1) / 2);
+}
+template <int BN, int CG>
 __host__ __device__ inline int problem_tiles(const Problem& p) {
-  const int mn = p.symmetric ? p.tiles_m * (p.tiles_n - p.tiles_m + 1) : p.tiles_m * p.tiles_n;
-  return mn * p.batch * p.splits;
+  return (p.symmetric ? symmetric_tiles(p, kBM * CG / BN) : p.tiles_m * p.tiles_n) * p.batch * p.splits;
 }
 
 // `rank`: of the CTA in its pair.
@@ -79,12 +90,13 @@ __device__ __forceinline__ Tile problem_tile(const Problem& p, int t, int rank) 
   Tile x;
   int mn;
   if (p.symmetric) {
-    const int per = p.tiles_m * (p.tiles_n - p.tiles_m + 1);
+    constexpr int high = kBM * CG / BN;
+    const int per = symmetric_tiles(p, high);
     mn = t % per;
     t /= per;
     int i = 0;
-    for (; mn >= p.tiles_n - 2 * i; ++i) mn -= p.tiles_n - 2 * i;
-    x.m0 = i * kBM * CG + rank * kBM, x.n0 = (2 * i + mn) * BN;
+    for (; mn >= p.tiles_n - high * i; ++i) mn -= p.tiles_n - high * i;
+    x.m0 = i * kBM * CG + rank * kBM, x.n0 = (high * i + mn) * BN;
   } else {
     const int per = p.tiles_m * p.tiles_n;
     mn = t % per;
@@ -306,7 +318,7 @@ __device__ __forceinline__ void load_v8(const void* p, uint32_t (&v)[8]) {
 // What a CTA's warps share beside the stages.
 template <int PL, int BN, int CG, int EW>
 struct Shared {
-  uint64_t bars[2 * Config<PL, BN, CG, EW>::kStages + 5 + Config<PL, BN, CG, EW>::kExtras];
+  uint64_t bars[2 * Config<PL, BN, CG, EW>::kStages + 2 * Config<PL, BN, CG, EW>::kAccs + 1 + Config<PL, BN, CG, EW>::kExtras];
   uint32_t tmem_slot;
   int abort, extra_readers[Config<PL, BN, CG, EW>::kExtras];
 };
@@ -337,9 +349,9 @@ struct Engine {
   __device__ __forceinline__ uint32_t full(int i) const { return bar0 + 8 * i; }
   __device__ __forceinline__ uint32_t empty(int i) const { return bar0 + 8 * (C::kStages + i); }
   __device__ __forceinline__ uint32_t acc_full(int i) const { return bar0 + 8 * (2 * C::kStages + i); }
-  __device__ __forceinline__ uint32_t acc_empty(int i) const { return bar0 + 8 * (2 * C::kStages + 2 + i); }
-  __device__ __forceinline__ uint32_t drain() const { return bar0 + 8 * (2 * C::kStages + 4); }
-  __device__ __forceinline__ uint32_t extra_full(int i) const { return bar0 + 8 * (2 * C::kStages + 5 + i); }
+  __device__ __forceinline__ uint32_t acc_empty(int i) const { return bar0 + 8 * (2 * C::kStages + C::kAccs + i); }
+  __device__ __forceinline__ uint32_t drain() const { return bar0 + 8 * (2 * C::kStages + 2 * C::kAccs); }
+  __device__ __forceinline__ uint32_t extra_full(int i) const { return bar0 + 8 * (2 * C::kStages + 2 * C::kAccs + 1 + i); }
 
   // By the whole CTA, before it reads anything that an earlier kernel wrote.  `raw`: the dynamic
   // shared memory, on 1024 bytes.
@@ -357,13 +369,13 @@ struct Engine {
     ph = warp == kEpiWarps;   // the loader starts on empty stages
     if (threadIdx.x == 0) {
       for (int i = 0; i < C::kStages; ++i) bar_init(full(i), 1), bar_init(empty(i), 1);
-      for (int i = 0; i < 2; ++i) bar_init(acc_full(i), 1), bar_init(acc_empty(i), kEpiWarps * CG);
+      for (int i = 0; i < C::kAccs; ++i) bar_init(acc_full(i), 1), bar_init(acc_empty(i), kEpiWarps * CG);
       bar_init(drain(), 1);
       for (int i = 0; i < C::kExtras; ++i) bar_init(extra_full(i), 1), sh->extra_readers[i] = 0;
       sh->abort = 0;
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == kEpiWarps + 1) tmem_alloc<CG>(smem_addr(&sh->tmem_slot), 2 * BN);
+    if (warp == kEpiWarps + 1) tmem_alloc<CG>(smem_addr(&sh->tmem_slot), C::kAccs * BN);
     fence_before();
     __syncthreads();
     if constexpr (CG == 2) cluster_sync();
@@ -457,8 +469,7 @@ struct Engine {
         __syncwarp();
         if (++s == C::kStages) s = 0, ph ^= 1;
       }
-      buf ^= 1;
-      if (buf == 0) aph ^= 1;
+      if (++buf == C::kAccs) buf = 0, aph ^= 1;
     }
   }
 
@@ -479,7 +490,7 @@ struct Engine {
         float v[32];
         tmem_load(lanes + buf * BN + i, v);
 #pragma unroll
-        for (int j = 0; j < 32; ++j) acc[i + j] = PL == 1 ? v[j] : acc[i + j] + v[j];   // one plane, one chunk
+        for (int j = 0; j < 32; ++j) acc[i + j] = PL == 1 ? v[j] : fmaf(v[j], kRestore, acc[i + j]);   // one plane, one chunk
       }
       fence_before();
       if ((threadIdx.x & 31) == 0) {
@@ -489,8 +500,7 @@ struct Engine {
           bar_arrive_remote(acc_empty(buf), lead);
       }
       __syncwarp();
-      buf ^= 1;
-      if (buf == 0) ph ^= 1;
+      if (++buf == C::kAccs) buf = 0, ph ^= 1;
     }
     es = (es + x.kt1 - x.kt0) % C::kStages;
   }
@@ -545,7 +555,7 @@ struct Engine {
     if constexpr (CG == 2) cluster_sync();
     if (warp == kEpiWarps + 1) {
       fence_after();
-      tmem_free<CG>(tmem, 2 * BN);
+      tmem_free<CG>(tmem, C::kAccs * BN);
     }
   }
 };
@@ -561,7 +571,7 @@ __global__ void __launch_bounds__(32 * (EW + 2), 1) product_kernel(const __grid_
   __shared__ Shared<PL, BN, CG, EW> sh;
   E e(raw, &sh, p.status);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int first = blockIdx.x / CG, stride = gridDim.x / CG, tiles = problem_tiles(p);
+  const int first = blockIdx.x / CG, stride = gridDim.x / CG, tiles = problem_tiles<BN, CG>(p);
   pdl_enter();
   if (warp == EW) {
     if (lane == 0)
@@ -614,7 +624,7 @@ nc_status launch_product(const Problem& p, const Epi& epi, cudaStream_t st, cons
   auto k = product_kernel<PL, BN, CG, EW, Epi>;
   constexpr int smem = Config<PL, BN, CG, EW>::kSmem;
   NC_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  const int tiles = problem_tiles(p), most = sm_count() / CG;
+  const int tiles = problem_tiles<BN, CG>(p), most = sm_count() / CG;
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
