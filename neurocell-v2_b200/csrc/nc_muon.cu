@@ -38,11 +38,12 @@ __device__ __forceinline__ double block_sum_f64(double v, double* red) {
 // The CTAs of a cluster hold slices of the long side in shared memory for all steps, as
 // X[l][i] (i along the short side, padded to S).  A step: every CTA adds up its slice's part
 // of A = X X^T, the cluster sums the parts (each CTA its share of A, read from and written to
-// the others' shared memory), and every CTA updates its slice, Y = A X, X <- a X + b Y + c A Y,
-// which needs no other slice and no A^2.  The momentum, the norm and the final update are in
-// the same launch, so the cost is the two cluster barriers of a step and the FMAs, 3 S^2 per
-// column of a slice.
-constexpr int kSmallThreads = 256;
+// the others' shared memory), and every CTA updates its slice, which needs no other slice:
+//   narrow slices (up to S):  Y = A X,  X <- a X + b Y + c A Y       2 S^2 FMAs a column
+//   wide ones:  Q = b A + c A^2 in every CTA (S^3),  X <- a X + Q X  S^2 a column
+// The momentum, the norm and the final update are in the same launch, so the cost is the two
+// cluster barriers of a step and the FMAs.
+constexpr int kSmallThreads = 512;
 constexpr size_t kSmallSmem = 200 * 1024;
 
 struct SmallArgs {
@@ -60,46 +61,77 @@ struct SmallArgs {
 };
 
 template <int S>
+struct Small {
+  static constexpr int kPitch = S + 4, kPer = S / 4, kCell = kPer * kPer;   // threads of one S x S product
+  static constexpr int kGroups = kSmallThreads / kCell;                     // that split the slice's columns
+  static constexpr int kParts = kGroups * S * S > S * kPitch ? kGroups * S * S : S * kPitch;   // Q fits too
+  static_assert(kCell <= kSmallThreads, "a thread takes 4 x 4 of A");
+};
+
+template <int S>
 __host__ __device__ constexpr size_t small_smem(int slice) {
-  return (size_t)(2 * slice * (S + 4) + 4096 + S * (S + 4)) * 4;
+  return (size_t)(2 * slice * Small<S>::kPitch + Small<S>::kParts + S * Small<S>::kPitch) * 4;
 }
 
-// out[l][i..i+3] for 4 columns l: sum over k of A[k][i] in[l][k].
-template <int S>
-__device__ __forceinline__ void small_product(const float* A, const float* in, int i, float (&acc)[4][4]) {
+// N columns l of sum over k of A[k][i..i+3] in[l][k].
+template <int S, int N>
+__device__ __forceinline__ void small_product(const float* A, const float* in, int i, float (&acc)[N][4]) {
+  constexpr int kPitch = Small<S>::kPitch;
 #pragma unroll
-  for (int q = 0; q < 4; ++q)
+  for (int q = 0; q < N; ++q)
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[q][e] = 0.f;
 #pragma unroll 4
   for (int k = 0; k < S; k += 4) {
-    float m[4][4], v[4][4];
+    float m[4][4], v[N][4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) *reinterpret_cast<float4*>(m[e]) = *reinterpret_cast<const float4*>(A + (k + e) * (S + 4) + i);
+    for (int e = 0; e < 4; ++e) *reinterpret_cast<float4*>(m[e]) = *reinterpret_cast<const float4*>(A + (k + e) * kPitch + i);
 #pragma unroll
-    for (int q = 0; q < 4; ++q) *reinterpret_cast<float4*>(v[q]) = *reinterpret_cast<const float4*>(in + q * (S + 4) + k);
+    for (int q = 0; q < N; ++q) *reinterpret_cast<float4*>(v[q]) = *reinterpret_cast<const float4*>(in + q * kPitch + k);
 #pragma unroll
     for (int e = 0; e < 4; ++e)
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
+      for (int q = 0; q < N; ++q)
 #pragma unroll
         for (int r = 0; r < 4; ++r) acc[q][r] = fmaf(m[e][r], v[q][e], acc[q][r]);
+  }
+}
+
+// put(l, i, sums) for all columns l of `count` and rows i..i+3 of A in: by threads of 4 columns
+// each, or where those would be few, of one.
+template <int S, typename Put>
+__device__ __forceinline__ void small_products(const float* A, const float* in, int count, Put put) {
+  constexpr int kPer = Small<S>::kPer, kPitch = Small<S>::kPitch;
+  if (count * kPer <= 2 * kSmallThreads) {
+    for (int t = threadIdx.x; t < count * kPer; t += kSmallThreads) {
+      const int i = t % kPer * 4, l = t / kPer;
+      float acc[1][4];
+      small_product<S, 1>(A, in + l * kPitch, i, acc);
+      put(l, i, acc[0]);
+    }
+  } else {
+    for (int t = threadIdx.x; t < count / 4 * kPer; t += kSmallThreads) {
+      const int i = t % kPer * 4, l = t / kPer * 4;
+      float acc[4][4];
+      small_product<S, 4>(A, in + l * kPitch, i, acc);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) put(l + q, i, acc[q]);
+    }
   }
 }
 
 template <int S, typename T>
 __global__ void __launch_bounds__(kSmallThreads) ns_small_kernel(SmallArgs p) {
   namespace cg = cooperative_groups;
-  constexpr int kPitch = S + 4, kPer = S / 4, kCell = kPer * kPer;   // threads of one S x S product
-  constexpr int kGroups = kSmallThreads / kCell;                     // that split the slice's columns
+  constexpr int kPitch = Small<S>::kPitch, kPer = Small<S>::kPer, kCell = Small<S>::kCell, kGroups = Small<S>::kGroups;
   extern __shared__ __align__(16) float sm[];
   __shared__ double red[kSmallThreads / 32], total;
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = cluster.num_blocks(), rank = cluster.block_rank(), tid = threadIdx.x;
   float* X = sm;
   float* Y = X + p.slice * kPitch;
-  float* part = Y + p.slice * kPitch;   // (kGroups, S, S)
-  float* A = part + 4096;               // (S, pitch)
+  float* part = Y + p.slice * kPitch;       // (kGroups, S, S)
+  float* A = part + Small<S>::kParts;       // (S, pitch)
   const bool tall = p.rows > p.cols;
   const int s = tall ? p.cols : p.rows, len = tall ? p.rows : p.cols;
   const int l0 = rank * p.slice;
@@ -179,24 +211,38 @@ __global__ void __launch_bounds__(kSmallThreads) ns_small_kernel(SmallArgs p) {
       for (int r = 0; r < ranks; ++r) cluster.map_shared_rank(A, r)[o] = v;
     }
     cluster.sync();
-    for (int t = tid; t < p.slice / 4 * kPer; t += kSmallThreads) {
-      const int i = t % kPer * 4, l = t / kPer * 4;
-      small_product<S>(A, X + l * kPitch, i, acc);
+    auto put4 = [](float* at, float x, float y, float z, float w) {
+      *reinterpret_cast<float4*>(at) = make_float4(x, y, z, w);
+    };
+    if (p.slice <= S) {
+      small_products<S>(A, X, p.slice, [&](int l, int i, float (&v)[4]) { put4(Y + l * kPitch + i, v[0], v[1], v[2], v[3]); });
+      __syncthreads();
+      small_products<S>(A, Y, p.slice, [&](int l, int i, float (&v)[4]) {
+        float* x = X + l * kPitch + i;
+        const float* y = Y + l * kPitch + i;
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        *reinterpret_cast<float4*>(Y + (l + q) * kPitch + i) = make_float4(acc[q][0], acc[q][1], acc[q][2], acc[q][3]);
-    }
-    __syncthreads();
-    for (int t = tid; t < p.slice / 4 * kPer; t += kSmallThreads) {
-      const int i = t % kPer * 4, l = t / kPer * 4;
-      small_product<S>(A, Y + l * kPitch, i, acc);
+        for (int e = 0; e < 4; ++e) v[e] = fmaf(p.a, x[e], fmaf(p.b, y[e], p.c * v[e]));
+        put4(x, v[0], v[1], v[2], v[3]);
+      });
+    } else {
+      // A is symmetric, so its rows serve as columns; the parts' place takes Q (its readers have
+      // passed the cluster's barrier)
+      float* Q = part;
+      small_products<S>(A, A, S, [&](int l, int i, float (&v)[4]) {
+        const float* x = A + l * kPitch + i;
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
+        for (int e = 0; e < 4; ++e) v[e] = fmaf(p.b, x[e], p.c * v[e]);
+        put4(Q + l * kPitch + i, v[0], v[1], v[2], v[3]);
+      });
+      __syncthreads();
+      small_products<S>(Q, X, p.slice, [&](int l, int i, float (&v)[4]) {
+        const float* x = X + l * kPitch + i;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int o = (l + q) * kPitch + i + e;
-          X[o] = fmaf(p.a, X[o], fmaf(p.b, Y[o], p.c * acc[q][e]));
-        }
+        for (int e = 0; e < 4; ++e) v[e] = fmaf(p.a, x[e], v[e]);
+        put4(Y + l * kPitch + i, v[0], v[1], v[2], v[3]);
+      });
+      float* t = X;
+      X = Y, Y = t;
     }
     __syncthreads();
   }
@@ -224,7 +270,7 @@ SmallPlan small_plan(const nc_newton_schulz* d) {
   const int s = d->rows < d->cols ? d->rows : d->cols, len = d->rows < d->cols ? d->cols : d->rows;
   SmallPlan r{};
   r.pad = s <= 16 ? 16 : s <= 32 ? 32 : 64;
-  r.ranks = len > 28 ? 8 : len > 12 ? 4 : len > 4 ? 2 : 1;
+  r.ranks = len > 1024 ? 16 : len > 28 ? 8 : len > 12 ? 4 : len > 4 ? 2 : 1;
   r.slice = ((len + r.ranks - 1) / r.ranks + 3) / 4 * 4;
   const size_t need = r.pad == 16 ? small_smem<16>(r.slice) : r.pad == 32 ? small_smem<32>(r.slice) : small_smem<64>(r.slice);
   r.fits = s <= 64 && need <= kSmallSmem;
@@ -236,6 +282,7 @@ nc_status launch_small(const SmallArgs& a, const SmallPlan& r, int batch, cudaSt
   auto k = ns_small_kernel<S, T>;
   const size_t smem = small_smem<S>(r.slice);
   NC_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  if (r.ranks > 8) NC_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
