@@ -264,14 +264,14 @@ typedef enum nc_reduction { NC_REDUCE_MEAN = 0, NC_REDUCE_SUM = 1, NC_REDUCE_NON
  * (rows, classes) logits in memory: z = features weight^T + bias, and for every row
  * loss = log sum exp z - z[label].
  *   features (rows, dim), weight (classes, dim), bias (classes) or null: row-major, `dtype`;
- *   with more than 32 rows and a dim of whole 8s a bfloat16 weight starts on 16 bytes
+ *   a bfloat16 weight with a dim of whole 8s starts on 16 bytes
  *   labels (rows) int32.  A row whose label is ignore_index (which must lie outside
  *   [0, classes)) takes no part: its loss and feature gradient are 0 and its features are
  *   not used, whatever they hold.  Any other label outside [0, classes) makes the loss and
  *   the gradients NaN; nothing is read out of range.
  * A bias of -inf takes its class out; a row with every class taken out has a NaN loss, as
  * has one with a logit of NaN or +inf.  Sums and statistics are held in float32.
- * Precision with float32 operands and more than 32 rows: as of float32 products, where the
+ * Precision with float32 operands and more than 16 rows: as of float32 products, where the
  * entries of a tensor below 2^-18 of its largest finite one count with an absolute error of
  * 2^-38 of that one, and dz = p - onehot with one of at most 2^-40 of the largest |g_loss|.
  */

@@ -7,11 +7,17 @@
 // The value keeps one running (maximum, sum) per row and block of classes; the gradient
 // computes the logits of a block of classes again and multiplies them out while they are
 // on chip.
+//
+// Few rows (here): a CTA streams its share of the weight through shared memory once, in chunks
+// that bulk copies bring while it works on the one before, and everything a chunk is needed
+// for happens there.  Bound by reading the weight (and writing its gradient).  More rows:
+// nc_readout_tc.cu.
 #include <math.h>
 
 #include "nc_common.cuh"
 #include "nc_errors.h"
 #include "nc_readout.h"
+#include "nc_tc.cuh"
 
 namespace nc {
 
@@ -19,8 +25,11 @@ namespace {
 
 constexpr int kRowThreads = 256;
 constexpr int kRowWarps = kRowThreads / 32;
-constexpr int kRowDimChunk = 1024;   // features staged in shared memory at a time
-constexpr int kRowTile = 4;          // classes a warp takes together
+constexpr int kRowDim = 4 * kRowThreads;       // most columns: four a thread
+constexpr int kRowBuffers = 2;
+constexpr size_t kRowChunkBytes = 64 * 1024;   // two in flight cover the memory's latency
+constexpr int kRowsMost = 16, kRowsMostBf16 = 16;
+constexpr int kRowStats = 512;                 // logits a row collects before its statistics take them in
 
 template <int VEC, typename T>
 __device__ __forceinline__ void load_vec(const T* p, float (&v)[VEC]) {
@@ -36,268 +45,361 @@ __device__ __forceinline__ void load_vec(const T* p, float (&v)[VEC]) {
   }
 }
 
-template <int VEC, typename T>
-__device__ __forceinline__ void store_vec(T* p, const float (&v)[VEC]) {
-  if constexpr (VEC == 1) {
-    store_as(p, v[0]);
-  } else if constexpr (sizeof(T) == 4) {
-    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+template <typename T>
+__device__ __forceinline__ void store4(T* p, const float (&v)[4]) {
+  if constexpr (sizeof(T) == 4) {
+    __stcs(reinterpret_cast<float4*>(p), make_float4(v[0], v[1], v[2], v[3]));
   } else {
-    __nv_bfloat162 lo = __floats2bfloat162_rn(v[0], v[1]), hi = __floats2bfloat162_rn(v[2], v[3]);
-    uint2 q;
-    q.x = *reinterpret_cast<uint32_t*>(&lo);
-    q.y = *reinterpret_cast<uint32_t*>(&hi);
-    *reinterpret_cast<uint2*>(p) = q;
+    const __nv_bfloat162 lo = __floats2bfloat162_rn(v[0], v[1]), hi = __floats2bfloat162_rn(v[2], v[3]);
+    __stcs(reinterpret_cast<uint2*>(p),
+           make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi)));
   }
 }
 
-// Logits of the row group [row0, row0 + RN) and the classes [v0, v0 + vb) into
-// z[r * vb + v] (no bias); vb is a multiple of kRowWarps * kRowTile.  A warp takes kRowTile classes at a time, its lanes split the
-// dimension; the group's features are in shared memory, where one 16-byte read serves
-// kRowTile * 4 products.  Rows that are ignored or past the end read as zeros; classes past the end
-// repeat the last one and are dropped by the caller.
-template <typename T, int RN, int VEC>
-__device__ void group_logits(const CeArgs& a, int row0, int v0, int vb, float* hs, float* z) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const T* f = static_cast<const T*>(a.features);
-  const T* w = static_cast<const T*>(a.weight);
-  const int chunks = (a.dim + kRowDimChunk - 1) / kRowDimChunk;
-  const int pitch = min(a.dim, kRowDimChunk);
-  for (int vp = 0; vp < vb; vp += kRowWarps * kRowTile) {
-    float acc[kRowTile * RN];
-#pragma unroll
-    for (int i = 0; i < kRowTile * RN; ++i) acc[i] = 0.f;
-    const int vw = vp + warp * kRowTile;
-    for (int c = 0; c < chunks; ++c) {
-      const int d0 = c * kRowDimChunk, len = min(kRowDimChunk, a.dim - d0);
-      if (chunks > 1 || vp == 0) {
-        __syncthreads();
-        for (int i = tid * VEC; i < RN * len; i += kRowThreads * VEC) {
-          const int r = i / len, d = i - r * len, row = row0 + r;
-          float v[VEC];
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) v[e] = 0.f;
-          if (row < a.rows && ce_kept(a, row)) load_vec<VEC>(f + (size_t)row * a.dim + d0 + d, v);
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) hs[r * pitch + d + e] = v[e];
-        }
-        __syncthreads();
+// What the streaming kernels share.  chunk: classes per chunk; chunks: of all classes.
+struct RowArgs {
+  CeArgs a;
+  int chunk, chunks;
+  int bulk;           // the weight starts on 16 bytes
+  int32_t* status;
+};
+
+// The stream of this CTA's chunks [c0, c1) of the weight.
+template <typename T>
+struct RowStream {
+  const RowArgs& r;
+  uint8_t* ring;
+  uint32_t bars;
+  int* abort;
+  int c0, c1;
+  bool ok = true;
+
+  __device__ __forceinline__ RowStream(const RowArgs& args, uint8_t* buffers, uint64_t* barriers, int* flag)
+      : r(args), ring(buffers), bars(tc::smem_addr(barriers)), abort(flag) {
+    c0 = (int)((int64_t)r.chunks * blockIdx.x / gridDim.x), c1 = (int)((int64_t)r.chunks * (blockIdx.x + 1) / gridDim.x);
+    if (threadIdx.x == 0) {
+      for (int i = 0; i < kRowBuffers; ++i) tc::bar_init(bars + 8 * i, 1);
+      *abort = 0;
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+  }
+  __device__ __forceinline__ int classes(int c) const { return min(r.chunk, r.a.classes - c * r.chunk); }
+  __device__ __forceinline__ const T* at(int c) const {
+    return static_cast<const T*>(r.a.weight) + (size_t)c * r.chunk * r.a.dim;
+  }
+  __device__ __forceinline__ T* buffer(int c) const {
+    return reinterpret_cast<T*>(ring + (size_t)((c - c0) % kRowBuffers) * r.chunk * r.a.dim * sizeof(T));
+  }
+  __device__ __forceinline__ uint32_t bytes(int c) const { return (uint32_t)(classes(c) * r.a.dim * sizeof(T)); }
+  // Thread 0 asks for chunk c; its buffer is free.
+  __device__ __forceinline__ void ask(int c) const {
+    if (!r.bulk || c >= c1 || threadIdx.x != 0) return;
+    const uint32_t bar = bars + 8 * ((c - c0) % kRowBuffers), n = bytes(c) & ~15u;
+    tc::bar_expect(bar, n);
+    if (n > 0)
+      asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                       tc::smem_addr(buffer(c))),
+                   "l"(at(c)), "r"(n), "r"(bar)
+                   : "memory");
+  }
+  // The whole CTA: chunk c is in its buffer.  Chunks start on 16 bytes; what a last one has
+  // behind whole 16s, and chunks of a weight that does not start so, are loaded here.
+  __device__ __forceinline__ bool wait(int c) {
+    const int i = c - c0;
+    if (r.bulk) ok = tc::bar_wait(bars + 8 * (i % kRowBuffers), i / kRowBuffers & 1, abort, r.status);
+    const int n = classes(c) * r.a.dim, from = r.bulk ? (int)((bytes(c) & ~15u) / sizeof(T)) : 0;
+    T* to = buffer(c);
+    for (int e = from + threadIdx.x; e < n; e += kRowThreads) to[e] = at(c)[e];
+    ok = __syncthreads_and(ok);
+    return ok;
+  }
+  // After an abort: the copies in flight land before the CTA ends.
+  __device__ __forceinline__ void drain(int c) const {
+    if (ok || !r.bulk || threadIdx.x != 0) return;
+    for (int k = c; k < min(c + kRowBuffers, c1); ++k)
+      for (int j = 0; j < tc::kWaitLimit && !tc::bar_try(bars + 8 * ((k - c0) % kRowBuffers), (k - c0) / kRowBuffers & 1); ++j) {
       }
-      const T* wr[kRowTile];
+  }
+};
+
+// The features in shared memory, zeros for rows that take no part or do not exist.
+template <typename T, int RN>
+__device__ __forceinline__ void stage_features(const CeArgs& a, float* hs) {
+  const T* f = static_cast<const T*>(a.features);
+  for (int i = threadIdx.x; i < RN * a.dim; i += kRowThreads) {
+    const int row = i / a.dim;
+    hs[i] = row < a.rows && ce_kept(a, row) ? to_f32(f[i]) : 0.f;
+  }
+}
+
+// Logits (no bias) of the chunk's classes: put(v, r, z).  A warp takes VT classes at a time, its
+// lanes split the columns; a 16-byte read of the features serves 4 VT products.  Classes past
+// `n` read what the buffer holds and are not put.
+template <typename T, int RN, int VEC, int VT, typename Put>
+__device__ __forceinline__ void chunk_logits(const T* w, const float* hs, int dim, int n, Put put) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int v0 = warp * VT; v0 < n; v0 += kRowWarps * VT) {
+    float acc[VT * RN];
 #pragma unroll
-      for (int j = 0; j < kRowTile; ++j)
-        wr[j] = w + (size_t)min(v0 + vw + j, a.classes - 1) * a.dim + d0;
+    for (int i = 0; i < VT * RN; ++i) acc[i] = 0.f;
 #pragma unroll 2
-      for (int d = lane * VEC; d < len; d += 32 * VEC) {
-        float x[kRowTile][VEC];
+    for (int d = lane * VEC; d < dim; d += 32 * VEC) {
+      float x[VT][VEC];
 #pragma unroll
-        for (int j = 0; j < kRowTile; ++j) load_vec<VEC>(wr[j] + d, x[j]);
+      for (int j = 0; j < VT; ++j) load_vec<VEC>(w + min(v0 + j, n - 1) * dim + d, x[j]);
 #pragma unroll
-        for (int r = 0; r < RN; ++r) {
-          float h[VEC];
-          load_vec<VEC>(hs + r * pitch + d, h);
+      for (int r = 0; r < RN; ++r) {
+        float h[VEC];
+        load_vec<VEC>(hs + r * dim + d, h);
 #pragma unroll
-          for (int j = 0; j < kRowTile; ++j)
+        for (int j = 0; j < VT; ++j)
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) acc[j * RN + r] = fmaf(x[j][e], h[e], acc[j * RN + r]);
-        }
+          for (int e = 0; e < VEC; ++e) acc[j * RN + r] = fmaf(x[j][e], h[e], acc[j * RN + r]);
       }
     }
     int first;
     warp_sums(acc, lane, &first);
 #pragma unroll
-    for (int i = 0; i < (kRowTile * RN + 31) / 32; ++i) {
-      const int k = first + i;
-      z[(k % RN) * vb + vw + k / RN] = acc[i];
+    for (int i = 0; i < (VT * RN + 31) / 32; ++i) {
+      const int k = first + i, v = v0 + k / RN;
+      if (v < n) put(v, k % RN, acc[i]);
     }
   }
-  __syncthreads();
 }
 
-// grid (class blocks, row groups): the block's (maximum, sum) of each row, and the label's
-// logit where the block holds it.
-template <typename T, int RN, int VEC>
-__global__ void __launch_bounds__(kRowThreads) ce_rows_value_kernel(CeArgs a, int vb, int blocks,
-                                                                    float2* __restrict__ part,
+// Each CTA's (maximum, sum) of every row, and the label's logit where it has it.
+template <typename T, int RN, int VEC, int VT>
+__global__ void __launch_bounds__(kRowThreads) ce_rows_value_kernel(const RowArgs args, float2* __restrict__ part,
                                                                     float* __restrict__ zlabel) {
-  extern __shared__ __align__(16) float sm[];
-  float* hs = sm;
-  float* z = sm + RN * min(a.dim, kRowDimChunk);
-  const int v0 = blockIdx.x * vb, row0 = blockIdx.y * RN;
-  pdl_enter();
-  group_logits<T, RN, VEC>(a, row0, v0, vb, hs, z);
+  extern __shared__ __align__(128) uint8_t raw[];
+  __shared__ __align__(8) uint64_t bars[kRowBuffers];
+  __shared__ int flag;
+  const CeArgs& a = args.a;
+  float* hs = reinterpret_cast<float*>(raw + kRowBuffers * (size_t)args.chunk * a.dim * sizeof(T));
+  float* z = hs + RN * a.dim;   // (RN, kRowStats)
+  RowStream<T> s(args, raw, bars, &flag);
   const T* bias = static_cast<const T*>(a.bias);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int n = min(vb, a.classes - v0);
-  for (int r = warp; r < RN && row0 + r < a.rows; r += kRowWarps) {
-    const int row = row0 + r, label = a.labels[row];
-    float m = -INFINITY;
-    for (int v = lane; v < n; v += 32) {
-      const float x = z[r * vb + v] + (bias ? to_f32(bias[v0 + v]) : 0.f);
-      z[r * vb + v] = x;
-      m = fmaxf(m, x);
-      if (v0 + v == label) zlabel[row] = x;
-    }
+  constexpr int kMine = (RN + kRowWarps - 1) / kRowWarps;   // rows whose statistics a warp keeps
+  float2 mine[kMine];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    float s = 0.f;
-    for (int v = lane; v < n; v += 32) {
-      const float x = z[r * vb + v];
-      s += x == -INFINITY ? 0.f : expf(x - m);
-    }
-    s = warp_sum(s);
-    if (lane == 0) part[(size_t)row * blocks + blockIdx.x] = make_float2(m, s);
-  }
-}
-
-// One warp per row: the blocks' pairs merged in a fixed order, the row's loss.
-__global__ void ce_finish_rows_kernel(CeArgs a, int blocks, const float2* __restrict__ part,
-                                      const float* __restrict__ zlabel, float* __restrict__ lse,
-                                      float* __restrict__ row_loss) {
+  for (int k = 0; k < kMine; ++k) mine[k] = make_float2(-INFINITY, 0.f);
   pdl_enter();
-  const int row = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (row >= a.rows) return;
-  float2 x = make_float2(-INFINITY, 0.f);
-  for (int i = lane; i < blocks; i += 32) x = lse_merge(x, part[(size_t)row * blocks + i]);
+  for (int c = s.c0; c < s.c0 + kRowBuffers; ++c) s.ask(c);
+  stage_features<T, RN>(a, hs);
+  int held = 0, base = s.c0 * args.chunk;   // classes base .. base + held - 1 are in z
+  int c = s.c0;
+  for (; c < s.c1; ++c) {
+    if (!s.wait(c)) break;
+    const int n = s.classes(c);
+    chunk_logits<T, RN, VEC, VT>(s.buffer(c), hs, a.dim, n,
+                                 [&](int v, int r, float x) { z[r * kRowStats + held + v] = x; });
+    __syncthreads();
+    s.ask(c + kRowBuffers);
+    held += n;
+    if (held + args.chunk <= kRowStats && c + 1 < s.c1) continue;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float2 y = make_float2(__shfl_xor_sync(0xffffffffu, x.x, o), __shfl_xor_sync(0xffffffffu, x.y, o));
-    x = lse_merge(x, y);
-  }
-  if (lane != 0) return;
-  finish_row(a, row, x, zlabel, lse, row_loss);
-}
-
-// One block: the sum or mean of the row losses, in a fixed order.
-__global__ void __launch_bounds__(1024) ce_sum_kernel(CeArgs a, const float* __restrict__ row_loss,
-                                                      float* __restrict__ loss) {
-  pdl_enter();
-  __shared__ double red[32];
-  const int n = count_kept(a);
-  double s = 0.0;
-  for (int i = threadIdx.x; i < a.rows; i += blockDim.x) s += row_loss[i];
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    double t = 0.0;
-    for (int i = 0; i < (int)(blockDim.x >> 5); ++i) t += red[i];
-    loss[0] = (float)(a.reduction == NC_REDUCE_MEAN ? t / (double)max(n, 1) : t);
-  }
-}
-
-// Gradients of one block of classes over all rows.  The logits of each row group are
-// computed again and left as p = g_n (exp(z - lse) - onehot) in shared memory; then the
-// threads own columns d: dw[v] = sum_n p f[n] (8 classes in registers) and the block's part
-// of df[n] = sum_v p w[v] (a row group in registers), written to its own slot.
-template <typename T, int RN, int VEC>
-__global__ void __launch_bounds__(kRowThreads) ce_rows_grad_kernel(
-    CeArgs a, int vb, int slots_per_block, int td, const float* __restrict__ lse,
-    const float* __restrict__ g_loss, T* __restrict__ g_weight, T* __restrict__ g_bias,
-    float* __restrict__ df_part) {
-  extern __shared__ __align__(16) float sm[];
-  const int rows_pad = (a.rows + RN - 1) / RN * RN;
-  float* p = sm;                          // (rows_pad, vb)
-  float* hs = sm + rows_pad * vb;
-  const int v0 = blockIdx.x * vb, tid = threadIdx.x;
-  const T* bias = static_cast<const T*>(a.bias);
-  pdl_enter();
-  float scale = 1.f;
-  if (a.reduction == NC_REDUCE_MEAN) scale = 1.f / (float)max(count_kept(a), 1);
-  for (int row0 = 0; row0 < a.rows; row0 += RN) {
-    float* z = p + row0 * vb;
-    group_logits<T, RN, VEC>(a, row0, v0, vb, hs, z);
-    for (int i = tid; i < RN * vb; i += kRowThreads) {
-      const int r = i / vb, v = v0 + i - r * vb, row = row0 + r;
-      float x = 0.f;
-      if (row < a.rows && v < a.classes && ce_kept(a, row)) {
-        const float g = g_loss ? g_loss[a.reduction == NC_REDUCE_NONE ? row : 0] * scale : scale;
-        x = z[i] + (bias ? to_f32(bias[v]) : 0.f);
-        x = g * (expf(x - lse[row]) - (v == a.labels[row] ? 1.f : 0.f));
+    for (int k = 0; k < kMine; ++k) {
+      const int r = warp + k * kRowWarps;
+      if (r >= a.rows || r >= RN) continue;
+      const int label = a.labels[r];
+      float m = -INFINITY;
+      for (int v = lane; v < held; v += 32) {
+        const float x = z[r * kRowStats + v] + (bias ? to_f32(bias[base + v]) : 0.f);
+        z[r * kRowStats + v] = x;
+        m = fmaxf(m, x);
+        if (base + v == label) zlabel[r] = x;
       }
-      z[i] = x;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      float t = 0.f;
+      for (int v = lane; v < held; v += 32) {
+        const float x = z[r * kRowStats + v];
+        t += x == -INFINITY ? 0.f : expf(x - m);
+      }
+      mine[k] = lse_merge(mine[k], make_float2(m, warp_sum(t)));
     }
+    base += held, held = 0;
     __syncthreads();
   }
-  if (g_bias) {
-    for (int v = tid; v < vb && v0 + v < a.classes; v += kRowThreads) {
-      float s = 0.f;
-      for (int n = 0; n < a.rows; ++n) s += p[n * vb + v];
-      store_as(g_bias + v0 + v, s);
-    }
-  }
-  const T* f = static_cast<const T*>(a.features);
-  const T* w = static_cast<const T*>(a.weight);
-  const int nd = (a.dim + VEC - 1) / VEC, dt = tid & (td - 1), vg = tid / td, groups = kRowThreads / td;
-  if (g_weight) {
-    for (int dv = dt; dv < nd; dv += td) {
-      for (int v8 = vg * 8; v8 < vb && v0 + v8 < a.classes; v8 += groups * 8) {
-        float acc[8][VEC];
+  s.drain(c);
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) acc[j][e] = 0.f;
-        for (int n = 0; n < a.rows; ++n) {
-          if (!ce_kept(a, n)) continue;   // its features may hold anything
-          float h[VEC], q[8];
-          load_vec<VEC>(f + (size_t)n * a.dim + dv * VEC, h);
-          *reinterpret_cast<float4*>(q) = *reinterpret_cast<const float4*>(p + n * vb + v8);
-          *reinterpret_cast<float4*>(q + 4) = *reinterpret_cast<const float4*>(p + n * vb + v8 + 4);
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) acc[j][e] = fmaf(q[j], h[e], acc[j][e]);
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (v0 + v8 + j < a.classes) store_vec<VEC>(g_weight + (size_t)(v0 + v8 + j) * a.dim + dv * VEC, acc[j]);
-      }
-    }
-  }
-  if (!df_part || vg >= slots_per_block) return;
-  float* out = df_part + ((size_t)blockIdx.x * slots_per_block + vg) * a.rows * a.dim;
-  for (int row0 = 0; row0 < a.rows; row0 += RN) {
-    for (int dv = dt; dv < nd; dv += td) {
-      float acc[RN][VEC];
-#pragma unroll
-      for (int r = 0; r < RN; ++r)
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) acc[r][e] = 0.f;
-      for (int v4 = vg * 4; v4 < vb; v4 += slots_per_block * 4) {
-        float x[4][VEC];
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          load_vec<VEC>(w + (size_t)min(v0 + v4 + j, a.classes - 1) * a.dim + dv * VEC, x[j]);
-#pragma unroll
-        for (int r = 0; r < RN; ++r) {
-          const float4 q = *reinterpret_cast<const float4*>(p + (row0 + r) * vb + v4);
-#pragma unroll
-          for (int e = 0; e < VEC; ++e)
-            acc[r][e] += q.x * x[0][e] + q.y * x[1][e] + q.z * x[2][e] + q.w * x[3][e];
-        }
-      }
-#pragma unroll
-      for (int r = 0; r < RN; ++r)
-        if (row0 + r < a.rows) store_vec<VEC>(out + (size_t)(row0 + r) * a.dim + dv * VEC, acc[r]);
-    }
+  for (int k = 0; k < kMine; ++k) {
+    const int r = warp + k * kRowWarps;
+    if (lane == 0 && r < RN && r < a.rows) part[(size_t)r * gridDim.x + blockIdx.x] = mine[k];
   }
 }
 
-// df: the slots' parts summed in order.
-template <typename T>
-__global__ void ce_sum_parts_kernel(const float* __restrict__ part, int64_t n, int slots, T* __restrict__ out) {
+// One block, a warp a row: the CTAs' pairs merged in a fixed order, the rows' losses, and their
+// sum or mean into `loss` unless that is null.
+__global__ void __launch_bounds__(512) ce_rows_finish_kernel(CeArgs a, int blocks, const float2* __restrict__ part,
+                                                             const float* __restrict__ zlabel, float* __restrict__ lse,
+                                                             float* row_loss, float* __restrict__ loss) {
   pdl_enter();
-  const int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x;
-  if (i >= n) return;
+  const int row = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (row < a.rows) {
+    float2 x = make_float2(-INFINITY, 0.f);
+    for (int i = lane; i < blocks; i += 32) x = lse_merge(x, part[(size_t)row * blocks + i]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const float2 y = make_float2(__shfl_xor_sync(0xffffffffu, x.x, o), __shfl_xor_sync(0xffffffffu, x.y, o));
+      x = lse_merge(x, y);
+    }
+    if (lane == 0) finish_row(a, row, x, zlabel, lse, row_loss);
+  }
+  __syncthreads();
+  if (!loss || threadIdx.x != 0) return;
+  double t = 0.0;
+  int kept = 0;
+  for (int i = 0; i < a.rows; ++i) t += row_loss[i], kept += ce_kept(a, i);
+  loss[0] = (float)(a.reduction == NC_REDUCE_MEAN ? t / (double)max(kept, 1) : t);
+}
+
+// Gradients.  Of each chunk the logits again, left as p = g_n (exp(z - lse) - onehot); then a thread
+// owns four columns, with the features' and df's in registers for all rows, and goes through
+// the classes: dw[v] = sum_n p f[n] is stored, df[n] += p w[v] stays.  Where the columns need
+// fewer threads (td of them), groups of td share the classes and meet at the end.
+template <typename T, int RN, int VEC, int VT>
+__global__ void __launch_bounds__(kRowThreads) ce_rows_grad_kernel(
+    const RowArgs args, int td, const float* __restrict__ lse, const float* __restrict__ g_loss, T* __restrict__ g_weight,
+    T* __restrict__ g_bias, float* __restrict__ df_part) {
+  extern __shared__ __align__(128) uint8_t raw[];
+  __shared__ __align__(8) uint64_t bars[kRowBuffers];
+  __shared__ int flag;
+  __shared__ float row_g[RN], row_lse[RN];
+  __shared__ int row_label[RN];
+  const CeArgs& a = args.a;
+  float* hs = reinterpret_cast<float*>(raw + kRowBuffers * (size_t)args.chunk * a.dim * sizeof(T));
+  float* p = hs + RN * a.dim;   // (chunk, RN)
+  RowStream<T> s(args, raw, bars, &flag);
+  const T* bias = static_cast<const T*>(a.bias);
+  const int tid = threadIdx.x;
+  pdl_enter();
+  for (int c = s.c0; c < s.c0 + kRowBuffers; ++c) s.ask(c);
+  if (tid < RN) {
+    int kept = 0;
+    for (int i = 0; i < a.rows; ++i) kept += ce_kept(a, i);
+    const bool in = tid < a.rows && ce_kept(a, tid);
+    const float g = g_loss && in ? g_loss[a.reduction == NC_REDUCE_NONE ? tid : 0] : 1.f;
+    row_g[tid] = !in ? 0.f : a.reduction == NC_REDUCE_MEAN ? g / (float)max(kept, 1) : g;
+    row_lse[tid] = in ? lse[tid] : 0.f;
+    row_label[tid] = in ? a.labels[tid] : -1;
+  }
+  stage_features<T, RN>(a, hs);
+  __syncthreads();
+  const int dt = tid % td, group = tid / td, groups = kRowThreads / td;
+  int col[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) col[e] = VEC == 4 ? 4 * dt + e : dt + e * td;
+  float h[RN][4], acc[RN][4];
+#pragma unroll
+  for (int r = 0; r < RN; ++r)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) h[r][e] = col[e] < a.dim ? hs[r * a.dim + col[e]] : 0.f, acc[r][e] = 0.f;
+  int c = s.c0;
+  for (; c < s.c1; ++c) {
+    if (!s.wait(c)) break;
+    const int n = s.classes(c), v0 = c * args.chunk;
+    const T* w = s.buffer(c);
+    chunk_logits<T, RN, VEC, VT>(w, hs, a.dim, n, [&](int v, int r, float x) { p[v * RN + r] = x; });
+    __syncthreads();
+    for (int i = tid; i < n * RN; i += kRowThreads) {
+      const int v = i / RN, r = i % RN;
+      const float x = p[i] + (bias ? to_f32(bias[v0 + v]) : 0.f);
+      p[i] = row_g[r] == 0.f ? 0.f : row_g[r] * (expf(x - row_lse[r]) - (v0 + v == row_label[r] ? 1.f : 0.f));
+    }
+    __syncthreads();
+    if (g_bias) {
+      for (int v = tid; v < n; v += kRowThreads) {
+        float t = 0.f;
+#pragma unroll
+        for (int r = 0; r < RN; ++r) t += p[v * RN + r];
+        store_as(g_bias + v0 + v, t);
+      }
+    }
+    if (col[0] < a.dim) {
+#pragma unroll 2
+      for (int v = group; v < n; v += groups) {
+        float x[4], q[RN], out[4] = {0.f, 0.f, 0.f, 0.f};
+        if constexpr (VEC == 4) {
+          load_vec<4>(w + v * a.dim + col[0], x);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] = col[e] < a.dim ? to_f32(w[v * a.dim + col[e]]) : 0.f;
+        }
+#pragma unroll
+        for (int r = 0; r < RN; ++r) q[r] = p[v * RN + r];
+#pragma unroll
+        for (int r = 0; r < RN; ++r)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            out[e] = fmaf(q[r], h[r][e], out[e]);
+            acc[r][e] = fmaf(q[r], x[e], acc[r][e]);
+          }
+        if (g_weight) {
+          T* o = g_weight + (size_t)(v0 + v) * a.dim;
+          if constexpr (VEC == 4) {
+            store4(o + col[0], out);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (col[e] < a.dim) store_as(o + col[e], out[e]);
+          }
+        }
+      }
+    }
+    __syncthreads();
+    s.ask(c + kRowBuffers);
+  }
+  s.drain(c);
+  if (!df_part) return;
+  // the groups' sums, in order; the ring's place is free
+  float* sum = reinterpret_cast<float*>(raw);   // (groups, RN, 4 td)
+  if (groups > 1) {
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < RN; ++r)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum[(group * RN + r) * 4 * td + e * td + dt] = acc[r][e];
+    __syncthreads();
+    for (int i = tid; i < RN * 4 * td; i += kRowThreads) {
+      const int r = i / (4 * td), k = i % (4 * td), d = VEC == 4 ? k % td * 4 + k / td : k % td + k / td * td;
+      float t = 0.f;
+      for (int g = 0; g < groups; ++g) t += sum[g * RN * 4 * td + i];
+      if (r < a.rows && d < a.dim) df_part[((size_t)blockIdx.x * a.rows + r) * a.dim + d] = t;
+    }
+  } else {
+#pragma unroll
+    for (int r = 0; r < RN; ++r)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (r < a.rows && col[e] < a.dim) df_part[((size_t)blockIdx.x * a.rows + r) * a.dim + col[e]] = acc[r][e];
+  }
+}
+
+// df: the CTAs' parts, 8 threads an element, in a fixed order.
+template <typename T>
+__global__ void __launch_bounds__(256) ce_sum_parts_kernel(const float* __restrict__ part, int n, int slots,
+                                                           T* __restrict__ out) {
+  __shared__ float sm[8][32];
+  pdl_enter();
+  const int i = blockIdx.x * 32 + threadIdx.x % 32, g = threadIdx.x / 32;
   float s = 0.f;
+  if (i < n) {
 #pragma unroll 4
-  for (int k = 0; k < slots; ++k) s += part[(size_t)k * n + i];
+    for (int k = g; k < slots; k += 8) s += part[(size_t)k * n + i];
+  }
+  sm[g][threadIdx.x % 32] = s;
+  __syncthreads();
+  if (g != 0 || i >= n) return;
+#pragma unroll
+  for (int k = 1; k < 8; ++k) s += sm[k][threadIdx.x];
   store_as(out + i, s);
 }
 
 struct RowsPlan {
-  int rn, vec, vb, blocks, groups, td, slots;
+  int rn, vec, vt, chunk, chunks, blocks, td;
   size_t smem_value, smem_grad;
 };
 
@@ -307,34 +409,30 @@ int pow2_at_least(int x) {
   return p;
 }
 
-// `vec`: elements per load, 4 or 1.  A plan of 1 never has more slots than one of 4.
+// `vec`: columns per load, 4 or 1.
 RowsPlan rows_plan(const nc_linear_ce* d, int vec) {
   RowsPlan r;
   r.rn = d->rows <= 1 ? 1 : d->rows <= 4 ? 4 : d->rows <= 8 ? 8 : 16;
-  r.groups = (d->rows + r.rn - 1) / r.rn;
-  // two blocks of classes per SM, within the shared memory that the gradient's p takes
-  const int rows_pad = r.groups * r.rn;
-  const int even = ((d->classes + 295) / 296 + 31) / 32 * 32;
-  const int fit = (int)(96 * 1024 / (4 * (size_t)rows_pad)) / 32 * 32;
-  r.vb = even < 32 ? 32 : even;
-  if (r.vb > 256) r.vb = 256;
-  if (r.vb > fit) r.vb = fit < 32 ? 32 : fit;
-  r.blocks = (d->classes + r.vb - 1) / r.vb;
   r.vec = vec;
-  const int nd = d->dim / r.vec;
-  r.td = pow2_at_least(nd < kRowThreads ? nd : kRowThreads);
-  const int groups = kRowThreads / r.td, most = r.vb / 4;
-  r.slots = groups < most ? groups : most;
-  const size_t hs = (size_t)r.rn * (d->dim < kRowDimChunk ? d->dim : kRowDimChunk) * 4;
-  r.smem_value = hs + (size_t)r.rn * r.vb * 4;
-  r.smem_grad = hs + (size_t)rows_pad * r.vb * 4;
+  const size_t row = (size_t)d->dim * (d->dtype == NC_BF16 ? 2 : 4);
+  r.chunk = 64;   // 16 classes of up to 4 KB fit a buffer
+  while (r.chunk > 16 && (r.chunk * row > kRowChunkBytes || d->classes < r.chunk * 148)) r.chunk /= 2;
+  r.vt = r.chunk >= 32 ? 4 : 2;
+  r.chunks = (d->classes + r.chunk - 1) / r.chunk;
+  r.blocks = r.chunks < 148 ? r.chunks : 148;
+  r.td = pow2_at_least((d->dim + 3) / 4);
+  const size_t ring = kRowBuffers * r.chunk * row, hs = (size_t)r.rn * d->dim * 4, sums = (size_t)r.rn * 4 * kRowThreads * 4;
+  r.smem_value = ring + hs + (size_t)r.rn * kRowStats * 4;
+  r.smem_grad = ring + hs + (size_t)r.rn * r.chunk * 4;
+  if (r.smem_grad < sums) r.smem_grad = sums;   // the groups' sums of df
   return r;
 }
 
-// Few rows: the row-group kernels, which read the weight once as it is.  From kRowsMost on
-// the tensor cores.
-constexpr int kRowsMost = 32;
-bool on_tensor_cores(const nc_linear_ce* d) { return d->rows > kRowsMost; }
+// Few rows take the streaming kernels, which read the weight as it is; from then on the tensor
+// cores are faster.
+bool on_tensor_cores(const nc_linear_ce* d) {
+  return d->dim > kRowDim || d->rows > (d->dtype == NC_BF16 ? kRowsMostBf16 : kRowsMost);
+}
 
 struct CeLayout {
   size_t status, row_loss, part, zlabel, df_part, tc, total;
@@ -354,10 +452,10 @@ CeLayout ce_layout(const nc_linear_ce* d, bool grad) {
     if (on_tensor_cores(d)) {
       L.tc = take(ce_tc_bytes(d, grad));
     } else {
-      const RowsPlan r = rows_plan(d, d->dim % 4 == 0 ? 4 : 1);
+      const RowsPlan r = rows_plan(d, 1);
       L.part = take((size_t)d->rows * r.blocks * sizeof(float2));
       L.zlabel = take((size_t)d->rows * 4);
-      if (grad) L.df_part = take((size_t)r.blocks * r.slots * d->rows * d->dim * 4);
+      if (grad) L.df_part = take((size_t)r.blocks * d->rows * d->dim * 4);
     }
   }
   L.total = at;
@@ -407,66 +505,66 @@ nc_status allow_smem(K kernel, size_t bytes) {
   return NC_OK;
 }
 
-template <typename T, int RN, int VEC>
-nc_status launch_rows_value(const CeArgs& a, const RowsPlan& r, float2* part, float* zlabel, cudaStream_t st) {
-  auto k = ce_rows_value_kernel<T, RN, VEC>;
-  NC_CHECK(allow_smem(k, r.smem_value));
-  PdlLaunch l(dim3(r.blocks, r.groups), dim3(kRowThreads), r.smem_value, st);
-  NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, k, a, r.vb, r.blocks, part, zlabel));
-  return launch_check("ce_rows_value_kernel launch");
-}
+// What a call of the streaming kernels takes along.
+struct RowsCall {
+  RowArgs args;
+  RowsPlan r;
+  cudaStream_t st;
+  // value
+  float2* part;
+  float* zlabel;
+  // gradient
+  const CeGrads* g;
+  float* df_part;
+};
 
-template <typename T, int RN, int VEC>
-nc_status launch_rows_grad(const CeArgs& a, const RowsPlan& r, const float* lse, const float* g_loss, void* gw,
-                           void* gb, float* df_part, cudaStream_t st) {
-  auto k = ce_rows_grad_kernel<T, RN, VEC>;
-  NC_CHECK(allow_smem(k, r.smem_grad));
-  PdlLaunch l(dim3(r.blocks), dim3(kRowThreads), r.smem_grad, st);
-  NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, k, a, r.vb, r.slots, r.td, lse, g_loss, static_cast<T*>(gw),
-                                   static_cast<T*>(gb), df_part));
+template <typename T, int RN, int VEC, int VT>
+nc_status launch_rows(const RowsCall& c) {
+  if (!c.g) {
+    auto k = ce_rows_value_kernel<T, RN, VEC, VT>;
+    NC_CHECK(allow_smem(k, c.r.smem_value));
+    PdlLaunch l(dim3(c.r.blocks), dim3(kRowThreads), c.r.smem_value, c.st);
+    NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, k, c.args, c.part, c.zlabel));
+    return launch_check("ce_rows_value_kernel launch");
+  }
+  auto k = ce_rows_grad_kernel<T, RN, VEC, VT>;
+  NC_CHECK(allow_smem(k, c.r.smem_grad));
+  PdlLaunch l(dim3(c.r.blocks), dim3(kRowThreads), c.r.smem_grad, c.st);
+  NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, k, c.args, c.r.td, c.g->lse, c.g->g_loss, static_cast<T*>(c.g->weight),
+                                   static_cast<T*>(c.g->bias), c.df_part));
   return launch_check("ce_rows_grad_kernel launch");
 }
 
-// Calls fn<T, RN, VEC>::run for the call's element type, row group and vector width.
-#define NC_ROWS_DISPATCH(FN, ...)                                                     \
-  do {                                                                                \
-    if (bf16) {                                                                       \
-      if (r.vec == 4) {                                                               \
-        return r.rn == 1   ? FN<__nv_bfloat16, 1, 4>(__VA_ARGS__)                     \
-               : r.rn == 4 ? FN<__nv_bfloat16, 4, 4>(__VA_ARGS__)                     \
-               : r.rn == 8 ? FN<__nv_bfloat16, 8, 4>(__VA_ARGS__)                     \
-                           : FN<__nv_bfloat16, 16, 4>(__VA_ARGS__);                   \
-      }                                                                               \
-      return r.rn == 1   ? FN<__nv_bfloat16, 1, 1>(__VA_ARGS__)                       \
-             : r.rn == 4 ? FN<__nv_bfloat16, 4, 1>(__VA_ARGS__)                       \
-             : r.rn == 8 ? FN<__nv_bfloat16, 8, 1>(__VA_ARGS__)                       \
-                         : FN<__nv_bfloat16, 16, 1>(__VA_ARGS__);                     \
-    }                                                                                 \
-    if (r.vec == 4) {                                                                 \
-      return r.rn == 1   ? FN<float, 1, 4>(__VA_ARGS__)                               \
-             : r.rn == 4 ? FN<float, 4, 4>(__VA_ARGS__)                               \
-             : r.rn == 8 ? FN<float, 8, 4>(__VA_ARGS__)                               \
-                         : FN<float, 16, 4>(__VA_ARGS__);                             \
-    }                                                                                 \
-    return r.rn == 1   ? FN<float, 1, 1>(__VA_ARGS__)                                 \
-           : r.rn == 4 ? FN<float, 4, 1>(__VA_ARGS__)                                 \
-           : r.rn == 8 ? FN<float, 8, 1>(__VA_ARGS__)                                 \
-                       : FN<float, 16, 1>(__VA_ARGS__);                               \
-  } while (0)
-
-nc_status rows_value(bool bf16, const CeArgs& a, const RowsPlan& r, float2* part, float* zlabel, cudaStream_t st) {
-  NC_ROWS_DISPATCH(launch_rows_value, a, r, part, zlabel, st);
+template <typename T, int RN>
+nc_status launch_rows_of(const RowsCall& c) {
+  if (c.r.vec == 1) return c.r.vt == 2 ? launch_rows<T, RN, 1, 2>(c) : launch_rows<T, RN, 1, 4>(c);
+  return c.r.vt == 2 ? launch_rows<T, RN, 4, 2>(c) : launch_rows<T, RN, 4, 4>(c);
 }
 
-nc_status rows_grad(bool bf16, const CeArgs& a, const RowsPlan& r, const float* lse, const float* g_loss, void* gw,
-                    void* gb, float* df_part, cudaStream_t st) {
-  NC_ROWS_DISPATCH(launch_rows_grad, a, r, lse, g_loss, gw, gb, df_part, st);
+template <typename T>
+nc_status launch_rows_as(const RowsCall& c) {
+  return c.r.rn == 1   ? launch_rows_of<T, 1>(c)
+         : c.r.rn == 4 ? launch_rows_of<T, 4>(c)
+         : c.r.rn == 8 ? launch_rows_of<T, 8>(c)
+                       : launch_rows_of<T, 16>(c);
 }
 
-// Vector loads need rows and base addresses on multiples of four elements.
-int vec_of(const nc_linear_ce* d, const void* p, const void* q, const void* out) {
-  const uintptr_t at = reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out);
-  return d->dim % 4 == 0 && at % (d->dtype == NC_BF16 ? 8 : 16) == 0 ? 4 : 1;
+// Vector loads and stores need rows and base addresses on multiples of four elements.
+RowsCall rows_call(const nc_linear_ce* d, const CeArgs& a, const void* g_weight, char* ws, const CeLayout& L,
+                   cudaStream_t st) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(a.weight) | reinterpret_cast<uintptr_t>(g_weight);
+  RowsCall c{};
+  c.r = rows_plan(d, d->dim % 4 == 0 && at % (d->dtype == NC_BF16 ? 8 : 16) == 0 ? 4 : 1);
+  c.args = RowArgs{a, c.r.chunk, c.r.chunks, reinterpret_cast<uintptr_t>(a.weight) % 16 == 0,
+                   reinterpret_cast<int32_t*>(ws + L.status)};
+  c.st = st;
+  return c;
+}
+
+// Before the streaming kernels: a call's status word is 0.
+nc_status rows_begin(char* ws, const CeLayout& L, cudaStream_t st) {
+  NC_CUDA_CHECK(cudaMemsetAsync(ws + L.status, 0, 4, st));
+  return NC_OK;
 }
 
 // lse and row losses, then the reduced loss.  `grad`: the layout of the workspace.
@@ -475,40 +573,38 @@ nc_status value(const nc_linear_ce* d, const CeArgs& a, bool grad, float* loss, 
   const bool none = d->reduction == NC_REDUCE_NONE;
   float* row_loss = none ? loss : reinterpret_cast<float*>(ws + L.row_loss);
   if (on_tensor_cores(d)) return ce_tc_value(d, a, grad, lse, row_loss, none ? nullptr : loss, ws + L.tc, st);
-  {
-    const RowsPlan r = rows_plan(d, vec_of(d, a.features, a.weight, nullptr));
-    float2* part = reinterpret_cast<float2*>(ws + L.part);
-    float* zlabel = reinterpret_cast<float*>(ws + L.zlabel);
-    NC_CHECK(rows_value(d->dtype == NC_BF16, a, r, part, zlabel, st));
-    PdlLaunch l(dim3((d->rows + 3) / 4), dim3(128), 0, st);
-    NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, ce_finish_rows_kernel, a, r.blocks, (const float2*)part,
-                                     (const float*)zlabel, lse, row_loss));
-    NC_CHECK(launch_check("ce_finish_rows_kernel launch"));
-  }
-  if (none) return NC_OK;
-  PdlLaunch l(dim3(1), dim3(1024), 0, st);
-  NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, ce_sum_kernel, a, (const float*)row_loss, loss));
-  return launch_check("ce_sum_kernel launch");
+  RowsCall c = rows_call(d, a, nullptr, ws, L, st);
+  c.part = reinterpret_cast<float2*>(ws + L.part), c.zlabel = reinterpret_cast<float*>(ws + L.zlabel);
+  NC_CHECK(d->dtype == NC_BF16 ? launch_rows_as<__nv_bfloat16>(c) : launch_rows_as<float>(c));
+  PdlLaunch l(dim3(1), dim3(512), 0, st);
+  NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, ce_rows_finish_kernel, a, c.r.blocks, (const float2*)c.part,
+                                   (const float*)c.zlabel, lse, row_loss, none ? (float*)nullptr : loss));
+  return launch_check("ce_rows_finish_kernel launch");
 }
 
 nc_status gradients(const nc_linear_ce* d, const CeArgs& a, const CeGrads& g, char* ws, cudaStream_t st) {
   const CeLayout L = ce_layout(d, true);
   if (on_tensor_cores(d)) return ce_tc_grad(d, a, g, ws + L.tc, st);
+  RowsCall c = rows_call(d, a, g.weight, ws, L, st);
+  c.g = &g, c.df_part = g.features ? reinterpret_cast<float*>(ws + L.df_part) : nullptr;
   const bool bf16 = d->dtype == NC_BF16;
-  const RowsPlan r = rows_plan(d, vec_of(d, a.features, a.weight, g.weight));
-  float* df_part = g.features ? reinterpret_cast<float*>(ws + L.df_part) : nullptr;
-  NC_CHECK(rows_grad(bf16, a, r, g.lse, g.g_loss, g.weight, g.bias, df_part, st));
+  NC_CHECK(bf16 ? launch_rows_as<__nv_bfloat16>(c) : launch_rows_as<float>(c));
   if (!g.features) return NC_OK;
-  const int64_t n = (int64_t)d->rows * d->dim;
-  PdlLaunch l(dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st);
-  const int slots = r.blocks * r.slots;
+  const int n = d->rows * d->dim;
+  PdlLaunch l(dim3((n + 31) / 32), dim3(256), 0, st);
   if (bf16)
-    NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, ce_sum_parts_kernel<__nv_bfloat16>, (const float*)df_part, n, slots,
+    NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, ce_sum_parts_kernel<__nv_bfloat16>, (const float*)c.df_part, n, c.r.blocks,
                                      static_cast<__nv_bfloat16*>(g.features)));
   else
-    NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, ce_sum_parts_kernel<float>, (const float*)df_part, n, slots,
+    NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, ce_sum_parts_kernel<float>, (const float*)c.df_part, n, c.r.blocks,
                                      static_cast<float*>(g.features)));
   return launch_check("ce_sum_parts_kernel launch");
+}
+
+// What the value and the gradient share, once before either.
+nc_status prepare(const nc_linear_ce* d, const CeArgs& a, bool grad, const float* g_loss, char* ws, cudaStream_t st) {
+  const CeLayout L = ce_layout(d, grad);
+  return on_tensor_cores(d) ? ce_tc_prepare(d, a, grad, g_loss, ws + L.tc, st) : rows_begin(ws, L, st);
 }
 
 nc_status check_inputs(const nc_linear_ce* d, const void* features, const void* weight, const void* bias,
@@ -516,6 +612,8 @@ nc_status check_inputs(const nc_linear_ce* d, const void* features, const void* 
   NC_CHECK(check_elems(d, features, "features"));
   NC_CHECK(check_elems(d, weight, "weight"));
   if (bias) NC_CHECK(check_elems(d, bias, "bias"));
+  if (d->dtype == NC_BF16 && d->dim % 8 == 0 && reinterpret_cast<uintptr_t>(weight) % 16 != 0)
+    return set_error(NC_ERR_INVALID, "a bfloat16 weight with a dim of whole 8s must start on 16 bytes");
   NC_CHECK(check_ptr(labels, "labels"));
   return check_ptr(lse, "lse");
 }
@@ -561,7 +659,7 @@ nc_status nc_linear_ce_forward(const nc_linear_ce* desc, const void* features, c
   NC_CHECK(check_ws(d_ws, ws_bytes, ce_layout(desc, false).total));
   char* ws = static_cast<char*>(d_ws);
   const CeArgs a = make_args(desc, features, weight, bias, labels);
-  if (on_tensor_cores(desc)) NC_CHECK(ce_tc_prepare(desc, a, false, nullptr, ws + ce_layout(desc, false).tc, st));
+  NC_CHECK(prepare(desc, a, false, nullptr, ws, st));
   NC_CHECK(value(desc, a, false, loss, lse, ws, st));
   clear_error();
   return NC_OK;
@@ -580,7 +678,7 @@ nc_status nc_linear_ce_backward(const nc_linear_ce* desc, const void* features, 
   NC_CHECK(check_ws(d_ws, ws_bytes, ce_layout(desc, true).total));
   char* ws = static_cast<char*>(d_ws);
   const CeArgs a = make_args(desc, features, weight, bias, labels);
-  if (on_tensor_cores(desc)) NC_CHECK(ce_tc_prepare(desc, a, true, g_loss, ws + ce_layout(desc, true).tc, st));
+  NC_CHECK(prepare(desc, a, true, g_loss, ws, st));
   const CeGrads g{lse, g_loss, g_features, g_weight, g_bias};
   NC_CHECK(gradients(desc, a, g, ws, st));
   clear_error();
@@ -600,7 +698,7 @@ nc_status nc_linear_ce_value_and_grad(const nc_linear_ce* desc, const void* feat
   NC_CHECK(check_ws(d_ws, ws_bytes, ce_layout(desc, true).total));
   char* ws = static_cast<char*>(d_ws);
   const CeArgs a = make_args(desc, features, weight, bias, labels);
-  if (on_tensor_cores(desc)) NC_CHECK(ce_tc_prepare(desc, a, true, nullptr, ws + ce_layout(desc, true).tc, st));
+  NC_CHECK(prepare(desc, a, true, nullptr, ws, st));
   NC_CHECK(value(desc, a, true, loss, lse, ws, st));
   const CeGrads g{lse, nullptr, g_features, g_weight, g_bias};
   NC_CHECK(gradients(desc, a, g, ws, st));

@@ -738,8 +738,6 @@ size_t ce_tc_bytes(const nc_linear_ce* d, bool grad) { return make_plan(d, grad)
 
 nc_status ce_tc_prepare(const nc_linear_ce* d, const CeArgs& a, bool grad, const float* g_loss, char* ws,
                         cudaStream_t st) {
-  if (!make_plan(d, grad).copy_w && !aligned16(a.weight))
-    return set_error(NC_ERR_INVALID, "a bfloat16 weight must start on a 16-byte boundary for more than 32 rows");
   NC_TC_CALL(grad, prepare(g_loss));
 }
 
