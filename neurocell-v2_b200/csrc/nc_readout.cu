@@ -26,9 +26,9 @@ namespace {
 constexpr int kRowThreads = 256;
 constexpr int kRowWarps = kRowThreads / 32;
 constexpr int kRowDim = 4 * kRowThreads;       // most columns: four a thread
-constexpr int kRowBuffers = 2;
+constexpr int kRowBuffers = 2, kRowChunk = 64;   // most classes of a chunk
 constexpr size_t kRowChunkBytes = 64 * 1024;   // two in flight cover the memory's latency
-constexpr int kRowsMost = 16, kRowsMostBf16 = 16;
+constexpr int kRowsMost = 16, kRowsMostBf16 = 4;
 constexpr int kRowStats = 512;                 // logits a row collects before its statistics take them in
 
 template <int VEC, typename T>
@@ -90,6 +90,11 @@ struct RowStream {
   }
   __device__ __forceinline__ T* buffer(int c) const {
     return reinterpret_cast<T*>(ring + (size_t)((c - c0) % kRowBuffers) * r.chunk * r.a.dim * sizeof(T));
+  }
+  // This thread's class of chunk c: its bias, asked for a chunk ahead of its use.
+  __device__ __forceinline__ float bias(int c) const {
+    const T* b = static_cast<const T*>(r.a.bias);
+    return b && c < c1 && (int)threadIdx.x < classes(c) ? to_f32(b[(size_t)c * r.chunk + threadIdx.x]) : 0.f;
   }
   __device__ __forceinline__ uint32_t bytes(int c) const { return (uint32_t)(classes(c) * r.a.dim * sizeof(T)); }
   // Thread 0 asks for chunk c; its buffer is free.
@@ -175,26 +180,30 @@ __global__ void __launch_bounds__(kRowThreads) ce_rows_value_kernel(const RowArg
   extern __shared__ __align__(128) uint8_t raw[];
   __shared__ __align__(8) uint64_t bars[kRowBuffers];
   __shared__ int flag;
+  __shared__ float bias[kRowChunk];
   const CeArgs& a = args.a;
   float* hs = reinterpret_cast<float*>(raw + kRowBuffers * (size_t)args.chunk * a.dim * sizeof(T));
   float* z = hs + RN * a.dim;   // (RN, kRowStats)
   RowStream<T> s(args, raw, bars, &flag);
-  const T* bias = static_cast<const T*>(a.bias);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   constexpr int kMine = (RN + kRowWarps - 1) / kRowWarps;   // rows whose statistics a warp keeps
   float2 mine[kMine];
 #pragma unroll
   for (int k = 0; k < kMine; ++k) mine[k] = make_float2(-INFINITY, 0.f);
   pdl_enter();
+  if (blockIdx.x == 0 && threadIdx.x == 0) *args.status = 0;
   for (int c = s.c0; c < s.c0 + kRowBuffers; ++c) s.ask(c);
   stage_features<T, RN>(a, hs);
   int held = 0, base = s.c0 * args.chunk;   // classes base .. base + held - 1 are in z
   int c = s.c0;
+  float next = s.bias(c);
   for (; c < s.c1; ++c) {
+    if (threadIdx.x < kRowChunk) bias[threadIdx.x] = next;
+    next = s.bias(c + 1);
     if (!s.wait(c)) break;
     const int n = s.classes(c);
     chunk_logits<T, RN, VEC, VT>(s.buffer(c), hs, a.dim, n,
-                                 [&](int v, int r, float x) { z[r * kRowStats + held + v] = x; });
+                                 [&](int v, int r, float x) { z[r * kRowStats + held + v] = x + bias[v]; });
     __syncthreads();
     s.ask(c + kRowBuffers);
     held += n;
@@ -206,8 +215,7 @@ __global__ void __launch_bounds__(kRowThreads) ce_rows_value_kernel(const RowArg
       const int label = a.labels[r];
       float m = -INFINITY;
       for (int v = lane; v < held; v += 32) {
-        const float x = z[r * kRowStats + v] + (bias ? to_f32(bias[base + v]) : 0.f);
-        z[r * kRowStats + v] = x;
+        const float x = z[r * kRowStats + v];
         m = fmaxf(m, x);
         if (base + v == label) zlabel[r] = x;
       }
@@ -267,15 +275,16 @@ __global__ void __launch_bounds__(kRowThreads) ce_rows_grad_kernel(
   extern __shared__ __align__(128) uint8_t raw[];
   __shared__ __align__(8) uint64_t bars[kRowBuffers];
   __shared__ int flag;
+  __shared__ float bias[kRowChunk];
   __shared__ float row_g[RN], row_lse[RN];
   __shared__ int row_label[RN];
   const CeArgs& a = args.a;
   float* hs = reinterpret_cast<float*>(raw + kRowBuffers * (size_t)args.chunk * a.dim * sizeof(T));
   float* p = hs + RN * a.dim;   // (chunk, RN)
   RowStream<T> s(args, raw, bars, &flag);
-  const T* bias = static_cast<const T*>(a.bias);
   const int tid = threadIdx.x;
   pdl_enter();
+  if (blockIdx.x == 0 && tid == 0) *args.status = 0;
   for (int c = s.c0; c < s.c0 + kRowBuffers; ++c) s.ask(c);
   if (tid < RN) {
     int kept = 0;
@@ -298,7 +307,10 @@ __global__ void __launch_bounds__(kRowThreads) ce_rows_grad_kernel(
 #pragma unroll
     for (int e = 0; e < 4; ++e) h[r][e] = col[e] < a.dim ? hs[r * a.dim + col[e]] : 0.f, acc[r][e] = 0.f;
   int c = s.c0;
+  float next = s.bias(c);
   for (; c < s.c1; ++c) {
+    if (tid < kRowChunk) bias[tid] = next;
+    next = s.bias(c + 1);
     if (!s.wait(c)) break;
     const int n = s.classes(c), v0 = c * args.chunk;
     const T* w = s.buffer(c);
@@ -306,7 +318,7 @@ __global__ void __launch_bounds__(kRowThreads) ce_rows_grad_kernel(
     __syncthreads();
     for (int i = tid; i < n * RN; i += kRowThreads) {
       const int v = i / RN, r = i % RN;
-      const float x = p[i] + (bias ? to_f32(bias[v0 + v]) : 0.f);
+      const float x = p[i] + bias[v];
       p[i] = row_g[r] == 0.f ? 0.f : row_g[r] * (expf(x - row_lse[r]) - (v0 + v == row_label[r] ? 1.f : 0.f));
     }
     __syncthreads();
@@ -321,15 +333,21 @@ __global__ void __launch_bounds__(kRowThreads) ce_rows_grad_kernel(
     if (col[0] < a.dim) {
 #pragma unroll 2
       for (int v = group; v < n; v += groups) {
-        float x[4], q[RN], out[4] = {0.f, 0.f, 0.f, 0.f};
+        static_assert(RN == 1 || RN % 4 == 0, "rows come in fours");
+        float x[4], out[4] = {0.f, 0.f, 0.f, 0.f};
+        alignas(16) float q[RN];
         if constexpr (VEC == 4) {
           load_vec<4>(w + v * a.dim + col[0], x);
         } else {
 #pragma unroll
           for (int e = 0; e < 4; ++e) x[e] = col[e] < a.dim ? to_f32(w[v * a.dim + col[e]]) : 0.f;
         }
+        if constexpr (RN % 4 == 0) {
 #pragma unroll
-        for (int r = 0; r < RN; ++r) q[r] = p[v * RN + r];
+          for (int r = 0; r < RN; r += 4) *reinterpret_cast<float4*>(q + r) = *reinterpret_cast<const float4*>(p + v * RN + r);
+        } else {
+          q[0] = p[v];
+        }
 #pragma unroll
         for (int r = 0; r < RN; ++r)
 #pragma unroll
@@ -415,7 +433,7 @@ RowsPlan rows_plan(const nc_linear_ce* d, int vec) {
   r.rn = d->rows <= 1 ? 1 : d->rows <= 4 ? 4 : d->rows <= 8 ? 8 : 16;
   r.vec = vec;
   const size_t row = (size_t)d->dim * (d->dtype == NC_BF16 ? 2 : 4);
-  r.chunk = 64;   // 16 classes of up to 4 KB fit a buffer
+  r.chunk = kRowChunk;   // 16 classes of up to 4 KB fit a buffer
   while (r.chunk > 16 && (r.chunk * row > kRowChunkBytes || d->classes < r.chunk * 148)) r.chunk /= 2;
   r.vt = r.chunk >= 32 ? 4 : 2;
   r.chunks = (d->classes + r.chunk - 1) / r.chunk;
@@ -561,12 +579,6 @@ RowsCall rows_call(const nc_linear_ce* d, const CeArgs& a, const void* g_weight,
   return c;
 }
 
-// Before the streaming kernels: a call's status word is 0.
-nc_status rows_begin(char* ws, const CeLayout& L, cudaStream_t st) {
-  NC_CUDA_CHECK(cudaMemsetAsync(ws + L.status, 0, 4, st));
-  return NC_OK;
-}
-
 // lse and row losses, then the reduced loss.  `grad`: the layout of the workspace.
 nc_status value(const nc_linear_ce* d, const CeArgs& a, bool grad, float* loss, float* lse, char* ws, cudaStream_t st) {
   const CeLayout L = ce_layout(d, grad);
@@ -604,7 +616,7 @@ nc_status gradients(const nc_linear_ce* d, const CeArgs& a, const CeGrads& g, ch
 // What the value and the gradient share, once before either.
 nc_status prepare(const nc_linear_ce* d, const CeArgs& a, bool grad, const float* g_loss, char* ws, cudaStream_t st) {
   const CeLayout L = ce_layout(d, grad);
-  return on_tensor_cores(d) ? ce_tc_prepare(d, a, grad, g_loss, ws + L.tc, st) : rows_begin(ws, L, st);
+  return on_tensor_cores(d) ? ce_tc_prepare(d, a, grad, g_loss, ws + L.tc, st) : NC_OK;
 }
 
 nc_status check_inputs(const nc_linear_ce* d, const void* features, const void* weight, const void* bias,
