@@ -7,8 +7,8 @@ Mirrors the parts of ``neurocell/trainer.py`` that drive the hot path:
 with the reference's epoch, evaluation, adaptive sub-ROI, annealed-temperature and
 multi-epoch entry points (trainer.py:108-156, 164-268, 270-356, 358-398).  The
 ``lax.scan`` programs become either an eager loop over the library's operators
-(``VNNTrainer``) or one CUDA graph per step or per epoch (``VNNTrainStep``).  Optimizers
-other than SGD are not part of the B200 hot path.
+(``VNNTrainer``) or one CUDA graph per step or per epoch (``VNNTrainStep``).  Both update by
+SGD or by orthogonalised momentum (``optimizer="muon"``, ``ops.muon_``).
 """
 from __future__ import annotations
 
@@ -49,6 +49,14 @@ def default_exact_match_metric(logits: torch.Tensor, targets: torch.Tensor) -> t
 
 def softmax_cross_entropy_loss(logits: torch.Tensor, labels: torch.Tensor) -> torch.Tensor:
     return ops.softmax_ce_loss(logits, labels)
+
+
+OPTIMIZERS = ("sgd", "muon")
+
+
+def _check_optimizer(optimizer: str) -> None:
+    if optimizer not in OPTIMIZERS:
+        raise ValueError(f"Unsupported optimizer '{optimizer}'; choose from {OPTIMIZERS}.")
 
 
 BIT_WEIGHTS_U8 = (128, 64, 32, 16, 8, 4, 2, 1)
@@ -204,6 +212,10 @@ class VNNTrainStep:
     page-locked host scalar, returned by ``step()`` and valid once the stream has reached
     the end of the step (``torch.cuda.synchronize()`` or an event); otherwise ``step()``
     returns the device loss.  ``capture()`` records the launch sequence into a CUDA graph.
+    ``optimizer="muon"`` updates by orthogonalised momentum (``nc_muon_update``) instead of
+    SGD: the three cell grids as matrices (H, W), the filters as one matrix (M, Kh Kw), with
+    ``beta``, Nesterov momentum and ``weight_decay``; over several ranks it takes the
+    ``"nccl"`` exchange.
     Every kernel of the step except NCCL's comes from ``libneurocell_b200.so``.
     """
 
@@ -213,7 +225,8 @@ class VNNTrainStep:
                  codd_mode: str = "continuous", state_temperature: float = 1.0,
                  active_threshold: float = 0.6, in_shapes=None, process_group=None,
                  exchange: str = "nccl", conv: str = "auto", spatial_mask=None,
-                 host_loss: bool = False):
+                 host_loss: bool = False, optimizer: str = "sgd", beta: float = 0.95,
+                 weight_decay: float = 0.0):
         import ctypes
         from . import _lib
         from .params import check_codd_mode
@@ -222,6 +235,7 @@ class VNNTrainStep:
             raise ValueError(f"Unsupported loss '{loss}'; choose from ('mse', 'ce').")
         if exchange not in ("nccl", "nvlink"):
             raise ValueError(f"Unsupported exchange '{exchange}'; choose from ('nccl', 'nvlink').")
+        _check_optimizer(optimizer)
         dev = params.cell_params.device
         ops._require_cuda(params.cell_params, "params.cell_params")
         if not topology.out_in_roi:
@@ -251,6 +265,8 @@ class VNNTrainStep:
         if process_group is not None:
             import torch.distributed as dist
             self.world = dist.get_world_size(process_group)
+        if optimizer == "muon" and exchange == "nvlink" and self.world > 1:
+            raise NotImplementedError("the nvlink exchange applies SGD; optimizer='muon' takes exchange='nccl'")
         cell = params.cell_params.detach()
         self._full_cell = None
         if self.window is not None:
@@ -265,6 +281,15 @@ class VNNTrainStep:
         self.flat[: self.n_cell].copy_(cell.reshape(-1))
         self.flat[self.n_cell:].copy_(params.greens_filters.reshape(-1))
         self.grads = torch.zeros_like(self.flat)
+        # muon: (descriptor, offset) of the cells and of the filters, their momentum and workspace
+        self.momentum = None
+        if optimizer == "muon":
+            self.beta, self.weight_decay = float(beta), float(weight_decay)
+            m = params.greens_filters.shape[0]
+            self._muon = [(ops._newton_schulz_desc(shape, "float32", 5, ops.NEWTON_SCHULZ_COEFFICIENTS, 1e-7), at)
+                          for shape, at in ((tuple(cell.shape), 0), ((m, self.n_filt // m), self.n_cell))]
+            self.momentum = torch.zeros_like(self.flat)
+            self._muon_ws = [ops._newton_schulz_ws(self.lib, d, dev) for d, _ in self._muon]
         self._cell_view = self.flat[: self.n_cell].view(tuple(cell.shape))
         self._filt_view = self.flat[self.n_cell:].view(params.greens_filters.shape)
         self.ws_bytes = self.lib.nc_workspace_bytes(ctypes.byref(self.plan.topo), self.B,
@@ -352,9 +377,17 @@ class VNNTrainStep:
             self.exchange.allreduce_sgd(gcell, cell, self.lr, st)
         else:
             world = allreduce_mean_(self.grads, self.pg)
-            lr = self.lr / world            # mean of the per-rank mean-loss gradients
-            self._lib.check(lib.nc_sgd_update(c.c_void_p(cell), c.c_void_p(gcell),
-                                              self.n_cell + self.n_filt, lr, st), "nc_sgd_update")
+            if self.momentum is not None:
+                # an orthogonalised update does not depend on the gradient's scale (1 / world)
+                for (d, at), ws in zip(self._muon, self._muon_ws):
+                    self._lib.check(lib.nc_muon_update(
+                        c.byref(d), c.c_void_p(cell + 4 * at), c.c_void_p(gcell + 4 * at),
+                        c.c_void_p(self.momentum.data_ptr() + 4 * at), self.lr, self.beta, 1,
+                        self.weight_decay, P(ws), ws.numel(), st), "nc_muon_update")
+            else:
+                lr = self.lr / world            # mean of the per-rank mean-loss gradients
+                self._lib.check(lib.nc_sgd_update(c.c_void_p(cell), c.c_void_p(gcell),
+                                                  self.n_cell + self.n_filt, lr, st), "nc_sgd_update")
         if timed:
             self.exchange_events[1].record()
         self._launches = int(lib.nc_launch_count() - n0)
@@ -391,7 +424,7 @@ class VNNTrainStep:
             dist.barrier(group=self.pg)      # ranks enter the first exchange together
         s = torch.cuda.Stream(self.device)
         s.wait_stream(torch.cuda.current_stream(self.device))
-        saved = self.flat.clone()
+        saved, momentum = self.flat.clone(), None if self.momentum is None else self.momentum.clone()
         with torch.cuda.stream(s):
             for _ in range(2):
                 self._launch()
@@ -400,6 +433,8 @@ class VNNTrainStep:
         with torch.cuda.graph(g):
             self._launch()
         self.flat.copy_(saved)             # warm-up and capture must not move the parameters
+        if momentum is not None:
+            self.momentum.copy_(momentum)
         self.graph = g
 
     def exchange_status(self) -> int:
@@ -424,7 +459,7 @@ class VNNTrainStep:
             dist.barrier(group=self.pg)
         s = torch.cuda.Stream(self.device)
         s.wait_stream(torch.cuda.current_stream(self.device))
-        saved = self.flat.clone()
+        saved, momentum = self.flat.clone(), None if self.momentum is None else self.momentum.clone()
         with torch.cuda.stream(s):
             for i in range(min(nb, 2)):      # warm-up (kernel attributes, lazy loading)
                 self.x.copy_(xs[i])
@@ -438,6 +473,8 @@ class VNNTrainStep:
                 self.y.copy_(ys[i])
                 self._launch(self.epoch_losses[i])
         self.flat.copy_(saved)
+        if momentum is not None:
+            self.momentum.copy_(momentum)
         self.epoch_graph = g
         self._epoch_src = (xs, ys)           # the graph reads these buffers
 
@@ -459,14 +496,19 @@ class VNNTrainStep:
 
 
 class VNNTrainer:
-    """value_and_grad + SGD over ``apply_fn`` (trainer.py:71-106, optimizer = SGD(lr)).
+    """value_and_grad + update over ``apply_fn`` (trainer.py:71-106, optimizer = SGD(lr), or
+    ``optimizer="muon"``: orthogonalised momentum as in :class:`VNNTrainStep`).
 
     ``apply_fn(params, batch_x, **kw)`` is ``VonNeumannNetwork.apply`` or a closure over
     ``propagate_vnn_2d``; the adaptive and annealed entry points pass ``spatial_mask``,
     ``codd_mode`` and ``state_temperature`` through it as the reference does."""
 
     def __init__(self, apply_fn, lr: float = 1e-2, batch_size: int = 128, loss_fn=None,
-                 eval_metric_fn=None):
+                 eval_metric_fn=None, optimizer: str = "sgd", beta: float = 0.95,
+                 weight_decay: float = 0.0):
+        _check_optimizer(optimizer)
+        self.optimizer, self.beta, self.weight_decay = optimizer, float(beta), float(weight_decay)
+        self.momentum = None      # VNNParams of the parameters last trained (muon)
         self.apply_fn = apply_fn
         self.lr = float(lr)
         self.batch_size = batch_size
@@ -485,9 +527,23 @@ class VNNTrainer:
         """Returns ``(new_params, loss)``; the update runs in place on ``params``' storage."""
         loss, grads = self.value_and_grad(params, batch_x, batch_y, **apply_kw)
         with torch.no_grad():
-            ops.sgd_(params.cell_params, grads.cell_params, self.lr)
-            ops.sgd_(params.greens_filters, grads.greens_filters, self.lr)
+            if self.optimizer == "muon":
+                self._muon_update(params, grads)
+            else:
+                ops.sgd_(params.cell_params, grads.cell_params, self.lr)
+                ops.sgd_(params.greens_filters, grads.greens_filters, self.lr)
         return params, loss
+
+    def _muon_update(self, params: VNNParams, grads: VNNParams) -> None:
+        """The momentum starts at zero and lives in the trainer; set ``momentum = None`` to
+        start over."""
+        if self.momentum is None:
+            self.momentum = VNNParams(torch.zeros_like(params.cell_params),
+                                      torch.zeros_like(params.greens_filters))
+        for p, g, m in zip(params, grads, self.momentum):
+            shape = p.shape if p.ndim == 3 else (p.shape[0], p.numel() // p.shape[0])
+            ops.muon_(p.view(shape), g.contiguous().view(shape), m.view(shape), self.lr, beta=self.beta,
+                      weight_decay=self.weight_decay)
 
     def train_epoch(self, params: VNNParams, x_epoch, y_epoch, **apply_kw):
         """Steps over the batches of ``x_epoch`` / ``y_epoch`` in order (trainer.py:108-119);
