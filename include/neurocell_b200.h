@@ -442,7 +442,9 @@ const char* nc_last_error(void);
  * the latest nc_vnn_forward / nc_vnn_forward_universe on d_ws, or of a backward after it,
  * gave up a bounded wait for its own asynchronous copies into shared memory (every result
  * of that call is then invalid).  Each forward clears it when it starts; calls on other
- * workspaces never touch it.  Copies the word to *status and synchronises the stream;
+ * workspaces never touch it.  The nc_linear_ce_*, nc_orthogonalize and nc_muon_update calls
+ * clear and set it the same way, each for itself (not where there are no rows or matrices,
+ * which launch nothing).  Copies the word to *status and synchronises the stream;
  * not for the hot path.
  */
 nc_status nc_workspace_status(const void* d_ws, int32_t* status, void* stream);

@@ -61,7 +61,6 @@ struct RowArgs {
   CeArgs a;
   int chunk, chunks;
   int bulk;           // the weight starts on 16 bytes
-  int32_t* status;
 };
 
 // The stream of this CTA's chunks [c0, c1) of the weight.
@@ -112,7 +111,7 @@ struct RowStream {
   // behind whole 16s, and chunks of a weight that does not start so, are loaded here.
   __device__ __forceinline__ bool wait(int c) {
     const int i = c - c0;
-    if (r.bulk) ok = tc::bar_wait(bars + 8 * (i % kRowBuffers), i / kRowBuffers & 1, abort, r.status);
+    if (r.bulk) ok = tc::bar_wait(bars + 8 * (i % kRowBuffers), i / kRowBuffers & 1, abort, r.a.status);
     const int n = classes(c) * r.a.dim, from = r.bulk ? (int)((bytes(c) & ~15u) / sizeof(T)) : 0;
     T* to = buffer(c);
     for (int e = from + threadIdx.x; e < n; e += kRowThreads) to[e] = at(c)[e];
@@ -191,7 +190,7 @@ __global__ void __launch_bounds__(kRowThreads) ce_rows_value_kernel(const RowArg
 #pragma unroll
   for (int k = 0; k < kMine; ++k) mine[k] = make_float2(-INFINITY, 0.f);
   pdl_enter();
-  if (blockIdx.x == 0 && threadIdx.x == 0) *args.status = 0;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *a.status = 0;
   for (int c = s.c0; c < s.c0 + kRowBuffers; ++c) s.ask(c);
   stage_features<T, RN>(a, hs);
   int held = 0, base = s.c0 * args.chunk;   // classes base .. base + held - 1 are in z
@@ -284,7 +283,7 @@ __global__ void __launch_bounds__(kRowThreads) ce_rows_grad_kernel(
   RowStream<T> s(args, raw, bars, &flag);
   const int tid = threadIdx.x;
   pdl_enter();
-  if (blockIdx.x == 0 && tid == 0) *args.status = 0;
+  if (blockIdx.x == 0 && tid == 0) *a.status = 0;
   for (int c = s.c0; c < s.c0 + kRowBuffers; ++c) s.ask(c);
   if (tid < RN) {
     int kept = 0;
@@ -508,11 +507,12 @@ nc_status check_ws(const void* ws, size_t have, size_t need) {
   return NC_OK;
 }
 
-CeArgs make_args(const nc_linear_ce* d, const void* f, const void* w, const void* b, const int32_t* labels) {
+CeArgs make_args(const nc_linear_ce* d, const void* f, const void* w, const void* b, const int32_t* labels, char* ws) {
   CeArgs a;
   a.features = f, a.weight = w, a.bias = b, a.labels = labels;
   a.rows = d->rows, a.dim = d->dim, a.classes = d->classes;
   a.ignore_index = d->ignore_index, a.reduction = d->reduction;
+  a.status = reinterpret_cast<int32_t*>(ws);   // the layout's first word
   return a;
 }
 
@@ -568,13 +568,11 @@ nc_status launch_rows_as(const RowsCall& c) {
 }
 
 // Vector loads and stores need rows and base addresses on multiples of four elements.
-RowsCall rows_call(const nc_linear_ce* d, const CeArgs& a, const void* g_weight, char* ws, const CeLayout& L,
-                   cudaStream_t st) {
+RowsCall rows_call(const nc_linear_ce* d, const CeArgs& a, const void* g_weight, cudaStream_t st) {
   const uintptr_t at = reinterpret_cast<uintptr_t>(a.weight) | reinterpret_cast<uintptr_t>(g_weight);
   RowsCall c{};
   c.r = rows_plan(d, d->dim % 4 == 0 && at % (d->dtype == NC_BF16 ? 8 : 16) == 0 ? 4 : 1);
-  c.args = RowArgs{a, c.r.chunk, c.r.chunks, reinterpret_cast<uintptr_t>(a.weight) % 16 == 0,
-                   reinterpret_cast<int32_t*>(ws + L.status)};
+  c.args = RowArgs{a, c.r.chunk, c.r.chunks, reinterpret_cast<uintptr_t>(a.weight) % 16 == 0};
   c.st = st;
   return c;
 }
@@ -585,7 +583,7 @@ nc_status value(const nc_linear_ce* d, const CeArgs& a, bool grad, float* loss, 
   const bool none = d->reduction == NC_REDUCE_NONE;
   float* row_loss = none ? loss : reinterpret_cast<float*>(ws + L.row_loss);
   if (on_tensor_cores(d)) return ce_tc_value(d, a, grad, lse, row_loss, none ? nullptr : loss, ws + L.tc, st);
-  RowsCall c = rows_call(d, a, nullptr, ws, L, st);
+  RowsCall c = rows_call(d, a, nullptr, st);
   c.part = reinterpret_cast<float2*>(ws + L.part), c.zlabel = reinterpret_cast<float*>(ws + L.zlabel);
   NC_CHECK(d->dtype == NC_BF16 ? launch_rows_as<__nv_bfloat16>(c) : launch_rows_as<float>(c));
   PdlLaunch l(dim3(1), dim3(512), 0, st);
@@ -597,7 +595,7 @@ nc_status value(const nc_linear_ce* d, const CeArgs& a, bool grad, float* loss, 
 nc_status gradients(const nc_linear_ce* d, const CeArgs& a, const CeGrads& g, char* ws, cudaStream_t st) {
   const CeLayout L = ce_layout(d, true);
   if (on_tensor_cores(d)) return ce_tc_grad(d, a, g, ws + L.tc, st);
-  RowsCall c = rows_call(d, a, g.weight, ws, L, st);
+  RowsCall c = rows_call(d, a, g.weight, st);
   c.g = &g, c.df_part = g.features ? reinterpret_cast<float*>(ws + L.df_part) : nullptr;
   const bool bf16 = d->dtype == NC_BF16;
   NC_CHECK(bf16 ? launch_rows_as<__nv_bfloat16>(c) : launch_rows_as<float>(c));
@@ -670,7 +668,7 @@ nc_status nc_linear_ce_forward(const nc_linear_ce* desc, const void* features, c
   NC_CHECK(check_inputs(desc, features, weight, bias, labels, lse));
   NC_CHECK(check_ws(d_ws, ws_bytes, ce_layout(desc, false).total));
   char* ws = static_cast<char*>(d_ws);
-  const CeArgs a = make_args(desc, features, weight, bias, labels);
+  const CeArgs a = make_args(desc, features, weight, bias, labels, ws);
   NC_CHECK(prepare(desc, a, false, nullptr, ws, st));
   NC_CHECK(value(desc, a, false, loss, lse, ws, st));
   clear_error();
@@ -689,7 +687,7 @@ nc_status nc_linear_ce_backward(const nc_linear_ce* desc, const void* features, 
   if (g_loss) NC_CHECK(check_ptr(g_loss, "g_loss"));
   NC_CHECK(check_ws(d_ws, ws_bytes, ce_layout(desc, true).total));
   char* ws = static_cast<char*>(d_ws);
-  const CeArgs a = make_args(desc, features, weight, bias, labels);
+  const CeArgs a = make_args(desc, features, weight, bias, labels, ws);
   NC_CHECK(prepare(desc, a, true, g_loss, ws, st));
   const CeGrads g{lse, g_loss, g_features, g_weight, g_bias};
   NC_CHECK(gradients(desc, a, g, ws, st));
@@ -709,7 +707,7 @@ nc_status nc_linear_ce_value_and_grad(const nc_linear_ce* desc, const void* feat
   NC_CHECK(check_inputs(desc, features, weight, bias, labels, lse));
   NC_CHECK(check_ws(d_ws, ws_bytes, ce_layout(desc, true).total));
   char* ws = static_cast<char*>(d_ws);
-  const CeArgs a = make_args(desc, features, weight, bias, labels);
+  const CeArgs a = make_args(desc, features, weight, bias, labels, ws);
   NC_CHECK(prepare(desc, a, true, nullptr, ws, st));
   NC_CHECK(value(desc, a, true, loss, lse, ws, st));
   const CeGrads g{lse, nullptr, g_features, g_weight, g_bias};

@@ -21,6 +21,7 @@ struct CeArgs {
   int rows, dim, classes;
   int ignore_index;
   int reduction;
+  int32_t* status;   // the workspace's status word (nc_workspace_status)
 };
 
 // What the gradient kernels read of the loss's own gradient, and where the results go.

@@ -105,7 +105,7 @@ Plan make_plan(const nc_linear_ce* d, bool grad) {
     at += pad256(bytes);
     return o;
   };
-  p.scales = take(sizeof(Scales) + 4);   // and the wait status
+  p.scales = take(sizeof(Scales));
   p.max_part = take(2 * kMaxBlocks * 4);
   if (p.copy_w) p.w = take((size_t)d->classes * p.pitch * 2 * planes);
   p.f = take((size_t)d->rows * p.pitch * 2 * planes);
@@ -234,7 +234,7 @@ template <typename T>
 __global__ void __launch_bounds__(kPrepThreads) ce_planes_kernel(CeArgs a, int copy_w, int pitch, int classes_pad,
                                                                  int wide_w, int wide_f,
                                                                  const float* __restrict__ max_part, Scales* scales,
-                                                                 int32_t* status, uint16_t* __restrict__ w,
+                                                                 uint16_t* __restrict__ w,
                                                                  uint16_t* __restrict__ f, float* __restrict__ bias,
                                                                  const float* __restrict__ g_loss,
                                                                  float* __restrict__ fac) {
@@ -264,7 +264,7 @@ __global__ void __launch_bounds__(kPrepThreads) ce_planes_kernel(CeArgs a, int c
   if (blockIdx.x == 0 && threadIdx.x == 0) {
     scales->w = sw, scales->f = sf, scales->w_inv = 1.f / sw, scales->f_inv = 1.f / sf;
     scales->blocks_done = 0;
-    *status = 0;
+    *a.status = 0;
   }
   const int64_t step = (int64_t)(gridDim.x - 1) * kPrepThreads, i0 = (int64_t)blockIdx.x * kPrepThreads + threadIdx.x;
   const int per = pitch / 8;
@@ -593,7 +593,6 @@ struct Call {
     return reinterpret_cast<U*>(ws + o);
   }
   Scales* scales() const { return at<Scales>(p.scales); }
-  int32_t* status() const { return reinterpret_cast<int32_t*>(at<Scales>(p.scales) + 1); }
 
   template <int BN, int CG, int EW>
   tc::Problem problem(int m, int n, int k, int splits) const {
@@ -601,7 +600,7 @@ struct Call {
     q.m = m, q.n = n, q.k = k, q.batch = 1, q.splits = splits, q.bf16 = p.bf16;
     tc::set_tiles<BN, CG>(&q);
     q.chunk = PL == 1 ? 1 << 30 : kChunk;
-    q.status = status();
+    q.status = a.status;
     return q;
   }
 
@@ -641,7 +640,7 @@ struct Call {
     const int even = d->dim % 8 == 0;
     NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, ce_planes_kernel<T>, a, (int)p.copy_w, p.pitch, p.classes_pad,
                                      (int)(even && aligned16(a.weight)), (int)(even && aligned16(a.features)),
-                                     (const float*)at<float>(p.max_part), scales(), status(), at<uint16_t>(p.w),
+                                     (const float*)at<float>(p.max_part), scales(), at<uint16_t>(p.w),
                                      at<uint16_t>(p.f), at<float>(p.bias), g_loss,
                                      p.grad ? at<float>(p.fac) : nullptr));
     return launch_check("ce_planes_kernel launch");

@@ -6,6 +6,7 @@ every FLOP runs in ``libneurocell_b200.so``.  Nothing here computes on the CPU.
 from __future__ import annotations
 
 import ctypes
+import math
 from dataclasses import dataclass
 
 import numpy as np
@@ -584,6 +585,8 @@ def _linear_ce_forward(lib, d, f, w, labels, b):
     _lib.check(lib.nc_linear_ce_forward(ctypes.byref(d), _ptr(f), _ptr(w), _ptr(b), _ptr(labels),
                                         _ptr(loss), _ptr(lse), _ptr(ws), ws.numel(), _stream(dev)),
                "nc_linear_ce_forward")
+    if d.rows:
+        _after_call(ws, "nc_linear_ce_forward")
     return loss, lse
 
 
@@ -597,6 +600,8 @@ def _linear_ce_backward(lib, d, f, w, labels, b, lse, g_loss, need_f, need_w, ne
                                          _ptr(lse), _ptr(g_loss), _ptr(g_f), _ptr(g_w), _ptr(g_b),
                                          _ptr(ws), ws.numel(), _stream(dev)),
                "nc_linear_ce_backward")
+    if d.rows:
+        _after_call(ws, "nc_linear_ce_backward")
     return g_f, g_w, g_b
 
 
@@ -659,6 +664,8 @@ def linear_softmax_ce_value_and_grad(features: torch.Tensor, weight: torch.Tenso
                                                    _ptr(loss), _ptr(lse), _ptr(g_f), _ptr(g_w), _ptr(g_b),
                                                    _ptr(ws), ws.numel(), _stream(dev)),
                    "nc_linear_ce_value_and_grad")
+        if d.rows:
+            _after_call(ws, "nc_linear_ce_value_and_grad")
     return loss, g_f, g_w, g_b
 
 
@@ -674,7 +681,7 @@ def _newton_schulz_desc(shape, dtype: str, steps, coefficients, eps) -> _lib.NcN
     if dtype not in _lib.NC_DTYPE:
         raise ValueError(f"float32 or bfloat16 expected, got {dtype}")
     a, b, c = coefficients
-    batch = int(np.prod(shape[:-2], dtype=np.int64))
+    batch = math.prod(shape[:-2])
     return _lib.NcNewtonSchulz(batch, shape[-2], shape[-1], _lib.NC_DTYPE[dtype], int(steps), float(a),
                                float(b), float(c), float(eps))
 
@@ -701,6 +708,8 @@ def orthogonalize(x: torch.Tensor, steps: int = 5, coefficients=NEWTON_SCHULZ_CO
         ws = _newton_schulz_ws(lib, d, x.device)
         _lib.check(lib.nc_orthogonalize(ctypes.byref(d), _ptr(x), _ptr(out), _ptr(ws), ws.numel(),
                                         _stream(x.device)), "nc_orthogonalize")
+        if d.batch:
+            _after_call(ws, "nc_orthogonalize")
     return out
 
 
@@ -726,3 +735,5 @@ def muon_(params: torch.Tensor, grads: torch.Tensor, momentum: torch.Tensor, lr:
         _lib.check(lib.nc_muon_update(ctypes.byref(d), _ptr(params), _ptr(grads), _ptr(momentum), float(lr),
                                       float(beta), int(nesterov), float(weight_decay), _ptr(ws), ws.numel(),
                                       _stream(params.device)), "nc_muon_update")
+        if d.batch:
+            _after_call(ws, "nc_muon_update")

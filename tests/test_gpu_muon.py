@@ -19,6 +19,15 @@ import torch
 from neurocell_b200 import _lib, ops
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _check_wait_status(monkeypatch, request):
+    """Every call's bounded waits are checked (not inside a capture, which cannot read them)."""
+    if "replayed" not in request.node.name and "captured" not in request.node.name:
+        monkeypatch.setattr(ops, "CHECK_WAIT_STATUS", True)
+
+
 DEV = torch.device("cuda:0")
 U = 2.0 ** -24
 COEFFS = ops.NEWTON_SCHULZ_COEFFICIENTS

@@ -23,6 +23,15 @@ import torch
 from neurocell_b200 import _lib, ops
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _check_wait_status(monkeypatch, request):
+    """Every call's bounded waits are checked (not inside a capture, which cannot read them)."""
+    if "replayed" not in request.node.name and "captured" not in request.node.name:
+        monkeypatch.setattr(ops, "CHECK_WAIT_STATUS", True)
+
+
 U = 2.0 ** -24
 DEV = torch.device("cuda:0")
 IGNORE = -100

@@ -10,6 +10,15 @@ from neurocell_b200 import ops
 from oracle import vnn_oracle as O
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _check_wait_status(monkeypatch, request):
+    """Every call's bounded waits are checked (not inside a capture, which cannot read them)."""
+    if "replayed" not in request.node.name and "captured" not in request.node.name:
+        monkeypatch.setattr(ops, "CHECK_WAIT_STATUS", True)
+
+
 DEV = torch.device("cuda:0")
 
 
