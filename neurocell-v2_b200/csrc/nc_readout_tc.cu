@@ -28,7 +28,7 @@ constexpr int kMaxBlocks = 296;        // blocks of the largest-value pass, per 
 constexpr float kDzScale = 32768.f;    // dz planes hold dz 2^15 (|dz| <= 1)
 constexpr int kChunk = 3;              // k-tiles (of 64) per accumulator beside float32 operands
 constexpr size_t kPieceBytes = 160u << 20;  // most that dz of one piece takes
-constexpr int kMaxSplits = 16;
+constexpr int kMaxSplits = 48;
 
 // Device scalars of a call.
 struct Scales {
@@ -55,7 +55,9 @@ struct Plan {
 // Pieces and splits by a count of k-tiles on the busiest SM (or pair): a product takes
 // ceil(tiles / SMs) times its k-tiles, so a piece is good where its tiles fill whole rounds.
 // 2048 x 512 x 32768 in float32: five pieces of 26 tiles of 256 classes, which fit L2, leave a
-// third of the pairs idle in dw and take 949 us; see DESIGN for what the choice here takes.
+// third of the pairs idle in dw and take 949 us; the choice here takes 759. Splits keep SMs busy
+// in df where it has few tiles: 333 x 128 x 10007 takes 79 us with them priced at the traffic of
+// their parts, 87 us at a flat 4 k-tiles each (which left df to 18 CTAs).
 void choose_pieces(const nc_linear_ce* d, int planes, Plan* p) {
   auto ceil_div = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
   const int sms = 148, bk = 64;
@@ -76,8 +78,9 @@ void choose_pieces(const nc_linear_ce* d, int planes, Plan* p) {
     const int64_t one = ceil_div(t * dz_tiles, dz_at) * ceil_div(d->dim, bk) + ceil_div(t * w_tiles, w_at) * ceil_div(d->rows, bk) +
                         3 * launch;
     for (int splits = 1; splits <= kMaxSplits && splits <= t; ++splits) {
-      // each split adds a pass over df's parts: about 4 k-tiles
-      const int64_t all = (one + ceil_div(f_tiles * splits, f_at) * ceil_div(t * (256 / bk), splits)) * ceil_div(tiles, t) + 4 * splits;
+      // a split's part of df is written and read once: about a k-tile for 250,000 elements
+      const int64_t all = (one + ceil_div(f_tiles * splits, f_at) * ceil_div(t * (256 / bk), splits)) * ceil_div(tiles, t) +
+                          splits * ((int64_t)d->rows * p->pitch / 250000 + 1) / 2;
       if (all < best) best = all, p->piece = (int)t * 256, p->splits = splits;
     }
   }
@@ -485,40 +488,44 @@ struct WeightEpilogue {
   const Scales* scales;
   T* out;          // of the piece's first class
   int classes, dim;
-  bool wide;       // rows on 32 bytes
+  bool wide;       // rows on 16 bytes
+  struct State {
+    float scale, g;
+    uint8_t* patch;
+  };
   template <int COLS>
-  __device__ __forceinline__ float2 begin(const tc::Tile&, int, int, uint8_t*) const {
-    return make_float2(scales->f_inv * (sizeof(T) == 4 ? 1.f / kDzScale : 1.f), scales->g);
+  __device__ __forceinline__ State begin(const tc::Tile&, int, int, uint8_t* patch) const {
+    return State{scales->f_inv * (sizeof(T) == 4 ? 1.f / kDzScale : 1.f), scales->g, patch};
   }
   template <int COLS>
-  __device__ __forceinline__ void run(float2 st, const tc::Tile&, int row, int col, float (&v)[COLS]) const {
-    if (row >= classes) return;
-    const float s = st.x, g = st.y;
-    T* o = out + (size_t)row * dim + col;
+  __device__ __forceinline__ void run(const State& st, const tc::Tile&, int row, int col, float (&v)[COLS]) const {
+    const int lane = threadIdx.x & 31, row0 = row - lane, rows = min(32, classes - row0);
+    if (rows <= 0) return;
+    constexpr int kGroup = sizeof(T) == 4 ? 32 : 64;   // columns in 128 bytes
 #pragma unroll
-    for (int j = 0; j < COLS; j += 16) {
+    for (int j = 0; j < COLS; j += kGroup) {
       if (col + j >= dim) break;
-      if (wide && col + j + 16 <= dim) {
-        uint32_t q[8];
+      const int cols = min(kGroup, dim - col - j);
+#pragma unroll
+      for (int e = 0; e < kGroup; ++e) v[j + e] *= st.scale * st.g;
+      if (wide) {
+        T* o = out + (size_t)row0 * dim + col + j;
         if constexpr (sizeof(T) == 4) {
-#pragma unroll
-          for (int e = 0; e < 16; e += 8) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) q[i] = __float_as_uint(v[j + e + i] * s * g);
-            tc::store_v8(o + j + e, q);
-          }
+          tc::patch_store_f32(st.patch, v + j, o, dim, rows, cols / 4, false);
         } else {
+          uint32_t q[32];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const __nv_bfloat162 b = __floats2bfloat162_rn(v[j + 2 * i] * s * g, v[j + 2 * i + 1] * s * g);
+          for (int i = 0; i < 32; ++i) {
+            const __nv_bfloat162 b = __floats2bfloat162_rn(v[j + 2 * i], v[j + 2 * i + 1]);
             q[i] = *reinterpret_cast<const uint32_t*>(&b);
           }
-          tc::store_v8(o + j, q);
+          tc::patch_store<64>(st.patch, q, reinterpret_cast<uint16_t*>(o), dim, rows, cols / 8);
         }
-      } else {
+      } else if (row < classes) {
+        T* o = out + (size_t)row * dim + col + j;
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (col + j + e < dim) store_as(o + j + e, v[j + e] * s * g);
+        for (int e = 0; e < kGroup; ++e)
+          if (e < cols) store_as(o + e, v[j + e]);
       }
     }
   }
@@ -527,26 +534,28 @@ struct WeightEpilogue {
 // df of a piece and split, added to that split's part (one CTA owns an element).
 struct FeatureEpilogue {
   const Scales* scales;
-  float* part;     // (splits, rows, pitch)
+  float* part;     // (splits, rows, pitch); the pitch is whole 8s
   int rows, dim, pitch, first;
   float mul;
+  struct State {
+    float scale;
+    uint8_t* patch;
+  };
   template <int COLS>
-  __device__ __forceinline__ float begin(const tc::Tile&, int, int, uint8_t*) const {
-    return scales->w_inv * mul;
+  __device__ __forceinline__ State begin(const tc::Tile&, int, int, uint8_t* patch) const {
+    return State{scales->w_inv * mul, patch};
   }
   template <int COLS>
-  __device__ __forceinline__ void run(float s, const tc::Tile& x, int row, int col, float (&v)[COLS]) const {
-    if (row >= rows) return;
-    float* o = part + ((size_t)x.split * rows + row) * pitch + col;
+  __device__ __forceinline__ void run(const State& st, const tc::Tile& x, int row, int col, float (&v)[COLS]) const {
+    const int lane = threadIdx.x & 31, row0 = row - lane, count = min(32, rows - row0);
+    if (count <= 0) return;
+    float* o = part + ((size_t)x.split * rows + row0) * pitch + col;
 #pragma unroll
-    for (int j = 0; j < COLS; j += 8) {
-      if (col + j >= dim) break;   // the pitch is whole 8s
-      uint32_t q[8];
-      if (!first) tc::load_v8(o + j, q);
+    for (int j = 0; j < COLS; j += 32) {
+      if (col + j >= pitch) break;
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        q[i] = __float_as_uint(v[j + i] * s + (first ? 0.f : __uint_as_float(q[i])));
-      tc::store_v8(o + j, q);
+      for (int e = 0; e < 32; ++e) v[j + e] *= st.scale;
+      tc::patch_store_f32(st.patch, v + j, o + j, pitch, count, min(8, (pitch - col - j) / 4), !first);
     }
   }
 };
@@ -560,6 +569,7 @@ __global__ void __launch_bounds__(256) ce_features_kernel(const float* __restric
   if (i >= (int64_t)rows * dim) return;
   const int row = (int)(i / dim), c = (int)(i - (int64_t)row * dim);
   float s = 0.f;
+#pragma unroll 8
   for (int k = 0; k < splits; ++k) s += part[((size_t)k * rows + row) * pitch + c];
   store_as(out + i, s * scales->g);
 }
@@ -681,7 +691,7 @@ struct Call {
     NC_CHECK((dz_op<BN, CG, EW>(&q, true)));
     NC_CHECK((features_op<BN, CG, EW>(&q, false, true)));
     T* out = static_cast<T*>(g.weight) + (size_t)v0 * d->dim;
-    const bool wide = reinterpret_cast<uintptr_t>(out) % 32 == 0 && (size_t)d->dim * sizeof(T) % 32 == 0;
+    const bool wide = reinterpret_cast<uintptr_t>(out) % 16 == 0 && (size_t)d->dim * sizeof(T) % 16 == 0;
     const WeightEpilogue<T> e{scales(), out, classes, d->dim, wide};
     return tc::launch_product<PL, BN, CG, EW>(q, e, st, "readout weight gradient launch");
   }

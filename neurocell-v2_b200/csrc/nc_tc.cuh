@@ -302,17 +302,31 @@ __device__ __forceinline__ void patch_store(uint8_t* patch, const uint32_t* v, u
   }
 }
 
-// 32-byte global accesses (one full sector per thread).
-__device__ __forceinline__ void store_v8(void* p, const uint32_t (&v)[8]) {
-  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
-               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
-               : "memory");
-}
-__device__ __forceinline__ void load_v8(const void* p, uint32_t (&v)[8]) {
-  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
-               : "l"(p)
-               : "memory");
+// The same for rows of 32 float32 values (a patch of 128-byte rows), stored or added to what is
+// there; the first 4 * pieces of each.
+__device__ __forceinline__ void patch_store_f32(uint8_t* patch, const float* v, float* p, int64_t pitch, int rows,
+                                                int pieces, bool add) {
+  const int lane = threadIdx.x & 31, q = lane & 7;
+  float4 old[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = i * 4 + (lane >> 3);
+    old[i] = add && r < rows && q < pieces ? *reinterpret_cast<const float4*>(p + r * pitch + 4 * q)
+                                           : make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    *reinterpret_cast<float4*>(patch_at<64>(patch, lane, i)) = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = i * 4 + (lane >> 3);
+    const float4 x = *reinterpret_cast<const float4*>(patch_at<64>(patch, r, q));
+    if (r < rows && q < pieces)
+      *reinterpret_cast<float4*>(p + r * pitch + 4 * q) =
+          make_float4(old[i].x + x.x, old[i].y + x.y, old[i].z + x.z, old[i].w + x.w);
+  }
 }
 
 // What a CTA's warps share beside the stages.
