@@ -273,7 +273,10 @@ typedef enum nc_reduction { NC_REDUCE_MEAN = 0, NC_REDUCE_SUM = 1, NC_REDUCE_NON
  * has one with a logit of NaN or +inf.  Sums and statistics are held in float32.
  * Precision with float32 operands and more than 16 rows: as of float32 products, where the
  * entries of a tensor below 2^-18 of its largest finite one count with an absolute error of
- * 2^-38 of that one, and dz = p - onehot with one of at most 2^-40 of the largest |g_loss|.
+ * 2^-38 of that one, and dz = p - onehot with one of at most 2^-40 of the largest |g_loss|
+ * (gradients are computed relative to that one: an infinite g_loss makes them all NaN).
+ * What a call writes (loss, lse, gradients, workspace) overlaps nothing else of it.
+ * Sizes up to 2^24 rows, classes and dim, 2^44 logits, 2^38 elements of features or weight.
  */
 typedef struct nc_linear_ce {
   int32_t rows, dim, classes;   /* rows may be 0: the loss and the weight's gradients are 0 */
@@ -301,6 +304,13 @@ nc_status nc_linear_ce_backward(const nc_linear_ce* desc, const void* features, 
                                 const float* g_loss, void* g_features, void* g_weight, void* g_bias,
                                 void* d_ws, size_t ws_bytes, void* stream);
 
+/* Both in one call, on a workspace of nc_linear_ce_workspace_bytes(desc, 1): what the two
+   share is computed once.  lse (rows) is scratch. */
+nc_status nc_linear_ce_value_and_grad(const nc_linear_ce* desc, const void* features, const void* weight,
+                                      const void* bias, const int32_t* labels, float* loss, float* lse,
+                                      void* g_features, void* g_weight, void* g_bias, void* d_ws,
+                                      size_t ws_bytes, void* stream);
+
 /*
  * Batch staging without the copy engine (no counterpart in the reference): copies `nseg`
  * (1..NC_MAX_STAGE_SEGS) byte ranges into device buffers with one kernel that reads the
@@ -323,19 +333,16 @@ nc_status nc_stage_from_host(const nc_stage_seg* segs, int32_t nseg, void* strea
 /* In-place SGD: params[i] -= lr * grads[i]  (lr read from host scalar). */
 nc_status nc_sgd_update(float* params, const float* grads, int64_t n, float lr, void* stream);
 
-/* Both in one call, on a workspace of nc_linear_ce_workspace_bytes(desc, 1): what the two
-   share is computed once.  lse (rows) is scratch. */
-nc_status nc_linear_ce_value_and_grad(const nc_linear_ce* desc, const void* features, const void* weight,
-                                      const void* bias, const int32_t* labels, float* loss, float* lse,
-                                      void* g_features, void* g_weight, void* g_bias, void* d_ws,
-                                      size_t ws_bytes, void* stream);
-
 /*
  * Newton-Schulz orthogonalisation of `batch` matrices (rows, cols), row-major and packed:
  * X0 = x / (|x|_F + eps), then `steps` times A = X X^T, X <- a X + (b A + c A^2) X (A = X^T X
  * and X <- a X + X (b A + c A^2) when rows > cols).  Each singular value goes through the
- * polynomial a s + b s^3 + c s^5; the singular vectors stay.  A zero matrix stays zero; a
- * matrix that holds NaN or an infinity gives NaN in that matrix.
+ * polynomial a s + b s^3 + c s^5; the singular vectors stay.  A zero matrix stays zero (with
+ * an eps of 0 it gives NaN); a matrix that holds NaN or an infinity gives NaN in that matrix.
+ * Entries of X, A and b A + c A^2 stay below 16 in magnitude with coefficients that orthogonalise;
+ * others may take them past it, and a matrix whose short side is over 64 (or whose long side
+ * is too long for shared memory) then gives NaN or infinities.  Up to 65535 matrices of up
+ * to 2^30 elements.
  */
 typedef struct nc_newton_schulz {
   int32_t batch, rows, cols;   /* batch may be 0                      */
@@ -347,7 +354,7 @@ typedef struct nc_newton_schulz {
 
 size_t nc_newton_schulz_workspace_bytes(const nc_newton_schulz* desc);
 
-/* out = the orthogonalised x; out may be x itself. */
+/* out = the orthogonalised x; out is x itself or apart from it. */
 nc_status nc_orthogonalize(const nc_newton_schulz* desc, const void* x, void* out, void* d_ws,
                            size_t ws_bytes, void* stream);
 
@@ -355,7 +362,7 @@ nc_status nc_orthogonalize(const nc_newton_schulz* desc, const void* x, void* ou
  * In-place update of `batch` float32 parameter matrices by orthogonalised momentum:
  *   momentum <- beta momentum + grads;  u = grads + beta momentum (nesterov) or momentum
  *   params <- (1 - lr weight_decay) params - lr sqrt(max(1, rows / cols)) orthogonalised(u)
- * params, grads and momentum are different buffers.
+ * params, grads and momentum do not overlap.
  */
 nc_status nc_muon_update(const nc_newton_schulz* desc, float* params, const float* grads,
                          float* momentum, float lr, float beta, int32_t nesterov,

@@ -1,6 +1,8 @@
 // nc_errors.h -- thread-local error reporting for the C ABI.
 #pragma once
 
+#include <cstdint>
+
 #include <cuda_runtime.h>
 
 #include "neurocell_b200.h"
@@ -21,6 +23,12 @@ nc_status launch_check(const char* what);
 nc_status check_ptr(const void* p, const char* name);
 // The device address of `p`; memory that the device cannot access is refused.
 nc_status device_address(const void* p, const char* name, const void** dev);
+
+// Whether two buffers share a byte.
+inline bool overlap(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return a && b && x < y + b_bytes && y < x + a_bytes;
+}
 
 // Launch configuration with programmatic dependent launch: the grid may be scheduled
 // before the kernel it follows on the stream has finished, once every CTA of that kernel

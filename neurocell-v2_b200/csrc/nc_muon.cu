@@ -348,6 +348,7 @@ struct NsArgs {
   MuonArgs mu;
   float decay, step;
   int32_t* status;
+  int first;            // of the call's launches: clears the status
 };
 
 // The transposed store of 32 rows (a lane each) and 32 columns: through the warp's patch, as 32
@@ -529,7 +530,7 @@ __global__ void __launch_bounds__(NsEngine<CLUSTER>::C::kThreads, 1) ns_kernel(c
   __shared__ tc::Shared<2, kBN, 1, kWarps> sh;
   __shared__ double red[kThreads / 32];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  if (blockIdx.x == 0 && tid == 0) *p.status = 0;
+  if (p.first && blockIdx.x == 0 && tid == 0) *p.status = 0;
   E e(raw, &sh, p.status);
   // The CTAs that work together: the whole grid on all matrices, or a cluster on one.
   const int size = CLUSTER ? kCluster : gridDim.x, rank = CLUSTER ? (int)tc::cluster_rank() : blockIdx.x;
@@ -735,9 +736,15 @@ int choose_splits(int64_t tiles, int k, int at_once) {
   return splits;
 }
 
+// Matrices that clusters take in one launch. More go by several launches on the same workspace,
+// which has planes (and parts of split products) for a launch's matrices: eight rounds of the 18
+// clusters that run at a time. 64000 x 65 x 520 would need 266 GiB at once.
+constexpr int kLaunchMatrices = 144;
+
 struct NsLayout {
   size_t status, norms, x, y, gram, poly, parts, total;
   bool cluster;
+  int batch;   // matrices of a launch
   int splits[3], blocks;
   int64_t parts_each;
 };
@@ -761,6 +768,7 @@ NsLayout ns_layout(const nc_newton_schulz* d) {
   // where the matrices fill the SMs
   const auto tiles_of = [](int64_t m, int64_t n, int wide) { return ((m + 127) / 128) * ((n + wide - 1) / wide); };
   L.cluster = tiles_of(d->rows, d->cols, 64) <= kCluster || (int64_t)d->batch * kCluster >= 2 * 148;
+  L.batch = L.cluster && d->batch > kLaunchMatrices ? kLaunchMatrices : d->batch;
   tc::Problem q{};
   q.m = q.n = (int)s, q.batch = L.cluster ? 1 : d->batch, q.splits = 1, q.symmetric = 1;
   if (L.cluster)
@@ -783,13 +791,13 @@ NsLayout ns_layout(const nc_newton_schulz* d) {
   // as many CTAs as any product keeps busy, or as share the element-wise passes well
   int64_t blocks = (int64_t)(d->batch * n / 4096);
   if (most > blocks) blocks = most;
-  L.blocks = L.cluster ? kCluster * d->batch : (int)(blocks < 148 ? blocks : 148);
-  L.norms = take((size_t)d->batch * L.blocks * 8);
-  L.x = take(d->batch * x * 4);
-  L.y = take(d->batch * x * 4);
-  L.gram = take(d->batch * g * 4);
-  L.poly = take(d->batch * g * 4);
-  L.parts = take((size_t)L.parts_each * (L.cluster ? d->batch : 1) * 16);
+  L.blocks = L.cluster ? kCluster * L.batch : (int)(blocks < 148 ? blocks : 148);
+  L.norms = take((size_t)L.batch * (L.cluster ? kCluster : L.blocks) * 8);
+  L.x = take(L.batch * x * 4);
+  L.y = take(L.batch * x * 4);
+  L.gram = take(L.batch * g * 4);
+  L.poly = take(L.batch * g * 4);
+  L.parts = take((size_t)L.parts_each * (L.cluster ? L.batch : 1) * 16);
   L.total = at;
   return L;
 }
@@ -801,8 +809,8 @@ nc_status check_desc(const nc_newton_schulz* d) {
   if (d->dtype != NC_F32 && d->dtype != NC_BF16) return set_error(NC_ERR_INVALID, "unknown dtype %d", d->dtype);
   if (d->steps < 0 || d->steps > 64) return set_error(NC_ERR_INVALID, "steps %d is not in 0..64", d->steps);
   if (!(d->eps >= 0.f)) return set_error(NC_ERR_INVALID, "eps is negative or NaN");
-  if (d->batch > 65535 || (int64_t)d->rows * d->cols > INT32_MAX)
-    return set_error(NC_ERR_UNSUPPORTED, "more than 65535 matrices, or more than 2^31 - 1 elements in one");
+  if (d->batch > 65535 || (int64_t)d->rows * d->cols > 1 << 30)
+    return set_error(NC_ERR_UNSUPPORTED, "more than 65535 matrices, or more than 2^30 elements in one");
   return NC_OK;
 }
 
@@ -829,7 +837,7 @@ nc_status run_tensor(const nc_newton_schulz* d, const T* x, float* momentum, Muo
   // k (boxes of 64 by 64)
   const int a_rows = 128, b_rows = L.cluster ? 64 : 128;
   auto map = [&](CUtensorMap* m, const Planes& q, int rows, int cols, int box) {
-    return tc::make_map(m, q.p, false, 2, cols, rows, q.pitch, q.plane, d->batch, 2 * q.plane, 64, box);
+    return tc::make_map(m, q.p, false, 2, cols, rows, q.pitch, q.plane, L.batch, 2 * q.plane, 64, box);
   };
   for (int i = 0; i < 2; ++i) {
     NC_CHECK(map(&a.k_a[i], a.X[i], d->rows, d->cols, a_rows));
@@ -841,10 +849,9 @@ nc_status run_tensor(const nc_newton_schulz* d, const T* x, float* momentum, Muo
   NC_CHECK(map(&a.gram_b, a.G, s, s, b_rows));
   NC_CHECK(map(&a.poly_a, a.Q, s, s, a_rows));
   NC_CHECK(map(&a.poly_b, a.Q, s, s, b_rows));
-  a.x = x, a.momentum = momentum, a.params = params, a.out = out;
   a.norms = reinterpret_cast<double*>(ws + L.norms), a.parts = reinterpret_cast<float4*>(ws + L.parts);
   a.parts_each = L.parts_each;
-  a.batch = d->batch, a.rows = d->rows, a.cols = d->cols, a.steps = d->steps;
+  a.rows = d->rows, a.cols = d->cols, a.steps = d->steps;
   for (int f = 0; f < 3; ++f) a.splits[f] = L.splits[f];
   a.vec = d->cols % 4 == 0 && (reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(momentum)) % 16 == 0;
   a.a = d->a, a.b = d->b, a.c = d->c, a.eps = d->eps, a.mu = mu, a.decay = decay, a.step = step;
@@ -861,11 +868,19 @@ nc_status run_tensor(const nc_newton_schulz* d, const T* x, float* momentum, Muo
     attr[0].id = cudaLaunchAttributeCooperative;
     attr[0].val.cooperative = 1;
   }
-  cfg.gridDim = dim3((unsigned)L.blocks);
   cfg.blockDim = dim3(L.cluster ? NsEngine<true>::C::kThreads : NsEngine<false>::C::kThreads);
   cfg.dynamicSmemBytes = smem, cfg.stream = st, cfg.attrs = attr, cfg.numAttrs = 1;
-  NC_CUDA_CHECK(cudaLaunchKernelEx(&cfg, k, a));
-  return launch_check("ns_kernel launch");
+  const size_t n = (size_t)d->rows * d->cols;
+  for (int b = 0; b < d->batch; b += L.batch) {
+    a.batch = d->batch - b < L.batch ? d->batch - b : L.batch;
+    a.x = x + b * n, a.momentum = momentum ? momentum + b * n : nullptr;
+    a.params = params ? params + b * n : nullptr, a.out = out ? out + b * n : nullptr;
+    a.first = b == 0;
+    cfg.gridDim = dim3((unsigned)(L.cluster ? kCluster * a.batch : L.blocks));
+    NC_CUDA_CHECK(cudaLaunchKernelEx(&cfg, k, a));
+    NC_CHECK(launch_check("ns_kernel launch"));
+  }
+  return NC_OK;
 }
 
 // From the source x (or x and momentum) to the orthogonalised matrix; `out` or `params`.
@@ -911,6 +926,10 @@ nc_status nc_orthogonalize(const nc_newton_schulz* desc, const void* x, void* ou
   if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(out)) % (bf16 ? 2 : 4) != 0)
     return set_error(NC_ERR_INVALID, "x or out is not on an element's boundary");
   NC_CHECK(check_ws(d_ws, ws_bytes, ns_layout(desc).total));
+  const size_t bytes = (size_t)desc->batch * desc->rows * desc->cols * (bf16 ? 2 : 4);
+  if ((x != out && overlap(x, bytes, out, bytes)) || overlap(x, bytes, d_ws, ws_bytes) ||
+      overlap(out, bytes, d_ws, ws_bytes))
+    return set_error(NC_ERR_INVALID, "x, out and the workspace overlap (out may only be x itself)");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const MuonArgs mu{};
   if (bf16)
@@ -934,9 +953,14 @@ nc_status nc_muon_update(const nc_newton_schulz* desc, float* params, const floa
   NC_CHECK(check_ptr(params, "params"));
   NC_CHECK(check_ptr(grads, "grads"));
   NC_CHECK(check_ptr(momentum, "momentum"));
-  if (params == momentum || params == grads || momentum == grads)
+  const size_t bytes = (size_t)desc->batch * desc->rows * desc->cols * 4;
+  if (overlap(params, bytes, momentum, bytes) || overlap(params, bytes, grads, bytes) ||
+      overlap(momentum, bytes, grads, bytes))
     return set_error(NC_ERR_INVALID, "params, grads and momentum must be different buffers");
   NC_CHECK(check_ws(d_ws, ws_bytes, ns_layout(desc).total));
+  if (overlap(params, bytes, d_ws, ws_bytes) || overlap(momentum, bytes, d_ws, ws_bytes) ||
+      overlap(grads, bytes, d_ws, ws_bytes))
+    return set_error(NC_ERR_INVALID, "the workspace overlaps params, grads or momentum");
   const MuonArgs mu{beta, nesterov};
   const double tall = (double)desc->rows / desc->cols;
   const float step = (float)((double)lr * sqrt(tall > 1.0 ? tall : 1.0));

@@ -14,6 +14,8 @@
 // nc_readout_tc.cu.
 #include <math.h>
 
+#include <initializer_list>
+
 #include "nc_common.cuh"
 #include "nc_errors.h"
 #include "nc_readout.h"
@@ -488,6 +490,11 @@ nc_status check_desc(const nc_linear_ce* d) {
     return set_error(NC_ERR_INVALID, "unknown reduction %d", d->reduction);
   if (d->ignore_index >= 0 && d->ignore_index < d->classes)
     return set_error(NC_ERR_INVALID, "ignore_index %d is one of the %d classes", d->ignore_index, d->classes);
+  // what tile counts, block counts (int) and the tensor maps' strides (40 bits) hold
+  const int64_t side = 1 << 24, rows = d->rows, dim = d->dim, classes = d->classes;
+  if (rows > side || dim > side || classes > side || rows * classes > (int64_t)1 << 44 ||
+      rows * dim > (int64_t)1 << 38 || classes * dim > (int64_t)1 << 38)
+    return set_error(NC_ERR_UNSUPPORTED, "readout too large (rows %d, dim %d, classes %d)", d->rows, d->dim, d->classes);
   return NC_OK;
 }
 
@@ -635,6 +642,37 @@ nc_status check_grads(const nc_linear_ce* d, const void* g_features, const void*
   return NC_OK;
 }
 
+// A buffer of a call.
+struct Span {
+  const void* p;
+  size_t bytes;
+  const char* name;
+};
+
+// Refuses what is written where something else of the call lies: the pieces of the gradient
+// products read their inputs while earlier pieces' results are stored.
+nc_status check_apart(std::initializer_list<Span> written, std::initializer_list<Span> read) {
+  for (const Span* x = written.begin(); x != written.end(); ++x) {
+    for (const Span* y = x + 1; y != written.end(); ++y)
+      if (overlap(x->p, x->bytes, y->p, y->bytes))
+        return set_error(NC_ERR_INVALID, "%s and %s overlap", x->name, y->name);
+    for (const Span& y : read)
+      if (overlap(x->p, x->bytes, y.p, y.bytes))
+        return set_error(NC_ERR_INVALID, "%s and %s overlap", x->name, y.name);
+  }
+  return NC_OK;
+}
+
+// Bytes of the call's buffers.
+struct Sizes {
+  size_t features, weight, bias, rows, loss;
+  explicit Sizes(const nc_linear_ce* d) {
+    const size_t size = d->dtype == NC_BF16 ? 2 : 4;
+    features = size * d->rows * d->dim, weight = size * d->classes * d->dim, bias = size * d->classes;
+    rows = (size_t)d->rows * 4, loss = d->reduction == NC_REDUCE_NONE ? rows : 4;
+  }
+};
+
 // No rows: a loss of 0 and gradients of 0.
 nc_status no_rows(const nc_linear_ce* d, float* loss, void* g_weight, void* g_bias, cudaStream_t st) {
   const size_t size = d->dtype == NC_BF16 ? 2 : 4;
@@ -667,6 +705,10 @@ nc_status nc_linear_ce_forward(const nc_linear_ce* desc, const void* features, c
   if (desc->rows == 0) return no_rows(desc, loss, nullptr, nullptr, st);
   NC_CHECK(check_inputs(desc, features, weight, bias, labels, lse));
   NC_CHECK(check_ws(d_ws, ws_bytes, ce_layout(desc, false).total));
+  const Sizes n(desc);
+  NC_CHECK(check_apart({{loss, n.loss, "loss"}, {lse, n.rows, "lse"}, {d_ws, ws_bytes, "the workspace"}},
+                       {{features, n.features, "features"}, {weight, n.weight, "weight"}, {bias, n.bias, "bias"},
+                        {labels, n.rows, "labels"}}));
   char* ws = static_cast<char*>(d_ws);
   const CeArgs a = make_args(desc, features, weight, bias, labels, ws);
   NC_CHECK(prepare(desc, a, false, nullptr, ws, st));
@@ -686,6 +728,11 @@ nc_status nc_linear_ce_backward(const nc_linear_ce* desc, const void* features, 
   NC_CHECK(check_inputs(desc, features, weight, bias, labels, lse));
   if (g_loss) NC_CHECK(check_ptr(g_loss, "g_loss"));
   NC_CHECK(check_ws(d_ws, ws_bytes, ce_layout(desc, true).total));
+  const Sizes n(desc);
+  NC_CHECK(check_apart({{g_features, n.features, "g_features"}, {g_weight, n.weight, "g_weight"},
+                        {g_bias, n.bias, "g_bias"}, {d_ws, ws_bytes, "the workspace"}},
+                       {{features, n.features, "features"}, {weight, n.weight, "weight"}, {bias, n.bias, "bias"},
+                        {labels, n.rows, "labels"}, {lse, n.rows, "lse"}, {g_loss, n.loss, "g_loss"}}));
   char* ws = static_cast<char*>(d_ws);
   const CeArgs a = make_args(desc, features, weight, bias, labels, ws);
   NC_CHECK(prepare(desc, a, true, g_loss, ws, st));
@@ -706,6 +753,12 @@ nc_status nc_linear_ce_value_and_grad(const nc_linear_ce* desc, const void* feat
   if (desc->rows == 0) return no_rows(desc, loss, g_weight, g_bias, st);
   NC_CHECK(check_inputs(desc, features, weight, bias, labels, lse));
   NC_CHECK(check_ws(d_ws, ws_bytes, ce_layout(desc, true).total));
+  const Sizes n(desc);
+  NC_CHECK(check_apart({{loss, n.loss, "loss"}, {lse, n.rows, "lse"}, {g_features, n.features, "g_features"},
+                        {g_weight, n.weight, "g_weight"}, {g_bias, n.bias, "g_bias"},
+                        {d_ws, ws_bytes, "the workspace"}},
+                       {{features, n.features, "features"}, {weight, n.weight, "weight"}, {bias, n.bias, "bias"},
+                        {labels, n.rows, "labels"}}));
   char* ws = static_cast<char*>(d_ws);
   const CeArgs a = make_args(desc, features, weight, bias, labels, ws);
   NC_CHECK(prepare(desc, a, true, nullptr, ws, st));

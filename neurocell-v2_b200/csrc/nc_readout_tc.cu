@@ -226,8 +226,10 @@ __device__ void row_factors(const CeArgs& a, const float* g_loss, float* fac, Sc
     __syncthreads();
     for (int i = 0; i < kPrepThreads / 32; ++i) m = fmaxf(m, red[i]);
   }
-  for (int i = threadIdx.x; i < a.rows; i += kPrepThreads)
-    fac[i] = !ce_kept(a, i) || m == 0.f ? 0.f : (each ? g_loss[i] : all) / m;
+  for (int i = threadIdx.x; i < a.rows; i += kPrepThreads) {
+    const float g = each ? g_loss[i] : all;
+    fac[i] = !ce_kept(a, i) ? 0.f : m > 0.f ? g / m : g;   // else g is 0 or NaN
+  }
   if (threadIdx.x == 0) scales->g = m;
 }
 

@@ -512,6 +512,11 @@ def _dtype_name(t: torch.Tensor) -> str:
     return str(t.dtype).replace("torch.", "")
 
 
+def _fits_int32(*sizes: int) -> None:
+    if max(sizes) > 2 ** 31 - 1:
+        raise ValueError(f"sizes {sizes} do not fit 32 bits")
+
+
 class _on:
     """Makes ``device`` current for the calls inside (launches go to the current device)."""
 
@@ -554,6 +559,9 @@ def _linear_ce_args(features, weight, labels, bias, ignore_index, reduction):
     for t, n in ((weight, "weight"), (bias, "bias"), (labels, "labels")):
         if t is not None and t.device != features.device:
             raise ValueError(f"{n} is on {t.device}, features are on {features.device}")
+    _fits_int32(features.shape[0], features.shape[1], weight.shape[0])
+    if not -2 ** 31 < int(ignore_index) < 2 ** 31 - 1:     # the ends stand for int64 labels beyond int32
+        raise ValueError(f"ignore_index {ignore_index} does not fit 32 bits")
     d = _lib.NcLinearCe(features.shape[0], features.shape[1], weight.shape[0],
                         _lib.NC_DTYPE[_dtype_name(features)], int(ignore_index),
                         _lib.NC_REDUCE[reduction])
@@ -639,7 +647,11 @@ def linear_softmax_ce_loss(features: torch.Tensor, weight: torch.Tensor, labels:
     type, float32 or bfloat16; the loss is float32.  ``reduction``: "mean" over the rows
     whose label is not ``ignore_index`` (0 when there are none), "sum", or "none" (one loss
     per row).  Any other label outside the classes gives NaN.  Differentiable once in
-    features, weight and bias (the gradient computes the logits a second time)."""
+    features, weight and bias (the gradient computes the logits a second time).
+
+    Inside a CUDA graph capture use :func:`linear_softmax_ce_value_and_grad`, which needs no
+    autograd: a captured backward pass whose leaves still belong to a live graph built outside
+    the capture can end the process."""
     return _LinearCE.apply(features, weight, bias, labels, ignore_index, reduction)
 
 
@@ -682,6 +694,7 @@ def _newton_schulz_desc(shape, dtype: str, steps, coefficients, eps) -> _lib.NcN
         raise ValueError(f"float32 or bfloat16 expected, got {dtype}")
     a, b, c = coefficients
     batch = math.prod(shape[:-2])
+    _fits_int32(batch, shape[-2], shape[-1], abs(int(steps)))
     return _lib.NcNewtonSchulz(batch, shape[-2], shape[-1], _lib.NC_DTYPE[dtype], int(steps), float(a),
                                float(b), float(c), float(eps))
 
@@ -698,7 +711,10 @@ def orthogonalize(x: torch.Tensor, steps: int = 5, coefficients=NEWTON_SCHULZ_CO
     """Newton-Schulz orthogonalisation of the matrices of ``x`` (..., rows, cols), float32 or
     bfloat16: ``x / (|x| + eps)``, then ``steps`` times ``X <- a X + (b A + c A^2) X`` with
     the Gram matrix ``A`` of the short side.  Returns a new tensor of ``x``'s type; products
-    and sums are as exact as float32 ones for either type.  Not differentiable."""
+    and sums are as exact as float32 ones for either type.  Not differentiable.
+
+    Coefficients far from orthogonalising ones, under which entries of an iterate or its Gram
+    products reach 16, give NaN where the short side is over 64."""
     _require_cuda(x, "x")
     lib = _lib.load()
     d = _newton_schulz_desc(x.shape, _dtype_name(x), steps, coefficients, eps)
@@ -719,7 +735,8 @@ def muon_(params: torch.Tensor, grads: torch.Tensor, momentum: torch.Tensor, lr:
     """In-place update of the float32 matrices ``params`` (..., rows, cols) by orthogonalised
     momentum, on the current stream: ``momentum = beta momentum + grads``, then
     ``params = (1 - lr weight_decay) params - lr sqrt(max(1, rows / cols)) O`` with O the
-    orthogonalised ``grads + beta momentum`` (``nesterov``) or ``momentum``."""
+    orthogonalised ``grads + beta momentum`` (``nesterov``) or ``momentum``.  Autograd sees
+    ``params`` and ``momentum`` as changed in place."""
     for t, n in ((params, "params"), (grads, "grads"), (momentum, "momentum")):
         _require_cuda(t, n)
         if t.dtype != torch.float32:
@@ -737,3 +754,4 @@ def muon_(params: torch.Tensor, grads: torch.Tensor, momentum: torch.Tensor, lr:
                                       _stream(params.device)), "nc_muon_update")
         if d.batch:
             _after_call(ws, "nc_muon_update")
+    torch.autograd.graph.increment_version([t for t in (params, momentum) if not t.is_inference()])

@@ -24,7 +24,7 @@ pytestmark = pytest.mark.gpu
 @pytest.fixture(autouse=True)
 def _check_wait_status(monkeypatch, request):
     """Every call's bounded waits are checked (not inside a capture, which cannot read them)."""
-    if "replayed" not in request.node.name and "captured" not in request.node.name:
+    if not any(k in request.node.name for k in ("replayed", "captured", "at_once")):
         monkeypatch.setattr(ops, "CHECK_WAIT_STATUS", True)
 
 
@@ -222,3 +222,67 @@ def test_refusals():
     ws = torch.empty(n, dtype=torch.uint8, device=DEV)
     assert lib.nc_orthogonalize(ctypes.byref(d), ops._ptr(x), ops._ptr(x), ops._ptr(ws), n - 1,
                                 None) == _lib.NC_ERR_WORKSPACE
+
+
+def test_calls_at_once_on_several_streams():
+    xs = [_matrices(140, 260, seed=21), _matrices(3, 62, 62, seed=22), _matrices(700, 300, seed=23),
+          _matrices(40, 70, 96, seed=24), _matrices(32, 2000, seed=25)]
+    want = [ops.orthogonalize(x) for x in xs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in xs]
+    got = []
+    for _ in range(5):
+        for s, x in zip(streams, xs):
+            with torch.cuda.stream(s):
+                got.append(ops.orthogonalize(x))
+    torch.cuda.synchronize()
+    for i, y in enumerate(got):
+        assert torch.equal(y, want[i % len(xs)]), i
+
+
+@pytest.mark.parametrize("batch,rows,cols,dtype", [(36_000, 62, 1000, torch.bfloat16), (64_000, 65, 520, torch.float32)])
+def test_offsets_past_32_bits(batch, rows, cols, dtype):
+    gen = torch.Generator(device=DEV).manual_seed(31)
+    x = torch.empty(batch, rows, cols, dtype=dtype, device=DEV).normal_(generator=gen)
+    got = ops.orthogonalize(x)
+    torch.cuda.synchronize()
+    for k in (0, batch // 2, batch - 1):
+        want, tol = _formula(x[k])
+        if dtype == torch.bfloat16:
+            tol = tol + 2.0 ** -8 * torch.linalg.matrix_norm(want)
+        assert torch.linalg.matrix_norm(got[k].double() - want) <= tol, k
+
+
+def test_a_batch_of_several_launches():
+    p, g, m = (_matrices(311, 70, 96, seed=k) for k in (35, 36, 37))
+    p2, m2 = p.clone(), m.clone()
+    ops.muon_(p, g, m, 0.1)
+    for k in range(0, 311, 100):      # as many as one launch takes
+        part = slice(k, min(311, k + 100))
+        ops.muon_(p2[part], g[part], m2[part], 0.1)
+    torch.cuda.synchronize()
+    assert torch.equal(p, p2) and torch.equal(m, m2)
+
+
+def test_autograd_sees_the_update():
+    p = _matrices(6, 8).requires_grad_()
+    m = torch.zeros_like(p)
+    y = (p * p).sum()
+    with torch.no_grad():
+        ops.muon_(p, torch.ones_like(p), m, 0.1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
+@pytest.mark.parametrize("shape", [(24, 40), (130, 200)])
+def test_no_eps(shape):
+    x = _matrices(2, *shape, seed=33)
+    _check(x, eps=0.0)
+    x[1] = 0
+    got = ops.orthogonalize(x, eps=0.0)
+    assert torch.isfinite(got[0]).all() and got[1].isnan().all()
+
+
+def test_coefficients_that_diverge_show():
+    got = ops.orthogonalize(_matrices(130, 200, seed=34), coefficients=(40.0, 0.0, 0.0))
+    assert not torch.isfinite(got).all()

@@ -28,7 +28,7 @@ pytestmark = pytest.mark.gpu
 @pytest.fixture(autouse=True)
 def _check_wait_status(monkeypatch, request):
     """Every call's bounded waits are checked (not inside a capture, which cannot read them)."""
-    if "replayed" not in request.node.name and "captured" not in request.node.name:
+    if not any(k in request.node.name for k in ("replayed", "captured", "at_once")):
         monkeypatch.setattr(ops, "CHECK_WAIT_STATUS", True)
 
 
@@ -322,3 +322,121 @@ def test_c_entry_points_refuse_bad_workspaces():
     assert lib.nc_linear_ce_forward(*args, None, n, None) == _lib.NC_ERR_WORKSPACE
     assert lib.nc_linear_ce_forward(ctypes.byref(d), None, P(w), P(b), P(lab), P(loss), P(lse), P(ws), n,
                                     None) == _lib.NC_ERR_INVALID
+
+
+def _past_32_bits(rows, dim, classes, dtype):
+    """A weight of more than 2^31 elements: the formula by pieces of the classes."""
+    gen = torch.Generator(device=DEV).manual_seed(41)
+    w = torch.empty(classes, dim, dtype=dtype, device=DEV).normal_(generator=gen).mul_(2.0 / dim ** 0.5)
+    f = torch.randn(rows, dim, device=DEV, generator=gen).to(dtype)
+    lab = torch.randint(0, classes, (rows,), device=DEV, generator=gen)
+    lab[0], lab[1] = classes - 1, 0
+    loss, g_f, g_w, _ = ops.linear_softmax_ce_value_and_grad(f, w, lab)
+    torch.cuda.synchronize()
+    step, fd = 100_000, f.double()
+    pieces = [(k, min(classes, k + step)) for k in range(0, classes, step)]
+    lse = torch.full((rows,), -float("inf"), dtype=torch.float64, device=DEV)
+    mag, at = torch.zeros_like(lse), torch.zeros_like(lse)
+    for a, b in pieces:
+        y = w[a:b].double()
+        z = fd @ y.T
+        lse = torch.logaddexp(lse, torch.logsumexp(z, 1))
+        mag = torch.maximum(mag, (fd.abs() @ y.abs().T).amax(1))
+        here = (lab >= a) & (lab < b)
+        at = torch.where(here, z.gather(1, (lab - a).clamp(0, b - a - 1)[:, None])[:, 0], at)
+    ez = ((dim + 4) * U + 2.0 ** -21) * mag
+    # the statistics join at most `classes` terms, in float32 sums of a few hundred terms joined as a tree
+    tol = 2 * ez + 8 * U * (lse.abs() + mag + 1) + 1024 * U
+    _within(loss, (lse - at).mean(), tol.mean() + 2 * U * (lse - at).abs().mean(), "loss")
+    bf16 = dtype == torch.bfloat16
+    rel = 2 * ez + 1032 * U + (2.0 ** -8 if bf16 else 2.0 ** -21)
+    out = 2.0 ** -8 if bf16 else 2 * U
+    df, t_df, size_f = (torch.zeros(rows, dim, dtype=torch.float64, device=DEV) for _ in range(3))
+    for a, b in pieces:
+        y = w[a:b].double()
+        p = torch.exp(fd @ y.T - lse[:, None])
+        hot = torch.zeros_like(p)
+        here = ((lab >= a) & (lab < b)).nonzero()[:, 0]
+        hot[here, lab[here] - a] = 1.0
+        dz, size = (p - hot) / rows, (p + hot) / rows
+        e = size * rel[:, None] + (0.0 if bf16 else 2.0 ** -40 / rows)
+        df += dz @ y
+        t_df += e @ y.abs()
+        size_f += size @ y.abs()
+        if a in (0, pieces[len(pieces) // 2][0], pieces[-1][0]):
+            dw = dz.T @ fd
+            t = e.T @ fd.abs() + (rows + 4) * U * (size.T @ fd.abs()) + out * dw.abs() + 1e-30
+            _within(g_w[a:b], dw, t, f"gradient of the weight from {a}")
+    # a sum over the classes: roundings of a random sign, eight standard deviations of them
+    _within(g_f, df, t_df + 8 * classes ** 0.5 * U * size_f + out * df.abs() + 1e-30, "gradient of the features")
+
+
+@pytest.mark.parametrize("rows,dim,classes,dtype", [(3, 1024, 2_200_001, torch.float32),
+                                                    (3, 1024, 2_200_001, torch.bfloat16),
+                                                    (20, 520, 4_200_001, torch.bfloat16),
+                                                    (20, 520, 4_200_001, torch.float32)])
+def test_offsets_past_32_bits(rows, dim, classes, dtype):
+    _past_32_bits(rows, dim, classes, dtype)
+
+
+@pytest.mark.parametrize("rows,dim,classes,dtype", [(1100, 40, 40001, torch.float32),
+                                                    (1100, 72, 80001, torch.bfloat16)])
+def test_several_pieces_of_the_classes(rows, dim, classes, dtype):
+    # more than 160 MB of dz, so the gradients' products go by pieces and add up df
+    _check(*_case(rows, dim, classes, dtype, seed=43, drop=0.1))
+
+
+def test_calls_at_once_on_several_streams():
+    cases = [_case(8, 1024, 3001, seed=1), _case(200, 72, 700, seed=2), _case(400, 260, 5000, torch.bfloat16, seed=3),
+             _case(2, 64, 50_000, torch.bfloat16, seed=4)]
+    want = [ops.linear_softmax_ce_value_and_grad(f, w, lab, bias=b) for f, w, b, lab in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    got = []
+    for _ in range(5):
+        for s, (f, w, b, lab) in zip(streams, cases):
+            with torch.cuda.stream(s):
+                got.append(ops.linear_softmax_ce_value_and_grad(f, w, lab, bias=b))
+    torch.cuda.synchronize()
+    for i, out in enumerate(got):
+        for x, y in zip(want[i % len(cases)], out):
+            assert torch.equal(x, y), i
+
+
+@pytest.mark.parametrize("rows", [3, 140])
+def test_loss_gradients_of_zero_and_nan(rows):
+    f, w, b, lab = _case(rows, 24, 70, seed=47)
+    for t in (f, w, b):
+        t.requires_grad_()
+    for bad in (None, 1):
+        g = torch.zeros(rows, device=DEV)
+        if bad is not None:
+            g[bad] = float("nan")
+        loss = ops.linear_softmax_ce_loss(f, w, lab, bias=b, reduction="none")
+        gf, gw, gb = torch.autograd.grad(loss, (f, w, b), g)
+        if bad is None:
+            assert not gf.any() and not gw.any() and not gb.any()
+        else:      # a NaN is passed on
+            assert gf[bad].isnan().all() and gw.isnan().all() and gb.isnan().all()
+
+
+def test_two_captures_replayed_at_once():
+    # each graph holds its own workspace
+    graphs, outs, wants = [], [], []
+    for seed, (rows, dim, classes) in enumerate(((8, 64, 3001), (200, 72, 700), (200, 72, 700))):
+        f, w, b, lab = _case(rows, dim, classes, seed=60 + seed)
+        wants.append(ops.linear_softmax_ce_value_and_grad(f, w, lab, bias=b))
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(ops.linear_softmax_ce_value_and_grad(f, w, lab, bias=b))
+        graphs.append((g, torch.cuda.Stream(), (f, w, b, lab)))
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for g, s, _ in graphs:
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for want, out in zip(wants, outs):
+        for x, y in zip(want, out):
+            assert torch.equal(x, y)

@@ -41,3 +41,29 @@ def test_host_tensors_are_refused():
         ops.orthogonalize(x)
     with pytest.raises(ValueError, match="no CPU path"):
         ops.muon_(x, x.clone(), x.clone(), 0.1)
+
+
+def test_sizes_past_the_limits_are_refused():
+    assert _bytes(rows=1, cols=1 << 30) > 0 and _bytes(rows=1 << 15, cols=1 << 15) > 0
+    assert _bytes(rows=1, cols=(1 << 30) + 1) == 0 and _bytes(rows=2 ** 31 - 1, cols=1) == 0
+    for shape, steps in (((2 ** 32 + 1, 4, 4), 5), ((4, 2 ** 32 + 1), 5), ((4, 4), 2 ** 32 + 5), ((4, 4), -2 ** 32)):
+        with pytest.raises(ValueError, match="32 bits"):
+            ops._newton_schulz_desc(shape, "float32", steps, ops.NEWTON_SCHULZ_COEFFICIENTS, 1e-7)
+
+
+def test_overlapping_buffers_are_refused():
+    lib = _lib.load()
+    d = _lib.NcNewtonSchulz(2, 4, 8, 0, 5, 3.4445, -4.775, 2.0315, 1e-7)     # 256 bytes
+    r, n = ctypes.byref(d), _bytes(batch=2)
+    x, ws, P = 1 << 20, 1 << 22, ctypes.c_void_p
+    for out, w in ((x + 4, ws), (x - 252, ws), (x + 512, x), (ws, ws)):
+        assert lib.nc_orthogonalize(r, P(x), P(out), P(w), n, None) == _lib.NC_ERR_INVALID, (out, w)
+        assert b"overlap" in lib.nc_last_error()
+    for p, g, m, w in ((x, x + 252, x + 512, ws), (x, x + 512, x + 252, ws), (x, x + 512, x + 764, ws),
+                       (x, x + 512, x + 1024, x + 512)):
+        assert lib.nc_muon_update(r, P(p), P(g), P(m), 0.1, 0.9, 1, 0.0, P(w), n, None) == _lib.NC_ERR_INVALID
+
+
+def test_workspaces_of_large_batches_stay_small():
+    # a launch's matrices share it: past a few rounds of the GPU the batch does not count
+    assert _bytes(batch=65535, rows=65, cols=520) == _bytes(batch=1000, rows=65, cols=520) < 2 ** 30

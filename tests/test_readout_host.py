@@ -68,3 +68,56 @@ def test_arguments_are_checked(change, match):
     with pytest.raises(ValueError, match=match):
         ops._linear_ce_args(args["features"], args["weight"], args["labels"], args["bias"], args["ignore_index"],
                             args["reduction"])
+
+
+def test_sizes_past_the_tile_counts_are_refused():
+    most = 1 << 24
+    assert _bytes(rows=most, dim=1, classes=1) > 0 and _bytes(rows=1, dim=1, classes=most, grad=1) > 0
+    for bad in (dict(rows=most + 1), dict(dim=most + 1), dict(classes=2 ** 31 - 1), dict(rows=2 ** 31 - 1),
+                dict(rows=most, classes=1 << 21), dict(rows=most, dim=1 << 15), dict(classes=most, dim=1 << 15)):
+        for grad in (0, 1):
+            assert _bytes(grad=grad, **bad) == 0, bad
+    assert b"too large" in _lib.load().nc_last_error()
+
+
+def test_overlapping_buffers_are_refused():
+    lib = _lib.load()
+    d = _lib.NcLinearCe(4, 8, 16, 0, -100, 0)
+    n = lib.nc_linear_ce_workspace_bytes(ctypes.byref(d), 1)
+    step = 1 << 20
+    names = ["f", "w", "b", "lab", "loss", "lse", "gl", "gf", "gw", "gb", "ws"]
+    assert n < step
+
+    def call(which, **change):
+        p = {k: ctypes.c_void_p(step * (i + 1)) for i, k in enumerate(names)}
+        p.update({k: ctypes.c_void_p(v) for k, v in change.items()})
+        if which == "forward":
+            return lib.nc_linear_ce_forward(ctypes.byref(d), p["f"], p["w"], p["b"], p["lab"], p["loss"], p["lse"],
+                                            p["ws"], n, None)
+        if which == "backward":
+            return lib.nc_linear_ce_backward(ctypes.byref(d), p["f"], p["w"], p["b"], p["lab"], p["lse"], p["gl"],
+                                             p["gf"], p["gw"], p["gb"], p["ws"], n, None)
+        return lib.nc_linear_ce_value_and_grad(ctypes.byref(d), p["f"], p["w"], p["b"], p["lab"], p["loss"],
+                                               p["lse"], p["gf"], p["gw"], p["gb"], p["ws"], n, None)
+
+    at = {k: step * (i + 1) for i, k in enumerate(names)}
+    for which, change in (("forward", dict(loss=at["lse"] + 12)), ("forward", dict(lse=at["f"] + 124)),
+                          ("forward", dict(ws=at["w"])), ("backward", dict(gw=at["w"])),
+                          ("backward", dict(gf=at["f"] + 4)), ("backward", dict(gb=at["gw"] + 508)),
+                          ("backward", dict(gf=at["gl"])), ("backward", dict(lse=at["ws"] + 8)),
+                          ("both", dict(gw=at["w"] - 4)), ("both", dict(loss=at["lab"])),
+                          ("both", dict(gf=at["gw"] + 4))):
+        assert call(which, **change) == _lib.NC_ERR_INVALID, (which, change)
+        assert b"overlap" in lib.nc_last_error()
+
+
+@pytest.mark.parametrize("ignore", [2 ** 32 - 100, -2 ** 31, 2 ** 31 - 1, -2 ** 40])
+def test_ignore_index_has_to_fit(ignore):
+    with pytest.raises(ValueError, match="32 bits"):
+        ops._linear_ce_args(_fake(2, 3), _fake(4, 3), _fake(2, dtype=torch.int64), None, ignore, "mean")
+
+
+def test_sizes_past_32_bits_are_refused():
+    wide = torch.zeros(1, 1).expand(2 ** 32 + 2, 1).as_subclass(_Fake)
+    with pytest.raises(ValueError, match="32 bits"):
+        ops._linear_ce_args(_fake(2, 1), wide, _fake(2, dtype=torch.int64), None, -100, "mean")
