@@ -10,8 +10,10 @@
 //
 // Few rows (here): a CTA streams its share of the weight through shared memory once, in chunks
 // that bulk copies bring while it works on the one before, and everything a chunk is needed
-// for happens there.  Bound by reading the weight (and writing its gradient).  More rows:
-// nc_readout_tc.cu.
+// for happens there.  Bound by reading the weight (and writing its gradient): one float32 row
+// x 1024 x 50000 is scored in 40 us (5.1 TB/s, 79 % of a copy's rate).  With more rows the FFMAs
+// and their shared memory reads take over: value and gradients of 8 rows take 201 us, 0.6 GB at
+// 3.1 TB/s (from global memory without the copies 240 us).  More rows: nc_readout_tc.cu.
 #include <math.h>
 
 #include <initializer_list>
@@ -266,7 +268,8 @@ __global__ void __launch_bounds__(512) ce_rows_finish_kernel(CeArgs a, int block
 }
 
 // Gradients.  Of each chunk the logits again, left as p = g_n (exp(z - lse) - onehot); then a thread
-// owns four columns, with the features' and df's in registers for all rows, and goes through
+// owns four columns (a sum over classes needs no other thread until the end), with the features'
+// and df's in registers for all rows, and goes through
 // the classes: dw[v] = sum_n p f[n] is stored, df[n] += p w[v] stays.  Where the columns need
 // fewer threads (td of them), groups of td share the classes and meet at the end.
 template <typename T, int RN, int VEC, int VT>
@@ -448,7 +451,9 @@ RowsPlan rows_plan(const nc_linear_ce* d, int vec) {
 }
 
 // Few rows take the streaming kernels, which read the weight as it is; from then on the tensor
-// cores are faster.
+// cores are faster.  In bfloat16 they need no planes of the weight and win from
+// 5 rows on.  Value and gradients of rows x 1024 x 50000: float32 16 rows 325 us here, 17 rows
+// 367 us there; bfloat16 4 rows 130 us here, 5 rows 190 and 16 rows 174 us there.
 bool on_tensor_cores(const nc_linear_ce* d) {
   return d->dim > kRowDim || d->rows > (d->dtype == NC_BF16 ? kRowsMostBf16 : kRowsMost);
 }

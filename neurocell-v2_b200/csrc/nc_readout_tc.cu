@@ -12,6 +12,12 @@
 // tensor's largest finite value to [2^13, 2^14): an entry down to 2^-18 of it keeps float32's
 // precision, smaller ones an absolute error of 2^-38 of it.  bfloat16 operands are used as
 // they are, and dz is rounded to bfloat16 (2^-9 of an entry, as the products read it).
+// Bound by the tensor pipe where rows, dim and classes are large: 2048 x 512 x 32768 in float32
+// takes 0.76 ms in a burst and 0.93 ms at the power cap (885 TFLOP/s of 16-bit products), 4096 x
+// 1024 x 50000 in bfloat16 1.57 and 1.83 ms (916 TFLOP/s); the value alone of 4096 x 1024 x 50000
+// takes 0.31 ms (1350 TFLOP/s).  Small calls are bound by nine dependent launches: 128 x 8 x 256
+// 39 us as a graph.
+//
 // f_n = g_n / max |g| lies in [-1, 1], so dz needs no more than a fixed scale: 22 bits down
 // to 2^-29, and an absolute error of 2^-40 below.
 #include <math.h>
@@ -409,7 +415,7 @@ __global__ void __launch_bounds__(1024) ce_finish_kernel(CeArgs a, int slots, in
 // ---- gradient ------------------------------------------------------------------------------
 
 template <bool BF16>
-struct DzEpilogue {
+struct DzEpilogue {   // bias sums and all: 4096 x 1024 x 50000 takes 1574 us with db, 1450 without a bias
   CeArgs a;
   const Scales* scales;
   const float* bias;
