@@ -739,10 +739,10 @@ int choose_splits(int64_t tiles, int k, int at_once) {
   return splits;
 }
 
-// Matrices that clusters take in one launch. More go by several launches on the same workspace,
-// which has planes (and parts of split products) for a launch's matrices: eight rounds of the 18
-// clusters that run at a time. 64000 x 65 x 520 would need 266 GiB at once.
-constexpr int kLaunchMatrices = 144;
+// Planes (and so matrices) of one launch; more matrices go by several launches on the same
+// workspace. 64000 x 65 x 520 would take 23 GB at once; a launch's start and end are about 170 us
+// beside several milliseconds.
+constexpr size_t kLaunchBytes = (size_t)1 << 30;
 
 struct NsLayout {
   size_t status, norms, x, y, gram, poly, parts, total;
@@ -768,14 +768,17 @@ NsLayout ns_layout(const nc_newton_schulz* d) {
     return L;
   }
   // A cluster's barrier takes a tenth of the grid's; worth it where its CTAs have up to two tiles
-  // each, or where the matrices fill the SMs.  Five steps, cluster and grid: 128 x 576 125 and 184
-  // us, 128 x 1024 (16 tiles) 132 and 199, 256 x 512 149 and 213; 384 x 384 (18 tiles) 226 and 220,
-  // 512 x 512 (32) 360 and 240.
+  // each.  Five steps, cluster and grid: 128 x 576 125 and 184 us, 128 x 1024 (16 tiles) 132 and
+  // 199, 256 x 512 149 and 213; 384 x 384 (18 tiles) 226 and 220, 512 x 512 (32) 360 and 240.
+  // Not for many matrices, as some 14 clusters run at a time while the grid shares all tiles: 20
+  // times 128 x 128 176 and 214 us, 36 times 260 and 253; 16 times 256 x 512 303 and 263.
   const auto tiles_of = [](int64_t m, int64_t n, int wide) { return ((m + 127) / 128) * ((n + wide - 1) / wide); };
-  L.cluster = tiles_of(d->rows, d->cols, 64) <= 2 * kCluster || (int64_t)d->batch * kCluster >= 2 * 148;
-  L.batch = L.cluster && d->batch > kLaunchMatrices ? kLaunchMatrices : d->batch;
+  const int64_t narrow = tiles_of(d->rows, d->cols, 64);
+  L.cluster = (narrow <= kCluster && d->batch <= 20) || (narrow <= 2 * kCluster && d->batch <= 14);
+  const size_t most_batch = kLaunchBytes / (8 * (x + g)) + 1;
+  L.batch = (size_t)d->batch < most_batch ? d->batch : (int)most_batch;
   tc::Problem q{};
-  q.m = q.n = (int)s, q.batch = L.cluster ? 1 : d->batch, q.splits = 1, q.symmetric = 1;
+  q.m = q.n = (int)s, q.batch = L.cluster ? 1 : L.batch, q.splits = 1, q.symmetric = 1;
   if (L.cluster)
     tc::set_tiles<64, 1>(&q);
   else
@@ -794,7 +797,7 @@ NsLayout ns_layout(const nc_newton_schulz* d) {
   }
   L.parts_each = parts * tile / 4;
   // as many CTAs as any product keeps busy, or as share the element-wise passes well
-  int64_t blocks = (int64_t)(d->batch * n / 4096);
+  int64_t blocks = (int64_t)(L.batch * n / 4096);
   if (most > blocks) blocks = most;
   L.blocks = L.cluster ? kCluster * L.batch : (int)(blocks < 148 ? blocks : 148);
   L.norms = take((size_t)L.batch * (L.cluster ? kCluster : L.blocks) * 8);

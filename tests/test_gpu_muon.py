@@ -254,11 +254,11 @@ def test_offsets_past_32_bits(batch, rows, cols, dtype):
 
 
 def test_a_batch_of_several_launches():
-    p, g, m = (_matrices(311, 70, 96, seed=k) for k in (35, 36, 37))
+    p, g, m = (_matrices(8000, 70, 96, seed=k) for k in (35, 36, 37))
     p2, m2 = p.clone(), m.clone()
     ops.muon_(p, g, m, 0.1)
-    for k in range(0, 311, 100):      # as many as one launch takes
-        part = slice(k, min(311, k + 100))
+    for k in range(0, 8000, 3000):      # a launch's worth or less
+        part = slice(k, min(8000, k + 3000))
         ops.muon_(p2[part], g[part], m2[part], 0.1)
     torch.cuda.synchronize()
     assert torch.equal(p, p2) and torch.equal(m, m2)
