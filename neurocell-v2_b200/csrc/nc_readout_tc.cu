@@ -51,43 +51,67 @@ struct Plan {
   int classes_pad;            // classes, whole 256s
   int slots;                  // half tiles of classes
   int piece, pieces;          // classes per piece (whole 256s)
-  // CTA pairs on 256 x 256 tiles, or one CTA on 128 x 128 where a side has at most 128: the
-  // logits' products, dw's and df's
-  bool pair, pair_w, pair_f;
+  // CTA pairs on 256 x 256 tiles, or one CTA on 128 x 128: the value's product, dz's, dw's, df's
+  bool pair, pair_dz, pair_w, pair_f;
   int splits;                 // of df over a piece's classes
   size_t scales, max_part, w, f, bias, part, zlabel, fac, dz, df_part, db_part, total;
 };
 
-// Pieces and splits by a count of k-tiles on the busiest SM (or pair): a product takes
-// ceil(tiles / SMs) times its k-tiles, so a piece is good where its tiles fill whole rounds.
+// Time of a product (m, n) over `depth` k-tiles, as 20ths of a pair's k-tile: its rounds of tiles
+// over the SMs, each with a fixed part (fill, drain, epilogue) and its k-tiles.  The constants are
+// fitted to the value's products of 512 .. 4096 rows, 256 .. 1024 columns and 4096 .. 16384 classes: a
+// round of pairs takes 4.5 + 0.87 kt us in float32 and 1.8 + 0.4 kt (5 at least, the epilogue's) in
+// bfloat16, one of single CTAs 1.5 + 0.8 kt and 1.2 + 0.34 kt.  So pairs win where there are many rounds (1024 x 512 x
+// 16384: 67 us and 76), single CTAs where tiles are few (333 x 512 x 10007: 41 us and 37).
+// dz's epilogue beside float32 operands (`dz`: both planes of 128 columns a thread) costs a pair
+// more: 1024 x 512 x 16384 takes 245 us with pairs there and 233 without, 4096 x 1024 x 50000 4.3 ms
+// and 4.6.
+int64_t product_time(int64_t m, int64_t n, int64_t depth, bool pair, bool bf16, bool dz = false) {
+  const int64_t side = pair ? 256 : 128, at = pair ? 74 : 148;
+  const int64_t rounds = (((m + side - 1) / side) * ((n + side - 1) / side) + at - 1) / at;
+  if (bf16) return rounds * (pair ? (depth > 8 ? 90 + 20 * depth : 250) : 60 + 17 * depth);
+  return rounds * (pair ? (dz ? 300 : 100) + 20 * depth : (dz ? 64 : 34) + 18 * depth);
+}
+
+bool pairs_win(int64_t m, int64_t n, int64_t depth, bool bf16, bool dz = false) {
+  return product_time(m, n, depth, true, bf16, dz) < product_time(m, n, depth, false, bf16, dz);
+}
+
+// Pieces, splits and tiles by product_time.
 // 2048 x 512 x 32768 in float32: five pieces of 26 tiles of 256 classes, which fit L2, leave a
-// third of the pairs idle in dw and take 949 us; the choice here takes 759. Splits keep SMs busy
-// in df where it has few tiles: 333 x 128 x 10007 takes 79 us with them priced at the traffic of
-// their parts, 87 us at a flat 4 k-tiles each (which left df to 18 CTAs).
+// third of the pairs idle in dw and take 949 us; the choice here takes 760 to 780. Splits keep SMs busy
+// in df where it has few tiles: 333 x 128 x 10007 (all by pairs) took 79 us with them priced at the
+// traffic of their parts, 87 us at a flat 4 k-tiles each (which left df to 18 CTAs).
 void choose_pieces(const nc_linear_ce* d, int planes, Plan* p) {
   auto ceil_div = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
-  const int sms = 148, bk = 64;
+  const int bk = 64;
   const int tiles = p->classes_pad / 256;
   const size_t tile_bytes = (size_t)p->rows_pad * 256 * 2 * planes;
   int64_t most = (int64_t)(kPieceBytes / tile_bytes);
   if (most < 1) most = 1;
   const int64_t fewest = ceil_div(tiles, most);
-  // products: tiles per 256 classes, and how many run at a time
-  const int64_t dz_tiles = p->pair ? ceil_div(d->rows, 256) : ceil_div(d->rows, 128) * 2, dz_at = p->pair ? sms / 2 : sms;
-  const int64_t w_tiles = p->pair_w ? ceil_div(d->dim, 256) : ceil_div(d->dim, 128) * 2, w_at = p->pair_w ? sms / 2 : sms;
-  const int f_side = p->pair_f ? 256 : 128;
-  const int64_t f_tiles = ceil_div(d->rows, f_side) * ceil_div(d->dim, f_side), f_at = p->pair_f ? sms / 2 : sms;
-  const int64_t launch = 12;   // k-tiles that a launch's start and end are worth
+  const int64_t launch = 240;   // a launch's start and end
   int64_t best = INT64_MAX;
   for (int64_t pieces = fewest; pieces < fewest + 4 && pieces <= tiles; ++pieces) {
-    const int64_t t = ceil_div(tiles, pieces);
-    const int64_t one = ceil_div(t * dz_tiles, dz_at) * ceil_div(d->dim, bk) + ceil_div(t * w_tiles, w_at) * ceil_div(d->rows, bk) +
-                        3 * launch;
+    const int64_t t = ceil_div(tiles, pieces), classes = 256 * t;
+    const bool pair_dz = pairs_win(d->rows, classes, ceil_div(d->dim, bk), p->bf16, true);
+    const bool pair_w = pairs_win(classes, d->dim, ceil_div(d->rows, bk), p->bf16);
+    const int64_t one = product_time(d->rows, classes, ceil_div(d->dim, bk), pair_dz, p->bf16, true) +
+                        product_time(classes, d->dim, ceil_div(d->rows, bk), pair_w, p->bf16) + 3 * launch;
     for (int splits = 1; splits <= kMaxSplits && splits <= t; ++splits) {
-      // a split's part of df is written and read once: about a k-tile for 250,000 elements
-      const int64_t all = (one + ceil_div(f_tiles * splits, f_at) * ceil_div(t * (256 / bk), splits)) * ceil_div(tiles, t) +
-                          splits * ((int64_t)d->rows * p->pitch / 250000 + 1) / 2;
-      if (all < best) best = all, p->piece = (int)t * 256, p->splits = splits;
+      const int64_t depth = ceil_div(t * (256 / bk), splits);
+      for (int pair_f = 0; pair_f < 2; ++pair_f) {
+        // splits as rows of tiles; a split's part of df is written and read once: about a k-tile
+        // for 250,000 elements
+        const int64_t side = pair_f ? 256 : 128;
+        const int64_t all = (one + product_time(ceil_div(d->rows, side) * side * splits, d->dim, depth, pair_f, p->bf16)) *
+                                ceil_div(tiles, t) +
+                            10 * splits * ((int64_t)d->rows * p->pitch / 250000 + 1);
+        if (all < best) {
+          best = all, p->piece = (int)classes, p->splits = splits;
+          p->pair_dz = pair_dz, p->pair_w = pair_w, p->pair_f = pair_f;
+        }
+      }
     }
   }
   p->pieces = (int)ceil_div(tiles, p->piece / 256);
@@ -101,9 +125,7 @@ Plan make_plan(const nc_linear_ce* d, bool grad) {
   p.pitch = (d->dim + 7) / 8 * 8;
   p.rows_pad = (d->rows + 255) / 256 * 256;
   p.classes_pad = (d->classes + 255) / 256 * 256;
-  p.pair = d->rows > 128;
-  p.pair_w = d->dim > 128;
-  p.pair_f = d->dim > 128 && d->rows > 128;
+  p.pair = pairs_win(d->rows, d->classes, (d->dim + 63) / 64, p.bf16);
   const int tile = p.pair ? 256 : 128;
   p.slots = (d->classes + tile - 1) / tile * 2;
   const int planes = p.bf16 ? 1 : 2;
@@ -721,7 +743,7 @@ struct Call {
       // the last piece may be shorter; `width` is whole tiles
       const int width = p.classes_pad - v0 < p.piece ? p.classes_pad - v0 : p.piece;
       const int classes = d->classes - v0 < width ? d->classes - v0 : width;
-      NC_CHECK(p.pair ? (dz_product<256, 2, 8>(g, v0, width)) : (dz_product<128, 1, 8>(g, v0, width)));
+      NC_CHECK(p.pair_dz ? (dz_product<256, 2, 8>(g, v0, width)) : (dz_product<128, 1, 8>(g, v0, width)));
       if (g.weight)
         NC_CHECK(p.pair_w ? (weight_product<256, 2, 8>(g, v0, classes)) : (weight_product<128, 1, 8>(g, v0, classes)));
       if (g.features)

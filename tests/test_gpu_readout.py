@@ -386,6 +386,15 @@ def test_several_pieces_of_the_classes(rows, dim, classes, dtype):
     _check(*_case(rows, dim, classes, dtype, seed=43, drop=0.1))
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,dim,classes", [(1001, 1010, 18690), (1024, 1024, 18944), (2048, 512, 4100),
+                                              (520, 264, 30000)])
+def test_products_by_pairs_of_ctas(rows, dim, classes, dtype):
+    # enough rounds of 256 x 256 tiles for the value, dz, dw and df to go by pairs (the first two; the
+    # others some of them)
+    _check(*_case(rows, dim, classes, dtype, seed=45, drop=0.1))
+
+
 def test_calls_at_once_on_several_streams():
     cases = [_case(8, 1024, 3001, seed=1), _case(200, 72, 700, seed=2), _case(400, 260, 5000, torch.bfloat16, seed=3),
              _case(2, 64, 50_000, torch.bfloat16, seed=4)]
