@@ -301,12 +301,16 @@ nc_status launch_small(const SmallArgs& a, const SmallPlan& r, int batch, cudaSt
 // 2^12: |entries| stay below 16 while the singular values do, and an entry of 2^-26 still has
 // its 11 bits in the high plane.
 //
+// Bound by shared memory where matrices are large: per k-tile a 128 x 128 tile's three products
+// read 96 KB of operands and the copies write 64 KB, 1250 cycles at 128 bytes a cycle (768 on the
+// tensor pipe alone); a k-tile takes about 1400.
+//
 // All steps are one cooperative launch: a product of such sizes takes a few microseconds, and
 // a launch, its set-up of tensor memory and its first loads as much again.  Between products
 // the grid meets (cooperative_groups); the symmetric ones compute the tiles on and above the
 // diagonal and store them twice; a product with fewer tiles than SMs is split along k, its
 // float32 parts summed in order by the whole grid.  2001 x 513 takes 286 us (19 a product, mostly
-// meetings, split sums, fill and drain), three 1024 x 1024 updates 480 us (tensor pipe), three
+// meetings, split sums, fill and drain), three 1024 x 1024 updates 482 us, three
 // 256 x 256 on a cluster each 133 us.
 constexpr float kPlaneScale = 4096.f, kPlaneInv = 1.f / 4096.f;
 constexpr int kNsChunk = 1;  // k-tiles (of 64) per accumulator: Gram sums of one sign show the additions' truncation

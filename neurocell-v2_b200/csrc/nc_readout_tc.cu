@@ -13,8 +13,8 @@
 // precision, smaller ones an absolute error of 2^-38 of it.  bfloat16 operands are used as
 // they are, and dz is rounded to bfloat16 (2^-9 of an entry, as the products read it).
 // Bound by the tensor pipe where rows, dim and classes are large: 2048 x 512 x 32768 in float32
-// takes 0.76 ms in a burst and 0.93 ms at the power cap (885 TFLOP/s of 16-bit products), 4096 x
-// 1024 x 50000 in bfloat16 1.57 and 1.83 ms (916 TFLOP/s); the value alone of 4096 x 1024 x 50000
+// takes 0.78 ms in a burst and 0.92 ms at the power cap (895 TFLOP/s of 16-bit products), 4096 x
+// 1024 x 50000 in bfloat16 1.41 and 1.70 ms (987 TFLOP/s); the value alone of 4096 x 1024 x 50000
 // takes 0.31 ms (1350 TFLOP/s).  Small calls are bound by nine dependent launches: 128 x 8 x 256
 // 39 us as a graph.
 //
@@ -437,7 +437,7 @@ __global__ void __launch_bounds__(1024) ce_finish_kernel(CeArgs a, int slots, in
 // ---- gradient ------------------------------------------------------------------------------
 
 template <bool BF16>
-struct DzEpilogue {   // bias sums and all: 4096 x 1024 x 50000 takes 1574 us with db, 1450 without a bias
+struct DzEpilogue {   // bias sums and all: with all by pairs 4096 x 1024 x 50000 took 1574 us with db, 1450 without a bias
   CeArgs a;
   const Scales* scales;
   const float* bias;
