@@ -437,7 +437,7 @@ __global__ void __launch_bounds__(1024) ce_finish_kernel(CeArgs a, int slots, in
 // ---- gradient ------------------------------------------------------------------------------
 
 template <bool BF16>
-struct DzEpilogue {   // bias sums and all: with all by pairs 4096 x 1024 x 50000 took 1574 us with db, 1450 without a bias
+struct DzEpilogue {   // its sums for db cost 8 % of a call in bfloat16 (4096 x 1024 x 50000)
   CeArgs a;
   const Scales* scales;
   const float* bias;
