@@ -132,6 +132,11 @@ __device__ __forceinline__ void bar_arrive_remote(uint32_t bar, uint32_t cta) {
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t n;
+  asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(n));
+  return n;
+}
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
@@ -332,7 +337,7 @@ __device__ __forceinline__ void patch_store_f32(uint8_t* patch, const float* v, 
 // What a CTA's warps share beside the stages.
 template <int PL, int BN, int CG, int EW>
 struct Shared {
-  uint64_t bars[2 * Config<PL, BN, CG, EW>::kStages + 2 * Config<PL, BN, CG, EW>::kAccs + 1 + Config<PL, BN, CG, EW>::kExtras];
+  uint64_t bars[2 * Config<PL, BN, CG, EW>::kStages + 2 * Config<PL, BN, CG, EW>::kAccs + 1 + 2 * Config<PL, BN, CG, EW>::kExtras];
   uint32_t tmem_slot;
   int abort, extra_readers[Config<PL, BN, CG, EW>::kExtras];
 };
@@ -366,6 +371,7 @@ struct Engine {
   __device__ __forceinline__ uint32_t acc_empty(int i) const { return bar0 + 8 * (2 * C::kStages + C::kAccs + i); }
   __device__ __forceinline__ uint32_t drain() const { return bar0 + 8 * (2 * C::kStages + 2 * C::kAccs); }
   __device__ __forceinline__ uint32_t extra_full(int i) const { return bar0 + 8 * (2 * C::kStages + 2 * C::kAccs + 1 + i); }
+  __device__ __forceinline__ uint32_t extra_read(int i) const { return extra_full(C::kExtras + i); }
 
   // By the whole CTA, before it reads anything that an earlier kernel wrote.  `raw`: the dynamic
   // shared memory, on 1024 bytes.
@@ -385,7 +391,7 @@ struct Engine {
       for (int i = 0; i < C::kStages; ++i) bar_init(full(i), 1), bar_init(empty(i), 1);
       for (int i = 0; i < C::kAccs; ++i) bar_init(acc_full(i), 1), bar_init(acc_empty(i), kEpiWarps * CG);
       bar_init(drain(), 1);
-      for (int i = 0; i < C::kExtras; ++i) bar_init(extra_full(i), 1), sh->extra_readers[i] = 0;
+      for (int i = 0; i < C::kExtras; ++i) bar_init(extra_full(i), 1), bar_init(extra_read(i), 1), sh->extra_readers[i] = 0;
       sh->abort = 0;
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -426,20 +432,22 @@ struct Engine {
   // Behind a tile's k-tiles, what the epilogue wants of a stored matrix: this CTA's rows of the
   // tile, both planes, a stage for every 64 columns.  It lands in this CTA (of a pair too) on
   // barriers of its own; the multiplying warp steps over it with skip_extra(), the epilogue
-  // takes it with extra() and extra_done().
+  // takes it with extra() and extra_done().  The next tile's waits until all warps have read this
+  // one: with fewer k-tiles than stages it could land first, and a slow warp would miss a phase.
   __device__ __forceinline__ void load_extra(const CUtensorMap* m, const Tile& x) {
     constexpr int bytes = PL * kBM * 128;
     static_assert(bytes <= C::kStage, "64 columns fit a stage");
 #pragma unroll
     for (int i = 0; i < C::kExtras; ++i) {
-      if (!ok || !(ok = bar_wait(empty(s), ph, abort, status))) return;
+      if (!ok || !(ok = bar_wait(extra_read(i), (extras / C::kExtras & 1) ^ 1, abort, status))) return;
+      if (!(ok = bar_wait(empty(s), ph, abort, status))) return;
       bar_expect(extra_full(i), bytes);
       tma_load<1>(stages + s * C::kStage, m, extra_full(i), x.n0 + 64 * i, x.m0, x.batch);
+      ++extras;
       if (rank == 0) bar_arrive(full(s));   // keeps the stage's phases in step
       if (issued < C::kStages) ++issued;
       if (++s == C::kStages) s = 0, ph ^= 1;
     }
-    ++extras;
   }
   __device__ __forceinline__ void skip_extra() {
 #pragma unroll
@@ -537,7 +545,10 @@ struct Engine {
     if ((threadIdx.x & 31) == 0) {
       __threadfence_block();
       constexpr int readers = EW / C::kExtras;
-      if (atomicAdd(extra_readers + i, 1) % readers == readers - 1) bar_arrive(empty(at >= C::kStages ? at - C::kStages : at));
+      if (atomicAdd(extra_readers + i, 1) % readers == readers - 1) {
+        bar_arrive(empty(at >= C::kStages ? at - C::kStages : at));
+        bar_arrive(extra_read(i));
+      }
     }
     eph ^= 1;
     es += C::kExtras;
@@ -554,9 +565,11 @@ struct Engine {
         for (int j = 0; j < kWaitLimit && !bar_try(full(s), ph ^ 1); ++j) {
         }
       }
-      for (int i = 0; i < C::kExtras && extras > 0; ++i)
-        for (int j = 0; j < kWaitLimit && !bar_try(extra_full(i), (extras - 1) & 1); ++j) {
+      for (int i = 0; i < C::kExtras; ++i) {
+        const int n = (extras + C::kExtras - 1 - i) / C::kExtras;   // copies on this barrier
+        for (int j = 0; j < kWaitLimit && n > 0 && !bar_try(extra_full(i), (n - 1) & 1); ++j) {
         }
+      }
     }
     if (warp == kEpiWarps + 1 && rank == 0) {
       // every product has finished before tensor memory is given back

@@ -253,6 +253,18 @@ def test_offsets_past_32_bits(batch, rows, cols, dtype):
         assert torch.linalg.matrix_norm(got[k].double() - want) <= tol, k
 
 
+@pytest.mark.parametrize("rows,cols", [(96, 1000), (1000, 96), (100, 576), (70, 2000), (128, 1024), (384, 384), (300, 400)])
+def test_several_tiles_of_a_cluster(rows, cols):
+    # rows past the end leave some warps without work, which then run ahead of the others
+    for batch in (1, 5):
+        x = _matrices(batch, rows, cols, seed=39)
+        want, tol = _formula(x)
+        first = ops.orthogonalize(x)
+        assert (torch.linalg.matrix_norm(first.double() - want) <= tol).all()
+        for _ in range(20):
+            assert torch.equal(ops.orthogonalize(x), first)
+
+
 def test_a_batch_of_several_launches():
     p, g, m = (_matrices(8000, 70, 96, seed=k) for k in (35, 36, 37))
     p2, m2 = p.clone(), m.clone()
