@@ -317,7 +317,7 @@ constexpr int kNsChunk = 1;  // k-tiles (of 64) per accumulator: Gram sums of on
 constexpr int kNsCols = 32;  // columns of an epilogue thread
 // Where matrices have many tiles: 128 x 128, the whole grid on all matrices (pairs of CTAs on
 // 256 x 128 took 146 cycles for a product of 16 k that one CTA does in 115 on its half).  Where
-// they have few: 128 x 64 and a cluster of 8 on each matrix.
+// they have few: 128 x 64 and a cluster of 8 or 16 on each matrix.
 template <bool CLUSTER>
 struct NsTile {
   static constexpr int kBN = CLUSTER ? 64 : 128, kWarps = CLUSTER ? 8 : 16;
@@ -334,7 +334,8 @@ struct Planes {   // (batch, plane, rows, pitch)
 
 enum NsProduct { kGram, kPoly, kUpdate };
 
-constexpr int kCluster = 8;
+constexpr int kCluster = 8, kLargeCluster = 16;   // CTAs
+constexpr int kLargeClusters = 7;                 // that run at a time
 
 struct NsArgs {
   // X and its next value, A and Q as operands a and b: with k contiguous, or by rows of k
@@ -540,8 +541,8 @@ __global__ void __launch_bounds__(NsEngine<CLUSTER>::C::kThreads, 1) ns_kernel(c
   if (p.first && blockIdx.x == 0 && tid == 0) *p.status = 0;
   E e(raw, &sh, p.status);
   // The CTAs that work together: the whole grid on all matrices, or a cluster on one.
-  const int size = CLUSTER ? kCluster : gridDim.x, rank = CLUSTER ? (int)tc::cluster_rank() : blockIdx.x;
-  const int b0 = CLUSTER ? blockIdx.x / kCluster : 0, batch = CLUSTER ? 1 : p.batch;
+  const int size = CLUSTER ? (int)tc::cluster_size() : gridDim.x, rank = CLUSTER ? (int)tc::cluster_rank() : blockIdx.x;
+  const int b0 = CLUSTER ? blockIdx.x / size : 0, batch = CLUSTER ? 1 : p.batch;
   // Everything stored so far is there for every CTA's loads, plain ones and tensor copies.
   auto meet = [&] {
     __threadfence();
@@ -750,7 +751,7 @@ constexpr size_t kLaunchBytes = (size_t)1 << 30;
 
 struct NsLayout {
   size_t status, norms, x, y, gram, poly, parts, total;
-  bool cluster;
+  int cluster;   // CTAs of one, or 0
   int batch;   // matrices of a launch
   int splits[3], blocks;
   int64_t parts_each;
@@ -771,14 +772,22 @@ NsLayout ns_layout(const nc_newton_schulz* d) {
     L.total = at;
     return L;
   }
-  // A cluster's barrier takes a tenth of the grid's; worth it where its CTAs have up to two tiles
-  // each.  Five steps, cluster and grid: 128 x 576 125 and 184 us, 128 x 1024 (16 tiles) 132 and
-  // 199, 256 x 512 149 and 213; 384 x 384 (18 tiles) 226 and 220, 512 x 512 (32) 360 and 240.
-  // Not for many matrices, as some 14 clusters run at a time while the grid shares all tiles: 20
-  // times 128 x 128 176 and 214 us, 36 times 260 and 253; 16 times 256 x 512 303 and 263.
+  // A meeting of a cluster takes half of the grid's, and a smaller tile's stores are sooner done.  Five
+  // steps of one matrix, us on a cluster of 8, of 16 and on the grid: 8 times 256 x 256 (8 tiles) 122, -
+  // and 226; 128 x 1024 (16) 133, 114 and 199; 256 x 512 (16) 151, 130 and 213; 384 x 384 (18) 226, 159 and
+  // 219; 128 x 2048 (32) 178, 141 and 203; 200 x 1500 (48) -, 196 and 219; 512 x 512 (32) 360, 240 and
+  // 241; 512 x 600 (40) -, 280 and 249.  So a cluster of 16 where its rounds of tiles come to at most
+  // 16 k-tiles.  Not for many matrices, as 7 clusters of 16 or some 14 of 8 run at a time while the
+  // grid shares all tiles: 20 times 128 x 128 176 on clusters of 8 and 214 on the grid, 36 times 260
+  // and 253; 16 times 256 x 512 303 and 263.
   const auto tiles_of = [](int64_t m, int64_t n, int wide) { return ((m + 127) / 128) * ((n + wide - 1) / wide); };
   const int64_t narrow = tiles_of(d->rows, d->cols, 64);
-  L.cluster = (narrow <= kCluster && d->batch <= 20) || (narrow <= 2 * kCluster && d->batch <= 14);
+  const int64_t deep = (narrow + kLargeCluster - 1) / kLargeCluster * ((s + tc::kBK - 1) / tc::kBK);
+  const bool large = narrow <= 4 * kLargeCluster && deep <= 16 && d->batch <= kLargeClusters;
+  L.cluster = narrow <= kCluster && d->batch <= 20          ? kCluster
+              : large                                       ? kLargeCluster
+              : narrow <= 2 * kCluster && d->batch <= 14 ? kCluster
+                                                         : 0;
   const size_t most_batch = kLaunchBytes / (8 * (x + g)) + 1;
   L.batch = (size_t)d->batch < most_batch ? d->batch : (int)most_batch;
   tc::Problem q{};
@@ -794,7 +803,7 @@ NsLayout ns_layout(const nc_newton_schulz* d) {
   const int tile = 128 * (L.cluster ? 64 : 128);
   int64_t most = 1, parts = 0;
   for (int f = 0; f < 3; ++f) {
-    L.splits[f] = choose_splits(count[f], depth[f], L.cluster ? kCluster : 148);
+    L.splits[f] = choose_splits(count[f], depth[f], L.cluster ? L.cluster : 148);
     const int64_t all = count[f] * L.splits[f];
     if (all > most) most = all;
     if (L.splits[f] > 1 && all > parts) parts = all;
@@ -803,8 +812,8 @@ NsLayout ns_layout(const nc_newton_schulz* d) {
   // as many CTAs as any product keeps busy, or as share the element-wise passes well
   int64_t blocks = (int64_t)(L.batch * n / 4096);
   if (most > blocks) blocks = most;
-  L.blocks = L.cluster ? kCluster * L.batch : (int)(blocks < 148 ? blocks : 148);
-  L.norms = take((size_t)L.batch * (L.cluster ? kCluster : L.blocks) * 8);
+  L.blocks = L.cluster ? L.cluster * L.batch : (int)(blocks < 148 ? blocks : 148);
+  L.norms = take((size_t)L.batch * (L.cluster ? L.cluster : L.blocks) * 8);
   L.x = take(L.batch * x * 4);
   L.y = take(L.batch * x * 4);
   L.gram = take(L.batch * g * 4);
@@ -871,11 +880,12 @@ nc_status run_tensor(const nc_newton_schulz* d, const T* x, float* momentum, Muo
   auto k = L.cluster ? ns_kernel<T, true> : ns_kernel<T, false>;
   const int smem = L.cluster ? NsEngine<true>::C::kSmem : NsEngine<false>::C::kSmem;
   NC_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  if (L.cluster > 8) NC_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr[1];
   if (L.cluster) {
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = kCluster, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+    attr[0].val.clusterDim.x = L.cluster, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
   } else {
     attr[0].id = cudaLaunchAttributeCooperative;
     attr[0].val.cooperative = 1;
@@ -888,7 +898,7 @@ nc_status run_tensor(const nc_newton_schulz* d, const T* x, float* momentum, Muo
     a.x = x + b * n, a.momentum = momentum ? momentum + b * n : nullptr;
     a.params = params ? params + b * n : nullptr, a.out = out ? out + b * n : nullptr;
     a.first = b == 0;
-    cfg.gridDim = dim3((unsigned)(L.cluster ? kCluster * a.batch : L.blocks));
+    cfg.gridDim = dim3((unsigned)(L.cluster ? L.cluster * a.batch : L.blocks));
     NC_CUDA_CHECK(cudaLaunchKernelEx(&cfg, k, a));
     NC_CHECK(launch_check("ns_kernel launch"));
   }

@@ -253,7 +253,7 @@ def test_offsets_past_32_bits(batch, rows, cols, dtype):
         assert torch.linalg.matrix_norm(got[k].double() - want) <= tol, k
 
 
-@pytest.mark.parametrize("rows,cols", [(96, 1000), (1000, 96), (100, 576), (70, 2000), (128, 1024), (384, 384), (300, 400)])
+@pytest.mark.parametrize("rows,cols", [(96, 1000), (1000, 96), (100, 576), (70, 2000), (128, 1024), (384, 384), (300, 400), (96, 4000), (200, 1500)])
 def test_several_tiles_of_a_cluster(rows, cols):
     # rows past the end leave some warps without work, which then run ahead of the others
     for batch in (1, 5):
