@@ -29,7 +29,10 @@ constexpr int kBK = 64;             // k of a stage: a swizzled row of 128 bytes
 // matrix) the sum of a k-tile comes out short by about 2^-22 of itself.  Given back, the
 // orthogonalised 96 x 4000 matrix is off by 1.3e-6 instead of 1.7e-6.
 constexpr float kRestore = 1.f + 2.3841858e-7f;
-constexpr int kWaitLimit = 1 << 20; // polls of a bounded wait
+#ifndef NC_TC_WAIT_LIMIT
+#define NC_TC_WAIT_LIMIT (1 << 20)
+#endif
+constexpr int kWaitLimit = NC_TC_WAIT_LIMIT; // polls of a bounded wait (a test lets them run out sooner)
 
 // One product of (batched) matrices, D (m, n) = A (m, k) B (n, k)^T.  An operand is stored
 // either with k contiguous, or (a_mn, b_mn) with its own row index contiguous.
@@ -154,7 +157,8 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
 }
 
 // Bounded wait.  Giving up (here or in another warp of the CTA) sets the abort flag and the
-// caller's status word; every role then leaves its loop.
+// caller's status word; every role then leaves its loop.  Lanes poll on their own and may
+// differ in the outcome: a whole warp takes it by warp_wait().
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* abort, int32_t* status) {
   for (int i = 0; i < kWaitLimit; ++i) {
     if (bar_try(bar, parity)) return true;
@@ -163,6 +167,10 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
   *abort = 1;
   *status = 1;
   return false;
+}
+// By a whole warp: true on every lane, or (where any of them gave up) false on every lane.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort, int32_t* status) {
+  return __all_sync(0xffffffffu, bar_wait(bar, parity, abort, status));
 }
 
 // A box into this CTA's shared memory; its bytes count on `bar`, for a pair the first CTA's.
@@ -466,12 +474,12 @@ struct Engine {
     const uint32_t a_step = p.a_mn ? 2048 >> 4 : 32 >> 4, b_step = p.b_mn ? 2048 >> 4 : 32 >> 4;
     const uint32_t a0 = desc_low(stages, p.a_mn, a_block), b0 = desc_low(stages + C::kA, p.b_mn, b_block);
     for (int c0 = x.kt0; c0 < x.kt1; c0 += p.chunk) {
-      if (!(ok = bar_wait(acc_empty(buf), aph, abort, status))) return;
+      if (!(ok = warp_wait(acc_empty(buf), aph, abort, status))) return;
       fence_after();
       const uint32_t d = tmem + buf * BN;
       const int c1 = min(c0 + p.chunk, x.kt1);
       for (int kt = c0; kt < c1; ++kt) {
-        if (!(ok = bar_wait(full(s), ph, abort, status))) return;
+        if (!(ok = warp_wait(full(s), ph, abort, status))) return;
         fence_after();
         const uint32_t a = a0 + s * (C::kStage >> 4), b = b0 + s * (C::kStage >> 4);
         if (elect_one()) {
