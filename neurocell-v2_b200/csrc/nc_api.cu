@@ -4,6 +4,9 @@
 #include <string.h>
 #include <atomic>
 #include <cmath>
+#include <map>
+#include <mutex>
+#include <utility>
 #include <vector>
 
 #include <cuda_runtime.h>
@@ -187,9 +190,21 @@ static bool g_fits(const Geo& g) {
   return sizeof(float) * ((size_t)g.M * g.K + 4 * (size_t)g.M + 128) <= kSmemBudget;
 }
 
-static nc_status set_smem_attr(const void* fn, size_t bytes) {
-  if (bytes <= 48 * 1024) return NC_OK;
-  NC_CUDA_CHECK(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+nc_status allow_smem(const void* kernel, size_t bytes) {
+  if (bytes <= 48 * 1024) return NC_OK;   // every kernel may
+  int dev = 0;
+  NC_CUDA_CHECK(cudaGetDevice(&dev));
+  try {
+    static std::mutex mutex;
+    static std::map<std::pair<const void*, int>, size_t> limits;
+    std::lock_guard<std::mutex> lock(mutex);
+    size_t& limit = limits[{kernel, dev}];
+    const size_t most = limit < bytes ? bytes : limit;
+    NC_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most));
+    limit = most;
+  } catch (...) {
+    return set_error(NC_ERR_CUDA, "no host memory for a kernel's shared memory limit");
+  }
   return NC_OK;
 }
 
@@ -514,7 +529,7 @@ static nc_status vnn_forward(const nc_topo* topo, const void* d_plan, const floa
   const FastKernels fk = universe ? FastKernels{} : fast_kernels(pr.g);
   const void* fn = fk.fwd ? fk.fwd : (const void*)vnn_fused_fwd_kernel;
   const size_t smem = fk.fwd ? fk.fwd_smem : fused_smem_bytes(pr.g, a.g_smem, a.f_smem, a.z_smem);
-  NC_CHECK(set_smem_attr(fn, smem));
+  NC_CHECK(allow_smem(fn, smem));
   if (g_prof.fs) NC_CUDA_CHECK(cudaEventRecord(g_prof.fs, st));
   {
     void* args[] = {&a};
@@ -673,7 +688,7 @@ static nc_status vnn_backward(const nc_topo* topo, const void* d_plan, const flo
   const FastKernels fk = g_universe ? FastKernels{} : fast_kernels(g);
   const void* fn = fk.bwd ? fk.bwd : (const void*)vnn_fused_bwd_kernel;
   const size_t smem = fk.bwd ? fk.bwd_smem : fused_smem_bytes(g, a.g_smem, a.f_smem, a.gz_smem);
-  NC_CHECK(set_smem_attr(fn, smem));
+  NC_CHECK(allow_smem(fn, smem));
   if (g_prof.bs) NC_CUDA_CHECK(cudaEventRecord(g_prof.bs, st));
   {
     FastBwdLayout bl = fk.bl;

@@ -19,6 +19,10 @@ void clear_error();
 void note_launch();
 // After a kernel launch: its error, or NC_OK with the launch counted.
 nc_status launch_check(const char* what);
+// Lets `kernel` take `bytes` of dynamic shared memory on the current device.  The limit belongs
+// to the process: host threads launch one kernel with different sizes, so it is only raised (a
+// call that lowered it between another's raise and launch would have that launch refused).
+nc_status allow_smem(const void* kernel, size_t bytes);
 // Refuses null and misaligned (4 bytes) pointers.
 nc_status check_ptr(const void* p, const char* name);
 // The device address of `p`; memory that the device cannot access is refused.

@@ -1091,12 +1091,6 @@ size_t cols_smem(int Nh, int C) {
   return sizeof(float2) * ((size_t)((TN + 1) & ~1) + (size_t)C * col_line_stride(Nh));
 }
 
-nc_status smem_attr(const void* fn, size_t bytes) {
-  if (bytes > 48 * 1024)
-    NC_CUDA_CHECK(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-  return NC_OK;
-}
-
 // RA of the transform kernels for N-point lines (see fft_ctas): a specialisation for
 // N = 128 ... 512, the run-time variant for 1024.
 int kernel_ra(int N) {
@@ -1109,7 +1103,7 @@ template <int RA>
 nc_status rows_fwd_ra(const Planes& a, float2* dst, int N, const float2* tw, cudaStream_t st) {
   const int L = rows_per_cta(N);
   const size_t smem = rows_smem(N, L);
-  NC_CHECK(smem_attr((const void*)rows_fwd_kernel<RA>, smem));
+  NC_CHECK(allow_smem((const void*)rows_fwd_kernel<RA>, smem));
   const int lines = a.units * a.rows;
   rows_fwd_kernel<RA><<<(lines + L - 1) / L, kFftThreads, smem, st>>>(a, dst, N, tw, L);
   return launched("rows_fwd_kernel launch");
@@ -1119,7 +1113,7 @@ template <int RA>
 nc_status rows_inv_ra(const float2* src, const Planes& a, int N, const float2* tw, cudaStream_t st) {
   const int L = rows_per_cta(N);
   const size_t smem = rows_smem(N, L);
-  NC_CHECK(smem_attr((const void*)rows_inv_kernel<RA>, smem));
+  NC_CHECK(allow_smem((const void*)rows_inv_kernel<RA>, smem));
   const int lines = a.units * a.rows;
   rows_inv_kernel<RA><<<(lines + L - 1) / L, kFftThreads, smem, st>>>(src, a, N, tw, L);
   return launched("rows_inv_kernel launch");
@@ -1155,7 +1149,7 @@ template <int MODE, int RA>
 nc_status cols_ra(const ColArgs& a, int units, const float2* tw, cudaStream_t st) {
   const int C = cols_per_cta(a.Nh, a.Nw, cols_big(MODE, RA));
   const size_t smem = cols_smem(a.Nh, C);
-  NC_CHECK(smem_attr((const void*)cols_kernel<MODE, RA>, smem));
+  NC_CHECK(allow_smem((const void*)cols_kernel<MODE, RA>, smem));
   cols_kernel<MODE, RA><<<dim3(a.Nw / C, units), cols_threads(MODE, RA), smem, st>>>(a, tw, C);
   return launched("cols_kernel launch");
 }

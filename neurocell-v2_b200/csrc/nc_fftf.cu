@@ -953,7 +953,7 @@ nc_status fftf_forward(const FftfArgs& args, cudaStream_t st) {
   const size_t smem = fftf_fwd_smem(a.g, a.stage != 0);
   const void* fn = fixed_acts(a.g) ? (const void*)fftf_fwd_kernel<NC_ACT_TANH, NC_ACT_NONE>
                                    : (const void*)fftf_fwd_kernel<kActRuntime, kActRuntime>;
-  NC_CUDA_CHECK(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  NC_CHECK(allow_smem(fn, smem));
   void* kargs[] = {&a};
   PdlLaunch l(dim3(a.batch), dim3(kThreadsF), smem, st);
   NC_CUDA_CHECK(cudaLaunchKernelExC(&l.cfg, fn, kargs));
@@ -968,7 +968,7 @@ nc_status fftf_backward(const FftfArgs& args, cudaStream_t st) {
   const size_t smem = fftf_bwd_smem(a.g, ring, a.stage != 0);
   const void* fn = fixed_acts(a.g) ? (const void*)fftf_bwd_kernel<NC_ACT_TANH, NC_ACT_NONE>
                                    : (const void*)fftf_bwd_kernel<kActRuntime, kActRuntime>;
-  NC_CUDA_CHECK(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  NC_CHECK(allow_smem(fn, smem));
   void* kargs[] = {&a};
   PdlLaunch l(dim3(a.batch), dim3(kThreadsF), smem, st);
   NC_CUDA_CHECK(cudaLaunchKernelExC(&l.cfg, fn, kargs));

@@ -282,7 +282,7 @@ template <int S, typename T>
 nc_status launch_small(const SmallArgs& a, const SmallPlan& r, int batch, cudaStream_t st) {
   auto k = ns_small_kernel<S, T>;
   const size_t smem = small_smem<S>(r.slice);
-  NC_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  NC_CHECK(allow_smem((const void*)k, smem));
   if (r.ranks > 8) NC_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr[2];
@@ -879,7 +879,7 @@ nc_status run_tensor(const nc_newton_schulz* d, const T* x, float* momentum, Muo
   a.status = reinterpret_cast<int32_t*>(ws + L.status);
   auto k = L.cluster ? ns_kernel<T, true> : ns_kernel<T, false>;
   const int smem = L.cluster ? NsEngine<true>::C::kSmem : NsEngine<false>::C::kSmem;
-  NC_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  NC_CHECK(allow_smem((const void*)k, smem));
   if (L.cluster > 8) NC_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr[1];

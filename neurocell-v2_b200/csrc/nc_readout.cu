@@ -528,13 +528,6 @@ CeArgs make_args(const nc_linear_ce* d, const void* f, const void* w, const void
   return a;
 }
 
-template <typename K>
-nc_status allow_smem(K kernel, size_t bytes) {
-  if (bytes > 48 * 1024)
-    NC_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-  return NC_OK;
-}
-
 // What a call of the streaming kernels takes along.
 struct RowsCall {
   RowArgs args;
@@ -552,13 +545,13 @@ template <typename T, int RN, int VEC, int VT>
 nc_status launch_rows(const RowsCall& c) {
   if (!c.g) {
     auto k = ce_rows_value_kernel<T, RN, VEC, VT>;
-    NC_CHECK(allow_smem(k, c.r.smem_value));
+    NC_CHECK(allow_smem((const void*)k, c.r.smem_value));
     PdlLaunch l(dim3(c.r.blocks), dim3(kRowThreads), c.r.smem_value, c.st);
     NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, k, c.args, c.part, c.zlabel));
     return launch_check("ce_rows_value_kernel launch");
   }
   auto k = ce_rows_grad_kernel<T, RN, VEC, VT>;
-  NC_CHECK(allow_smem(k, c.r.smem_grad));
+  NC_CHECK(allow_smem((const void*)k, c.r.smem_grad));
   PdlLaunch l(dim3(c.r.blocks), dim3(kRowThreads), c.r.smem_grad, c.st);
   NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, k, c.args, c.r.td, c.g->lse, c.g->g_loss, static_cast<T*>(c.g->weight),
                                    static_cast<T*>(c.g->bias), c.df_part));

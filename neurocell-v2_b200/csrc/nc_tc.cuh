@@ -658,7 +658,7 @@ template <int PL, int BN, int CG, int EW, class Epi>
 nc_status launch_product(const Problem& p, const Epi& epi, cudaStream_t st, const char* what) {
   auto k = product_kernel<PL, BN, CG, EW, Epi>;
   constexpr int smem = Config<PL, BN, CG, EW>::kSmem;
-  NC_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  NC_CHECK(allow_smem((const void*)k, smem));
   const int tiles = problem_tiles<BN, CG>(p), most = sm_count() / CG;
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr[2];
