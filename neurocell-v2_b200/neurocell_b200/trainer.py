@@ -501,14 +501,18 @@ class VNNTrainer:
 
     ``apply_fn(params, batch_x, **kw)`` is ``VonNeumannNetwork.apply`` or a closure over
     ``propagate_vnn_2d``; the adaptive and annealed entry points pass ``spatial_mask``,
-    ``codd_mode`` and ``state_temperature`` through it as the reference does."""
+    ``codd_mode`` and ``state_temperature`` through it as the reference does.
+
+    The momentum (``momentum``, a ``VNNParams``) belongs to the parameters it was built on, by
+    their storage: training other tensors starts from zero.  Assign it to go on from a stored
+    one; assign ``None`` after copying new values into the same tensors."""
 
     def __init__(self, apply_fn, lr: float = 1e-2, batch_size: int = 128, loss_fn=None,
                  eval_metric_fn=None, optimizer: str = "sgd", beta: float = 0.95,
                  weight_decay: float = 0.0):
         _check_optimizer(optimizer)
         self.optimizer, self.beta, self.weight_decay = optimizer, float(beta), float(weight_decay)
-        self.momentum = None      # VNNParams of the parameters last trained (muon)
+        self.momentum = None
         self.apply_fn = apply_fn
         self.lr = float(lr)
         self.batch_size = batch_size
@@ -534,13 +538,29 @@ class VNNTrainer:
                 ops.sgd_(params.greens_filters, grads.greens_filters, self.lr)
         return params, loss
 
+    @property
+    def momentum(self) -> VNNParams | None:
+        return self._momentum
+
+    @momentum.setter
+    def momentum(self, value: VNNParams | None) -> None:
+        self._momentum = value
+        self._momentum_of = None      # of whichever parameters are trained next
+
+    def _momentum_for(self, params: VNNParams) -> VNNParams:
+        """The momentum of ``params``, zeros where it is another's.  The parameters are kept
+        (detached) beside it, so that no other tensors come to lie at their addresses."""
+        of = self._momentum_of
+        known = of is None or all(a.data_ptr() == b.data_ptr() and a.shape == b.shape and a.device == b.device
+                                  for a, b in zip(of, params))
+        if self._momentum is None or not known:
+            self._momentum = VNNParams(torch.zeros_like(params.cell_params, requires_grad=False),
+                                       torch.zeros_like(params.greens_filters, requires_grad=False))
+        self._momentum_of = tuple(p.detach() for p in params)
+        return self._momentum
+
     def _muon_update(self, params: VNNParams, grads: VNNParams) -> None:
-        """The momentum starts at zero and lives in the trainer; set ``momentum = None`` to
-        start over."""
-        if self.momentum is None:
-            self.momentum = VNNParams(torch.zeros_like(params.cell_params),
-                                      torch.zeros_like(params.greens_filters))
-        for p, g, m in zip(params, grads, self.momentum):
+        for p, g, m in zip(params, grads, self._momentum_for(params)):
             shape = p.shape if p.ndim == 3 else (p.shape[0], p.numel() // p.shape[0])
             ops.muon_(p.view(shape), g.contiguous().view(shape), m.view(shape), self.lr, beta=self.beta,
                       weight_decay=self.weight_decay)
