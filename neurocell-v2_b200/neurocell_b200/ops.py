@@ -123,6 +123,13 @@ def _output_index(topology: ChipTopology2D) -> tuple[np.ndarray, tuple]:
     return (rr * W + cc).ravel().astype(np.int32), (oh, ow)
 
 
+def subroi_window(topology: ChipTopology2D, roi_bbox) -> tuple:
+    """Grid rows and columns (r0, r1, c0, c1) that a sub-ROI's kernels read: the sub-ROI with
+    its kernel halo."""
+    r0, r1, c0, c1 = (int(v) for v in roi_bbox)
+    return r0, r1 + 2 * topology.pad_h, c0, c1 + 2 * topology.pad_w
+
+
 def _window_tables(topology: ChipTopology2D, roi_bbox, in_idx, out_idx, universe=False):
     """Adaptive sub-ROI (propagator.py:228-241, 343-371) as its own VALID / SAME problem: the
     grid window that holds the sub-ROI and its kernel halo.  Returns the window slice, its
@@ -135,7 +142,7 @@ def _window_tables(topology: ChipTopology2D, roi_bbox, in_idx, out_idx, universe
     H, W = topology.grid_shape
     ph, pw = topology.pad_h, topology.pad_w
     r0, r1, c0, c1 = roi_bbox
-    gr0, gr1, gc0, gc1 = r0, r1 + 2 * ph, c0, c1 + 2 * pw       # grid rows / cols of the window
+    gr0, gr1, gc0, gc1 = subroi_window(topology, roi_bbox)       # grid rows / cols of the window
     wh, ww = gr1 - gr0, gc1 - gc0
 
     def remap(idx, required):

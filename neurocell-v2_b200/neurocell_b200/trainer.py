@@ -505,7 +505,9 @@ class VNNTrainer:
 
     The momentum (``momentum``, a ``VNNParams``) belongs to the parameters it was built on, by
     their storage: training other tensors starts from zero.  Assign it to go on from a stored
-    one; assign ``None`` after copying new values into the same tensors."""
+    one; assign ``None`` after copying new values into the same tensors.  On an adaptive
+    sub-ROI the window's cells are the matrices that are updated; the cells outside it and
+    their momentum stay as they are."""
 
     def __init__(self, apply_fn, lr: float = 1e-2, batch_size: int = 128, loss_fn=None,
                  eval_metric_fn=None, optimizer: str = "sgd", beta: float = 0.95,
@@ -532,7 +534,7 @@ class VNNTrainer:
         loss, grads = self.value_and_grad(params, batch_x, batch_y, **apply_kw)
         with torch.no_grad():
             if self.optimizer == "muon":
-                self._muon_update(params, grads)
+                self._muon_update(params, grads, apply_kw.get("spatial_mask"))
             else:
                 ops.sgd_(params.cell_params, grads.cell_params, self.lr)
                 ops.sgd_(params.greens_filters, grads.greens_filters, self.lr)
@@ -559,11 +561,37 @@ class VNNTrainer:
         self._momentum_of = tuple(p.detach() for p in params)
         return self._momentum
 
-    def _muon_update(self, params: VNNParams, grads: VNNParams) -> None:
+    def _muon_update(self, params: VNNParams, grads: VNNParams, mask_spec=None) -> None:
+        window = self._muon_window(mask_spec)
         for p, g, m in zip(params, grads, self._momentum_for(params)):
-            shape = p.shape if p.ndim == 3 else (p.shape[0], p.numel() // p.shape[0])
-            ops.muon_(p.view(shape), g.contiguous().view(shape), m.view(shape), self.lr, beta=self.beta,
-                      weight_decay=self.weight_decay)
+            if p.ndim == 3 and window is not None:
+                # the window's cells as matrices of their own; momentum and weight decay would
+                # move the cells outside it, which get no gradient
+                r0, r1, c0, c1 = window
+                pw, mw = (t[:, r0:r1, c0:c1].contiguous() for t in (p, m))
+                self._muon_matrices(pw, g[:, r0:r1, c0:c1].contiguous(), mw)
+                p[:, r0:r1, c0:c1].copy_(pw)
+                m[:, r0:r1, c0:c1].copy_(mw)
+            else:
+                shape = p.shape if p.ndim == 3 else (p.shape[0], p.numel() // p.shape[0])
+                self._muon_matrices(p.view(shape), g.contiguous().view(shape), m.view(shape))
+
+    def _muon_matrices(self, p: torch.Tensor, g: torch.Tensor, m: torch.Tensor) -> None:
+        ops.muon_(p, g, m, self.lr, beta=self.beta, weight_decay=self.weight_decay)
+
+    @staticmethod
+    def _muon_window(mask_spec) -> tuple | None:
+        """The cells that a step on ``mask_spec`` trains, as VNNTrainStep's window; None: all."""
+        if mask_spec is None or mask_spec.is_full_roi:
+            return None
+        topology = mask_spec.cropped_topology
+        if topology is None:
+            raise ValueError("optimizer='muon' needs the topology of the spatial mask (cropped_topology)")
+        if topology.padding_mode == "CIRCULAR":
+            return None               # the mask does not apply
+        if not topology.out_in_roi:
+            raise NotImplementedError("optimizer='muon' on a sub-ROI needs output ports inside the ROI")
+        return ops.subroi_window(topology, mask_spec.roi_bbox)
 
     def train_epoch(self, params: VNNParams, x_epoch, y_epoch, **apply_kw):
         """Steps over the batches of ``x_epoch`` / ``y_epoch`` in order (trainer.py:108-119);

@@ -1,5 +1,7 @@
 """``optimizer="muon"`` of VNNTrainer and VNNTrainStep: whose momentum it is, sub-ROIs, ranks and
 the update's own waits."""
+import dataclasses
+
 import numpy as np
 import pytest
 import torch
@@ -77,3 +79,60 @@ def test_momentum_goes_on_through_views_and_may_be_stored():
         t.copy_(v)
     tr.momentum = None
     assert _same(_run(tr, q, x, y, steps=4), want)
+
+
+@pytest.mark.parametrize("annealed", [False, True])
+@pytest.mark.parametrize("decay", [0.0, 0.1])
+def test_a_sub_roi_keeps_the_cells_outside(decay, annealed):
+    """A step on all cells, then steps on a sub-ROI: the cells outside the window and their
+    momentum keep their bits; inside, the update of the window as matrices of its own, as
+    VNNTrainStep takes it."""
+    topo = nc.ChipTopology2D.alu_chip()
+    spec = nc.compute_adaptive_spatial_mask(nc.init_vnn_params(701, topo, device=DEV), topo)
+    assert not spec.is_full_roi
+    x, y = _batch(32, 4)
+    codd = dict(codd_mode="annealed", state_temperature=0.7) if annealed else {}
+    tr, p = _trainer(weight_decay=decay), _params(6)
+    p, _ = tr.train_step(p, x, y, **codd)
+    st = nc.VNNTrainStep(topo, p, 32, lr=0.02, in_shapes=((8, 1),) * 3, spatial_mask=spec, optimizer="muon",
+                         weight_decay=decay, **codd)
+    r0, r1, c0, c1 = st.window
+    assert r1 - r0 != c1 - c0      # the step's factor sqrt(rows / cols) is the window's own
+    inside = torch.zeros(62, 62, dtype=torch.bool, device=DEV)
+    inside[r0:r1, c0:c1] = True
+    st.momentum[: st.n_cell].copy_(tr.momentum.cell_params[:, r0:r1, c0:c1].reshape(-1))
+    st.momentum[st.n_cell:].copy_(tr.momentum.greens_filters.reshape(-1))
+    before, mom = p.cell_params.clone(), tr.momentum.cell_params.clone()
+    for _ in range(2):
+        _, grads = tr.value_and_grad(p, x, y, spatial_mask=spec, **codd)
+        assert not grads.cell_params[:, ~inside].any()
+        want, m = (t[:, r0:r1, c0:c1].contiguous() for t in (p.cell_params, tr.momentum.cell_params))
+        ops.muon_(want, grads.cell_params[:, r0:r1, c0:c1].contiguous(), m, 0.02, weight_decay=decay)
+        if annealed:
+            tr.train_step_annealed(p, x, y, state_temperature=0.7, mask_spec=spec)
+        else:
+            tr.train_step_adaptive(p, x, y, spec)
+        assert torch.equal(p.cell_params[:, r0:r1, c0:c1], want)
+        st.step(x, y)
+    assert torch.equal(p.cell_params[:, ~inside], before[:, ~inside])
+    assert torch.equal(tr.momentum.cell_params[:, ~inside], mom[:, ~inside])
+    assert not torch.equal(p.cell_params, before)
+    assert _same(st.params, p)
+
+
+def test_sub_rois_that_cannot_be_updated_are_refused():
+    topo = nc.ChipTopology2D.alu_chip()
+    x, y = _batch(4, 4)
+    tr, p = _trainer(), _params(6)
+    spec = dataclasses.replace(nc.compute_adaptive_spatial_mask(nc.init_vnn_params(701, topo, device=DEV), topo),
+                               cropped_topology=None)
+    before = p.cell_params.clone()
+    with pytest.raises(ValueError, match="topology"):
+        tr.train_step_adaptive(p, x, y, spec)
+    outer = dataclasses.replace(spec, cropped_topology=dataclasses.replace(topo, out_in_roi=False))
+    with pytest.raises(NotImplementedError, match="output ports"):
+        tr.train_step_adaptive(p, x, y, outer)
+    assert torch.equal(p.cell_params, before)
+    # CIRCULAR chips take no mask: all cells are trained
+    ring = dataclasses.replace(spec, cropped_topology=dataclasses.replace(topo, padding_mode="CIRCULAR"))
+    assert tr._muon_window(ring) is None
