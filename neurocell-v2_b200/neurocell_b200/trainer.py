@@ -282,7 +282,7 @@ class VNNTrainStep:
         self.flat[self.n_cell:].copy_(params.greens_filters.reshape(-1))
         self.grads = torch.zeros_like(self.flat)
         # muon: (descriptor, offset) of the cells and of the filters, their momentum and workspace
-        self.momentum = None
+        self.momentum, self._muon_ws = None, []
         if optimizer == "muon":
             self.beta, self.weight_decay = float(beta), float(weight_decay)
             m = params.greens_filters.shape[0]
@@ -369,7 +369,10 @@ class VNNTrainStep:
                                             P(self.x), self.B, c.byref(self.codd), P(self.g_out),
                                             c.c_void_p(gcell), c.c_void_p(gfilt), P(self.ws),
                                             self.ws_bytes, st), "nc_vnn_backward")
-        timed = self.exchange_events is not None and not torch.cuda.is_current_stream_capturing()
+        capturing = torch.cuda.is_current_stream_capturing()
+        if not capturing:
+            ops._after_call(self.ws, "nc_vnn_forward / nc_vnn_backward")
+        timed = self.exchange_events is not None and not capturing
         if timed:
             self.exchange_events[0].record()
         if self.exchange is not None:
@@ -384,6 +387,8 @@ class VNNTrainStep:
                         c.byref(d), c.c_void_p(cell + 4 * at), c.c_void_p(gcell + 4 * at),
                         c.c_void_p(self.momentum.data_ptr() + 4 * at), self.lr, self.beta, 1,
                         self.weight_decay, P(ws), ws.numel(), st), "nc_muon_update")
+                    if not capturing:
+                        ops._after_call(ws, "nc_muon_update")
             else:
                 lr = self.lr / world            # mean of the per-rank mean-loss gradients
                 self._lib.check(lib.nc_sgd_update(c.c_void_p(cell), c.c_void_p(gcell),
@@ -436,6 +441,12 @@ class VNNTrainStep:
         if momentum is not None:
             self.momentum.copy_(momentum)
         self.graph = g
+
+    def wait_status(self) -> int:
+        """Status of the bounded waits of the latest step, replayed ones included: 0, or 1 where a
+        kernel of the forward, the backward or the update gave one up (the parameters are then
+        invalid).  Synchronises; not for the hot path."""
+        return max(ops.workspace_status(ws) for ws in (self.ws, *self._muon_ws))
 
     def exchange_status(self) -> int:
         """Status word of the NVLink exchange (0 ok, 1 a peer timed out); 0 without one."""

@@ -136,3 +136,40 @@ def test_sub_rois_that_cannot_be_updated_are_refused():
     # CIRCULAR chips take no mask: all cells are trained
     ring = dataclasses.replace(spec, cropped_topology=dataclasses.replace(topo, padding_mode="CIRCULAR"))
     assert tr._muon_window(ring) is None
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_the_updates_waits_are_seen(captured):
+    """The update's workspaces have status words of their own; here a host write stands for a wait
+    that ran out."""
+    x, y = _batch(16, 1)
+    st = nc.VNNTrainStep(nc.ChipTopology2D.alu_chip(), _params(3), 16, lr=0.02, in_shapes=((8, 1),) * 3,
+                         optimizer="muon")
+    if captured:
+        st.load_batch(x, y)
+        st.capture()
+    st.step(x, y)
+    assert st.wait_status() == 0
+    for ws in (st.ws, *st._muon_ws):
+        ws[:4].view(torch.int32).fill_(1)
+        assert st.wait_status() == 1
+        st.step(x, y)                       # each step clears them
+        assert st.wait_status() == 0
+
+
+def test_an_eager_step_checks_its_waits(monkeypatch):
+    x, y = _batch(16, 1)
+    st = nc.VNNTrainStep(nc.ChipTopology2D.alu_chip(), _params(3), 16, lr=0.02, in_shapes=((8, 1),) * 3,
+                         optimizer="muon")
+    monkeypatch.setattr(ops, "CHECK_WAIT_STATUS", True)
+    n = ops.STATUS_CHECKS
+    st.step(x, y)
+    assert ops.STATUS_CHECKS == n + 3         # propagation, cells, filters
+    st.capture()
+    st.step(x, y)
+    real = ops.workspace_status
+    monkeypatch.setattr(ops, "workspace_status", lambda ws: int(ws is st._muon_ws[1]) or real(ws))
+    assert st.wait_status() == 1
+    st.release()
+    with pytest.raises(RuntimeError, match="nc_muon_update"):
+        st.step(x, y)
