@@ -427,9 +427,9 @@ class VNNTrainStep:
             import torch.distributed as dist
             torch.cuda.synchronize(self.device)
             dist.barrier(group=self.pg)      # ranks enter the first exchange together
-        s = torch.cuda.Stream(self.device)
-        s.wait_stream(torch.cuda.current_stream(self.device))
         saved, momentum = self.flat.clone(), None if self.momentum is None else self.momentum.clone()
+        s = torch.cuda.Stream(self.device)
+        s.wait_stream(torch.cuda.current_stream(self.device))     # behind the copies
         with torch.cuda.stream(s):
             for _ in range(2):
                 self._launch()
@@ -468,9 +468,9 @@ class VNNTrainStep:
             import torch.distributed as dist
             torch.cuda.synchronize(self.device)
             dist.barrier(group=self.pg)
-        s = torch.cuda.Stream(self.device)
-        s.wait_stream(torch.cuda.current_stream(self.device))
         saved, momentum = self.flat.clone(), None if self.momentum is None else self.momentum.clone()
+        s = torch.cuda.Stream(self.device)
+        s.wait_stream(torch.cuda.current_stream(self.device))     # behind the copies
         with torch.cuda.stream(s):
             for i in range(min(nb, 2)):      # warm-up (kernel attributes, lazy loading)
                 self.x.copy_(xs[i])

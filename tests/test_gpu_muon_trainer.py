@@ -173,3 +173,34 @@ def test_an_eager_step_checks_its_waits(monkeypatch):
     st.release()
     with pytest.raises(RuntimeError, match="nc_muon_update"):
         st.step(x, y)
+
+
+@pytest.mark.parametrize("optimizer", ["sgd", "muon"])
+@pytest.mark.parametrize("epoch", [False, True])
+def test_a_capture_saves_the_parameters_before_its_warm_up(epoch, optimizer, monkeypatch):
+    """The warm-up steps run on a stream of their own, which has to wait for the copies: here what
+    follows the stream's wait on the current one is held up for about 50 ms."""
+    x, y = _batch(16, 1)
+    p = _params(3)
+    st = nc.VNNTrainStep(nc.ChipTopology2D.alu_chip(), p, 16, lr=0.5, in_shapes=((8, 1),) * 3, optimizer=optimizer)
+    st.load_batch(x, y)
+    st.step()
+    before = st.flat.clone()
+    mom = None if st.momentum is None else st.momentum.clone()
+    torch.cuda.synchronize()
+    real = torch.cuda.Stream.wait_stream
+
+    def wait_stream(self, other):
+        real(self, other)
+        if self != torch.cuda.current_stream():
+            torch.cuda._sleep(100_000_000)
+
+    with monkeypatch.context() as patch:
+        patch.setattr(torch.cuda.Stream, "wait_stream", wait_stream)
+        if epoch:
+            st.capture_epoch(x[None], y[None])
+        else:
+            st.capture()
+    torch.cuda.synchronize()
+    assert torch.equal(st.flat, before)
+    assert mom is None or torch.equal(st.momentum, mom)
