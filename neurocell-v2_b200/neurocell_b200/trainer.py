@@ -286,7 +286,10 @@ class VNNTrainStep:
         if optimizer == "muon":
             self.beta, self.weight_decay = float(beta), float(weight_decay)
             m = params.greens_filters.shape[0]
-            self._muon = [(ops._newton_schulz_desc(shape, "float32", 5, ops.NEWTON_SCHULZ_COEFFICIENTS, 1e-7), at)
+            # the gradients are sums over the ranks, so the momentum is `world` times that of their
+            # mean; with eps as many times as large the orthogonalised update is the mean's
+            eps = 1e-7 * self.world
+            self._muon = [(ops._newton_schulz_desc(shape, "float32", 5, ops.NEWTON_SCHULZ_COEFFICIENTS, eps), at)
                           for shape, at in ((tuple(cell.shape), 0), ((m, self.n_filt // m), self.n_cell))]
             self.momentum = torch.zeros_like(self.flat)
             self._muon_ws = [ops._newton_schulz_ws(self.lib, d, dev) for d, _ in self._muon]
@@ -381,7 +384,6 @@ class VNNTrainStep:
         else:
             world = allreduce_mean_(self.grads, self.pg)
             if self.momentum is not None:
-                # an orthogonalised update does not depend on the gradient's scale (1 / world)
                 for (d, at), ws in zip(self._muon, self._muon_ws):
                     self._lib.check(lib.nc_muon_update(
                         c.byref(d), c.c_void_p(cell + 4 * at), c.c_void_p(gcell + 4 * at),

@@ -204,3 +204,36 @@ def test_a_capture_saves_the_parameters_before_its_warm_up(epoch, optimizer, mon
     torch.cuda.synchronize()
     assert torch.equal(st.flat, before)
     assert mom is None or torch.equal(st.momentum, mom)
+
+
+def _step_of(world, monkeypatch, **kw):
+    """A step whose ranks all hold the same batch: the exchange's sum is `world` times its gradient."""
+    from neurocell_b200 import trainer
+
+    def exchange(flat, group=None):
+        flat.mul_(world)
+        return world
+
+    monkeypatch.setattr(trainer, "allreduce_mean_", exchange)
+    monkeypatch.setattr(torch.distributed, "get_world_size", lambda group=None: world)
+    return nc.VNNTrainStep(nc.ChipTopology2D.alu_chip(), _params(3), 16, lr=0.02, in_shapes=((8, 1),) * 3,
+                           optimizer="muon", process_group=object(), weight_decay=0.1, **kw)
+
+
+@pytest.mark.parametrize("world", [2, 8])
+def test_ranks_take_the_step_of_the_mean_gradient(world, monkeypatch):
+    """Ranks on the same batch step as one does.  Powers of two scale momentum, norm and eps without
+    a rounding, so the bits are the same."""
+    x, y = _batch(16, 1)
+    flats = []
+    for n in (1, world):
+        st = _step_of(n, monkeypatch)
+        for _ in range(3):
+            st.step(x, y)
+        flats.append((st.flat.clone(), st.momentum / n))
+    assert _same(*flats)
+
+
+def test_the_fused_exchange_is_refused_with_muon(monkeypatch):
+    with pytest.raises(NotImplementedError, match="nvlink"):
+        _step_of(2, monkeypatch, exchange="nvlink")
