@@ -400,9 +400,10 @@ __global__ void __launch_bounds__(kRowThreads) ce_rows_grad_kernel(
   }
 }
 
-// df: the CTAs' parts, 8 threads an element, in a fixed order.
+// df: the CTAs' parts, 8 threads an element, in a fixed order; 0 in rows that take no part, whatever
+// the weight (0 times an infinity) and g_loss hold.
 template <typename T>
-__global__ void __launch_bounds__(256) ce_sum_parts_kernel(const float* __restrict__ part, int n, int slots,
+__global__ void __launch_bounds__(256) ce_sum_parts_kernel(CeArgs a, const float* __restrict__ part, int n, int slots,
                                                            T* __restrict__ out) {
   __shared__ float sm[8][32];
   pdl_enter();
@@ -417,7 +418,7 @@ __global__ void __launch_bounds__(256) ce_sum_parts_kernel(const float* __restri
   if (g != 0 || i >= n) return;
 #pragma unroll
   for (int k = 1; k < 8; ++k) s += sm[k][threadIdx.x];
-  store_as(out + i, s);
+  store_as(out + i, ce_kept(a, i / a.dim) ? s : 0.f);
 }
 
 struct RowsPlan {
@@ -608,10 +609,10 @@ nc_status gradients(const nc_linear_ce* d, const CeArgs& a, const CeGrads& g, ch
   const int n = d->rows * d->dim;
   PdlLaunch l(dim3((n + 31) / 32), dim3(256), 0, st);
   if (bf16)
-    NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, ce_sum_parts_kernel<__nv_bfloat16>, (const float*)c.df_part, n, c.r.blocks,
+    NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, ce_sum_parts_kernel<__nv_bfloat16>, a, (const float*)c.df_part, n, c.r.blocks,
                                      static_cast<__nv_bfloat16*>(g.features)));
   else
-    NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, ce_sum_parts_kernel<float>, (const float*)c.df_part, n, c.r.blocks,
+    NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, ce_sum_parts_kernel<float>, a, (const float*)c.df_part, n, c.r.blocks,
                                      static_cast<float*>(g.features)));
   return launch_check("ce_sum_parts_kernel launch");
 }

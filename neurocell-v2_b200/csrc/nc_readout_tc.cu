@@ -590,18 +590,20 @@ struct FeatureEpilogue {
   }
 };
 
+// df: the splits' parts in order; 0 in rows that take no part, whatever the weight (0 times an
+// infinity) and g_loss hold.
 template <typename T>
-__global__ void __launch_bounds__(256) ce_features_kernel(const float* __restrict__ part, int splits, int rows, int dim,
+__global__ void __launch_bounds__(256) ce_features_kernel(CeArgs a, const float* __restrict__ part, int splits,
                                                           int pitch, const Scales* __restrict__ scales,
                                                           T* __restrict__ out) {
   pdl_enter();
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= (int64_t)rows * dim) return;
-  const int row = (int)(i / dim), c = (int)(i - (int64_t)row * dim);
+  if (i >= (int64_t)a.rows * a.dim) return;
+  const int row = (int)(i / a.dim), c = (int)(i - (int64_t)row * a.dim);
   float s = 0.f;
 #pragma unroll 8
-  for (int k = 0; k < splits; ++k) s += part[((size_t)k * rows + row) * pitch + c];
-  store_as(out + i, s * scales->g);
+  for (int k = 0; k < splits; ++k) s += part[((size_t)k * a.rows + row) * pitch + c];
+  store_as(out + i, ce_kept(a, row) ? s * scales->g : 0.f);
 }
 
 template <typename T>
@@ -752,8 +754,8 @@ struct Call {
     if (g.features) {
       const int64_t n = (int64_t)d->rows * d->dim;
       PdlLaunch l(dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st);
-      NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, ce_features_kernel<T>, (const float*)at<float>(p.df_part), p.splits,
-                                       d->rows, d->dim, p.pitch, (const Scales*)scales(),
+      NC_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, ce_features_kernel<T>, a, (const float*)at<float>(p.df_part), p.splits,
+                                       p.pitch, (const Scales*)scales(),
                                        static_cast<T*>(g.features)));
       NC_CHECK(launch_check("ce_features_kernel launch"));
     }
