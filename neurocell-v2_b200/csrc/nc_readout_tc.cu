@@ -33,6 +33,7 @@ constexpr int kPrepThreads = 256;
 constexpr int kMaxBlocks = 296;        // blocks of the largest-value pass, per tensor
 constexpr float kDzScale = 32768.f;    // dz planes hold dz 2^15 (|dz| <= 1)
 constexpr int kChunk = 3;              // k-tiles (of 64) per accumulator beside float32 operands
+constexpr int kLogitChunk = 32;        // of bfloat16 logits: the loss is float32 (see tc::kLongChunk)
 constexpr size_t kPieceBytes = 160u << 20;  // most that dz of one piece takes
 constexpr int kMaxSplits = 48;
 
@@ -641,7 +642,7 @@ struct Call {
     tc::Problem q{};
     q.m = m, q.n = n, q.k = k, q.batch = 1, q.splits = splits, q.bf16 = p.bf16;
     tc::set_tiles<BN, CG>(&q);
-    q.chunk = PL == 1 ? 1 << 30 : kChunk;
+    q.chunk = PL == 1 ? tc::kLongChunk : kChunk;
     q.status = a.status;
     return q;
   }
@@ -693,6 +694,7 @@ struct Call {
     tc::Problem q = problem<BN, CG, EW>(d->rows, d->classes, d->dim, 1);
     NC_CHECK((features_op<BN, CG, EW>(&q, true, false)));
     NC_CHECK((weight_op<BN, CG, EW>(&q, false)));
+    if (PL == 1) q.chunk = kLogitChunk;
     const ValueEpilogue e{a, scales(), at<float>(p.bias), at<float2>(p.part), at<float>(p.zlabel), p.rows_pad};
     return tc::launch_product<PL, BN, CG, EW>(q, e, st, "readout value product launch");
   }
@@ -712,6 +714,7 @@ struct Call {
     NC_CHECK((features_op<BN, CG, EW>(&q, true, false)));
     NC_CHECK((weight_op<BN, CG, EW>(&q, false)));
     q.b_n0 = v0;
+    if (PL == 1) q.chunk = kLogitChunk;
     const DzEpilogue<PL == 1> e{a,     scales(), at<float>(p.bias), g.lse,  at<float>(p.fac), at<uint16_t>(p.dz),
                                 g.bias ? at<float>(p.db_part) : nullptr, v0, p.piece, p.classes_pad};
     return tc::launch_product<PL, BN, CG, EW>(q, e, st, "readout logit gradient launch");

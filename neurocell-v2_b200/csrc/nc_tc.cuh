@@ -7,9 +7,10 @@
 // exact as float32 multiplications, for three 16-bit products (three bfloat16 planes would
 // take six).  bfloat16 operands are one plane and one product.
 //
-// The tensor core adds in float32 but not to nearest, which shows in long sums; with two
-// planes the accumulator is therefore drained every `chunk` k-tiles into float32 registers
-// (added to nearest there) while the other half of tensor memory takes the next chunk.
+// The tensor core adds in float32 but not to nearest, which shows in long sums; the accumulator is
+// therefore drained every `chunk` k-tiles into float32 registers (added to nearest there) while
+// the other half of tensor memory takes the next chunk.  One plane has long chunks (kLongChunk),
+// and most of its products are one.
 #pragma once
 
 #include <cuda.h>
@@ -29,6 +30,10 @@ constexpr int kBK = 64;             // k of a stage: a swizzled row of 128 bytes
 // matrix) the sum of a k-tile comes out short by about 2^-22 of itself.  Given back, the
 // orthogonalised 96 x 4000 matrix is off by 1.3e-6 instead of 1.7e-6.
 constexpr float kRestore = 1.f + 2.3841858e-7f;
+// k-tiles per accumulator of one plane.  A sum of one sign comes out short by about 4e-7 of itself per
+// k-tile of its accumulator: 5e-5 here, a fortieth of a bfloat16 rounding (2^20 terms in one
+// accumulator: 6.5e-3).
+constexpr int kLongChunk = 128;
 #ifndef NC_TC_WAIT_LIMIT
 #define NC_TC_WAIT_LIMIT (1 << 20)
 #endif
@@ -503,7 +508,9 @@ struct Engine {
     }
   }
 
-  // An epilogue warp: the sums of its 32 rows and COLS columns.
+  // An epilogue warp: the sums of its 32 rows and COLS columns.  DRAIN: of several chunks; one alone
+  // (one plane) needs no second set of registers.
+  template <bool DRAIN = PL == 2>
   __device__ __forceinline__ void collect(const Problem& p, const Tile& x, float (&acc)[COLS]) {
     const int warp = threadIdx.x >> 5;
     const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + (warp >> 2) * COLS;
@@ -520,7 +527,7 @@ struct Engine {
         float v[32];
         tmem_load(lanes + buf * BN + i, v);
 #pragma unroll
-        for (int j = 0; j < 32; ++j) acc[i + j] = PL == 1 ? v[j] : fmaf(v[j], kRestore, acc[i + j]);   // one plane, one chunk
+        for (int j = 0; j < 32; ++j) acc[i + j] = DRAIN ? fmaf(v[j], PL == 1 ? 1.f : kRestore, acc[i + j]) : v[j];
       }
       fence_before();
       if ((threadIdx.x & 31) == 0) {
@@ -599,7 +606,7 @@ struct Engine {
 // persistent over tiles.  Epi::run(state, tile, row, col, acc) gets COLS consecutive columns of a row as
 // float32 sums; Epi::begin(tile, row, col, patch) runs before the wait for them and returns the
 // state.
-template <int PL, int BN, int CG, int EW, class Epi>
+template <int PL, int BN, int CG, int EW, class Epi, bool DRAIN>
 __global__ void __launch_bounds__(32 * (EW + 2), 1) product_kernel(const __grid_constant__ Problem p, const Epi epi) {
   using E = Engine<PL, BN, CG, EW>;
   extern __shared__ __align__(1024) uint8_t raw[];
@@ -622,7 +629,7 @@ __global__ void __launch_bounds__(32 * (EW + 2), 1) product_kernel(const __grid_
       const auto state = epi.template begin<E::COLS>(x, row, col, e.patch);
       __syncwarp();
       float acc[E::COLS];
-      e.collect(p, x, acc);
+      e.template collect<DRAIN>(p, x, acc);
       if (e.ok) epi.template run<E::COLS>(state, x, row, col, acc);
     }
   }
@@ -656,7 +663,11 @@ __host__ __device__ inline void set_tiles(Problem* p) {
 
 template <int PL, int BN, int CG, int EW, class Epi>
 nc_status launch_product(const Problem& p, const Epi& epi, cudaStream_t st, const char* what) {
-  auto k = product_kernel<PL, BN, CG, EW, Epi>;
+  auto k = product_kernel<PL, BN, CG, EW, Epi, true>;
+  if constexpr (PL == 1) {
+    const int kt = (p.k + kBK - 1) / kBK;
+    if ((kt + p.splits - 1) / p.splits <= p.chunk) k = product_kernel<PL, BN, CG, EW, Epi, false>;
+  }
   constexpr int smem = Config<PL, BN, CG, EW>::kSmem;
   NC_CHECK(allow_smem((const void*)k, smem));
   const int tiles = problem_tiles<BN, CG>(p), most = sm_count() / CG;

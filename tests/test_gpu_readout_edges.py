@@ -41,3 +41,59 @@ def test_ignored_rows_have_no_gradient_whatever_the_others_hold(rows, what, dtyp
     if what == "weight":
         gf = ops.linear_softmax_ce_value_and_grad(f.detach(), w, lab)[1]
         assert (gf[1::2] == 0).all() and gf[0].isnan().any()
+
+
+# Long sums of bfloat16 operands.  Terms of one sign, so that what each addition loses adds up: a
+# float32 accumulator that rounds toward zero loses on average half of 2^-24 to 2^-23 of itself per
+# addition.  The mean error over many elements shows it; the roundings to nearest of dz and of the
+# result (2^-9 at most each) have random signs and leave 2^-9 / sqrt(elements), eight of which are allowed
+# beside 2^-14 for the sums.
+def _positive(*shape, gen):
+    return (torch.rand(*shape, device=DEV, generator=gen) + 0.5).to(torch.bfloat16)
+
+
+@pytest.mark.parametrize("rows,dim,classes", [(1 << 18, 16, 300), (1 << 18, 200, 600)])
+def test_a_weight_gradient_sums_many_rows(rows, dim, classes):
+    gen = torch.Generator(DEV).manual_seed(1)
+    f = _positive(rows, dim, gen=gen)
+    w = (torch.randn(classes, dim, device=DEV, generator=gen) * 1.2 / dim ** 0.5).to(torch.bfloat16)
+    lab = torch.zeros(rows, dtype=torch.int32, device=DEV)
+    gw = ops.linear_softmax_ce_value_and_grad(f, w, lab, reduction="sum")[2]
+    exact = torch.zeros(classes, dim, dtype=torch.float64, device=DEV)
+    for a in range(0, rows, 1 << 16):
+        fd = f[a:a + (1 << 16)].double()
+        p = torch.softmax(fd @ w.double().T, 1)
+        p[:, 0] -= 1
+        exact += p.T @ fd
+    off = ((gw.double() - exact) / exact)[1:]
+    assert abs(float(off.mean())) <= 8 * 2.0 ** -9 / off.numel() ** 0.5 + 2.0 ** -14
+
+
+def test_a_feature_gradient_sums_many_classes():
+    rows, dim, classes = 256, 4096, 200_000
+    gen = torch.Generator(DEV).manual_seed(2)
+    f = (torch.randn(rows, dim, device=DEV, generator=gen) / dim ** 0.5).to(torch.bfloat16)
+    w = _positive(classes, dim, gen=gen)
+    lab = torch.randint(0, classes, (rows,), device=DEV, generator=gen)
+    gf = ops.linear_softmax_ce_value_and_grad(f, w, lab, reduction="sum")[1]
+    z = torch.cat([f.double() @ w[a:a + 20_000].double().T for a in range(0, classes, 20_000)], 1)
+    p = torch.softmax(z, 1)
+    exact = -w[lab].double()
+    for a in range(0, classes, 20_000):
+        exact += p[:, a:a + 20_000] @ w[a:a + 20_000].double()
+    # the sum of p w is about 1 in every element
+    off = gf.double() - exact
+    assert abs(float(off.mean())) <= 8 * 2.0 ** -9 / off.numel() ** 0.5 + 2.0 ** -14
+
+
+def test_a_logit_sums_a_long_dim():
+    rows, dim, classes = 40, 1 << 17, 300
+    gen = torch.Generator(DEV).manual_seed(3)
+    f = _positive(rows, dim, gen=gen)
+    size = torch.linspace(0, 20, classes, device=DEV)[:, None] / dim
+    w = (_positive(classes, dim, gen=gen) * size).to(torch.bfloat16)
+    lab = torch.randint(0, 20, (rows,), device=DEV, generator=gen)
+    loss = ops.linear_softmax_ce_loss(f, w, lab, reduction="none")
+    z = f.double() @ w.double().T
+    exact = torch.logsumexp(z, 1) - z.gather(1, lab[:, None])[:, 0]
+    assert (loss.double() - exact).abs().max() <= 2.0 ** -14 * float(z.max()) + 2.0 ** -20 * float(exact.max())
