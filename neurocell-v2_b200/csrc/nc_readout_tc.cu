@@ -538,7 +538,7 @@ struct WeightEpilogue {
       if (col + j >= dim) break;
       const int cols = min(kGroup, dim - col - j);
 #pragma unroll
-      for (int e = 0; e < kGroup; ++e) v[j + e] *= st.scale * st.g;
+      for (int e = 0; e < kGroup; ++e) v[j + e] = v[j + e] * st.scale * st.g;   // a power of two first: exact
       if (wide) {
         T* o = out + (size_t)row0 * dim + col + j;
         if constexpr (sizeof(T) == 4) {

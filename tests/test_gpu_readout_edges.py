@@ -97,3 +97,18 @@ def test_a_logit_sums_a_long_dim():
     z = f.double() @ w.double().T
     exact = torch.logsumexp(z, 1) - z.gather(1, lab[:, None])[:, 0]
     assert (loss.double() - exact).abs().max() <= 2.0 ** -14 * float(z.max()) + 2.0 ** -20 * float(exact.max())
+
+
+@pytest.mark.parametrize("exponent", [112, -112, 90, -90])
+@pytest.mark.parametrize("rows", [4, 140])
+def test_far_scales_that_meet_in_the_logits(rows, exponent):
+    """Features of 2^e and a weight of 2^-e: logits of ordinary size.  Relative to the largest entry of
+    each result: sums of `dim`, `rows` or `classes` products as float32 ones, 2^-20 of their size."""
+    f, w, lab = _inputs(rows, 40, 90, torch.float32, seed=5)
+    f, w = f * 2.0 ** exponent, w * (0.3 * 2.0 ** -exponent)
+    loss, gf, gw, _ = ops.linear_softmax_ce_value_and_grad(f, w, lab)
+    fd, wd = f.double().requires_grad_(), w.double().requires_grad_()
+    want = torch.nn.functional.cross_entropy(fd @ wd.T, lab)
+    assert abs(float(loss) - float(want.detach())) <= 2.0 ** -20 * 10
+    for got, e in zip((gf, gw), torch.autograd.grad(want, (fd, wd))):
+        assert (got.double() - e).abs().max() <= 2.0 ** -18 * e.abs().max()
