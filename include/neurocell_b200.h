@@ -274,7 +274,9 @@ typedef enum nc_reduction { NC_REDUCE_MEAN = 0, NC_REDUCE_SUM = 1, NC_REDUCE_NON
  * Precision with float32 operands and more than 16 rows: as of float32 products, where the
  * entries of a tensor below 2^-18 of its largest finite one count with an absolute error of
  * 2^-38 of that one, and dz = p - onehot with one of at most 2^-40 of the largest |g_loss|
- * (gradients are computed relative to that one: an infinite g_loss makes them all NaN).
+ * (gradients are computed relative to that one: an infinite g_loss makes them all NaN, but for
+ * the features' in ignored rows, which are 0 always).  An infinity in the features or the weight
+ * makes the logits it enters NaN there.
  * What a call writes (loss, lse, gradients, workspace) overlaps nothing else of it.
  * Sizes up to 2^24 rows, classes and dim, 2^44 logits, 2^38 elements of features or weight.
  */

@@ -309,8 +309,8 @@ nc_status launch_small(const SmallArgs& a, const SmallPlan& r, int batch, cudaSt
 // a launch, its set-up of tensor memory and its first loads as much again.  Between products
 // the grid meets (cooperative_groups); the symmetric ones compute the tiles on and above the
 // diagonal and store them twice; a product with fewer tiles than SMs is split along k, its
-// float32 parts summed in order by the whole grid.  2001 x 513 takes 286 us (19 a product, mostly
-// meetings, split sums, fill and drain), three 1024 x 1024 updates 482 us, three
+// float32 parts summed in order by the whole grid.  2001 x 513 takes 280 us (18 a product, mostly
+// meetings, split sums, fill and drain), three 1024 x 1024 updates 455 us, three
 // 256 x 256 on a cluster each 133 us.
 constexpr float kPlaneScale = 4096.f, kPlaneInv = 1.f / 4096.f;
 constexpr int kNsChunk = 1;  // k-tiles (of 64) per accumulator: Gram sums of one sign show the additions' truncation

@@ -3,23 +3,28 @@
 //   value:     z tile = features weight^T; the epilogue keeps each row's (maximum, sum of exp)
 //              over its half of the tile's classes, and the label's logit.
 //   gradient:  the classes go by in pieces.  A piece's logits are computed again and their
-//              epilogue writes dz = f_n (exp(z - lse) - onehot) as 16-bit planes, small
-//              enough to stay in L2; two products read them there, dw = dz^T features (whole
-//              for the piece) and df += dz weight (split over the piece's classes, parts
-//              summed in order at the end).
+//              epilogue writes dz = f_n (exp(z - lse) - onehot) as 16-bit planes; two
+//              products read them soon after, dw = dz^T features (whole for the piece) and df
+//              += dz weight (split over the piece's classes, parts summed in order at the end).
+//              A piece's dz takes up to 160 MB beside 126 MB of L2 (2048 x 512 x 32768: 134 MB),
+//              so part of it comes from memory again; pieces that fit L2 measured slower.
 //
 // float32 operands are two float16 planes each, scaled by a power of two that brings the
 // tensor's largest finite value to [2^13, 2^14): an entry down to 2^-18 of it keeps float32's
 // precision, smaller ones an absolute error of 2^-38 of it.  bfloat16 operands are used as
-// they are, and dz is rounded to bfloat16 (2^-9 of an entry, as the products read it).
+// they are, and dz is rounded to bfloat16 (2^-9 of an entry, as the products read it); their sums
+// leave the accumulator every 128 k-tiles, logits every 32 (tc::kLongChunk).
 // Bound by the tensor pipe where rows, dim and classes are large: 2048 x 512 x 32768 in float32
-// takes 0.78 ms in a burst and 0.92 ms at the power cap (895 TFLOP/s of 16-bit products), 4096 x
-// 1024 x 50000 in bfloat16 1.41 and 1.70 ms (987 TFLOP/s); the value alone of 4096 x 1024 x 50000
-// takes 0.31 ms (1350 TFLOP/s).  Small calls are bound by nine dependent launches: 128 x 8 x 256
+// takes 0.80 ms in a burst and 0.94 ms at the power cap (880 TFLOP/s of 16-bit products), 4096 x
+// 1024 x 50000 in bfloat16 1.50 and 1.69 ms (993 TFLOP/s); the value alone of 4096 x 1024 x 50000
+// takes 0.32 ms (1320 TFLOP/s). The tensor pipe is active 60 % of the value's time (2048 x 1024 x
+// 16384 in bfloat16), 49 of dz's, 49 of dw's, 54 of df's; warps wait for their accumulators (long
+// scoreboard).  Small calls are bound by nine dependent launches: 128 x 8 x 256
 // 39 us as a graph.
 //
-// f_n = g_n / max |g| lies in [-1, 1], so dz needs no more than a fixed scale: 22 bits down
-// to 2^-29, and an absolute error of 2^-40 below.
+// f_n = g_n / max |g| lies in [-1, 1], and dz has a fixed scale of 2^15: 22 bits down to 2^-18 (the low
+// plane's smallest step is 2^-24), an absolute error of 2^-40 below. A class that is improbable in
+// every row (p of 1e-11) therefore keeps one digit of its weight gradient.
 #include <math.h>
 
 #include "nc_readout.h"

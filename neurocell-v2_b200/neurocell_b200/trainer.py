@@ -215,7 +215,7 @@ class VNNTrainStep:
     ``optimizer="muon"`` updates by orthogonalised momentum (``nc_muon_update``) instead of
     SGD: the three cell grids as matrices (H, W), the filters as one matrix (M, Kh Kw), with
     ``beta``, Nesterov momentum and ``weight_decay``; over several ranks it takes the
-    ``"nccl"`` exchange.
+    ``"nccl"`` exchange and updates by the mean gradient (``momentum`` holds the ranks' sum).
     Every kernel of the step except NCCL's comes from ``libneurocell_b200.so``.
     """
 
