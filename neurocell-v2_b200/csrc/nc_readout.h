@@ -60,15 +60,16 @@ __device__ __forceinline__ float2 lse_merge(float2 x, float2 y) {
   return make_float2(m, sx + sy);
 }
 
-// A row's log-sum-exp and loss from the merged pair.  Labels outside the classes, other than
-// ignore_index, make both NaN.
+// A row's log-sum-exp and loss from the merged pair.  The loss is not taken from the log-sum-exp:
+// rounded to float32 that has lost what the other classes add to a large logit.  Labels outside the
+// classes, other than ignore_index, make both NaN.
 __device__ __forceinline__ void finish_row(const CeArgs& a, int row, float2 x, const float* zlabel, float* lse,
                                            float* row_loss) {
   const int label = a.labels[row];
-  float l = x.x + logf(x.y);
-  if (label < 0 || label >= a.classes) l = NAN;
-  lse[row] = l;
-  row_loss[row] = label == a.ignore_index ? 0.f : l - zlabel[row];
+  const bool in = label >= 0 && label < a.classes;
+  const float l = logf(x.y);
+  lse[row] = in ? x.x + l : NAN;
+  row_loss[row] = label == a.ignore_index ? 0.f : in ? x.x - zlabel[row] + l : NAN;
 }
 
 // Rows that take part, counted by a whole block (every thread gets the count).

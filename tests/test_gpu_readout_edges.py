@@ -112,3 +112,33 @@ def test_far_scales_that_meet_in_the_logits(rows, exponent):
     assert abs(float(loss) - float(want.detach())) <= 2.0 ** -20 * 10
     for got, e in zip((gf, gw), torch.autograd.grad(want, (fd, wd))):
         assert (got.double() - e).abs().max() <= 2.0 ** -18 * e.abs().max()
+
+
+# A label's logit of 64 and the others 12 below it, all exact: loss log(1 + (classes - 1) exp(-12)).  exp
+# and log are off by 2^-20 of the small part.  The sum that holds the label's 1 takes further terms by
+# float32 additions, each rounded by at most 2^-24: up to 32 in a tile of 128 classes (four chains, 16 in
+# one of 64; 16 a lane in a window of 512 classes), 2 to join the chains, at most 5 tiles or windows or 5
+# per lane of 300 classes' blocks, and 5 in a warp's tree: under 48.  The rounding of a log-sum-exp of
+# 64.0018 would be 3.3e-6 here, 48 2^-24 is 2.9e-6.
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows", [1, 16, 140])
+def test_the_loss_of_a_confident_row(rows, dtype):
+    classes = 300
+    f = torch.zeros(rows, 24, device=DEV, dtype=dtype)
+    f[:, 0] = 8.0
+    w = torch.zeros(classes, 24, device=DEV, dtype=dtype)
+    w[:, 0] = 6.5
+    w[7, 0] = 8.0
+    lab = torch.full((rows,), 7, device=DEV)
+    loss = ops.linear_softmax_ce_loss(f, w, lab, reduction="none")
+    want = torch.log1p((classes - 1) * torch.exp(torch.tensor(-12.0, dtype=torch.float64)))
+    assert (loss.double() - want.item()).abs().max() <= 48 * 2.0 ** -24 + 2.0 ** -20 * want.item()
+
+
+@pytest.mark.parametrize("rows", [4, 140])
+def test_the_loss_where_every_class_has_the_lowest_bias(rows):
+    f, w, lab = _inputs(rows, 40, 90, torch.float32)
+    b = torch.full((90,), torch.finfo(torch.float32).min, device=DEV)
+    loss = ops.linear_softmax_ce_loss(f, w, lab, bias=b, reduction="none")
+    want = torch.log(torch.tensor(90.0, dtype=torch.float64)).item()
+    assert (loss[::2].double() - want).abs().max() <= 2.0 ** -22 * want and (loss[1::2] == 0).all()
