@@ -271,9 +271,9 @@ typedef enum nc_reduction { NC_REDUCE_MEAN = 0, NC_REDUCE_SUM = 1, NC_REDUCE_NON
  *   the gradients NaN; nothing is read out of range.
  * A bias of -inf takes its class out; a row with every class taken out has a NaN loss, as
  * has one with a logit of NaN or +inf.  Sums and statistics are held in float32.
- * The gradients' probabilities are exp(z - lse), off by 2^-24 |lse| of themselves: a row whose logits
- * are all past 2^22 in magnitude (every class masked by a finite value) has a loss but gradients that
- * mean nothing.
+ * The gradients' probabilities are exp(z - lse), off by 2^-24 |lse| of themselves.  Where that would
+ * be more than an eighth (every class masked by a finite value past 2^20) lse and the gradients are
+ * NaN, beside a loss that is not.
  * Precision with float32 operands and more than 16 rows: as of float32 products, where the
  * entries of a tensor below 2^-18 of its largest finite one count with an absolute error of
  * 2^-38 of that one, and dz = p - onehot with one of at most 2^-40 of the largest |g_loss|

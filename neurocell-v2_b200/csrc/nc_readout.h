@@ -61,14 +61,16 @@ __device__ __forceinline__ float2 lse_merge(float2 x, float2 y) {
 }
 
 // A row's log-sum-exp and loss from the merged pair.  The loss is not taken from the log-sum-exp:
-// rounded to float32 that has lost what the other classes add to a large logit.  Labels outside the
-// classes, other than ignore_index, make both NaN.
+// rounded to float32 that has lost what the other classes add to a large logit.  The gradients do
+// go by the log-sum-exp, which is NaN where its rounding would put them off by more than an eighth (and
+// where no class is left).  Labels outside the classes, other than ignore_index, make both NaN.
 __device__ __forceinline__ void finish_row(const CeArgs& a, int row, float2 x, const float* zlabel, float* lse,
                                            float* row_loss) {
   const int label = a.labels[row];
   const bool in = label >= 0 && label < a.classes;
   const float l = logf(x.y);
-  lse[row] = in ? x.x + l : NAN;
+  const float sum = x.x + l;
+  lse[row] = in && fabsf((sum - x.x) - l) <= 0.125f ? sum : NAN;
   row_loss[row] = label == a.ignore_index ? 0.f : in ? x.x - zlabel[row] + l : NAN;
 }
 

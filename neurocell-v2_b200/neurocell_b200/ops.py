@@ -655,7 +655,7 @@ def linear_softmax_ce_loss(features: torch.Tensor, weight: torch.Tensor, labels:
     whose label is not ``ignore_index`` (0 when there are none), "sum", or "none" (one loss
     per row).  Any other label outside the classes gives NaN.  Differentiable once in
     features, weight and bias (the gradient computes the logits a second time).  A bias of -inf
-    takes its class out; a finite mask has to leave a class for the gradients to mean anything.
+    takes its class out; where every class is masked by a huge finite value the gradients are NaN.
 
     Inside a CUDA graph capture use :func:`linear_softmax_ce_value_and_grad`, which needs no
     autograd: a captured backward pass whose leaves still belong to a live graph built outside

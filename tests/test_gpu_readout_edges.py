@@ -142,3 +142,20 @@ def test_the_loss_where_every_class_has_the_lowest_bias(rows):
     loss = ops.linear_softmax_ce_loss(f, w, lab, bias=b, reduction="none")
     want = torch.log(torch.tensor(90.0, dtype=torch.float64)).item()
     assert (loss[::2].double() - want).abs().max() <= 2.0 ** -22 * want and (loss[1::2] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows", [4, 140])
+def test_gradients_without_a_class_left_are_nan(rows, dtype):
+    f, w, lab = _inputs(rows, 40, 90, dtype)
+    for low in (torch.finfo(dtype).min, -1e9):
+        b = torch.full((90,), low, device=DEV, dtype=dtype)
+        loss, gf, gw, gb = ops.linear_softmax_ce_value_and_grad(f, w, lab, bias=b)
+        assert torch.isfinite(loss)
+        assert gf[::2].isnan().all() and (gf[1::2] == 0).all() and gw.isnan().all() and gb.isnan().all()
+        # one class left, or one far above the others: as ever
+        for high in (0.0, 1e9):
+            b[7] = high
+            one = torch.where(lab == IGNORE, lab, torch.full_like(lab, 7))
+            loss, gf, gw, gb = ops.linear_softmax_ce_value_and_grad(f, w, one, bias=b)
+            assert float(loss) == 0 and not gf.any() and not gw.any() and not gb.any()
