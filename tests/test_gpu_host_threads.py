@@ -44,12 +44,13 @@ def _readout(rows, dim, classes, grad, stream):
     s = ctypes.c_void_p(stream.cuda_stream)
     P = ops._ptr
 
-    def call(keep=(f, w, lab, ws, loss, lse, gf, gw)):
+    def call(keep=(f, w, lab, ws, lse)):
         if grad:
             return lib.nc_linear_ce_value_and_grad(ctypes.byref(d), P(f), P(w), None, P(lab), P(loss), P(lse), P(gf),
                                                    P(gw), None, P(ws), n, s)
         return lib.nc_linear_ce_forward(ctypes.byref(d), P(f), P(w), None, P(lab), P(loss), P(lse), P(ws), n, s)
 
+    call.outputs = [loss, gf, gw] if grad else [loss]
     return call
 
 
@@ -63,9 +64,10 @@ def _orthogonalize(rows, cols, stream):
     s = ctypes.c_void_p(stream.cuda_stream)
     P = ops._ptr
 
-    def call(keep=(x, out, ws)):
+    def call(keep=(x, ws)):
         return lib.nc_orthogonalize(ctypes.byref(d), P(x), P(out), P(ws), n, s)
 
+    call.outputs = [out]
     return call
 
 
@@ -78,4 +80,11 @@ def test_sizes_of_one_kernel_from_two_threads(kind):
     else:
         calls = [_readout(8, dim, 3000, kind == "gradients", s) for dim, s in zip((520, 1024), streams)]
     torch.cuda.synchronize()
+    want = []
+    for c in calls:
+        assert c() == _lib.NC_OK
+        torch.cuda.synchronize()
+        want.append([t.clone() for t in c.outputs])
     assert _at_once(calls, 4000) == []
+    for c, w in zip(calls, want):
+        assert all(torch.equal(x, y) for x, y in zip(c.outputs, w))
